@@ -1,0 +1,578 @@
+// framewise_b200.cu -- the operators of framewise training behind the C ABI of include/framewise_b200.h: output layer
+// with softmax cross entropy (linear_ce_b200.inc), label embedding (embedding_b200.inc), AdamW (adamw_b200.inc).
+// This file holds their host side: sizes, launch shapes, tensor maps.
+#include "framewise_b200.h"
+#include "tensor_core.h"
+
+#include <cuda_runtime.h>
+#include <math_constants.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cfloat>
+#include <cmath>
+#include <cstdint>
+
+namespace {
+
+std::atomic<int64_t> g_launches{0};
+
+#define FW_TRY(call)                                     \
+    do {                                                 \
+        if ((call) != cudaSuccess) return FRAMEWISE_B200_CUDA_ERROR; \
+    } while (0)
+#define FW_LAUNCHED()                                    \
+    do {                                                 \
+        g_launches.fetch_add(1, std::memory_order_relaxed); \
+        FW_TRY(cudaGetLastError());                      \
+    } while (0)
+
+#define FW_DO(...)                                       \
+    do {                                                 \
+        const int status_ = (__VA_ARGS__);                     \
+        if (status_ != FRAMEWISE_B200_OK) return status_; \
+    } while (0)
+
+#include "embedding_b200.inc"
+#include "adamw_b200.inc"
+#include "linear_ce_b200.inc"
+
+constexpr size_t kAlign = 256;
+inline size_t aligned(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
+inline bool   misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & (kAlign - 1)) != 0; }
+inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+// A buffer's parts one after another, each aligned.
+struct Parts {
+    char*  base;
+    size_t used = 0;
+    explicit Parts(void* p) : base(static_cast<char*>(p)) {}
+    template <typename X>
+    X* take(int64_t n) {
+        X* at = base ? reinterpret_cast<X*>(base + used) : nullptr;
+        used += aligned((size_t)n * sizeof(X));
+        return at;
+    }
+};
+
+// The current device's; the device's context is current afterwards (a thread that has made no CUDA call yet, such as
+// torch's for backward passes, has none, and tensor maps need one).
+int bind_device() {
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess ? FRAMEWISE_B200_OK : FRAMEWISE_B200_CUDA_ERROR;
+}
+int sm_count() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return 0;
+    return n;
+}
+
+// ------------------------------------------------------------------------------------------ cross entropy
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static std::atomic<EncodeTiled> cached{nullptr};
+    EncodeTiled f = cached.load(std::memory_order_acquire);
+    if (f) return f;
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+        return nullptr;
+    f = reinterpret_cast<EncodeTiled>(p);
+    cached.store(f, std::memory_order_release);
+    return f;
+}
+
+// planes x rows x cols, rows `pitch` elements apart, read or written in boxes of box_cols x box_rows
+bool map_of(CUtensorMap* map, const void* base, bool f32, int64_t cols, int64_t rows, int64_t planes, int64_t pitch, int64_t plane,
+            int box_cols, int box_rows) {
+    const EncodeTiled f = encode_tiled();
+    if (!f) return false;
+    const int64_t    size = f32 ? 4 : 2;
+    const cuuint64_t dims[3]    = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)(pitch * size), (cuuint64_t)(plane * size)};
+    const cuuint32_t box[3]     = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
+    const cuuint32_t step[3]    = {1, 1, 1};
+    const int row_bytes = box_cols * (int)size;
+    return f(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims,
+             strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr int kPair = 1;  // CTAs per tile
+
+// What a call keeps and uses, from its sizes alone.
+struct CePlan {
+    int64_t N, V, D;
+    int     parts, pitch, chunks, chunk;
+    bool    copy_weight;
+    int     wide_v, wide_d;          // columns of the tiles over V and over D
+    int     splits_hidden, splits_weight;
+    int64_t q_pitch, out_pitch;
+    // saved
+    int32_t*       head;
+    int*           chunk_count;
+    int*           row_label;
+    int*           row_position;
+    uint8_t*       counted;  // per position
+    float*         bias;
+    float2*        stats;
+    __nv_bfloat16* rows;
+    __nv_bfloat16* weight;
+    size_t         saved_bytes;
+    // forward
+    float2* part;
+    float*  target;
+    size_t  forward_bytes;
+    // backward
+    __nv_bfloat16* q;
+    float*         hidden_part;
+    float*         weight_part;
+    float*         col_part;
+    size_t         backward_bytes;
+};
+
+// q of a chunk takes this much at most: some hundred rows of the largest vocabularies, all rows of small batches.
+constexpr int64_t kChunkBytes = (int64_t)768 << 20;
+constexpr int64_t kSplitBytes = (int64_t)256 << 20;
+
+int pick_splits(int64_t tiles, int64_t depth, int workers, int64_t bytes_per_split) {
+    if (tiles >= workers) return 1;
+    int64_t s = workers / std::max<int64_t>(tiles, 1);
+    s = std::min(s, std::max<int64_t>(1, depth / 8));
+    s = std::min(s, std::max<int64_t>(1, kSplitBytes / std::max<int64_t>(bytes_per_split, 1)));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
+}
+
+int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void* backward, CePlan* p) {
+    if (!sh) return FRAMEWISE_B200_BAD_ARGUMENT;
+    const int64_t kMost = (int64_t)1 << 31;
+    if (sh->B < 0 || sh->T < 0 || sh->V < 1 || sh->D < 1 || sh->B >= kMost || sh->T >= kMost || sh->V >= kMost - 256 ||
+        sh->D >= kMost - 256 || sh->B * sh->T >= kMost - 256)
+        return FRAMEWISE_B200_BAD_ARGUMENT;
+    if (sh->dtype != FRAMEWISE_B200_F32 && sh->dtype != FRAMEWISE_B200_BF16) return FRAMEWISE_B200_BAD_ARGUMENT;
+    const int workers = sm_count() / kPair;
+    if (workers < 1) return FRAMEWISE_B200_CUDA_ERROR;
+    p->N = sh->B * sh->T, p->V = sh->V, p->D = sh->D;
+    p->parts       = sh->dtype == FRAMEWISE_B200_F32 ? 3 : 1;
+    p->copy_weight = p->parts == 3 || sh->copy_weight != 0;
+    p->pitch       = (int)up(sh->D, 8);
+    p->chunks      = (int)((p->N + ce::kCountChunk - 1) / ce::kCountChunk);
+    const int     tile   = ce::kRowsPerCta * kPair;
+    const int64_t rows   = up(p->N, 256);
+    const int64_t mt     = rows / tile;
+    // narrower tiles where wide ones would leave SMs idle
+    p->wide_v = 256;
+    while (p->wide_v > 64 * kPair && (p->wide_v / 2 >= p->V || mt * ((p->V + p->wide_v - 1) / p->wide_v) < workers)) p->wide_v /= 2;
+    p->wide_d  = (int)std::min<int64_t>(256, up(p->D, 64 * kPair));
+    p->q_pitch = up(p->V, 8);
+    p->chunk   = (int)std::min(rows, std::max<int64_t>(256, kChunkBytes / (2 * p->parts * p->q_pitch) / 256 * 256));
+    p->out_pitch = up(p->D, 4);
+    const int64_t nt_d = (p->D + p->wide_d - 1) / p->wide_d;
+    p->splits_hidden = pick_splits(p->chunk / tile * nt_d, (p->V + 63) / 64, workers, 4 * p->chunk * p->out_pitch);
+    p->splits_weight = pick_splits((p->V + tile - 1) / tile * nt_d, p->chunk / 64, workers, 4 * p->V * p->out_pitch);
+
+    Parts s(saved);
+    p->head         = s.take<int32_t>(64);
+    p->chunk_count  = s.take<int>(p->chunks);
+    p->row_label    = s.take<int>(rows);
+    p->row_position = s.take<int>(rows);
+    p->counted      = s.take<uint8_t>(sh->train ? p->N : 0);
+    p->bias         = s.take<float>(up(p->V, 256));
+    p->stats        = s.take<float2>(sh->train ? rows : 0);
+    p->rows         = s.take<__nv_bfloat16>(p->parts * rows * p->pitch);
+    p->weight       = s.take<__nv_bfloat16>(p->copy_weight ? p->parts * p->V * p->pitch : 0);
+    p->saved_bytes  = s.used;
+    Parts f(forward);
+    p->part   = f.take<float2>((workers + mt) * 2 * tile);
+    p->target = f.take<float>(rows);
+    p->forward_bytes = f.used;
+    Parts b(backward);
+    p->q           = b.take<__nv_bfloat16>(p->parts * p->chunk * p->q_pitch);
+    p->hidden_part = b.take<float>((int64_t)p->splits_hidden * p->chunk * p->out_pitch);
+    p->weight_part = b.take<float>((int64_t)p->splits_weight * p->V * p->out_pitch);
+    p->col_part    = b.take<float>(sh->has_bias ? rows / 32 * up(p->V, 256) : 0);
+    p->backward_bytes = b.used;
+    return FRAMEWISE_B200_OK;
+}
+
+template <int KIND, int PARTS>
+int launch_tiles(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const ce::Params& p, int workers, cudaStream_t stream) {
+    using L = ce::Layout<KIND, kPair>;
+    auto kernel = ce::k_ce_tiles<KIND, kPair, PARTS>;
+    FW_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+    cudaLaunchConfig_t c = {};
+    c.gridDim          = dim3(workers * kPair);
+    c.blockDim         = dim3(ce::kThreads);
+    c.dynamicSmemBytes = L::kBytes;
+    c.stream           = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = kPair, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    c.attrs    = at;
+    c.numAttrs = kPair > 1 ? 1 : 0;
+    FW_TRY(cudaLaunchKernelEx(&c, kernel, a, b, out, p));
+    FW_LAUNCHED();
+    return FRAMEWISE_B200_OK;
+}
+
+template <typename X, typename L>
+int ce_forward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* hidden, const X* weight, const X* bias, const L* targets,
+               const int32_t* lens, float* loss, cudaStream_t stream) {
+    constexpr int PARTS = sizeof(X) == 4 ? 3 : 1;
+    const int workers = sm_count() / kPair, tile = ce::kRowsPerCta * kPair;
+    const int64_t rows = up(p.N, 256);
+    FW_DO(bind_device());
+    ce::k_count_rows<<<p.chunks + (int)(up(p.V, 256) / 256), 256, 0, stream>>>(p.N, (int)sh.T, targets, lens, sh.ignore_index, p.chunks,
+                                                                            p.chunk_count, bias, p.bias, (int)p.V, p.head);
+    FW_LAUNCHED();
+    ce::k_gather_rows<X, L, PARTS><<<(unsigned)((p.N + ce::kGatherRows - 1) / ce::kGatherRows), 256, 0, stream>>>(
+        p.N, (int)sh.T, hidden, sh.hidden_stride_b, sh.hidden_stride_t, targets, lens, sh.ignore_index, p.chunk_count, p.head, (int)p.V,
+        (int)p.D, p.pitch, p.rows, rows * p.pitch, p.row_label, p.row_position, sh.train ? p.counted : nullptr, loss);
+    FW_LAUNCHED();
+    if (p.copy_weight) {
+        ce::k_split_weight<X, PARTS><<<(unsigned)((p.V + 7) / 8), 256, 0, stream>>>(weight, p.weight, p.V * p.pitch, (int)p.V, (int)p.D, p.pitch);
+        FW_LAUNCHED();
+    }
+    const void*   w       = p.copy_weight ? (const void*)p.weight : (const void*)weight;
+    const int64_t w_pitch = p.copy_weight ? p.pitch : p.D;
+    CUtensorMap a, b;
+    if (!map_of(&a, p.rows, false, p.D, rows, PARTS, p.pitch, rows * p.pitch, 64, ce::kRowsPerCta) ||
+        !map_of(&b, w, false, p.D, p.V, PARTS, w_pitch, p.V * w_pitch, 64, p.wide_v / kPair))
+        return FRAMEWISE_B200_TENSOR_MAP;
+    ce::Params q = {};
+    q.head = p.head, q.V = (int)p.V, q.D = (int)p.D, q.wide = p.wide_v, q.splits = 1;
+    q.bias = p.bias, q.label = p.row_label, q.part = p.part, q.target = p.target;
+    FW_DO(launch_tiles<ce::kLogits, PARTS>(a, b, a, q, workers, stream));
+    ce::k_join_rows<<<(unsigned)((p.N + 127) / 128), 128, 0, stream>>>(p.head, (int)((p.V + p.wide_v - 1) / p.wide_v), tile, workers, p.part,
+                                                                    p.target, p.row_label, p.row_position, loss, sh.train ? p.stats : nullptr);
+    FW_LAUNCHED();
+    return FRAMEWISE_B200_OK;
+}
+
+template <typename X>
+int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* weight, const float* grad, int64_t grad_b, int64_t grad_t,
+                X* grad_hidden, X* grad_weight, X* grad_bias, cudaStream_t stream) {
+    constexpr int PARTS = sizeof(X) == 4 ? 3 : 1;
+    const int workers = sm_count() / kPair;
+    const int64_t rows = up(p.N, 256);
+    const void*   w       = p.copy_weight ? (const void*)p.weight : (const void*)weight;
+    const int64_t w_pitch = p.copy_weight ? p.pitch : p.D, V = p.V, D = p.D;
+    FW_DO(bind_device());
+    CUtensorMap x_k, w_k, q_out, q_k, w_mn, q_mn, x_mn, h_out, w_out;
+    if (!map_of(&x_k, p.rows, false, D, rows, PARTS, p.pitch, rows * p.pitch, 64, ce::kRowsPerCta) ||
+        !map_of(&w_k, w, false, D, V, PARTS, w_pitch, V * w_pitch, 64, p.wide_v / kPair) ||
+        !map_of(&q_out, p.q, false, V, p.chunk, PARTS, p.q_pitch, p.chunk * p.q_pitch, 32, 32) ||
+        !map_of(&q_k, p.q, false, V, p.chunk, PARTS, p.q_pitch, p.chunk * p.q_pitch, 64, ce::kRowsPerCta) ||
+        !map_of(&q_mn, p.q, false, V, p.chunk, PARTS, p.q_pitch, p.chunk * p.q_pitch, 64, 64) ||
+        !map_of(&w_mn, w, false, D, V, PARTS, w_pitch, V * w_pitch, 64, 64) ||
+        !map_of(&x_mn, p.rows, false, D, rows, PARTS, p.pitch, rows * p.pitch, 64, 64) ||
+        !map_of(&h_out, p.hidden_part, true, D, p.chunk, p.splits_hidden, p.out_pitch, p.chunk * p.out_pitch, 32, 32) ||
+        !map_of(&w_out, p.weight_part, true, D, V, p.splits_weight, p.out_pitch, V * p.out_pitch, 32, 32))
+        return FRAMEWISE_B200_TENSOR_MAP;
+    if (grad_hidden) {
+        ce::k_hidden_zero<X><<<(unsigned)((p.N + 7) / 8), 256, 0, stream>>>(p.N, p.counted, (int)D, grad_hidden);
+        FW_LAUNCHED();
+    }
+    ce::Params g = {};
+    g.head = p.head, g.V = (int)V, g.D = (int)D, g.chunk = p.chunk;
+    g.bias = p.bias, g.label = p.row_label, g.position = p.row_position, g.stats = p.stats;
+    g.grad = grad, g.grad_b = grad_b, g.grad_t = grad_t, g.T = (int)sh.T;
+    g.col_part = grad_bias ? p.col_part : nullptr, g.col_pitch = (int)up(V, 256);
+    for (int64_t row0 = 0; row0 < rows; row0 += p.chunk) {
+        g.row0 = (int)row0, g.add = row0 > 0;
+        g.wide = p.wide_v, g.splits = 1;
+        FW_DO(launch_tiles<ce::kGradients, PARTS>(x_k, w_k, q_out, g, workers, stream));
+        g.wide = p.wide_d;
+        if (grad_hidden) {
+            g.splits = p.splits_hidden;
+            FW_DO(launch_tiles<ce::kToHidden, PARTS>(q_k, w_mn, h_out, g, workers, stream));
+            ce::k_hidden_out<X><<<(unsigned)(p.chunk / 8), 256, 0, stream>>>(p.head, (int)row0, p.chunk, p.splits_hidden, p.hidden_part, (int)D,
+                                                                          (int)p.out_pitch, p.row_position, grad_hidden);
+            FW_LAUNCHED();
+        }
+        if (grad_weight) {
+            g.splits = p.splits_weight;
+            FW_DO(launch_tiles<ce::kToWeight, PARTS>(q_mn, x_mn, w_out, g, workers, stream));
+        }
+    }
+    if (grad_weight) {
+        ce::k_weight_out<X><<<(unsigned)((V + 7) / 8), 256, 0, stream>>>(p.head, p.splits_weight, p.weight_part, (int)V, (int)D, (int)p.out_pitch, grad_weight);
+        FW_LAUNCHED();
+    }
+    if (grad_bias) {
+        ce::k_bias_out<X><<<(unsigned)((V + 31) / 32), 256, 0, stream>>>(p.head, p.col_part, (int)up(V, 256), (int)V, grad_bias);
+        FW_LAUNCHED();
+    }
+    return FRAMEWISE_B200_OK;
+}
+
+// ------------------------------------------------------------------------------------------ embedding
+
+struct EmbedPlan {
+    int64_t   N;
+    int       chunks, passes, digits[2];
+    uint32_t *keys[2], *places[2];
+    int32_t * counts, *before, *total, *all;
+    float*    edge;
+    size_t    bytes;
+};
+
+bool embed_sizes_ok(int64_t B, int64_t T, int64_t V, int64_t D) {
+    const int64_t kMost = (int64_t)1 << 31;
+    return B >= 0 && T >= 0 && B < kMost && T < kMost && B * T < kMost - 1024 && V >= 1 && V < ((int64_t)1 << 28) && D >= 1 && D < kMost - 256;
+}
+
+EmbedPlan embed_plan(int64_t B, int64_t T, int64_t V, int64_t D, void* work) {
+    EmbedPlan p;
+    p.N         = B * T;
+    p.chunks    = (int)((p.N + embed::kChunk - 1) / embed::kChunk);
+    p.passes    = V + 1 > embed::kDigits ? 2 : 1;  // keys up to V: labels outside the vocabulary
+    p.digits[0] = (int)std::min<int64_t>(V + 1, embed::kDigits);
+    p.digits[1] = (int)(V / embed::kDigits) + 1;
+    const int digits = std::max(p.digits[0], p.passes == 2 ? p.digits[1] : 0);
+    Parts b(work);
+    for (int i = 0; i < 2; ++i) {
+        p.keys[i]   = b.take<uint32_t>(i < p.passes ? p.N : 0);
+        p.places[i] = b.take<uint32_t>(i < p.passes ? p.N : 0);
+    }
+    p.counts = b.take<int32_t>((int64_t)p.chunks * digits);
+    p.before = b.take<int32_t>(digits);
+    p.total  = b.take<int32_t>(digits / embed::kScanRow + 1);
+    p.all    = b.take<int32_t>(1);
+    p.edge   = b.take<float>((p.N + embed::kPiece - 1) / embed::kPiece * 2 * D);
+    p.bytes  = b.used;
+    return p;
+}
+
+template <typename S>
+int sort_pass(const S& src, const EmbedPlan& p, int pass, cudaStream_t stream) {
+    const int digits = p.digits[pass], shift = 14 * pass, scans = (digits + embed::kScanRow - 1) / embed::kScanRow;
+    static_assert(embed::kDigits == 1 << 14, "");
+    const size_t bytes = (size_t)digits * 4;
+    FW_TRY(cudaFuncSetAttribute(embed::k_sort_count<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, embed::kDigits * 4));
+    FW_TRY(cudaFuncSetAttribute(embed::k_sort_place<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, embed::kDigits * 4));
+    embed::k_sort_count<S><<<p.chunks, 256, bytes, stream>>>(src, shift, digits, p.counts);
+    FW_LAUNCHED();
+    embed::k_sort_scan<<<scans, embed::kScanRow, 0, stream>>>(p.counts, p.chunks, digits, p.before, p.total);
+    FW_LAUNCHED();
+    embed::k_sort_place<S><<<p.chunks, 32, bytes, stream>>>(src, shift, digits, p.counts, p.before, p.total, scans, p.keys[pass], p.places[pass], p.all);
+    FW_LAUNCHED();
+    return FRAMEWISE_B200_OK;
+}
+
+template <typename X, typename L>
+int embed_forward(int64_t N, int64_t T, int64_t V, int64_t D, int64_t ignore, float scale, const X* table, const L* labels,
+                  const int32_t* lens, X* out, cudaStream_t stream) {
+    const bool wide = D % 8 == 0 && ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+    const unsigned grid = (unsigned)((N + 7) / 8);
+    if (wide)
+        embed::k_embed<X, L, true><<<grid, 256, 0, stream>>>(N, (int)T, V, (int)D, table, labels, lens, ignore, scale, out);
+    else
+        embed::k_embed<X, L, false><<<grid, 256, 0, stream>>>(N, (int)T, V, (int)D, table, labels, lens, ignore, scale, out);
+    FW_LAUNCHED();
+    return FRAMEWISE_B200_OK;
+}
+
+template <typename X, typename L>
+int embed_backward(const EmbedPlan& p, int64_t T, int64_t V, int64_t D, int64_t ignore, float scale, const X* grad, int64_t grad_b,
+                   int64_t grad_t, const L* labels, const int32_t* lens, X* out, cudaStream_t stream) {
+    FW_DO(sort_pass(embed::FromLabels<L>{labels, lens, p.N, ignore, V, (int)T}, p, 0, stream));
+    if (p.passes == 2) FW_DO(sort_pass(embed::FromKeys{p.keys[0], p.places[0], p.all}, p, 1, stream));
+    const uint32_t *keys = p.keys[p.passes - 1], *places = p.places[p.passes - 1];
+    const int     slices = (int)((D + embed::kSlice - 1) / embed::kSlice);
+    const int64_t jobs   = (p.N + embed::kPiece - 1) / embed::kPiece * slices;
+    const int64_t lanes  = 16 / (int64_t)sizeof(X);
+    const bool wide = D % 8 == 0 && grad_b % lanes == 0 && grad_t % lanes == 0 && (reinterpret_cast<uintptr_t>(grad) & 15) == 0;
+    if ((jobs + 7) / 8 >= (int64_t)1 << 31) return FRAMEWISE_B200_BAD_ARGUMENT;
+    if (wide)
+        embed::k_embed_pieces<X, true><<<(unsigned)((jobs + 7) / 8), 256, 0, stream>>>(p.all, V, (int)D, slices, (int)T, grad, grad_b, grad_t, keys, places, scale, p.edge, out);
+    else
+        embed::k_embed_pieces<X, false><<<(unsigned)((jobs + 7) / 8), 256, 0, stream>>>(p.all, V, (int)D, slices, (int)T, grad, grad_b, grad_t, keys, places, scale, p.edge, out);
+    FW_LAUNCHED();
+    embed::k_embed_rows<X><<<(unsigned)((V + 7) / 8), 256, 0, stream>>>(p.all, V, (int)D, keys, scale, p.edge, out);
+    FW_LAUNCHED();
+    return FRAMEWISE_B200_OK;
+}
+
+// ------------------------------------------------------------------------------------------ AdamW
+
+// Calls `launch` for groups of up to kSlots tensors.
+template <typename F>
+int for_slots(const framewise_b200_tensor* tensors, int64_t count, bool codes, F&& launch) {
+    int64_t i = 0;
+    while (i < count) {
+        adamw::Slots s;
+        s.count = 0, s.blocks = 0;
+        for (; i < count && s.count < adamw::kSlots; ++i) {
+            const framewise_b200_tensor& t = tensors[i];
+            if (t.n == 0) continue;
+            adamw::Slot& o = s.slot[s.count++];
+            o.param = t.param, o.grad = t.grad, o.master = t.master, o.m = t.exp_avg, o.v = t.exp_avg_sq;
+            o.m_steps = t.exp_avg_steps, o.v_steps = t.exp_avg_sq_steps, o.n = t.n, o.first = s.blocks;
+            const uintptr_t all = reinterpret_cast<uintptr_t>(t.param) | reinterpret_cast<uintptr_t>(t.grad) | reinterpret_cast<uintptr_t>(t.master);
+            const uintptr_t held = reinterpret_cast<uintptr_t>(t.exp_avg) | reinterpret_cast<uintptr_t>(t.exp_avg_sq);
+            o.wide = all % 16 == 0 && held % (codes ? 8 : 16) == 0;
+            s.blocks += (t.n + adamw::kBlock - 1) / adamw::kBlock;
+        }
+        if (s.count) FW_DO(launch(s));
+    }
+    return FRAMEWISE_B200_OK;
+}
+
+unsigned adamw_grid(int64_t blocks) { return (unsigned)std::min<int64_t>((blocks + 7) / 8, (int64_t)sm_count() * 64); }
+
+}  // namespace
+
+extern "C" {
+
+int64_t framewise_b200_launch_count(void) { return g_launches.load(); }
+
+const char* framewise_b200_status_string(int status) {
+    switch (status) {
+        case FRAMEWISE_B200_OK: return "ok";
+        case FRAMEWISE_B200_BAD_ARGUMENT: return "bad argument";
+        case FRAMEWISE_B200_WORKSPACE: return "buffer too small";
+        case FRAMEWISE_B200_CUDA_ERROR: return "CUDA error";
+        case FRAMEWISE_B200_TENSOR_MAP: return "a tensor map could not be made";
+        default: return "unknown status";
+    }
+}
+
+int framewise_b200_ce_bytes(const framewise_b200_ce_shape* shape, size_t* saved_bytes, size_t* forward_work_bytes,
+                            size_t* backward_work_bytes) {
+    CePlan p;
+    if (!saved_bytes || !forward_work_bytes || !backward_work_bytes) return FRAMEWISE_B200_BAD_ARGUMENT;
+    FW_DO(ce_plan(shape, nullptr, nullptr, nullptr, &p));
+    *saved_bytes = p.saved_bytes, *forward_work_bytes = p.forward_bytes, *backward_work_bytes = p.backward_bytes;
+    return FRAMEWISE_B200_OK;
+}
+
+int framewise_b200_ce_forward(const framewise_b200_ce_shape* shape, const void* hidden, const void* weight, const void* bias,
+                              const void* targets, const int32_t* seq_lens, float* loss, void* saved, size_t saved_bytes, void* work,
+                              size_t work_bytes, framewise_b200_stream_t stream) {
+    CePlan p;
+    FW_DO(ce_plan(shape, saved, work, nullptr, &p));
+    if (p.N == 0) return FRAMEWISE_B200_OK;
+    if (!hidden || !weight || !targets || !loss || !saved || !work || misaligned(saved) || misaligned(work) || (shape->has_bias && !bias))
+        return FRAMEWISE_B200_BAD_ARGUMENT;
+    if (!p.copy_weight && (reinterpret_cast<uintptr_t>(weight) % 16 != 0 || p.D % 8 != 0)) return FRAMEWISE_B200_BAD_ARGUMENT;
+    if (saved_bytes < p.saved_bytes || work_bytes < p.forward_bytes) return FRAMEWISE_B200_WORKSPACE;
+    if (!shape->has_bias) bias = nullptr;
+    auto go = [&](auto x, auto l) {
+        using X = decltype(x);
+        using L = decltype(l);
+        return ce_forward<X, L>(*shape, p, (const X*)hidden, (const X*)weight, (const X*)bias, (const L*)targets, seq_lens, loss, stream);
+    };
+    if (shape->dtype == FRAMEWISE_B200_F32) return shape->labels64 ? go(float(), int64_t()) : go(float(), int32_t());
+    return shape->labels64 ? go(__nv_bfloat16(), int64_t()) : go(__nv_bfloat16(), int32_t());
+}
+
+int framewise_b200_ce_backward(const framewise_b200_ce_shape* shape, const void* weight, const float* grad_loss, int64_t grad_stride_b,
+                               int64_t grad_stride_t, void* grad_hidden, void* grad_weight, void* grad_bias, const void* saved,
+                               size_t saved_bytes, void* work, size_t work_bytes, framewise_b200_stream_t stream) {
+    CePlan p;
+    FW_DO(ce_plan(shape, const_cast<void*>(saved), nullptr, work, &p));
+    const size_t size = shape->dtype == FRAMEWISE_B200_F32 ? 4 : 2;
+    if (p.N == 0) {
+        if (grad_weight) FW_TRY(cudaMemsetAsync(grad_weight, 0, (size_t)p.V * p.D * size, stream));
+        if (grad_bias) FW_TRY(cudaMemsetAsync(grad_bias, 0, (size_t)p.V * size, stream));
+        return FRAMEWISE_B200_OK;
+    }
+    if (!shape->train || !weight || !grad_loss || !saved || !work || misaligned(saved) || misaligned(work) || (grad_bias && !shape->has_bias))
+        return FRAMEWISE_B200_BAD_ARGUMENT;
+    if (!p.copy_weight && (reinterpret_cast<uintptr_t>(weight) % 16 != 0 || p.D % 8 != 0)) return FRAMEWISE_B200_BAD_ARGUMENT;
+    if (saved_bytes < p.saved_bytes || work_bytes < p.backward_bytes) return FRAMEWISE_B200_WORKSPACE;
+    if (shape->dtype == FRAMEWISE_B200_F32)
+        return ce_backward<float>(*shape, p, (const float*)weight, grad_loss, grad_stride_b, grad_stride_t, (float*)grad_hidden,
+                                  (float*)grad_weight, (float*)grad_bias, stream);
+    return ce_backward<__nv_bfloat16>(*shape, p, (const __nv_bfloat16*)weight, grad_loss, grad_stride_b, grad_stride_t,
+                                      (__nv_bfloat16*)grad_hidden, (__nv_bfloat16*)grad_weight, (__nv_bfloat16*)grad_bias, stream);
+}
+
+int framewise_b200_embed_forward(int64_t B, int64_t T, int64_t V, int64_t D, int32_t dtype, int32_t labels64, int64_t ignore_index,
+                                 float scale, const void* table, const void* labels, const int32_t* seq_lens, void* out,
+                                 framewise_b200_stream_t stream) {
+    if (!embed_sizes_ok(B, T, V, D) || (dtype != FRAMEWISE_B200_F32 && dtype != FRAMEWISE_B200_BF16)) return FRAMEWISE_B200_BAD_ARGUMENT;
+    if (B * T == 0) return FRAMEWISE_B200_OK;
+    if (!table || !labels || !out) return FRAMEWISE_B200_BAD_ARGUMENT;
+    auto go = [&](auto x, auto l) {
+        using X = decltype(x);
+        using L = decltype(l);
+        return embed_forward<X, L>(B * T, T, V, D, ignore_index, scale, (const X*)table, (const L*)labels, seq_lens, (X*)out, stream);
+    };
+    if (dtype == FRAMEWISE_B200_F32) return labels64 ? go(float(), int64_t()) : go(float(), int32_t());
+    return labels64 ? go(__nv_bfloat16(), int64_t()) : go(__nv_bfloat16(), int32_t());
+}
+
+size_t framewise_b200_embed_bytes(int64_t B, int64_t T, int64_t V, int64_t D) {
+    return embed_sizes_ok(B, T, V, D) ? embed_plan(B, T, V, D, nullptr).bytes : 0;
+}
+
+int framewise_b200_embed_backward(int64_t B, int64_t T, int64_t V, int64_t D, int32_t dtype, int32_t labels64, int64_t ignore_index,
+                                  float scale, const void* grad_out, int64_t grad_stride_b, int64_t grad_stride_t, const void* labels,
+                                  const int32_t* seq_lens, void* grad_table, void* work, size_t work_bytes, framewise_b200_stream_t stream) {
+    if (!embed_sizes_ok(B, T, V, D) || (dtype != FRAMEWISE_B200_F32 && dtype != FRAMEWISE_B200_BF16) || !grad_table)
+        return FRAMEWISE_B200_BAD_ARGUMENT;
+    if (B * T == 0) {
+        FW_TRY(cudaMemsetAsync(grad_table, 0, (size_t)V * D * (dtype == FRAMEWISE_B200_F32 ? 4 : 2), stream));
+        return FRAMEWISE_B200_OK;
+    }
+    if (!grad_out || !labels || !work || misaligned(work)) return FRAMEWISE_B200_BAD_ARGUMENT;
+    const EmbedPlan p = embed_plan(B, T, V, D, work);
+    if (work_bytes < p.bytes) return FRAMEWISE_B200_WORKSPACE;
+    auto go = [&](auto x, auto l) {
+        using X = decltype(x);
+        using L = decltype(l);
+        return embed_backward<X, L>(p, T, V, D, ignore_index, scale, (const X*)grad_out, grad_stride_b, grad_stride_t, (const L*)labels, seq_lens,
+                                    (X*)grad_table, stream);
+    };
+    if (dtype == FRAMEWISE_B200_F32) return labels64 ? go(float(), int64_t()) : go(float(), int32_t());
+    return labels64 ? go(__nv_bfloat16(), int64_t()) : go(__nv_bfloat16(), int32_t());
+}
+
+int framewise_b200_adamw(const framewise_b200_tensor* tensors, int64_t count, int32_t dtype, int32_t state_bits, double lr, double beta1,
+                         double beta2, double eps, double weight_decay, int64_t step, framewise_b200_stream_t stream) {
+    if ((count > 0 && !tensors) || count < 0 || step < 1 || (state_bits != 8 && state_bits != 32) ||
+        (dtype != FRAMEWISE_B200_F32 && dtype != FRAMEWISE_B200_BF16))
+        return FRAMEWISE_B200_BAD_ARGUMENT;
+    for (int64_t i = 0; i < count; ++i) {
+        const framewise_b200_tensor& t = tensors[i];
+        if (t.n < 0 || (t.n > 0 && (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq ||
+                                    (state_bits == 8 && (!t.exp_avg_steps || !t.exp_avg_sq_steps)))))
+            return FRAMEWISE_B200_BAD_ARGUMENT;
+    }
+    const adamw::Rates r = {(float)beta1, (float)(1 - beta1), (float)beta2, (float)(1 - beta2), (float)(1 - lr * weight_decay),
+                            (float)(lr / (1 - std::pow(beta1, (double)step))), (float)(1 / std::sqrt(1 - std::pow(beta2, (double)step))), (float)eps};
+    return for_slots(tensors, count, state_bits == 8, [&](const adamw::Slots& s) -> int {
+        const unsigned grid = adamw_grid(s.blocks);
+        if (dtype == FRAMEWISE_B200_F32 && state_bits == 32) adamw::k_adamw<float, 32><<<grid, 256, 0, stream>>>(s, r);
+        else if (dtype == FRAMEWISE_B200_F32) adamw::k_adamw<float, 8><<<grid, 256, 0, stream>>>(s, r);
+        else if (state_bits == 32) adamw::k_adamw<__nv_bfloat16, 32><<<grid, 256, 0, stream>>>(s, r);
+        else adamw::k_adamw<__nv_bfloat16, 8><<<grid, 256, 0, stream>>>(s, r);
+        FW_LAUNCHED();
+        return FRAMEWISE_B200_OK;
+    });
+}
+
+int framewise_b200_adamw_decode(const framewise_b200_tensor* tensors, int64_t count, framewise_b200_stream_t stream) {
+    if ((count > 0 && !tensors) || count < 0) return FRAMEWISE_B200_BAD_ARGUMENT;
+    for (int64_t i = 0; i < count; ++i) {
+        const framewise_b200_tensor& t = tensors[i];
+        if (t.n < 0 || (t.n > 0 && (!t.param || !t.master || !t.exp_avg || !t.exp_avg_sq || !t.exp_avg_steps || !t.exp_avg_sq_steps)))
+            return FRAMEWISE_B200_BAD_ARGUMENT;
+    }
+    return for_slots(tensors, count, true, [&](const adamw::Slots& s) -> int {
+        adamw::k_adamw_decode<<<adamw_grid(s.blocks), 256, 0, stream>>>(s);
+        FW_LAUNCHED();
+        return FRAMEWISE_B200_OK;
+    });
+}
+
+}  // extern "C"
