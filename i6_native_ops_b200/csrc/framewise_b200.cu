@@ -105,15 +105,14 @@ bool map_of(CUtensorMap* map, const void* base, bool f32, int64_t cols, int64_t 
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-constexpr int kPair = 1;  // CTAs per tile
-
 // What a call keeps and uses, from its sizes alone.
 struct CePlan {
     int64_t N, V, D;
+    int     pair;                    // CTAs per tile
     int     parts, pitch, chunks, chunk;
     bool    copy_weight;
     int     wide_v, wide_d;          // columns of the tiles over V and over D
-    int     splits_hidden, splits_weight;
+    int     row_chunks;                  // chunks of rows
     int64_t q_pitch, out_pitch;
     // saved
     int32_t*       head;
@@ -132,23 +131,17 @@ struct CePlan {
     size_t  forward_bytes;
     // backward
     __nv_bfloat16* q;
-    float*         hidden_part;
-    float*         weight_part;
+    float*         pieces;
+    float*         acc;       // the weight's gradient in 32 bits, where it takes several chunks
     float*         col_part;
+    int64_t        col_chunk; // its values per chunk
     size_t         backward_bytes;
 };
 
 // q of a chunk takes this much at most: some hundred rows of the largest vocabularies, all rows of small batches.
 constexpr int64_t kChunkBytes = (int64_t)768 << 20;
-constexpr int64_t kSplitBytes = (int64_t)256 << 20;
-
-int pick_splits(int64_t tiles, int64_t depth, int workers, int64_t bytes_per_split) {
-    if (tiles >= workers) return 1;
-    int64_t s = workers / std::max<int64_t>(tiles, 1);
-    s = std::min(s, std::max<int64_t>(1, depth / 8));
-    s = std::min(s, std::max<int64_t>(1, kSplitBytes / std::max<int64_t>(bytes_per_split, 1)));
-    return (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
-}
+// Up to this many rows a tile is one CTA's.
+constexpr int64_t kOneCta = 128;
 
 int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void* backward, CePlan* p) {
     if (!sh) return FRAMEWISE_B200_BAD_ARGUMENT;
@@ -157,15 +150,16 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
         sh->D >= kMost - 256 || sh->B * sh->T >= kMost - 256)
         return FRAMEWISE_B200_BAD_ARGUMENT;
     if (sh->dtype != FRAMEWISE_B200_F32 && sh->dtype != FRAMEWISE_B200_BF16) return FRAMEWISE_B200_BAD_ARGUMENT;
-    const int workers = sm_count() / kPair;
-    if (workers < 1) return FRAMEWISE_B200_CUDA_ERROR;
     p->N = sh->B * sh->T, p->V = sh->V, p->D = sh->D;
+    p->pair = p->N > kOneCta ? 2 : 1;
+    const int kPair = p->pair, workers = sm_count() / kPair;
+    if (workers < 1) return FRAMEWISE_B200_CUDA_ERROR;
     p->parts       = sh->dtype == FRAMEWISE_B200_F32 ? 3 : 1;
     p->copy_weight = p->parts == 3 || sh->copy_weight != 0;
     p->pitch       = (int)up(sh->D, 8);
     p->chunks      = (int)((p->N + ce::kCountChunk - 1) / ce::kCountChunk);
     const int     tile   = ce::kRowsPerCta * kPair;
-    const int64_t rows   = up(p->N, 256);
+    const int64_t rows   = up(std::max<int64_t>(p->N, 1), 256);
     const int64_t mt     = rows / tile;
     // narrower tiles where wide ones would leave SMs idle
     p->wide_v = 256;
@@ -174,9 +168,7 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
     p->q_pitch = up(p->V, 8);
     p->chunk   = (int)std::min(rows, std::max<int64_t>(256, kChunkBytes / (2 * p->parts * p->q_pitch) / 256 * 256));
     p->out_pitch = up(p->D, 4);
-    const int64_t nt_d = (p->D + p->wide_d - 1) / p->wide_d;
-    p->splits_hidden = pick_splits(p->chunk / tile * nt_d, (p->V + 63) / 64, workers, 4 * p->chunk * p->out_pitch);
-    p->splits_weight = pick_splits((p->V + tile - 1) / tile * nt_d, p->chunk / 64, workers, 4 * p->V * p->out_pitch);
+    p->row_chunks = (int)((rows + p->chunk - 1) / p->chunk);
 
     Parts s(saved);
     p->head         = s.take<int32_t>(64);
@@ -195,14 +187,15 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
     p->forward_bytes = f.used;
     Parts b(backward);
     p->q           = b.take<__nv_bfloat16>(p->parts * p->chunk * p->q_pitch);
-    p->hidden_part = b.take<float>((int64_t)p->splits_hidden * p->chunk * p->out_pitch);
-    p->weight_part = b.take<float>((int64_t)p->splits_weight * p->V * p->out_pitch);
-    p->col_part    = b.take<float>(sh->has_bias ? rows / 32 * up(p->V, 256) : 0);
+    p->pieces   = b.take<float>((int64_t)2 * workers * tile * ce::kWide);
+    p->acc      = b.take<float>(p->row_chunks > 1 ? p->V * p->out_pitch : 0);
+    p->col_chunk = (workers + (p->V + p->wide_v - 1) / p->wide_v) * 4 * kPair * ce::kWide;
+    p->col_part = b.take<float>(sh->has_bias ? p->row_chunks * p->col_chunk : 0);
     p->backward_bytes = b.used;
     return FRAMEWISE_B200_OK;
 }
 
-template <int KIND, int PARTS>
+template <int KIND, int kPair, int PARTS>
 int launch_tiles(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const ce::Params& p, int workers, cudaStream_t stream) {
     using L = ce::Layout<KIND, kPair>;
     auto kernel = ce::k_ce_tiles<KIND, kPair, PARTS>;
@@ -222,7 +215,7 @@ int launch_tiles(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& 
     return FRAMEWISE_B200_OK;
 }
 
-template <typename X, typename L>
+template <int kPair, typename X, typename L>
 int ce_forward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* hidden, const X* weight, const X* bias, const L* targets,
                const int32_t* lens, float* loss, cudaStream_t stream) {
     constexpr int PARTS = sizeof(X) == 4 ? 3 : 1;
@@ -247,16 +240,21 @@ int ce_forward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* hidd
         !map_of(&b, w, false, p.D, p.V, PARTS, w_pitch, p.V * w_pitch, 64, p.wide_v / kPair))
         return FRAMEWISE_B200_TENSOR_MAP;
     ce::Params q = {};
-    q.head = p.head, q.V = (int)p.V, q.D = (int)p.D, q.wide = p.wide_v, q.splits = 1;
+    q.head = p.head, q.V = (int)p.V, q.D = (int)p.D, q.wide = p.wide_v;
     q.bias = p.bias, q.label = p.row_label, q.part = p.part, q.target = p.target;
-    FW_DO(launch_tiles<ce::kLogits, PARTS>(a, b, a, q, workers, stream));
-    ce::k_join_rows<<<(unsigned)((p.N + 127) / 128), 128, 0, stream>>>(p.head, (int)((p.V + p.wide_v - 1) / p.wide_v), tile, workers, p.part,
-                                                                    p.target, p.row_label, p.row_position, loss, sh.train ? p.stats : nullptr);
+    FW_DO(launch_tiles<ce::kLogits, kPair, PARTS>(a, b, a, q, workers, stream));
+    const int nt = (int)((p.V + p.wide_v - 1) / p.wide_v);
+    auto join = [&](auto* kernel, int64_t lanes) {
+        kernel<<<(unsigned)((p.N * lanes + 255) / 256), 256, 0, stream>>>(p.head, nt, tile, workers, p.part, p.target, p.row_label, p.row_position,
+                                                                       loss, sh.train ? p.stats : nullptr);
+    };
+    if (p.N > 4096) join(ce::k_join_rows<4>, 4);
+    else join(ce::k_join_rows<32>, 32);
     FW_LAUNCHED();
     return FRAMEWISE_B200_OK;
 }
 
-template <typename X>
+template <int kPair, typename X>
 int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* weight, const float* grad, int64_t grad_b, int64_t grad_t,
                 X* grad_hidden, X* grad_weight, X* grad_bias, cudaStream_t stream) {
     constexpr int PARTS = sizeof(X) == 4 ? 3 : 1;
@@ -265,7 +263,8 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
     const void*   w       = p.copy_weight ? (const void*)p.weight : (const void*)weight;
     const int64_t w_pitch = p.copy_weight ? p.pitch : p.D, V = p.V, D = p.D;
     FW_DO(bind_device());
-    CUtensorMap x_k, w_k, q_out, q_k, w_mn, q_mn, x_mn, h_out, w_out;
+    const bool several = p.row_chunks > 1;
+    CUtensorMap x_k, w_k, q_out, q_k, w_mn, q_mn, x_mn, w_out;
     if (!map_of(&x_k, p.rows, false, D, rows, PARTS, p.pitch, rows * p.pitch, 64, ce::kRowsPerCta) ||
         !map_of(&w_k, w, false, D, V, PARTS, w_pitch, V * w_pitch, 64, p.wide_v / kPair) ||
         !map_of(&q_out, p.q, false, V, p.chunk, PARTS, p.q_pitch, p.chunk * p.q_pitch, 32, 32) ||
@@ -273,43 +272,43 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
         !map_of(&q_mn, p.q, false, V, p.chunk, PARTS, p.q_pitch, p.chunk * p.q_pitch, 64, 64) ||
         !map_of(&w_mn, w, false, D, V, PARTS, w_pitch, V * w_pitch, 64, 64) ||
         !map_of(&x_mn, p.rows, false, D, rows, PARTS, p.pitch, rows * p.pitch, 64, 64) ||
-        !map_of(&h_out, p.hidden_part, true, D, p.chunk, p.splits_hidden, p.out_pitch, p.chunk * p.out_pitch, 32, 32) ||
-        !map_of(&w_out, p.weight_part, true, D, V, p.splits_weight, p.out_pitch, V * p.out_pitch, 32, 32))
+        (several && !map_of(&w_out, p.acc, true, D, V, 1, p.out_pitch, V * p.out_pitch, 32, 32)))
         return FRAMEWISE_B200_TENSOR_MAP;
-    if (grad_hidden) {
-        ce::k_hidden_zero<X><<<(unsigned)((p.N + 7) / 8), 256, 0, stream>>>(p.N, p.counted, (int)D, grad_hidden);
-        FW_LAUNCHED();
-    }
+    if (!several) w_out = x_mn;  // not used
     ce::Params g = {};
     g.head = p.head, g.V = (int)V, g.D = (int)D, g.chunk = p.chunk;
     g.bias = p.bias, g.label = p.row_label, g.position = p.row_position, g.stats = p.stats;
-    g.grad = grad, g.grad_b = grad_b, g.grad_t = grad_t, g.T = (int)sh.T;
-    g.col_part = grad_bias ? p.col_part : nullptr, g.col_pitch = (int)up(V, 256);
-    for (int64_t row0 = 0; row0 < rows; row0 += p.chunk) {
-        g.row0 = (int)row0, g.add = row0 > 0;
-        g.wide = p.wide_v, g.splits = 1;
-        FW_DO(launch_tiles<ce::kGradients, PARTS>(x_k, w_k, q_out, g, workers, stream));
+    g.grad = grad, g.grad_b = grad_b, g.grad_t = grad_t, g.T = (int)sh.T, g.pieces = p.pieces;
+    auto wide = [&](const X* out) { return D * sizeof(X) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0; };
+    const unsigned joins = (unsigned)((workers - 1) * (ce::kRowsPerCta * kPair / 32) * (p.wide_d / 32));
+    for (int c = 0; c < p.row_chunks; ++c) {
+        g.row0 = c * p.chunk, g.add = c > 0;
+        g.wide = p.wide_v, g.col_part = grad_bias ? p.col_part + c * p.col_chunk : nullptr;
+        FW_DO(launch_tiles<ce::kGradients, kPair, PARTS>(x_k, w_k, q_out, g, workers, stream));
         g.wide = p.wide_d;
         if (grad_hidden) {
-            g.splits = p.splits_hidden;
-            FW_DO(launch_tiles<ce::kToHidden, PARTS>(q_k, w_mn, h_out, g, workers, stream));
-            ce::k_hidden_out<X><<<(unsigned)(p.chunk / 8), 256, 0, stream>>>(p.head, (int)row0, p.chunk, p.splits_hidden, p.hidden_part, (int)D,
-                                                                          (int)p.out_pitch, p.row_position, grad_hidden);
+            g.out = grad_hidden, g.out_wide = wide(grad_hidden);
+            FW_DO(launch_tiles<ce::kToHidden, kPair, PARTS>(q_k, w_mn, w_mn, g, workers, stream));
+            ce::k_join_pieces<ce::kToHidden, kPair, X><<<joins, 256, 0, stream>>>(g, workers, grad_hidden, nullptr, 0);
             FW_LAUNCHED();
         }
         if (grad_weight) {
-            g.splits = p.splits_weight;
-            FW_DO(launch_tiles<ce::kToWeight, PARTS>(q_mn, x_mn, w_out, g, workers, stream));
+            g.out = several ? nullptr : grad_weight, g.out_wide = wide(grad_weight);
+            FW_DO(launch_tiles<ce::kToWeight, kPair, PARTS>(q_mn, x_mn, w_out, g, workers, stream));
+            ce::k_join_pieces<ce::kToWeight, kPair, X><<<joins, 256, 0, stream>>>(g, workers, grad_weight, several ? p.acc : nullptr, (int)p.out_pitch);
+            FW_LAUNCHED();
         }
     }
-    if (grad_weight) {
-        ce::k_weight_out<X><<<(unsigned)((V + 7) / 8), 256, 0, stream>>>(p.head, p.splits_weight, p.weight_part, (int)V, (int)D, (int)p.out_pitch, grad_weight);
+    if (grad_weight && several) {
+        ce::k_weight_out<X><<<(unsigned)((V * p.out_pitch / 4 + 255) / 256), 256, 0, stream>>>(p.acc, (int)V, (int)D, (int)p.out_pitch, grad_weight);
         FW_LAUNCHED();
     }
     if (grad_bias) {
-        ce::k_bias_out<X><<<(unsigned)((V + 31) / 32), 256, 0, stream>>>(p.head, p.col_part, (int)up(V, 256), (int)V, grad_bias);
+        ce::k_bias_out<X, kPair><<<(unsigned)((V + 31) / 32), 32, 0, stream>>>(p.head, p.col_part, p.col_chunk, p.chunk, p.wide_v, workers, (int)V, grad_bias);
         FW_LAUNCHED();
     }
+    ce::k_finish<X><<<(unsigned)((p.N + 7) / 8), 256, 0, stream>>>(p.head, p.N, (int)V, (int)D, p.counted, grad_hidden, grad_weight, grad_bias);
+    FW_LAUNCHED();
     return FRAMEWISE_B200_OK;
 }
 
@@ -468,7 +467,8 @@ int framewise_b200_ce_forward(const framewise_b200_ce_shape* shape, const void* 
     auto go = [&](auto x, auto l) {
         using X = decltype(x);
         using L = decltype(l);
-        return ce_forward<X, L>(*shape, p, (const X*)hidden, (const X*)weight, (const X*)bias, (const L*)targets, seq_lens, loss, stream);
+        return (p.pair == 2 ? ce_forward<2, X, L> : ce_forward<1, X, L>)(*shape, p, (const X*)hidden, (const X*)weight, (const X*)bias,
+                                                                       (const L*)targets, seq_lens, loss, stream);
     };
     if (shape->dtype == FRAMEWISE_B200_F32) return shape->labels64 ? go(float(), int64_t()) : go(float(), int32_t());
     return shape->labels64 ? go(__nv_bfloat16(), int64_t()) : go(__nv_bfloat16(), int32_t());
@@ -489,11 +489,12 @@ int framewise_b200_ce_backward(const framewise_b200_ce_shape* shape, const void*
         return FRAMEWISE_B200_BAD_ARGUMENT;
     if (!p.copy_weight && (reinterpret_cast<uintptr_t>(weight) % 16 != 0 || p.D % 8 != 0)) return FRAMEWISE_B200_BAD_ARGUMENT;
     if (saved_bytes < p.saved_bytes || work_bytes < p.backward_bytes) return FRAMEWISE_B200_WORKSPACE;
-    if (shape->dtype == FRAMEWISE_B200_F32)
-        return ce_backward<float>(*shape, p, (const float*)weight, grad_loss, grad_stride_b, grad_stride_t, (float*)grad_hidden,
-                                  (float*)grad_weight, (float*)grad_bias, stream);
-    return ce_backward<__nv_bfloat16>(*shape, p, (const __nv_bfloat16*)weight, grad_loss, grad_stride_b, grad_stride_t,
-                                      (__nv_bfloat16*)grad_hidden, (__nv_bfloat16*)grad_weight, (__nv_bfloat16*)grad_bias, stream);
+    auto go = [&](auto x) {
+        using X = decltype(x);
+        return (p.pair == 2 ? ce_backward<2, X> : ce_backward<1, X>)(*shape, p, (const X*)weight, grad_loss, grad_stride_b, grad_stride_t,
+                                                                   (X*)grad_hidden, (X*)grad_weight, (X*)grad_bias, stream);
+    };
+    return shape->dtype == FRAMEWISE_B200_F32 ? go(float()) : go(__nv_bfloat16());
 }
 
 int framewise_b200_embed_forward(int64_t B, int64_t T, int64_t V, int64_t D, int32_t dtype, int32_t labels64, int64_t ignore_index,

@@ -36,14 +36,15 @@ __device__ __forceinline__ void bar_init_fence() { asm volatile("fence.mbarrier_
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// `bar` may lie in another CTA of the cluster
+// `bar` may lie in another CTA of the cluster.  (What is handed over lies in tensor memory or is written by copies: the
+// default scope, the CTA, will do; wider ones would drop the first-level cache at every wait.)
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     uint32_t done;
     asm volatile(
-        "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
         : "=r"(done)
         : "r"(bar), "r"(parity)
         : "memory");
@@ -111,8 +112,9 @@ __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t columns) {  //
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// 32 columns of this warp's 32 lanes: register j of a lane holds column j of its row
-__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
+// 32 columns of this warp's 32 lanes: value j of a lane is column j of its row.  The values are there after
+// tmem_loaded; a load may run while values of another are worked on.
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float2 (&v)[16]) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -123,7 +125,7 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
         : "r"(addr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_loaded(float (&v)[32]) {
+__device__ __forceinline__ void tmem_loaded(float2 (&v)[16]) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
     // the registers pass through, so that no use of them moves ahead of the wait
     asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -174,6 +176,28 @@ __device__ __forceinline__ void products_commit(uint32_t bar) {
     }
 }
 
+// ---- arithmetic
+
+// two values an instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
