@@ -168,6 +168,11 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
     p->q_pitch = up(p->V, 8);
     p->chunk   = (int)std::min(rows, std::max<int64_t>(256, kChunkBytes / (2 * p->parts * p->q_pitch) / 256 * 256));
     p->out_pitch = up(p->D, 4);
+    // tiles, and stages of the tiles that are shared out, are counted in 32 bits
+    const int64_t depth = std::max(p->V, (int64_t)p->chunk) / ce::kDepth + 1;
+    if (mt * ((p->V + p->wide_v - 1) / p->wide_v) >= kMost / 2 || depth * workers >= kMost / 2 ||
+        (std::max(p->V, rows) / tile + 1) * ((p->D + p->wide_d - 1) / p->wide_d) >= kMost / 2)
+        return FRAMEWISE_B200_BAD_ARGUMENT;
     p->row_chunks = (int)((rows + p->chunk - 1) / p->chunk);
 
     Parts s(saved);
