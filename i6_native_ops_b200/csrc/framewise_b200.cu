@@ -165,7 +165,7 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
     p->wide_v = 256;
     while (p->wide_v > 64 * kPair && (p->wide_v / 2 >= p->V || mt * ((p->V + p->wide_v - 1) / p->wide_v) < workers)) p->wide_v /= 2;
     p->wide_d  = (int)std::min<int64_t>(256, up(p->D, 64 * kPair));
-    p->q_pitch = up(p->V, 8);
+    p->q_pitch = up(p->V, 16);
     p->chunk   = (int)std::min(rows, std::max<int64_t>(256, kChunkBytes / (2 * p->parts * p->q_pitch) / 256 * 256));
     p->out_pitch = up(p->D, 4);
     // tiles, and stages of the tiles that are shared out, are counted in 32 bits
@@ -187,7 +187,7 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
     p->weight       = s.take<__nv_bfloat16>(p->copy_weight ? p->parts * p->V * p->pitch : 0);
     p->saved_bytes  = s.used;
     Parts f(forward);
-    p->part   = f.take<float2>((workers + mt) * 2 * tile);
+    p->part   = f.take<float2>((workers + mt) * ce::Layout<ce::kLogits, 1>::kGroups * tile);
     p->target = f.take<float>(rows);
     p->forward_bytes = f.used;
     Parts b(backward);
@@ -207,7 +207,7 @@ int launch_tiles(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& 
     FW_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
     cudaLaunchConfig_t c = {};
     c.gridDim          = dim3(workers * kPair);
-    c.blockDim         = dim3(ce::kThreads);
+    c.blockDim         = dim3(L::kThreads);
     c.dynamicSmemBytes = L::kBytes;
     c.stream           = stream;
     cudaLaunchAttribute at[1];
@@ -269,10 +269,9 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
     const int64_t w_pitch = p.copy_weight ? p.pitch : p.D, V = p.V, D = p.D;
     FW_DO(bind_device());
     const bool several = p.row_chunks > 1;
-    CUtensorMap x_k, w_k, q_out, q_k, w_mn, q_mn, x_mn, w_out;
+    CUtensorMap x_k, w_k, q_k, w_mn, q_mn, x_mn, w_out;
     if (!map_of(&x_k, p.rows, false, D, rows, PARTS, p.pitch, rows * p.pitch, 64, ce::kRowsPerCta) ||
         !map_of(&w_k, w, false, D, V, PARTS, w_pitch, V * w_pitch, 64, p.wide_v / kPair) ||
-        !map_of(&q_out, p.q, false, V, p.chunk, PARTS, p.q_pitch, p.chunk * p.q_pitch, 32, 32) ||
         !map_of(&q_k, p.q, false, V, p.chunk, PARTS, p.q_pitch, p.chunk * p.q_pitch, 64, ce::kRowsPerCta) ||
         !map_of(&q_mn, p.q, false, V, p.chunk, PARTS, p.q_pitch, p.chunk * p.q_pitch, 64, 64) ||
         !map_of(&w_mn, w, false, D, V, PARTS, w_pitch, V * w_pitch, 64, 64) ||
@@ -284,12 +283,13 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
     g.head = p.head, g.V = (int)V, g.D = (int)D, g.chunk = p.chunk;
     g.bias = p.bias, g.label = p.row_label, g.position = p.row_position, g.stats = p.stats;
     g.grad = grad, g.grad_b = grad_b, g.grad_t = grad_t, g.T = (int)sh.T, g.pieces = p.pieces;
+    g.q = p.q, g.q_pitch = (int)p.q_pitch, g.q_plane = p.chunk * p.q_pitch;
     auto wide = [&](const X* out) { return D * sizeof(X) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0; };
     const unsigned joins = (unsigned)((workers - 1) * (ce::kRowsPerCta * kPair / 32) * (p.wide_d / 32));
     for (int c = 0; c < p.row_chunks; ++c) {
         g.row0 = c * p.chunk, g.add = c > 0;
         g.wide = p.wide_v, g.col_part = grad_bias ? p.col_part + c * p.col_chunk : nullptr;
-        FW_DO(launch_tiles<ce::kGradients, kPair, PARTS>(x_k, w_k, q_out, g, workers, stream));
+        FW_DO(launch_tiles<ce::kGradients, kPair, PARTS>(x_k, w_k, x_k, g, workers, stream));
         g.wide = p.wide_d;
         if (grad_hidden) {
             g.out = grad_hidden, g.out_wide = wide(grad_hidden);

@@ -176,6 +176,13 @@ __device__ __forceinline__ void products_commit(uint32_t bar) {
     }
 }
 
+// a sector of 32 bytes at once, to be read from memory rather than kept near
+__device__ __forceinline__ void store_sector(void* to, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f, uint32_t g, uint32_t h) {
+    asm volatile("st.global.L1::no_allocate.L2::evict_first.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(a), "r"(b), "r"(c), "r"(d),
+                 "r"(e), "r"(f), "r"(g), "r"(h)
+                 : "memory");
+}
+
 // ---- arithmetic
 
 // two values an instruction
