@@ -113,7 +113,8 @@ struct CePlan {
     bool    copy_weight;
     int     wide_v, wide_d;          // columns of the tiles over V and over D
     int     row_chunks;                  // chunks of rows
-    int64_t q_pitch, out_pitch;
+    int     q_blocks;                // columns of q in blocks of 64
+    int64_t out_pitch;
     // saved
     int32_t*       head;
     int*           chunk_count;
@@ -134,7 +135,6 @@ struct CePlan {
     float*         pieces;
     float*         acc;       // the weight's gradient in 32 bits, where it takes several chunks
     float*         col_part;
-    int64_t        col_chunk; // its values per chunk
     size_t         backward_bytes;
 };
 
@@ -156,7 +156,7 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
     if (workers < 1) return FRAMEWISE_B200_CUDA_ERROR;
     p->parts       = sh->dtype == FRAMEWISE_B200_F32 ? 3 : 1;
     p->copy_weight = p->parts == 3 || sh->copy_weight != 0;
-    p->pitch       = (int)up(sh->D, 8);
+    p->pitch       = (int)up(sh->D, 64);  // rows of whole lines of 128 bytes: copies of 128 would touch two lines each
     p->chunks      = (int)((p->N + ce::kCountChunk - 1) / ce::kCountChunk);
     const int     tile   = ce::kRowsPerCta * kPair;
     const int64_t rows   = up(std::max<int64_t>(p->N, 1), 256);
@@ -165,8 +165,8 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
     p->wide_v = 256;
     while (p->wide_v > 64 * kPair && (p->wide_v / 2 >= p->V || mt * ((p->V + p->wide_v - 1) / p->wide_v) < workers)) p->wide_v /= 2;
     p->wide_d  = (int)std::min<int64_t>(256, up(p->D, 64 * kPair));
-    p->q_pitch = up(p->V, 16);
-    p->chunk   = (int)std::min(rows, std::max<int64_t>(256, kChunkBytes / (2 * p->parts * p->q_pitch) / 256 * 256));
+    p->q_blocks = (int)((p->V + 63) / 64);
+    p->chunk   = (int)std::min(rows, std::max<int64_t>(256, kChunkBytes / (128 * (int64_t)p->parts * p->q_blocks) / 256 * 256));
     p->out_pitch = up(p->D, 4);
     // tiles, and stages of the tiles that are shared out, are counted in 32 bits
     const int64_t depth = std::max(p->V, (int64_t)p->chunk) / ce::kDepth + 1;
@@ -191,11 +191,10 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
     p->target = f.take<float>(rows);
     p->forward_bytes = f.used;
     Parts b(backward);
-    p->q           = b.take<__nv_bfloat16>(p->parts * p->chunk * p->q_pitch);
+    p->q           = b.take<__nv_bfloat16>((int64_t)p->parts * p->q_blocks * 64 * p->chunk);
     p->pieces   = b.take<float>((int64_t)2 * workers * tile * ce::kWide);
     p->acc      = b.take<float>(p->row_chunks > 1 ? p->V * p->out_pitch : 0);
-    p->col_chunk = (workers + (p->V + p->wide_v - 1) / p->wide_v) * 4 * kPair * ce::kWide;
-    p->col_part = b.take<float>(sh->has_bias ? p->row_chunks * p->col_chunk : 0);
+    p->col_part = b.take<float>(sh->has_bias ? rows / 32 * up(p->V, 64) : 0);
     p->backward_bytes = b.used;
     return FRAMEWISE_B200_OK;
 }
@@ -272,8 +271,8 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
     CUtensorMap x_k, w_k, q_k, w_mn, q_mn, x_mn, w_out;
     if (!map_of(&x_k, p.rows, false, D, rows, PARTS, p.pitch, rows * p.pitch, 64, ce::kRowsPerCta) ||
         !map_of(&w_k, w, false, D, V, PARTS, w_pitch, V * w_pitch, 64, p.wide_v / kPair) ||
-        !map_of(&q_k, p.q, false, V, p.chunk, PARTS, p.q_pitch, p.chunk * p.q_pitch, 64, ce::kRowsPerCta) ||
-        !map_of(&q_mn, p.q, false, V, p.chunk, PARTS, p.q_pitch, p.chunk * p.q_pitch, 64, 64) ||
+        !map_of(&q_k, p.q, false, 64, p.chunk, PARTS * p.q_blocks, 64, (int64_t)p.chunk * 64, 64, ce::kRowsPerCta) ||
+        !map_of(&q_mn, p.q, false, 64, p.chunk, PARTS * p.q_blocks, 64, (int64_t)p.chunk * 64, 64, 64) ||
         !map_of(&w_mn, w, false, D, V, PARTS, w_pitch, V * w_pitch, 64, 64) ||
         !map_of(&x_mn, p.rows, false, D, rows, PARTS, p.pitch, rows * p.pitch, 64, 64) ||
         (several && !map_of(&w_out, p.acc, true, D, V, 1, p.out_pitch, V * p.out_pitch, 32, 32)))
@@ -283,12 +282,12 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
     g.head = p.head, g.V = (int)V, g.D = (int)D, g.chunk = p.chunk;
     g.bias = p.bias, g.label = p.row_label, g.position = p.row_position, g.stats = p.stats;
     g.grad = grad, g.grad_b = grad_b, g.grad_t = grad_t, g.T = (int)sh.T, g.pieces = p.pieces;
-    g.q = p.q, g.q_pitch = (int)p.q_pitch, g.q_plane = p.chunk * p.q_pitch;
+    g.q = p.q, g.q_blocks = p.q_blocks, g.col_part = grad_bias ? p.col_part : nullptr, g.col_pitch = (int)up(V, 64);
     auto wide = [&](const X* out) { return D * sizeof(X) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0; };
     const unsigned joins = (unsigned)((workers - 1) * (ce::kRowsPerCta * kPair / 32) * (p.wide_d / 32));
     for (int c = 0; c < p.row_chunks; ++c) {
         g.row0 = c * p.chunk, g.add = c > 0;
-        g.wide = p.wide_v, g.col_part = grad_bias ? p.col_part + c * p.col_chunk : nullptr;
+        g.wide = p.wide_v;
         FW_DO(launch_tiles<ce::kGradients, kPair, PARTS>(x_k, w_k, x_k, g, workers, stream));
         g.wide = p.wide_d;
         if (grad_hidden) {
@@ -309,7 +308,7 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
         FW_LAUNCHED();
     }
     if (grad_bias) {
-        ce::k_bias_out<X, kPair><<<(unsigned)((V + 31) / 32), 32, 0, stream>>>(p.head, p.col_part, p.col_chunk, p.chunk, p.wide_v, workers, (int)V, grad_bias);
+        ce::k_bias_out<X><<<(unsigned)((V + 31) / 32), 256, 0, stream>>>(p.head, p.col_part, (int)up(V, 64), (int)V, grad_bias);
         FW_LAUNCHED();
     }
     ce::k_finish<X><<<(unsigned)((p.N + 7) / 8), 256, 0, stream>>>(p.head, p.N, (int)V, (int)D, p.counted, grad_hidden, grad_weight, grad_bias);
