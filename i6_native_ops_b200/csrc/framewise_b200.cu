@@ -355,17 +355,20 @@ EmbedPlan embed_plan(int64_t B, int64_t T, int64_t V, int64_t D, void* work) {
 }
 
 template <typename S>
-int sort_pass(const S& src, const EmbedPlan& p, int pass, cudaStream_t stream) {
+int sort_pass(const S& src, const EmbedPlan& p, int pass, void* zero, int64_t zero_bytes, cudaStream_t stream) {
     const int digits = p.digits[pass], shift = 14 * pass, scans = (digits + embed::kScanRow - 1) / embed::kScanRow;
     static_assert(embed::kDigits == 1 << 14, "");
     const size_t bytes = (size_t)digits * 4;
-    FW_TRY(cudaFuncSetAttribute(embed::k_sort_count<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, embed::kDigits * 4));
-    FW_TRY(cudaFuncSetAttribute(embed::k_sort_place<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, embed::kDigits * 4));
-    embed::k_sort_count<S><<<p.chunks, 256, bytes, stream>>>(src, shift, digits, p.counts);
+    if (bytes > 24 * 1024) {  // with the static arrays, more than a kernel gets without asking
+        FW_TRY(cudaFuncSetAttribute(embed::k_sort_count<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, embed::kDigits * 4));
+        FW_TRY(cudaFuncSetAttribute(embed::k_sort_place<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, embed::kDigits * 4));
+    }
+    const int grid = (int)std::max<int64_t>(p.chunks, std::min<int64_t>(zero ? zero_bytes / 16384 : 0, 1024));
+    embed::k_sort_count<S><<<grid, 256, bytes, stream>>>(src, shift, digits, p.chunks, p.counts, static_cast<char*>(zero), zero_bytes);
     FW_LAUNCHED();
     embed::k_sort_scan<<<scans, embed::kScanRow, 0, stream>>>(p.counts, p.chunks, digits, p.before, p.total);
     FW_LAUNCHED();
-    embed::k_sort_place<S><<<p.chunks, 32, bytes, stream>>>(src, shift, digits, p.counts, p.before, p.total, scans, p.keys[pass], p.places[pass], p.all);
+    embed::k_sort_place<S><<<p.chunks, 256, bytes, stream>>>(src, shift, digits, p.counts, p.before, p.total, scans, p.keys[pass], p.places[pass], p.all);
     FW_LAUNCHED();
     return FRAMEWISE_B200_OK;
 }
@@ -374,7 +377,7 @@ template <typename X, typename L>
 int embed_forward(int64_t N, int64_t T, int64_t V, int64_t D, int64_t ignore, float scale, const X* table, const L* labels,
                   const int32_t* lens, X* out, cudaStream_t stream) {
     const bool wide = D % 8 == 0 && ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-    const unsigned grid = (unsigned)((N + 7) / 8);
+    const unsigned grid = (unsigned)((N + 8 * embed::kRows - 1) / (8 * embed::kRows));
     if (wide)
         embed::k_embed<X, L, true><<<grid, 256, 0, stream>>>(N, (int)T, V, (int)D, table, labels, lens, ignore, scale, out);
     else
@@ -386,8 +389,9 @@ int embed_forward(int64_t N, int64_t T, int64_t V, int64_t D, int64_t ignore, fl
 template <typename X, typename L>
 int embed_backward(const EmbedPlan& p, int64_t T, int64_t V, int64_t D, int64_t ignore, float scale, const X* grad, int64_t grad_b,
                    int64_t grad_t, const L* labels, const int32_t* lens, X* out, cudaStream_t stream) {
-    FW_DO(sort_pass(embed::FromLabels<L>{labels, lens, p.N, ignore, V, (int)T}, p, 0, stream));
-    if (p.passes == 2) FW_DO(sort_pass(embed::FromKeys{p.keys[0], p.places[0], p.all}, p, 1, stream));
+    if (reinterpret_cast<uintptr_t>(out) % 16 != 0) return FRAMEWISE_B200_BAD_ARGUMENT;
+    FW_DO(sort_pass(embed::FromLabels<L>{labels, lens, p.N, ignore, V, (int)T}, p, 0, out, V * D * (int64_t)sizeof(X), stream));
+    if (p.passes == 2) FW_DO(sort_pass(embed::FromKeys{p.keys[0], p.places[0], p.all}, p, 1, nullptr, 0, stream));
     const uint32_t *keys = p.keys[p.passes - 1], *places = p.places[p.passes - 1];
     const int     slices = (int)((D + embed::kSlice - 1) / embed::kSlice);
     const int64_t jobs   = (p.N + embed::kPiece - 1) / embed::kPiece * slices;
@@ -399,7 +403,9 @@ int embed_backward(const EmbedPlan& p, int64_t T, int64_t V, int64_t D, int64_t 
     else
         embed::k_embed_pieces<X, false><<<(unsigned)((jobs + 7) / 8), 256, 0, stream>>>(p.all, V, (int)D, slices, (int)T, grad, grad_b, grad_t, keys, places, scale, p.edge, out);
     FW_LAUNCHED();
-    embed::k_embed_rows<X><<<(unsigned)((V + 7) / 8), 256, 0, stream>>>(p.all, V, (int)D, keys, scale, p.edge, out);
+    const int64_t columns = (D + 63) / 64, runs = (p.N + embed::kPiece - 1) / embed::kPiece * columns;
+    if (runs >= (int64_t)1 << 31) return FRAMEWISE_B200_BAD_ARGUMENT;
+    embed::k_embed_runs<X><<<(unsigned)runs, 256, 0, stream>>>(p.all, V, (int)D, (int)columns, keys, scale, p.edge, out);
     FW_LAUNCHED();
     return FRAMEWISE_B200_OK;
 }

@@ -6,7 +6,7 @@
  * All pointers are DEVICE pointers unless a comment says host.  Sizes are 64-bit.  No call allocates
  * device memory, synchronises, or keeps anything of a call for the next one; calls enqueue work on the
  * given stream and may be captured into a CUDA graph.  Buffers called `saved` and `work` must be 256-byte
- * aligned; tensors need the alignment of their element type only.
+ * aligned, grad_table 16-byte; other tensors need the alignment of their element type only.
  *
  * Positions.  Activations and labels are (B,T) padded batches.  A position (b,t) counts if
  * t < seq_lens[b] (all t where seq_lens is NULL) and its label is not `ignore_index`.  Nothing is read of
