@@ -55,17 +55,40 @@ struct Parts {
     }
 };
 
-// The current device's; the device's context is current afterwards (a thread that has made no CUDA call yet, such as
-// torch's for backward passes, has none, and tensor maps need one).
-int bind_device() {
-    int dev = 0;
-    return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess ? FRAMEWISE_B200_OK : FRAMEWISE_B200_CUDA_ERROR;
-}
+constexpr int kMostDevices = 64;
+
+// The current device's number of SMs.
 int sm_count() {
+    static std::atomic<int> known[kMostDevices];
     int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (dev < kMostDevices && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    if (dev < kMostDevices) known[dev].store(n, std::memory_order_relaxed);
     return n;
+}
+
+// The current device's context is current afterwards: a thread that has made no CUDA call yet, such as torch's for
+// backward passes, has none, and tensor maps need one.
+int bind_device() {
+    static thread_local int bound = -1;
+    int dev = 0;
+    FW_TRY(cudaGetDevice(&dev));
+    if (dev != bound) FW_TRY(cudaSetDevice(dev));
+    bound = dev;
+    return FRAMEWISE_B200_OK;
+}
+
+// Dynamic shared memory past 48 KB has to be asked for, once per kernel (each has a `done` of its own) and device.
+template <typename K>
+int allow_shared(K* kernel, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    FW_TRY(cudaGetDevice(&dev));
+    const uint64_t bit = dev < kMostDevices ? (uint64_t)1 << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return FRAMEWISE_B200_OK;
+    FW_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return FRAMEWISE_B200_OK;
 }
 
 // ------------------------------------------------------------------------------------------ cross entropy
@@ -132,7 +155,8 @@ struct CePlan {
     size_t  forward_bytes;
     // backward
     __nv_bfloat16* q;
-    float*         pieces;
+    float*         pieces;        // of the two products' shared tiles
+    int64_t        piece_values;  // of each
     float*         acc;       // the weight's gradient in 32 bits, where it takes several chunks
     float*         col_part;
     size_t         backward_bytes;
@@ -192,7 +216,8 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
     p->forward_bytes = f.used;
     Parts b(backward);
     p->q           = b.take<__nv_bfloat16>((int64_t)p->parts * p->q_blocks * 64 * p->chunk);
-    p->pieces   = b.take<float>((int64_t)2 * workers * tile * ce::kWide);
+    p->piece_values = (int64_t)2 * workers * tile * ce::kWide;
+    p->pieces   = b.take<float>(2 * p->piece_values);
     p->acc      = b.take<float>(p->row_chunks > 1 ? p->V * p->out_pitch : 0);
     p->col_part = b.take<float>(sh->has_bias ? rows / 32 * up(p->V, 64) : 0);
     p->backward_bytes = b.used;
@@ -203,7 +228,8 @@ template <int KIND, int kPair, int PARTS>
 int launch_tiles(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const ce::Params& p, int workers, cudaStream_t stream) {
     using L = ce::Layout<KIND, kPair>;
     auto kernel = ce::k_ce_tiles<KIND, kPair, PARTS>;
-    FW_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+    static std::atomic<uint64_t> allowed{0};
+    FW_DO(allow_shared(kernel, L::kBytes, allowed));
     cudaLaunchConfig_t c = {};
     c.gridDim          = dim3(workers * kPair);
     c.blockDim         = dim3(L::kThreads);
@@ -226,17 +252,16 @@ int ce_forward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* hidd
     const int workers = sm_count() / kPair, tile = ce::kRowsPerCta * kPair;
     const int64_t rows = up(p.N, 256);
     FW_DO(bind_device());
-    ce::k_count_rows<<<p.chunks + (int)(up(p.V, 256) / 256), 256, 0, stream>>>(p.N, (int)sh.T, targets, lens, sh.ignore_index, p.chunks,
-                                                                            p.chunk_count, bias, p.bias, (int)p.V, p.head);
-    FW_LAUNCHED();
-    ce::k_gather_rows<X, L, PARTS><<<(unsigned)((p.N + ce::kGatherRows - 1) / ce::kGatherRows), 256, 0, stream>>>(
-        p.N, (int)sh.T, hidden, sh.hidden_stride_b, sh.hidden_stride_t, targets, lens, sh.ignore_index, p.chunk_count, p.head, (int)p.V,
-        (int)p.D, p.pitch, p.rows, rows * p.pitch, p.row_label, p.row_position, sh.train ? p.counted : nullptr, loss);
-    FW_LAUNCHED();
-    if (p.copy_weight) {
-        ce::k_split_weight<X, PARTS><<<(unsigned)((p.V + 7) / 8), 256, 0, stream>>>(weight, p.weight, p.V * p.pitch, (int)p.V, (int)p.D, p.pitch);
+    if (p.chunks > 1) {
+        ce::k_count_rows<L><<<p.chunks, 256, 0, stream>>>(p.N, (int)sh.T, targets, lens, sh.ignore_index, p.chunk_count);
         FW_LAUNCHED();
     }
+    const int64_t gather = (p.N + ce::kGatherRows - 1) / ce::kGatherRows, biases = up(p.V, 256) / 256, splits = p.copy_weight ? (p.V + 7) / 8 : 0;
+    ce::k_prepare<X, L, PARTS><<<(unsigned)(gather + biases + splits), 256, 0, stream>>>(
+        p.N, (int)sh.T, hidden, sh.hidden_stride_b, sh.hidden_stride_t, targets, lens, sh.ignore_index, p.chunk_count, p.head, (int)p.V,
+        (int)p.D, p.pitch, p.rows, rows * p.pitch, p.row_label, p.row_position, sh.train ? p.counted : nullptr, loss, bias, p.bias, weight,
+        p.weight, (int)gather, (int)biases);
+    FW_LAUNCHED();
     const void*   w       = p.copy_weight ? (const void*)p.weight : (const void*)weight;
     const int64_t w_pitch = p.copy_weight ? p.pitch : p.D;
     CUtensorMap a, b;
@@ -281,38 +306,42 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
     ce::Params g = {};
     g.head = p.head, g.V = (int)V, g.D = (int)D, g.chunk = p.chunk;
     g.bias = p.bias, g.label = p.row_label, g.position = p.row_position, g.stats = p.stats;
-    g.grad = grad, g.grad_b = grad_b, g.grad_t = grad_t, g.T = (int)sh.T, g.pieces = p.pieces;
+    g.grad = grad, g.grad_b = grad_b, g.grad_t = grad_t, g.T = (int)sh.T;
     g.q = p.q, g.q_blocks = p.q_blocks, g.col_part = grad_bias ? p.col_part : nullptr, g.col_pitch = (int)up(V, 64);
     auto wide = [&](const X* out) { return D * sizeof(X) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0; };
-    const unsigned joins = (unsigned)((workers - 1) * (ce::kRowsPerCta * kPair / 32) * (p.wide_d / 32));
+    const int joins = (workers - 1) * (ce::kRowsPerCta * kPair / 32) * (p.wide_d / 32);
     for (int c = 0; c < p.row_chunks; ++c) {
+        const bool last = c + 1 == p.row_chunks;
+        ce::After after = {};
         g.row0 = c * p.chunk, g.add = c > 0;
         g.wide = p.wide_v;
         FW_DO(launch_tiles<ce::kGradients, kPair, PARTS>(x_k, w_k, x_k, g, workers, stream));
         g.wide = p.wide_d;
         if (grad_hidden) {
-            g.out = grad_hidden, g.out_wide = wide(grad_hidden);
+            g.out = grad_hidden, g.out_wide = wide(grad_hidden), g.pieces = p.pieces;
             FW_DO(launch_tiles<ce::kToHidden, kPair, PARTS>(q_k, w_mn, w_mn, g, workers, stream));
-            ce::k_join_pieces<ce::kToHidden, kPair, X><<<joins, 256, 0, stream>>>(g, workers, grad_hidden, nullptr, 0);
-            FW_LAUNCHED();
+            after.hidden_ctas = joins;
         }
+        after.hidden = g;
         if (grad_weight) {
-            g.out = several ? nullptr : grad_weight, g.out_wide = wide(grad_weight);
+            g.out = several ? nullptr : grad_weight, g.out_wide = wide(grad_weight), g.pieces = p.pieces + p.piece_values;
             FW_DO(launch_tiles<ce::kToWeight, kPair, PARTS>(q_mn, x_mn, w_out, g, workers, stream));
-            ce::k_join_pieces<ce::kToWeight, kPair, X><<<joins, 256, 0, stream>>>(g, workers, grad_weight, several ? p.acc : nullptr, (int)p.out_pitch);
+            after.weight_ctas = joins;
+        }
+        after.weight = g;
+        if (last) after.bias_ctas = grad_bias ? (int)((V + 31) / 32) : 0, after.finish_ctas = (int)((p.N + 7) / 8);
+        after.workers = workers, after.acc = several ? p.acc : nullptr, after.acc_pitch = (int)p.out_pitch;
+        after.N = p.N, after.counted = p.counted;
+        const int64_t ctas = (int64_t)after.hidden_ctas + after.weight_ctas + after.bias_ctas + after.finish_ctas;
+        if (ctas) {
+            ce::k_after<kPair, X><<<(unsigned)ctas, 256, 0, stream>>>(after, grad_hidden, grad_weight, grad_bias);
             FW_LAUNCHED();
         }
     }
     if (grad_weight && several) {
-        ce::k_weight_out<X><<<(unsigned)((V * p.out_pitch / 4 + 255) / 256), 256, 0, stream>>>(p.acc, (int)V, (int)D, (int)p.out_pitch, grad_weight);
+        ce::k_weight_out<X><<<(unsigned)((V * p.out_pitch / 4 + 255) / 256), 256, 0, stream>>>(p.head, p.acc, (int)V, (int)D, (int)p.out_pitch, grad_weight);
         FW_LAUNCHED();
     }
-    if (grad_bias) {
-        ce::k_bias_out<X><<<(unsigned)((V + 31) / 32), 256, 0, stream>>>(p.head, p.col_part, (int)up(V, 64), (int)V, grad_bias);
-        FW_LAUNCHED();
-    }
-    ce::k_finish<X><<<(unsigned)((p.N + 7) / 8), 256, 0, stream>>>(p.head, p.N, (int)V, (int)D, p.counted, grad_hidden, grad_weight, grad_bias);
-    FW_LAUNCHED();
     return FRAMEWISE_B200_OK;
 }
 
@@ -360,8 +389,9 @@ int sort_pass(const S& src, const EmbedPlan& p, int pass, void* zero, int64_t ze
     static_assert(embed::kDigits == 1 << 14, "");
     const size_t bytes = (size_t)digits * 4;
     if (bytes > 24 * 1024) {  // with the static arrays, more than a kernel gets without asking
-        FW_TRY(cudaFuncSetAttribute(embed::k_sort_count<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, embed::kDigits * 4));
-        FW_TRY(cudaFuncSetAttribute(embed::k_sort_place<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, embed::kDigits * 4));
+        static std::atomic<uint64_t> count{0}, place{0};
+        FW_DO(allow_shared(embed::k_sort_count<S>, embed::kDigits * 4, count));
+        FW_DO(allow_shared(embed::k_sort_place<S>, embed::kDigits * 4, place));
     }
     const int grid = (int)std::max<int64_t>(p.chunks, std::min<int64_t>(zero ? zero_bytes / 16384 : 0, 1024));
     embed::k_sort_count<S><<<grid, 256, bytes, stream>>>(src, shift, digits, p.chunks, p.counts, static_cast<char*>(zero), zero_bytes);

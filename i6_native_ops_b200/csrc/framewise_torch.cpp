@@ -1,11 +1,17 @@
 // framewise_torch.cpp -- torch extension `framewise_core`: the operators of framewise training over the C ABI of
-// include/framewise_b200.h, as autograd functions.  Input errors are RuntimeErrors; work is enqueued on torch's current
+// include/framewise_b200.h, as autograd nodes.  Input errors are RuntimeErrors; work is enqueued on torch's current
 // stream of the inputs' device under a device guard; scratch comes from torch's caching allocator.
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
+#include <memory>
+#include <string>
+#include <tuple>
 #include <vector>
 
 #include "framewise_b200.h"
@@ -13,7 +19,6 @@
 namespace {
 
 using torch::Tensor;
-using torch::autograd::AutogradContext;
 using OptTensor = c10::optional<Tensor>;
 
 void check_status(int status) {
@@ -118,42 +123,37 @@ std::pair<Tensor, Tensor> ce_forward(const CeInputs& in, const Tensor& targets) 
     return {loss, saved};
 }
 
-class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> {
-  public:
-    static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const OptTensor& bias, const Tensor& targets,
-                          const OptTensor& seq_lens, int64_t ignore_index) {
-        c10::cuda::CUDAGuard guard(hidden.device());
-        at::AutoDispatchBelowADInplaceOrView below;
-        const CeInputs in = ce_inputs(hidden, weight, bias, targets, seq_lens, ignore_index, true);
-        auto [loss, saved] = ce_forward(in, targets);
-        // the caller's weight where it was taken as it is: a change of it before the backward pass is noticed
-        ctx->save_for_backward({in.weight.is_same(weight) ? weight : in.weight, saved});
-        const auto& s = in.call.shape;
-        ctx->saved_data["shape"] = std::vector<int64_t>{s.B, s.T, s.V, s.D, s.dtype, s.has_bias, s.copy_weight, targets.dim()};
-        return loss;
+// The node of the graph that a call leaves behind.  (A node of its own, rather than torch::autograd::Function: that packs
+// sizes into a dictionary, some ten microseconds a step.)
+struct LinearCrossEntropyBackward : public torch::autograd::Node {
+    torch::autograd::SavedVariable weight;  // a change of it before the backward pass is noticed
+    Tensor  saved;
+    CeCall  call;
+    bool    flat = false;
+
+    std::string name() const override { return "LinearCrossEntropyBackward"; }
+    void release_variables() override {
+        weight.reset_data();
+        saved.reset();
     }
-    static torch::autograd::variable_list backward(AutogradContext* ctx, torch::autograd::variable_list grads) {
+    torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
         TORCH_CHECK(!torch::GradMode::is_enabled(), "framewise: there are no gradients of these gradients");
-        const auto   kept   = ctx->get_saved_variables();
-        const Tensor weight = kept[0], saved = kept[1];
-        const auto   sizes  = ctx->saved_data["shape"].toIntVector();
-        c10::cuda::CUDAGuard guard(weight.device());
-        CeCall call;
-        auto& s = call.shape;
-        s.B = sizes[0], s.T = sizes[1], s.V = sizes[2], s.D = sizes[3];
-        s.dtype = (int32_t)sizes[4], s.has_bias = (int32_t)sizes[5], s.copy_weight = (int32_t)sizes[6], s.train = 1;
-        const bool flat = sizes[7] == 1;
-        check_status(framewise_b200_ce_bytes(&s, &call.saved, &call.forward, &call.backward));
+        if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
+        const Tensor w = weight.unpack();
+        TORCH_CHECK(saved.defined(), "framewise: the graph has been freed");
+        c10::cuda::CUDAGuard guard(w.device());
+        const auto& s = call.shape;
         Tensor g = plain(grads[0]);
         if (g.scalar_type() != torch::kFloat32) g = g.to(torch::kFloat32);
-        Tensor dh, dw, db, work = bytes(call.backward, weight);
-        if (ctx->needs_input_grad(0)) dh = flat ? torch::empty({s.T, s.D}, weight.options()) : torch::empty({s.B, s.T, s.D}, weight.options());
-        if (ctx->needs_input_grad(1)) dw = torch::empty({s.V, s.D}, weight.options());
-        if (s.has_bias && ctx->needs_input_grad(2)) db = torch::empty({s.V}, weight.options());
+        Tensor dh, dw, db, work = bytes(call.backward, w);
+        const auto options = w.options().requires_grad(false);
+        if (task_should_compute_output(0)) dh = flat ? torch::empty({s.T, s.D}, options) : torch::empty({s.B, s.T, s.D}, options);
+        if (task_should_compute_output(1)) dw = torch::empty({s.V, s.D}, options);
+        if (s.has_bias && task_should_compute_output(2)) db = torch::empty({s.V}, options);
         auto ptr = [](const Tensor& x) { return x.defined() ? x.data_ptr() : nullptr; };
-        check_status(framewise_b200_ce_backward(&s, weight.data_ptr(), g.data_ptr<float>(), flat ? 0 : g.stride(0), g.stride(-1), ptr(dh), ptr(dw),
+        check_status(framewise_b200_ce_backward(&s, w.data_ptr(), g.data_ptr<float>(), flat ? 0 : g.stride(0), g.stride(-1), ptr(dh), ptr(dw),
                                                 ptr(db), saved.data_ptr(), call.saved, work.data_ptr(), call.backward, stream_of()));
-        return {dh, dw, db, Tensor(), Tensor(), Tensor()};
+        return {dh, dw, db};
     }
 };
 
@@ -162,9 +162,21 @@ Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Te
     dtype_of(hidden, "hidden");
     const bool train = torch::GradMode::is_enabled() &&
                        (hidden.requires_grad() || weight.requires_grad() || (bias.has_value() && bias->requires_grad()));
-    if (train) return LinearCrossEntropy::apply(hidden, weight, bias, targets, seq_lens, ignore_index);
     c10::cuda::CUDAGuard guard(hidden.device());
-    return ce_forward(ce_inputs(hidden, weight, bias, targets, seq_lens, ignore_index, false), targets).first;
+    if (!train) return ce_forward(ce_inputs(hidden, weight, bias, targets, seq_lens, ignore_index, false), targets).first;
+    Tensor loss;
+    std::shared_ptr<LinearCrossEntropyBackward> node(new LinearCrossEntropyBackward(), torch::autograd::deleteNode);
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const CeInputs in = ce_inputs(hidden, weight, bias, targets, seq_lens, ignore_index, true);
+        std::tie(loss, node->saved) = ce_forward(in, targets);
+        node->weight = torch::autograd::SavedVariable(in.weight, false);
+        node->call   = in.call;
+        node->flat   = targets.dim() == 1;
+    }
+    node->set_next_edges(torch::autograd::collect_next_edges(hidden, weight, bias.has_value() ? *bias : Tensor()));
+    torch::autograd::set_history(loss, node);
+    return loss;
 }
 
 // ------------------------------------------------------------------------------------------ embedding
@@ -181,44 +193,53 @@ Tensor embed_forward(const Tensor& weight, const Tensor& labels, const Positions
     return out;
 }
 
-class LabelEmbedding : public torch::autograd::Function<LabelEmbedding> {
-  public:
-    static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& labels, const OptTensor& seq_lens, double scale,
-                          int64_t ignore_index) {
-        c10::cuda::CUDAGuard guard(weight.device());
-        at::AutoDispatchBelowADInplaceOrView below;
-        const Positions at(labels, seq_lens, weight);
-        Tensor out = embed_forward(weight, labels, at, scale, ignore_index);
-        ctx->save_for_backward({at.labels.is_same(labels) ? labels : at.labels, at.lens.defined() ? (at.lens.is_same(*seq_lens) ? *seq_lens : at.lens) : Tensor()});
-        ctx->saved_data["sizes"] = std::vector<int64_t>{at.B, at.T, weight.size(0), weight.size(1), ignore_index, labels.dim()};
-        ctx->saved_data["scale"] = scale;
-        return out;
+struct LabelEmbeddingBackward : public torch::autograd::Node {
+    torch::autograd::SavedVariable labels, lens;
+    bool    has_lens = false, flat = false;
+    int64_t B = 0, T = 0, V = 0, D = 0, ignore_index = 0;
+    double  scale = 1.0;
+
+    std::string name() const override { return "LabelEmbeddingBackward"; }
+    void release_variables() override {
+        labels.reset_data();
+        lens.reset_data();
     }
-    static torch::autograd::variable_list backward(AutogradContext* ctx, torch::autograd::variable_list grads) {
+    torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
         TORCH_CHECK(!torch::GradMode::is_enabled(), "framewise: there are no gradients of these gradients");
-        const auto   kept   = ctx->get_saved_variables();
-        const Tensor labels = kept[0], lens = kept[1];
-        const auto   z      = ctx->saved_data["sizes"].toIntVector();
-        c10::cuda::CUDAGuard guard(labels.device());
+        if (!grads[0].defined()) return {Tensor()};
+        const Tensor t = labels.unpack(), n = has_lens ? lens.unpack() : Tensor();
+        c10::cuda::CUDAGuard guard(t.device());
         Tensor g = plain(grads[0]);
         if (g.stride(-1) != 1) g = g.contiguous();
-        const int64_t B = z[0], T = z[1], V = z[2], D = z[3];
         Tensor dw = torch::empty({V, D}, g.options());
-        const size_t n = framewise_b200_embed_bytes(B, T, V, D);
-        Tensor work = bytes(n, g);
-        check_status(framewise_b200_embed_backward(B, T, V, D, dtype_of(g, "the gradient"), labels.scalar_type() == torch::kInt64, z[4],
-                                                   (float)ctx->saved_data["scale"].toDouble(), g.data_ptr(), z[5] == 2 ? g.stride(0) : 0, g.stride(-2),
-                                                   labels.data_ptr(), lens.defined() ? lens.data_ptr<int32_t>() : nullptr, dw.data_ptr(),
-                                                   work.data_ptr(), n, stream_of()));
-        return {dw, Tensor(), Tensor(), Tensor(), Tensor()};
+        const size_t need = framewise_b200_embed_bytes(B, T, V, D);
+        Tensor work = bytes(need, g);
+        check_status(framewise_b200_embed_backward(B, T, V, D, dtype_of(g, "the gradient"), t.scalar_type() == torch::kInt64, ignore_index,
+                                                   (float)scale, g.data_ptr(), flat ? 0 : g.stride(0), g.stride(-2), t.data_ptr(),
+                                                   n.defined() ? n.data_ptr<int32_t>() : nullptr, dw.data_ptr(), work.data_ptr(), need, stream_of()));
+        return {dw};
     }
 };
 
 Tensor label_embedding(const Tensor& labels, const Tensor& weight, double scale, const OptTensor& seq_lens, int64_t ignore_index) {
     dtype_of(weight, "weight");
-    if (torch::GradMode::is_enabled() && weight.requires_grad()) return LabelEmbedding::apply(weight, labels, seq_lens, scale, ignore_index);
     c10::cuda::CUDAGuard guard(weight.device());
-    return embed_forward(weight, labels, Positions(labels, seq_lens, weight), scale, ignore_index);
+    if (!torch::GradMode::is_enabled() || !weight.requires_grad())
+        return embed_forward(weight, labels, Positions(labels, seq_lens, weight), scale, ignore_index);
+    Tensor out;
+    std::shared_ptr<LabelEmbeddingBackward> node(new LabelEmbeddingBackward(), torch::autograd::deleteNode);
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const Positions at(labels, seq_lens, weight);
+        out = embed_forward(weight, labels, at, scale, ignore_index);
+        node->labels = torch::autograd::SavedVariable(at.labels, false);
+        if ((node->has_lens = at.lens.defined())) node->lens = torch::autograd::SavedVariable(at.lens, false);
+        node->flat = labels.dim() == 1, node->B = at.B, node->T = at.T, node->V = weight.size(0), node->D = weight.size(1);
+        node->ignore_index = ignore_index, node->scale = scale;
+    }
+    node->set_next_edges(torch::autograd::collect_next_edges(weight));
+    torch::autograd::set_history(out, node);
+    return out;
 }
 
 // ------------------------------------------------------------------------------------------ AdamW
