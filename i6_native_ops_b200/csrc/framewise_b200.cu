@@ -164,8 +164,10 @@ struct CePlan {
 
 // q of a chunk takes this much at most: some hundred rows of the largest vocabularies, all rows of small batches.
 constexpr int64_t kChunkBytes = (int64_t)768 << 20;
-// Up to this many rows a tile is one CTA's.
-constexpr int64_t kOneCta = 128;
+// Up to this many rows a tile is one CTA's, a pair's above.  Device time of loss and gradients, one CTA / pairs:
+// 200 x 10025 x 512 79 / 82 us, 600 x 5000 x 512 85 / 88, 1000 x 12001 x 512 117 / 118, 2000 x 5000 x 512 (f32) 285 / 267,
+// 4000 x 12001 x 512 246 / 235.
+constexpr int64_t kOneCta = 1024;
 
 int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void* backward, CePlan* p) {
     if (!sh) return FRAMEWISE_B200_BAD_ARGUMENT;
@@ -256,11 +258,12 @@ int ce_forward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* hidd
         ce::k_count_rows<L><<<p.chunks, 256, 0, stream>>>(p.N, (int)sh.T, targets, lens, sh.ignore_index, p.chunk_count);
         FW_LAUNCHED();
     }
-    const int64_t gather = (p.N + ce::kGatherRows - 1) / ce::kGatherRows, biases = up(p.V, 256) / 256, splits = p.copy_weight ? (p.V + 7) / 8 : 0;
+    const int     per_cta = p.N > 64 * 128 ? ce::kGatherRows : ce::kGatherFew;
+    const int64_t gather = (p.N + per_cta - 1) / per_cta, biases = up(p.V, 256) / 256, splits = p.copy_weight ? (p.V + 7) / 8 : 0;
     ce::k_prepare<X, L, PARTS><<<(unsigned)(gather + biases + splits), 256, 0, stream>>>(
         p.N, (int)sh.T, hidden, sh.hidden_stride_b, sh.hidden_stride_t, targets, lens, sh.ignore_index, p.chunk_count, p.head, (int)p.V,
         (int)p.D, p.pitch, p.rows, rows * p.pitch, p.row_label, p.row_position, sh.train ? p.counted : nullptr, loss, bias, p.bias, weight,
-        p.weight, (int)gather, (int)biases);
+        p.weight, per_cta, (int)gather, (int)biases);
     FW_LAUNCHED();
     const void*   w       = p.copy_weight ? (const void*)p.weight : (const void*)weight;
     const int64_t w_pitch = p.copy_weight ? p.pitch : p.D;
@@ -309,9 +312,7 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
     g.grad = grad, g.grad_b = grad_b, g.grad_t = grad_t, g.T = (int)sh.T;
     g.q = p.q, g.q_blocks = p.q_blocks, g.col_part = grad_bias ? p.col_part : nullptr, g.col_pitch = (int)up(V, 64);
     auto wide = [&](const X* out) { return D * sizeof(X) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0; };
-    const int joins = (workers - 1) * (ce::kRowsPerCta * kPair / 32) * (p.wide_d / 32);
     for (int c = 0; c < p.row_chunks; ++c) {
-        const bool last = c + 1 == p.row_chunks;
         ce::After after = {};
         g.row0 = c * p.chunk, g.add = c > 0;
         g.wide = p.wide_v;
@@ -320,23 +321,20 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
         if (grad_hidden) {
             g.out = grad_hidden, g.out_wide = wide(grad_hidden), g.pieces = p.pieces;
             FW_DO(launch_tiles<ce::kToHidden, kPair, PARTS>(q_k, w_mn, w_mn, g, workers, stream));
-            after.hidden_ctas = joins;
+            after.with_hidden = true;
         }
         after.hidden = g;
         if (grad_weight) {
             g.out = several ? nullptr : grad_weight, g.out_wide = wide(grad_weight), g.pieces = p.pieces + p.piece_values;
             FW_DO(launch_tiles<ce::kToWeight, kPair, PARTS>(q_mn, x_mn, w_out, g, workers, stream));
-            after.weight_ctas = joins;
+            after.with_weight = true;
         }
         after.weight = g;
-        if (last) after.bias_ctas = grad_bias ? (int)((V + 31) / 32) : 0, after.finish_ctas = (int)((p.N + 7) / 8);
+        after.last = c + 1 == p.row_chunks, after.with_bias = grad_bias != nullptr;
         after.workers = workers, after.acc = several ? p.acc : nullptr, after.acc_pitch = (int)p.out_pitch;
         after.N = p.N, after.counted = p.counted;
-        const int64_t ctas = (int64_t)after.hidden_ctas + after.weight_ctas + after.bias_ctas + after.finish_ctas;
-        if (ctas) {
-            ce::k_after<kPair, X><<<(unsigned)ctas, 256, 0, stream>>>(after, grad_hidden, grad_weight, grad_bias);
-            FW_LAUNCHED();
-        }
+        ce::k_after<kPair, X><<<sm_count() * 8, 256, 0, stream>>>(after, grad_hidden, grad_weight, grad_bias);
+        FW_LAUNCHED();
     }
     if (grad_weight && several) {
         ce::k_weight_out<X><<<(unsigned)((V * p.out_pitch / 4 + 255) / 256), 256, 0, stream>>>(p.head, p.acc, (int)V, (int)D, (int)p.out_pitch, grad_weight);
