@@ -455,7 +455,7 @@ int for_slots(const framewise_b200_tensor* tensors, int64_t count, bool codes, F
             o.m_steps = t.exp_avg_steps, o.v_steps = t.exp_avg_sq_steps, o.n = t.n, o.first = s.blocks;
             const uintptr_t all = reinterpret_cast<uintptr_t>(t.param) | reinterpret_cast<uintptr_t>(t.grad) | reinterpret_cast<uintptr_t>(t.master);
             const uintptr_t held = reinterpret_cast<uintptr_t>(t.exp_avg) | reinterpret_cast<uintptr_t>(t.exp_avg_sq);
-            o.wide = all % 16 == 0 && held % (codes ? 8 : 16) == 0;
+            o.wide = all % 32 == 0 && held % (codes ? 8 : 32) == 0 ? 2 : all % 16 == 0 && held % (codes ? 8 : 16) == 0 ? 1 : 0;
             s.blocks += (t.n + adamw::kBlock - 1) / adamw::kBlock;
         }
         if (s.count) FW_DO(launch(s));
