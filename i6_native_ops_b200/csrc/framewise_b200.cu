@@ -132,7 +132,8 @@ bool map_of(CUtensorMap* map, const void* base, bool f32, int64_t cols, int64_t 
 struct CePlan {
     int64_t N, V, D;
     int     pair;                    // CTAs per tile
-    int     parts, pitch, chunks, chunk;
+    int     parts, q_parts;          // planes of X and the weight, of q
+    int     pitch, chunks, chunk;
     bool    copy_weight;
     int     wide_v, wide_d;          // columns of the tiles over V and over D
     int     row_chunks;                  // chunks of rows
@@ -169,6 +170,11 @@ constexpr int64_t kChunkBytes = (int64_t)768 << 20;
 // 4000 x 12001 x 512 246 / 235.
 constexpr int64_t kOneCta = 1024;
 
+// bf16: up to this many rows q is held in two parts, 16 bits: with few rows the gradients' error would be up to 1.8 times
+// that of their own rounding (1.4 times with many), and a product more each costs little beside launches (200 x 10025 x
+// 512: 69 us, 62 with one part).
+constexpr int64_t kTwoParts = 256;
+
 int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void* backward, CePlan* p) {
     if (!sh) return FRAMEWISE_B200_BAD_ARGUMENT;
     const int64_t kMost = (int64_t)1 << 31;
@@ -181,6 +187,7 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
     const int kPair = p->pair, workers = sm_count() / kPair;
     if (workers < 1) return FRAMEWISE_B200_CUDA_ERROR;
     p->parts       = sh->dtype == FRAMEWISE_B200_F32 ? 3 : 1;
+    p->q_parts     = p->parts == 1 && p->N <= kTwoParts ? 2 : p->parts;
     p->copy_weight = p->parts == 3 || sh->copy_weight != 0;
     p->pitch       = (int)up(sh->D, 64);  // rows of whole lines of 128 bytes: copies of 128 would touch two lines each
     p->chunks      = (int)((p->N + ce::kCountChunk - 1) / ce::kCountChunk);
@@ -192,7 +199,7 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
     while (p->wide_v > 64 * kPair && (p->wide_v / 2 >= p->V || mt * ((p->V + p->wide_v - 1) / p->wide_v) < workers)) p->wide_v /= 2;
     p->wide_d  = (int)std::min<int64_t>(256, up(p->D, 64 * kPair));
     p->q_blocks = (int)((p->V + 63) / 64);
-    p->chunk   = (int)std::min(rows, std::max<int64_t>(256, kChunkBytes / (128 * (int64_t)p->parts * p->q_blocks) / 256 * 256));
+    p->chunk   = (int)std::min(rows, std::max<int64_t>(256, kChunkBytes / (128 * (int64_t)p->q_parts * p->q_blocks) / 256 * 256));
     p->out_pitch = up(p->D, 4);
     // tiles, and stages of the tiles that are shared out, are counted in 32 bits
     const int64_t depth = std::max(p->V, (int64_t)p->chunk) / ce::kDepth + 1;
@@ -217,7 +224,7 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
     p->target = f.take<float>(rows);
     p->forward_bytes = f.used;
     Parts b(backward);
-    p->q           = b.take<__nv_bfloat16>((int64_t)p->parts * p->q_blocks * 64 * p->chunk);
+    p->q           = b.take<__nv_bfloat16>((int64_t)p->q_parts * p->q_blocks * 64 * p->chunk);
     p->piece_values = (int64_t)2 * workers * tile * ce::kWide;
     p->pieces   = b.take<float>(2 * p->piece_values);
     p->acc      = b.take<float>(p->row_chunks > 1 ? p->V * p->out_pitch : 0);
@@ -286,7 +293,7 @@ int ce_forward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* hidd
     return FRAMEWISE_B200_OK;
 }
 
-template <int kPair, typename X>
+template <int kPair, int Q_PARTS, typename X>
 int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* weight, const float* grad, int64_t grad_b, int64_t grad_t,
                 X* grad_hidden, X* grad_weight, X* grad_bias, cudaStream_t stream) {
     constexpr int PARTS = sizeof(X) == 4 ? 3 : 1;
@@ -299,8 +306,8 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
     CUtensorMap x_k, w_k, q_k, w_mn, q_mn, x_mn, w_out;
     if (!map_of(&x_k, p.rows, false, D, rows, PARTS, p.pitch, rows * p.pitch, 64, ce::kRowsPerCta) ||
         !map_of(&w_k, w, false, D, V, PARTS, w_pitch, V * w_pitch, 64, p.wide_v / kPair) ||
-        !map_of(&q_k, p.q, false, 64, p.chunk, PARTS * p.q_blocks, 64, (int64_t)p.chunk * 64, 64, ce::kRowsPerCta) ||
-        !map_of(&q_mn, p.q, false, 64, p.chunk, PARTS * p.q_blocks, 64, (int64_t)p.chunk * 64, 64, 64) ||
+        !map_of(&q_k, p.q, false, 64, p.chunk, Q_PARTS * p.q_blocks, 64, (int64_t)p.chunk * 64, 64, ce::kRowsPerCta) ||
+        !map_of(&q_mn, p.q, false, 64, p.chunk, Q_PARTS * p.q_blocks, 64, (int64_t)p.chunk * 64, 64, 64) ||
         !map_of(&w_mn, w, false, D, V, PARTS, w_pitch, V * w_pitch, 64, 64) ||
         !map_of(&x_mn, p.rows, false, D, rows, PARTS, p.pitch, rows * p.pitch, 64, 64) ||
         (several && !map_of(&w_out, p.acc, true, D, V, 1, p.out_pitch, V * p.out_pitch, 32, 32)))
@@ -316,17 +323,17 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
         ce::After after = {};
         g.row0 = c * p.chunk, g.add = c > 0;
         g.wide = p.wide_v;
-        FW_DO(launch_tiles<ce::kGradients, kPair, PARTS>(x_k, w_k, x_k, g, workers, stream));
+        FW_DO(launch_tiles<ce::kGradients, kPair, Q_PARTS>(x_k, w_k, x_k, g, workers, stream));
         g.wide = p.wide_d;
         if (grad_hidden) {
             g.out = grad_hidden, g.out_wide = wide(grad_hidden), g.pieces = p.pieces;
-            FW_DO(launch_tiles<ce::kToHidden, kPair, PARTS>(q_k, w_mn, w_mn, g, workers, stream));
+            FW_DO(launch_tiles<ce::kToHidden, kPair, Q_PARTS>(q_k, w_mn, w_mn, g, workers, stream));
             after.with_hidden = true;
         }
         after.hidden = g;
         if (grad_weight) {
             g.out = several ? nullptr : grad_weight, g.out_wide = wide(grad_weight), g.pieces = p.pieces + p.piece_values;
-            FW_DO(launch_tiles<ce::kToWeight, kPair, PARTS>(q_mn, x_mn, w_out, g, workers, stream));
+            FW_DO(launch_tiles<ce::kToWeight, kPair, Q_PARTS>(q_mn, x_mn, w_out, g, workers, stream));
             after.with_weight = true;
         }
         after.weight = g;
@@ -347,7 +354,7 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
 
 struct EmbedPlan {
     int64_t   N;
-    int       chunks, passes, digits[2];
+    int       chunks, passes, shift, digits[2];
     uint32_t *keys[2], *places[2];
     int32_t * counts, *before, *total, *all;
     float*    edge;
@@ -363,9 +370,14 @@ EmbedPlan embed_plan(int64_t B, int64_t T, int64_t V, int64_t D, void* work) {
     EmbedPlan p;
     p.N         = B * T;
     p.chunks    = (int)((p.N + embed::kChunk - 1) / embed::kChunk);
-    p.passes    = V + 1 > embed::kDigits ? 2 : 1;  // keys up to V: labels outside the vocabulary
-    p.digits[0] = (int)std::min<int64_t>(V + 1, embed::kDigits);
-    p.digits[1] = (int)(V / embed::kDigits) + 1;
+    // Keys up to V (labels outside the vocabulary).  One pass where a chunk's counters fit shared memory and all chunks'
+    // take some ten megabytes at most; else two of half the bits.
+    int bits = 1;
+    while (V >> bits) ++bits;
+    p.passes    = V + 1 > embed::kDigits || p.chunks > embed::kOnePassChunks ? 2 : 1;
+    p.shift     = p.passes == 1 ? bits : (bits + 1) / 2;
+    p.digits[0] = p.passes == 1 ? (int)(V + 1) : 1 << p.shift;
+    p.digits[1] = (int)(V >> p.shift) + 1;
     const int digits = std::max(p.digits[0], p.passes == 2 ? p.digits[1] : 0);
     Parts b(work);
     for (int i = 0; i < 2; ++i) {
@@ -383,8 +395,8 @@ EmbedPlan embed_plan(int64_t B, int64_t T, int64_t V, int64_t D, void* work) {
 
 template <typename S>
 int sort_pass(const S& src, const EmbedPlan& p, int pass, void* zero, int64_t zero_bytes, cudaStream_t stream) {
-    const int digits = p.digits[pass], shift = 14 * pass, scans = (digits + embed::kScanRow - 1) / embed::kScanRow;
-    static_assert(embed::kDigits == 1 << 14, "");
+    const int digits = p.digits[pass], shift = p.shift * pass, scans = (digits + embed::kScanRow - 1) / embed::kScanRow;
+    const uint32_t mask = p.passes == 2 && pass == 0 ? (1u << p.shift) - 1 : 0xffffffffu;
     const size_t bytes = (size_t)digits * 4;
     if (bytes > 24 * 1024) {  // with the static arrays, more than a kernel gets without asking
         static std::atomic<uint64_t> count{0}, place{0};
@@ -392,11 +404,11 @@ int sort_pass(const S& src, const EmbedPlan& p, int pass, void* zero, int64_t ze
         FW_DO(allow_shared(embed::k_sort_place<S>, embed::kDigits * 4, place));
     }
     const int grid = (int)std::max<int64_t>(p.chunks, std::min<int64_t>(zero ? zero_bytes / 16384 : 0, 1024));
-    embed::k_sort_count<S><<<grid, 256, bytes, stream>>>(src, shift, digits, p.chunks, p.counts, static_cast<char*>(zero), zero_bytes);
+    embed::k_sort_count<S><<<grid, 256, bytes, stream>>>(src, shift, mask, digits, p.chunks, p.counts, static_cast<char*>(zero), zero_bytes);
     FW_LAUNCHED();
     embed::k_sort_scan<<<scans, embed::kScanRow, 0, stream>>>(p.counts, p.chunks, digits, p.before, p.total);
     FW_LAUNCHED();
-    embed::k_sort_place<S><<<p.chunks, 256, bytes, stream>>>(src, shift, digits, p.counts, p.before, p.total, scans, p.keys[pass], p.places[pass], p.all);
+    embed::k_sort_place<S><<<p.chunks, 256, bytes, stream>>>(src, shift, mask, digits, p.counts, p.before, p.total, scans, p.keys[pass], p.places[pass], p.all);
     FW_LAUNCHED();
     return FRAMEWISE_B200_OK;
 }
@@ -529,8 +541,10 @@ int framewise_b200_ce_backward(const framewise_b200_ce_shape* shape, const void*
     if (saved_bytes < p.saved_bytes || work_bytes < p.backward_bytes) return FRAMEWISE_B200_WORKSPACE;
     auto go = [&](auto x) {
         using X = decltype(x);
-        return (p.pair == 2 ? ce_backward<2, X> : ce_backward<1, X>)(*shape, p, (const X*)weight, grad_loss, grad_stride_b, grad_stride_t,
-                                                                   (X*)grad_hidden, (X*)grad_weight, (X*)grad_bias, stream);
+        constexpr int P = sizeof(X) == 4 ? 3 : 1, FEW = sizeof(X) == 4 ? 3 : 2;
+        static_assert(kTwoParts <= kOneCta, "");
+        auto run = p.pair == 2 ? ce_backward<2, P, X> : p.q_parts == FEW ? ce_backward<1, FEW, X> : ce_backward<1, P, X>;
+        return run(*shape, p, (const X*)weight, grad_loss, grad_stride_b, grad_stride_t, (X*)grad_hidden, (X*)grad_weight, (X*)grad_bias, stream);
     };
     return shape->dtype == FRAMEWISE_B200_F32 ? go(float()) : go(__nv_bfloat16());
 }

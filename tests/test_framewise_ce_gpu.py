@@ -258,6 +258,54 @@ def test_another_stream_and_a_graph(fw, cuda):
         assert torch.equal(loss, fw.linear_cross_entropy(h * 0.5, w, t, bias=b, seq_lens=lens, ignore_index=IGNORE))
 
 
+def test_a_training_step_in_a_graph(fw, cuda):
+    h, w, b, t, lens, g = inputs(cuda, torch.bfloat16, 4, 100, 700, 128)
+    x = [v.clone().requires_grad_() for v in (h, w, b)]
+
+    def step():
+        loss = fw.linear_cross_entropy(x[0], x[1], t, bias=x[2], seq_lens=lens, ignore_index=IGNORE)
+        return [loss.detach(), *torch.autograd.grad(loss, x, g)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    with torch.no_grad():
+        x[0].mul_(0.5)
+    graph.replay()
+    want = run(fw, h * 0.5, w, b, t, lens, g)
+    for a, c in zip(out, (want["loss"], want["hidden"], want["weight"], want["bias"])):
+        assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_one_large_row_leaves_the_others_alone(fw, cuda, dtype):
+    """Rows meet only in the sums over rows: one with values of 1e20 changes nothing of the others' losses and gradients."""
+    h, w, b, t, lens, g = inputs(cuda, dtype, 2, 90, 300, 80, skip=0.0, short=False)
+    want = run(fw, h, w, b, t, lens, g)
+    h2 = h.clone()
+    h2[1, 40] *= 1e20
+    got = run(fw, h2, w, b, t, lens, g)
+    keep = torch.ones_like(t, dtype=torch.bool)
+    keep[1, 40] = False
+    assert torch.equal(got["loss"][keep], want["loss"][keep]) and torch.equal(got["hidden"][keep], want["hidden"][keep])
+
+
+def test_large_offsets(fw, cuda):
+    """Activations whose positions lie past 2^31 elements: rows of a buffer of 5 GB."""
+    big = torch.empty(2, 5, 2**28, dtype=torch.bfloat16, device=cuda)[..., :64]
+    h, w, b, t, lens, g = inputs(cuda, torch.bfloat16, 2, 5, 100, 64, short=False, skip=0.0)
+    big.copy_(h)
+    assert big.stride(0) * 1 + big.stride(1) * 4 > 2**31
+    want, got = run(fw, h, w, b, t, None, g), run(fw, big, w, b, t, None, g)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+
+
 def test_refusals(fw, cuda):
     h, w, b, t, lens, g = inputs(cuda, torch.float32, 2, 5, 11, 8)
     f = fw.linear_cross_entropy

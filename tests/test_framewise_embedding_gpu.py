@@ -75,6 +75,11 @@ def test_label_counts_around_the_digits_of_the_sort(fw, cuda, V):
     check(fw, t, w, lens, scale, g)
 
 
+@pytest.mark.parametrize("V", [1, 3, 121, 12001, 16383])
+def test_more_positions_than_one_pass_sorts(fw, cuda, V):
+    check(fw, *inputs(cuda, torch.float32, 600, 1000, V, 4, seed=V))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("few", [1, 2, 5])
 def test_labels_that_many_positions_share(fw, cuda, dtype, few):
