@@ -416,7 +416,7 @@ int sort_pass(const S& src, const EmbedPlan& p, int pass, void* zero, int64_t ze
 template <typename X, typename L>
 int embed_forward(int64_t N, int64_t T, int64_t V, int64_t D, int64_t ignore, float scale, const X* table, const L* labels,
                   const int32_t* lens, X* out, cudaStream_t stream) {
-    const bool wide = D % 8 == 0 && ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+    const bool wide = D % 8 == 0 && (reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(out)) % (8 * sizeof(X)) == 0;
     const unsigned grid = (unsigned)((N + 8 * embed::kRows - 1) / (8 * embed::kRows));
     if (wide)
         embed::k_embed<X, L, true><<<grid, 256, 0, stream>>>(N, (int)T, V, (int)D, table, labels, lens, ignore, scale, out);
@@ -443,9 +443,8 @@ int embed_backward(const EmbedPlan& p, int64_t T, int64_t V, int64_t D, int64_t 
     else
         embed::k_embed_pieces<X, false><<<(unsigned)((jobs + 7) / 8), 256, 0, stream>>>(p.all, V, (int)D, slices, (int)T, grad, grad_b, grad_t, keys, places, scale, p.edge, out);
     FW_LAUNCHED();
-    const int64_t columns = (D + 63) / 64, runs = (p.N + embed::kPiece - 1) / embed::kPiece * columns;
-    if (runs >= (int64_t)1 << 31) return FRAMEWISE_B200_BAD_ARGUMENT;
-    embed::k_embed_runs<X><<<(unsigned)runs, 256, 0, stream>>>(p.all, V, (int)D, (int)columns, keys, scale, p.edge, out);
+    const int64_t pieces = (p.N + embed::kPiece - 1) / embed::kPiece;
+    embed::k_embed_runs<X><<<(unsigned)((pieces + 7) / 8), 256, 0, stream>>>(p.all, V, (int)D, keys, scale, p.edge, out);
     FW_LAUNCHED();
     return FRAMEWISE_B200_OK;
 }
