@@ -220,7 +220,7 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
     p->weight       = s.take<__nv_bfloat16>(p->copy_weight ? p->parts * p->V * p->pitch : 0);
     p->saved_bytes  = s.used;
     Parts f(forward);
-    p->part   = f.take<float2>((workers + mt) * ce::Layout<ce::kLogits, 1>::kGroups * tile);
+    p->part   = f.take<float2>((workers + mt) * ce::Layout<ce::kLogits, 1, 1>::kGroups * tile);
     p->target = f.take<float>(rows);
     p->forward_bytes = f.used;
     Parts b(backward);
@@ -235,7 +235,7 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
 
 template <int KIND, int kPair, int PARTS>
 int launch_tiles(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const ce::Params& p, int workers, cudaStream_t stream) {
-    using L = ce::Layout<KIND, kPair>;
+    using L = ce::Layout<KIND, kPair, PARTS>;
     auto kernel = ce::k_ce_tiles<KIND, kPair, PARTS>;
     static std::atomic<uint64_t> allowed{0};
     FW_DO(allow_shared(kernel, L::kBytes, allowed));
@@ -303,9 +303,10 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
     const int64_t w_pitch = p.copy_weight ? p.pitch : p.D, V = p.V, D = p.D;
     FW_DO(bind_device());
     const bool several = p.row_chunks > 1;
-    CUtensorMap x_k, w_k, q_k, w_mn, q_mn, x_mn, w_out;
+    CUtensorMap x_k, w_k, q_out, q_k, w_mn, q_mn, x_mn, w_out;
     if (!map_of(&x_k, p.rows, false, D, rows, PARTS, p.pitch, rows * p.pitch, 64, ce::kRowsPerCta) ||
         !map_of(&w_k, w, false, D, V, PARTS, w_pitch, V * w_pitch, 64, p.wide_v / kPair) ||
+        !map_of(&q_out, p.q, false, 64, p.chunk, Q_PARTS * p.q_blocks, 64, (int64_t)p.chunk * 64, 32, 32) ||
         !map_of(&q_k, p.q, false, 64, p.chunk, Q_PARTS * p.q_blocks, 64, (int64_t)p.chunk * 64, 64, ce::kRowsPerCta) ||
         !map_of(&q_mn, p.q, false, 64, p.chunk, Q_PARTS * p.q_blocks, 64, (int64_t)p.chunk * 64, 64, 64) ||
         !map_of(&w_mn, w, false, D, V, PARTS, w_pitch, V * w_pitch, 64, 64) ||
@@ -323,7 +324,7 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
         ce::After after = {};
         g.row0 = c * p.chunk, g.add = c > 0;
         g.wide = p.wide_v;
-        FW_DO(launch_tiles<ce::kGradients, kPair, Q_PARTS>(x_k, w_k, x_k, g, workers, stream));
+        FW_DO(launch_tiles<ce::kGradients, kPair, Q_PARTS>(x_k, w_k, q_out, g, workers, stream));
         g.wide = p.wide_d;
         if (grad_hidden) {
             g.out = grad_hidden, g.out_wide = wide(grad_hidden), g.pieces = p.pieces;
