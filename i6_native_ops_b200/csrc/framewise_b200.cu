@@ -319,7 +319,10 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
     g.bias = p.bias, g.label = p.row_label, g.position = p.row_position, g.stats = p.stats;
     g.grad = grad, g.grad_b = grad_b, g.grad_t = grad_t, g.T = (int)sh.T;
     g.q = p.q, g.q_blocks = p.q_blocks, g.col_part = grad_bias ? p.col_part : nullptr, g.col_pitch = (int)up(V, 64);
-    auto wide = [&](const X* out) { return D * sizeof(X) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0; };
+    auto grain = [&](const X* out) {  // at least a value's size
+        const uintptr_t odd = (uintptr_t)(D * sizeof(X)) | reinterpret_cast<uintptr_t>(out) | 16;
+        return (int)(odd & (~odd + 1));
+    };
     for (int c = 0; c < p.row_chunks; ++c) {
         ce::After after = {};
         g.row0 = c * p.chunk, g.add = c > 0;
@@ -327,13 +330,13 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
         FW_DO(launch_tiles<ce::kGradients, kPair, Q_PARTS>(x_k, w_k, q_out, g, workers, stream));
         g.wide = p.wide_d;
         if (grad_hidden) {
-            g.out = grad_hidden, g.out_wide = wide(grad_hidden), g.pieces = p.pieces;
+            g.out = grad_hidden, g.out_grain = grain(grad_hidden), g.pieces = p.pieces;
             FW_DO(launch_tiles<ce::kToHidden, kPair, Q_PARTS>(q_k, w_mn, w_mn, g, workers, stream));
             after.with_hidden = true;
         }
         after.hidden = g;
         if (grad_weight) {
-            g.out = several ? nullptr : grad_weight, g.out_wide = wide(grad_weight), g.pieces = p.pieces + p.piece_values;
+            g.out = several ? nullptr : grad_weight, g.out_grain = grain(grad_weight), g.pieces = p.pieces + p.piece_values;
             FW_DO(launch_tiles<ce::kToWeight, kPair, Q_PARTS>(q_mn, x_mn, w_out, g, workers, stream));
             after.with_weight = true;
         }
