@@ -160,6 +160,7 @@ struct CePlan {
     int64_t        piece_values;  // of each
     float*         acc;       // the weight's gradient in 32 bits, where it takes several chunks
     float*         col_part;
+    float*         bias_acc;  // the bias's, likewise
     size_t         backward_bytes;
 };
 
@@ -228,7 +229,8 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
     p->piece_values = (int64_t)2 * workers * tile * ce::kWide;
     p->pieces   = b.take<float>(2 * p->piece_values);
     p->acc      = b.take<float>(p->row_chunks > 1 ? p->V * p->out_pitch : 0);
-    p->col_part = b.take<float>(sh->has_bias ? rows / 32 * up(p->V, 64) : 0);
+    p->col_part = b.take<float>(sh->has_bias ? (int64_t)p->chunk / 32 * up(p->V, 64) : 0);
+    p->bias_acc = b.take<float>(sh->has_bias ? p->V : 0);
     p->backward_bytes = b.used;
     return FRAMEWISE_B200_OK;
 }
@@ -342,7 +344,7 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
         }
         after.weight = g;
         after.last = c + 1 == p.row_chunks, after.with_bias = grad_bias != nullptr;
-        after.workers = workers, after.acc = several ? p.acc : nullptr, after.acc_pitch = (int)p.out_pitch;
+        after.workers = workers, after.acc = several ? p.acc : nullptr, after.acc_pitch = (int)p.out_pitch, after.bias_acc = p.bias_acc;
         after.N = p.N, after.counted = p.counted;
         ce::k_after<kPair, X><<<sm_count() * 8, 256, 0, stream>>>(after, grad_hidden, grad_weight, grad_bias);
         FW_LAUNCHED();
