@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
+#include <algorithm>
 #include <memory>
 #include <string>
 #include <tuple>
@@ -75,6 +76,12 @@ struct Positions {
 struct CeCall {
     framewise_b200_ce_shape shape = {};
     size_t saved = 0, forward = 0, backward = 0;
+
+    // One buffer: what is kept, then scratch, the backward pass's as well where that is small (an allocation less there).
+    static constexpr size_t kSmall = (size_t)32 << 20;
+    size_t work_at() const { return (saved + 255) / 256 * 256; }
+    bool   work_kept() const { return shape.train && backward <= kSmall; }
+    size_t buffer() const { return work_at() + (work_kept() ? std::max(forward, backward) : forward); }
 };
 
 struct CeInputs {
@@ -116,10 +123,11 @@ CeInputs ce_inputs(const Tensor& hidden_in, const Tensor& weight_in, const OptTe
 // (loss, what the backward pass needs)
 std::pair<Tensor, Tensor> ce_forward(const CeInputs& in, const Tensor& targets) {
     Tensor loss  = torch::empty(targets.sizes(), in.hidden.options().dtype(torch::kFloat32));
-    Tensor saved = bytes(in.call.saved, in.hidden), work = bytes(in.call.forward, in.hidden);
+    Tensor saved = bytes(in.call.buffer(), in.hidden);
+    char* const kept = static_cast<char*>(saved.data_ptr());
     check_status(framewise_b200_ce_forward(&in.call.shape, in.hidden.data_ptr(), in.weight.data_ptr(),
                                            in.bias.defined() ? in.bias.data_ptr() : nullptr, in.at.labels.data_ptr(), in.at.lens_ptr(),
-                                           loss.data_ptr<float>(), saved.data_ptr(), in.call.saved, work.data_ptr(), in.call.forward, stream_of()));
+                                           loss.data_ptr<float>(), kept, in.call.saved, kept + in.call.work_at(), in.call.forward, stream_of()));
     return {loss, saved};
 }
 
@@ -145,14 +153,17 @@ struct LinearCrossEntropyBackward : public torch::autograd::Node {
         const auto& s = call.shape;
         Tensor g = plain(grads[0]);
         if (g.scalar_type() != torch::kFloat32) g = g.to(torch::kFloat32);
-        Tensor dh, dw, db, work = bytes(call.backward, w);
+        Tensor dh, dw, db, work;
+        if (!call.work_kept()) work = bytes(call.backward, w);
+        char* const kept = static_cast<char*>(saved.data_ptr());
         const auto options = w.options().requires_grad(false);
         if (task_should_compute_output(0)) dh = flat ? torch::empty({s.T, s.D}, options) : torch::empty({s.B, s.T, s.D}, options);
         if (task_should_compute_output(1)) dw = torch::empty({s.V, s.D}, options);
         if (s.has_bias && task_should_compute_output(2)) db = torch::empty({s.V}, options);
         auto ptr = [](const Tensor& x) { return x.defined() ? x.data_ptr() : nullptr; };
         check_status(framewise_b200_ce_backward(&s, w.data_ptr(), g.data_ptr<float>(), flat ? 0 : g.stride(0), g.stride(-1), ptr(dh), ptr(dw),
-                                                ptr(db), saved.data_ptr(), call.saved, work.data_ptr(), call.backward, stream_of()));
+                                                ptr(db), kept, call.saved, call.work_kept() ? kept + call.work_at() : work.data_ptr(), call.backward,
+                                                stream_of()));
         return {dh, dw, db};
     }
 };
