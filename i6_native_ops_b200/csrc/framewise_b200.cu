@@ -412,7 +412,7 @@ int sort_pass(const S& src, const EmbedPlan& p, int pass, void* zero, int64_t ze
     const int grid = (int)std::max<int64_t>(p.chunks, std::min<int64_t>(zero ? zero_bytes / 16384 : 0, 1024));
     embed::k_sort_count<S><<<grid, 256, bytes, stream>>>(src, shift, mask, digits, p.chunks, p.counts, static_cast<char*>(zero), zero_bytes);
     FW_LAUNCHED();
-    embed::k_sort_scan<<<scans, embed::kScanRow, 0, stream>>>(p.counts, p.chunks, digits, p.before, p.total);
+    embed::k_sort_scan<<<scans, 256, 0, stream>>>(p.counts, p.chunks, digits, p.before, p.total);
     FW_LAUNCHED();
     embed::k_sort_place<S><<<p.chunks, 256, bytes, stream>>>(src, shift, mask, digits, p.counts, p.before, p.total, scans, p.keys[pass], p.places[pass], p.all);
     FW_LAUNCHED();
