@@ -171,6 +171,9 @@ constexpr int64_t kChunkBytes = (int64_t)768 << 20;
 // 4000 x 12001 x 512 246 / 235.
 constexpr int64_t kOneCta = 1024;
 
+// Up to this many positions each CTA of k_prepare counts those before its own by itself; above, a launch before does (us
+// by itself / with that launch: 4000 positions 7.4 / 11.5, 8000 11.7 / 12.5, 16000 16.8 / 12.5).
+constexpr int64_t kCountHere = 4096;
 // bf16: up to this many rows q is held in two parts, 16 bits: with few rows the gradients' error would be up to 1.8 times
 // that of their own rounding (1.4 times with many), and a product more each costs little beside launches (200 x 10025 x
 // 512: 69 us, 62 with one part).
@@ -263,14 +266,15 @@ int ce_forward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* hidd
     const int workers = sm_count() / kPair, tile = ce::kRowsPerCta * kPair;
     const int64_t rows = up(p.N, 256);
     FW_DO(bind_device());
-    if (p.chunks > 1) {
+    const bool count = p.N > kCountHere;
+    if (count) {
         ce::k_count_rows<L><<<p.chunks, 256, 0, stream>>>(p.N, (int)sh.T, targets, lens, sh.ignore_index, p.chunk_count);
         FW_LAUNCHED();
     }
     const int     per_cta = p.N > 64 * 128 ? ce::kGatherRows : ce::kGatherFew;
     const int64_t gather = (p.N + per_cta - 1) / per_cta, biases = up(p.V, 256) / 256, splits = p.copy_weight ? (p.V + 7) / 8 : 0;
     ce::k_prepare<X, L, PARTS><<<(unsigned)(gather + biases + splits), 256, 0, stream>>>(
-        p.N, (int)sh.T, hidden, sh.hidden_stride_b, sh.hidden_stride_t, targets, lens, sh.ignore_index, p.chunk_count, p.head, (int)p.V,
+        p.N, (int)sh.T, hidden, sh.hidden_stride_b, sh.hidden_stride_t, targets, lens, sh.ignore_index, count ? p.chunk_count : nullptr, p.head, (int)p.V,
         (int)p.D, p.pitch, p.rows, rows * p.pitch, p.row_label, p.row_position, sh.train ? p.counted : nullptr, loss, bias, p.bias, weight,
         p.weight, per_cta, (int)gather, (int)biases);
     FW_LAUNCHED();
