@@ -268,6 +268,12 @@ void check_steps(const Tensor& x, const Tensor& codes, const char* name) {
                 " must be contiguous float32, one per 256 values in a row");
 }
 
+// Autograd learns that a tensor has been written: a graph that needs its former values refuses to go on.
+void written(const Tensors& list) {
+    for (const Tensor& x : list)
+        if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+}
+
 // exp_avg_steps, exp_avg_sq_steps: empty (states of 32 bits), or one per parameter.  master: empty, or one per parameter.
 void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& master, const Tensors& exp_avg, const Tensors& exp_avg_sq,
                 const Tensors& exp_avg_steps, const Tensors& exp_avg_sq_steps, double lr, double beta1, double beta2, double eps,
@@ -312,6 +318,7 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& mast
         }
     }
     check_status(framewise_b200_adamw(list.data(), (int64_t)n, dtype, eight ? 8 : 32, lr, beta1, beta2, eps, weight_decay, step, stream_of()));
+    for (const Tensors* const x : {&params, &master, &exp_avg, &exp_avg_sq, &exp_avg_steps, &exp_avg_sq_steps}) written(*x);
 }
 
 // What 8-bit states stand for: (first moments, second moments), f32.

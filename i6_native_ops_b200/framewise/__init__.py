@@ -121,7 +121,8 @@ def adamw_step(
     eps: float = 1e-8,
     weight_decay: float = 0.01,
 ) -> None:
-    """One step of AdamW over a list of parameters, in place, in as few launches as there are 48 tensors.
+    """One step of AdamW over a list of parameters, in place, in as few launches as there are 48 tensors.  As after any
+    operation in place, graphs that saved a parameter before refuse their backward pass.
 
     :param params: contiguous CUDA tensors, all float32 or all bfloat16
     :param exp_avg, exp_avg_sq: per parameter a float32 tensor of its shape, or (8-bit states) ``(codes, steps)``: int8

@@ -1,0 +1,66 @@
+"""What autograd has to know of the framewise operators: that the optimizer changed a tensor, what a graph keeps."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def fw():
+    import i6_native_ops_b200.framewise as m
+
+    return m
+
+
+def layer(cuda, dtype, B=3, T=40, V=90, D=64, seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    kw = dict(device=cuda, generator=gen)
+    h = torch.randn(B, T, D, **kw).to(dtype).requires_grad_()
+    w = (torch.randn(V, D, **kw) / D**0.5).to(dtype)
+    t = torch.randint(0, V, (B, T), **kw)
+    return h, w, t
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_step_between_a_loss_and_its_gradients_is_an_error(fw, cuda, dtype, bits):
+    """The gradients are formed from the weight that the loss was formed from: changed by the optimizer, it is refused, as
+    one changed by torch is."""
+    h, w, t = layer(cuda, dtype)
+    w = torch.nn.Parameter(w)
+    optimizer = fw.AdamW([w], lr=1e-2, betas=(0.9, 0.98), state_bits=bits)
+    loss = fw.linear_cross_entropy(h, w, t).sum()
+    square = (w * w).sum()  # torch's own product saves the weight as well
+    w.grad = torch.ones_like(w)
+    optimizer.step()
+    for x in (loss, square):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            x.backward()
+    # and after the step all is as usual
+    fw.linear_cross_entropy(h, w, t).sum().backward()
+    assert bool(h.grad.isfinite().all())
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_step_moves_the_versions_of_what_it_writes(fw, cuda, bits):
+    p = [torch.ones(300, device=cuda, dtype=torch.bfloat16), torch.ones(7, 5, device=cuda, dtype=torch.bfloat16)]
+    g = [torch.ones_like(x) for x in p]
+    master = [x.float() for x in p]
+    if bits == 8:
+        m, v = ([(torch.zeros(x.shape, device=cuda, dtype=kind), torch.zeros(-(-x.numel() // 256), device=cuda)) for x in p]
+                for kind in (torch.int8, torch.uint8))
+        states = [y for x in m + v for y in x]
+    else:
+        m, v = ([torch.zeros(x.shape, device=cuda) for x in p] for _ in range(2))
+        states = m + v
+    written, read = p + master + states, g
+    before = [x._version for x in written], [x._version for x in read]
+    fw.adamw_step(p, g, m, v, step=1, master=master, betas=(0.9, 0.98))
+    assert all(x._version > n for x, n in zip(written, before[0]))
+    assert all(x._version == n for x, n in zip(read, before[1]))
+    # tensors without versions are written all the same
+    with torch.inference_mode():
+        q = torch.ones(300, device=cuda)
+        m, v = torch.zeros(300, device=cuda), torch.zeros(300, device=cuda)
+    fw.adamw_step([q], [torch.ones(300, device=cuda)], [m], [v], step=1)
+    assert bool((q < 1).all())
