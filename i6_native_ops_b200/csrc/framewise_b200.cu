@@ -611,13 +611,19 @@ int framewise_b200_adamw(const framewise_b200_tensor* tensors, int64_t count, in
             return FRAMEWISE_B200_BAD_ARGUMENT;
     }
     const adamw::Rates r = {(float)beta1, (float)(1 - beta1), (float)beta2, (float)(1 - beta2), (float)(1 - lr * weight_decay),
-                            (float)(lr / (1 - std::pow(beta1, (double)step))), (float)(1 / std::sqrt(1 - std::pow(beta2, (double)step))), (float)eps};
+                            (float)(lr / (1 - std::pow(beta1, (double)step))), (float)(1 / std::sqrt(1 - std::pow(beta2, (double)step))), (float)eps,
+                            (uint32_t)step * adamw::kTurn1, (uint32_t)step * adamw::kTurn2};
+    const bool dither = state_bits == 8 && std::max(beta1, beta2) > adamw::kNearest;
     return for_slots(tensors, count, state_bits == 8, [&](const adamw::Slots& s) -> int {
         const unsigned grid = adamw_grid(s.blocks);
-        if (dtype == FRAMEWISE_B200_F32 && state_bits == 32) adamw::k_adamw<float, 32><<<grid, 256, 0, stream>>>(s, r);
-        else if (dtype == FRAMEWISE_B200_F32) adamw::k_adamw<float, 8><<<grid, 256, 0, stream>>>(s, r);
-        else if (state_bits == 32) adamw::k_adamw<__nv_bfloat16, 32><<<grid, 256, 0, stream>>>(s, r);
-        else adamw::k_adamw<__nv_bfloat16, 8><<<grid, 256, 0, stream>>>(s, r);
+        auto go = [&](auto x) {
+            using X = decltype(x);
+            if (state_bits == 32) adamw::k_adamw<X, 32, false><<<grid, 256, 0, stream>>>(s, r);
+            else if (dither) adamw::k_adamw<X, 8, true><<<grid, 256, 0, stream>>>(s, r);
+            else adamw::k_adamw<X, 8, false><<<grid, 256, 0, stream>>>(s, r);
+        };
+        if (dtype == FRAMEWISE_B200_F32) go(float());
+        else go(__nv_bfloat16());
         FW_LAUNCHED();
         return FRAMEWISE_B200_OK;
     });

@@ -127,8 +127,10 @@ def adamw_step(
     :param params: contiguous CUDA tensors, all float32 or all bfloat16
     :param exp_avg, exp_avg_sq: per parameter a float32 tensor of its shape, or (8-bit states) ``(codes, steps)``: int8
         (first moment) or uint8 (root of the second) codes in the parameter's shape and a float32 step for each 256
-        values in a row, which stand for ``code * |code| * step``
-    :param step: of this call, counted from 1
+        values in a row, which stand for ``code * |code| * step``.  They are rounded to the nearest codes where both
+        betas are 0.98 at most, else up or down by offsets that change with ``step``, so that moments which shrink slower
+        than codes are apart do so on average (roots of the second moment are then within about ``1 / sqrt(2 code)``)
+    :param step: of this call, counted from 1; has to grow from step to step
     :param master: float32 copies that are updated in place of the parameters, which then get their rounded values"""
     m, m_steps = _split(exp_avg)
     v, v_steps = _split(exp_avg_sq)
@@ -147,7 +149,9 @@ class AdamW(torch.optim.Optimizer):
     """AdamW whose step takes all parameters of a group in one launch or a few.
 
     ``state_bits=8`` holds the moments in 8 bits (2 bytes a parameter instead of 8): per 256 values a step and quadratic
-    codes, 16 thousand to one (first moment) and 65 thousand to one (root of the second) between largest and smallest.
+    codes, 16 thousand to one (first moment) and 65 thousand to one (root of the second) between largest and smallest
+    (:func:`adamw_step` says how they are rounded: on average right at any betas, a root of the second moment that is a
+    hundredth of its block's largest to some 15 %).
     bfloat16 parameters get a float32 copy that the steps accumulate in (``state["master"]``).  Parameters without a
     gradient are passed over.  The learning rate may be changed between steps, as for any torch optimizer."""
 

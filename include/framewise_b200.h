@@ -115,7 +115,11 @@ typedef struct {
  * 8-bit states: a code c and its block's step k stand for c |c| k; the codes of the first moment are -127..127,
  * those of the ROOT of the second 0..255, at least 1 where the root is not zero.  A block's step is its largest
  * magnitude / 127^2 (255^2), zero where that is below 2^-120; a block with an infinity or a NaN stands for it
- * throughout. */
+ * throughout.  Where both betas are 0.98 at most, the root of |value| / k is rounded to the nearest whole number; where one
+ * is above, an offset is added first, for such codes would hardly ever follow a moment that shrinks.  For value i of its
+ * tensor at step s: ((i a + s b) mod 2^32 >> 9) 2^-23 - 1/2 with a, b = 2447445413, 3242174889 for the first moment and
+ * 3242174889, 2447445413 for the second.  The sum, rounded to f32, is rounded to the nearest whole number and limited
+ * to 0..127 (255). */
 int framewise_b200_adamw(const framewise_b200_tensor* tensors, int64_t count, int32_t dtype,
                          int32_t state_bits, double lr, double beta1, double beta2, double eps,
                          double weight_decay, int64_t step, framewise_b200_stream_t stream);
