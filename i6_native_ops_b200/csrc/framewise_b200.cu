@@ -12,6 +12,7 @@
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 namespace {
 
@@ -486,6 +487,38 @@ int for_slots(const framewise_b200_tensor* tensors, int64_t count, bool codes, F
 
 unsigned adamw_grid(int64_t blocks) { return (unsigned)std::min<int64_t>((blocks + 7) / 8, (int64_t)sm_count() * 64); }
 
+int adamw_step(const framewise_b200_tensor* tensors, int64_t count, int32_t dtype, int32_t state_bits, double lr, double beta1,
+                         double beta2, double eps, double weight_decay, int64_t step, bool follow, cudaStream_t stream) {
+    if ((count > 0 && !tensors) || count < 0 || step < 1 || (state_bits != 8 && state_bits != 32) ||
+        (dtype != FRAMEWISE_B200_F32 && dtype != FRAMEWISE_B200_BF16))
+        return FRAMEWISE_B200_BAD_ARGUMENT;
+    for (int64_t i = 0; i < count; ++i) {
+        const framewise_b200_tensor& t = tensors[i];
+        if (t.n < 0 || (t.n > 0 && (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq ||
+                                    (state_bits == 8 && (!t.exp_avg_steps || !t.exp_avg_sq_steps)))))
+            return FRAMEWISE_B200_BAD_ARGUMENT;
+    }
+    const adamw::Rates r = {(float)beta1, (float)(1 - beta1), (float)beta2, (float)(1 - beta2), (float)(1 - lr * weight_decay),
+                            (float)(lr / (1 - std::pow(beta1, (double)step))), (float)(1 / std::sqrt(1 - std::pow(beta2, (double)step))), (float)eps,
+                            (uint32_t)step * adamw::kTurn1, (uint32_t)step * adamw::kTurn2};
+    const bool dither = state_bits == 8 && std::max(beta1, beta2) > adamw::kNearest;
+    return for_slots(tensors, count, state_bits == 8, [&](const adamw::Slots& s) -> int {
+        const unsigned grid = adamw_grid(s.blocks);
+        auto go = [&](auto x, auto f) {
+            using X = decltype(x);
+            constexpr bool kFollow = decltype(f)::value;
+            if (state_bits == 32) adamw::k_adamw<X, 32, false, kFollow><<<grid, 256, 0, stream>>>(s, r);
+            else if (dither) adamw::k_adamw<X, 8, true, kFollow><<<grid, 256, 0, stream>>>(s, r);
+            else adamw::k_adamw<X, 8, false, kFollow><<<grid, 256, 0, stream>>>(s, r);
+        };
+        if (dtype == FRAMEWISE_B200_F32) go(float(), std::false_type());  // a copy of one would be the same
+        else if (follow) go(__nv_bfloat16(), std::true_type());
+        else go(__nv_bfloat16(), std::false_type());
+        FW_LAUNCHED();
+        return FRAMEWISE_B200_OK;
+    });
+}
+
 }  // namespace
 
 extern "C" {
@@ -601,32 +634,13 @@ int framewise_b200_embed_backward(int64_t B, int64_t T, int64_t V, int64_t D, in
 
 int framewise_b200_adamw(const framewise_b200_tensor* tensors, int64_t count, int32_t dtype, int32_t state_bits, double lr, double beta1,
                          double beta2, double eps, double weight_decay, int64_t step, framewise_b200_stream_t stream) {
-    if ((count > 0 && !tensors) || count < 0 || step < 1 || (state_bits != 8 && state_bits != 32) ||
-        (dtype != FRAMEWISE_B200_F32 && dtype != FRAMEWISE_B200_BF16))
-        return FRAMEWISE_B200_BAD_ARGUMENT;
-    for (int64_t i = 0; i < count; ++i) {
-        const framewise_b200_tensor& t = tensors[i];
-        if (t.n < 0 || (t.n > 0 && (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq ||
-                                    (state_bits == 8 && (!t.exp_avg_steps || !t.exp_avg_sq_steps)))))
-            return FRAMEWISE_B200_BAD_ARGUMENT;
-    }
-    const adamw::Rates r = {(float)beta1, (float)(1 - beta1), (float)beta2, (float)(1 - beta2), (float)(1 - lr * weight_decay),
-                            (float)(lr / (1 - std::pow(beta1, (double)step))), (float)(1 / std::sqrt(1 - std::pow(beta2, (double)step))), (float)eps,
-                            (uint32_t)step * adamw::kTurn1, (uint32_t)step * adamw::kTurn2};
-    const bool dither = state_bits == 8 && std::max(beta1, beta2) > adamw::kNearest;
-    return for_slots(tensors, count, state_bits == 8, [&](const adamw::Slots& s) -> int {
-        const unsigned grid = adamw_grid(s.blocks);
-        auto go = [&](auto x) {
-            using X = decltype(x);
-            if (state_bits == 32) adamw::k_adamw<X, 32, false><<<grid, 256, 0, stream>>>(s, r);
-            else if (dither) adamw::k_adamw<X, 8, true><<<grid, 256, 0, stream>>>(s, r);
-            else adamw::k_adamw<X, 8, false><<<grid, 256, 0, stream>>>(s, r);
-        };
-        if (dtype == FRAMEWISE_B200_F32) go(float());
-        else go(__nv_bfloat16());
-        FW_LAUNCHED();
-        return FRAMEWISE_B200_OK;
-    });
+    return adamw_step(tensors, count, dtype, state_bits, lr, beta1, beta2, eps, weight_decay, step, false, stream);
+}
+
+int framewise_b200_adamw_follow(const framewise_b200_tensor* tensors, int64_t count, int32_t dtype, int32_t state_bits, double lr,
+                                double beta1, double beta2, double eps, double weight_decay, int64_t step,
+                                framewise_b200_stream_t stream) {
+    return adamw_step(tensors, count, dtype, state_bits, lr, beta1, beta2, eps, weight_decay, step, true, stream);
 }
 
 int framewise_b200_adamw_decode(const framewise_b200_tensor* tensors, int64_t count, framewise_b200_stream_t stream) {

@@ -274,10 +274,11 @@ void written(const Tensors& list) {
         if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
 }
 
-// exp_avg_steps, exp_avg_sq_steps: empty (states of 32 bits), or one per parameter.  master: empty, or one per parameter.
+// exp_avg_steps, exp_avg_sq_steps: empty (states of 32 bits), or one per parameter.  master: empty, or one per parameter;
+// follow: the copies take over what has been changed in the parameters.
 void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& master, const Tensors& exp_avg, const Tensors& exp_avg_sq,
                 const Tensors& exp_avg_steps, const Tensors& exp_avg_sq_steps, double lr, double beta1, double beta2, double eps,
-                double weight_decay, int64_t step) {
+                double weight_decay, int64_t step, bool follow) {
     const size_t n = params.size();
     TORCH_CHECK(grads.size() == n && exp_avg.size() == n && exp_avg_sq.size() == n && (master.empty() || master.size() == n) &&
                     exp_avg_steps.size() == exp_avg_sq_steps.size() && (exp_avg_steps.empty() || exp_avg_steps.size() == n),
@@ -317,7 +318,8 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& mast
             t.exp_avg_steps = exp_avg_steps[i].data_ptr<float>(), t.exp_avg_sq_steps = exp_avg_sq_steps[i].data_ptr<float>();
         }
     }
-    check_status(framewise_b200_adamw(list.data(), (int64_t)n, dtype, eight ? 8 : 32, lr, beta1, beta2, eps, weight_decay, step, stream_of()));
+    const auto run = follow ? framewise_b200_adamw_follow : framewise_b200_adamw;
+    check_status(run(list.data(), (int64_t)n, dtype, eight ? 8 : 32, lr, beta1, beta2, eps, weight_decay, step, stream_of()));
     for (const Tensors* const x : {&params, &master, &exp_avg, &exp_avg_sq, &exp_avg_steps, &exp_avg_sq_steps}) written(*x);
 }
 

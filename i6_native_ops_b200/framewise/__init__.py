@@ -120,6 +120,7 @@ def adamw_step(
     betas: Tuple[float, float] = (0.9, 0.999),
     eps: float = 1e-8,
     weight_decay: float = 0.01,
+    follow: bool = False,
 ) -> None:
     """One step of AdamW over a list of parameters, in place, in as few launches as there are 48 tensors.  As after any
     operation in place, graphs that saved a parameter before refuse their backward pass.
@@ -131,11 +132,13 @@ def adamw_step(
         betas are 0.98 at most, else up or down by offsets that change with ``step``, so that moments which shrink slower
         than codes are apart do so on average (roots of the second moment are then within about ``1 / sqrt(2 code)``)
     :param step: of this call, counted from 1; has to grow from step to step
-    :param master: float32 copies that are updated in place of the parameters, which then get their rounded values"""
+    :param master: float32 copies that are updated in place of the parameters, which then get their rounded values
+    :param follow: a copy of which its parameter is not the rounded value starts from the parameter, which has been changed
+        since the last step; without, what the parameter holds makes no difference"""
     m, m_steps = _split(exp_avg)
     v, v_steps = _split(exp_avg_sq)
     core.adamw_step(list(params), list(grads), [] if master is None else list(master), m, v, m_steps, v_steps, float(lr),
-                    float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(step))
+                    float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(step), bool(follow))
 
 
 def adamw_values(exp_avg: Sequence[State], exp_avg_sq: Sequence[State]) -> Tuple[List[torch.Tensor], List[torch.Tensor]]:
@@ -152,7 +155,8 @@ class AdamW(torch.optim.Optimizer):
     codes, 16 thousand to one (first moment) and 65 thousand to one (root of the second) between largest and smallest
     (:func:`adamw_step` says how they are rounded: on average right at any betas, a root of the second moment that is a
     hundredth of its block's largest to some 15 %).
-    bfloat16 parameters get a float32 copy that the steps accumulate in (``state["master"]``).  Parameters without a
+    bfloat16 parameters get a float32 copy that the steps accumulate in (``state["master"]``); values that the program
+    changes between steps (a model loaded, weights clipped) are taken over from the parameter.  Parameters without a
     gradient are passed over.  The learning rate may be changed between steps, as for any torch optimizer."""
 
     def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -208,7 +212,7 @@ class AdamW(torch.optim.Optimizer):
                 core.adamw_step(params, [p.grad for p in params], [] if dtype == torch.float32 else pick("master"),
                                 pick("exp_avg"), pick("exp_avg_sq"), pick("exp_avg_steps") if eight else [],
                                 pick("exp_avg_sq_steps") if eight else [], float(group["lr"]), float(group["betas"][0]),
-                                float(group["betas"][1]), float(group["eps"]), float(group["weight_decay"]), int(step))
+                                float(group["betas"][1]), float(group["eps"]), float(group["weight_decay"]), int(step), True)
         return loss
 
 

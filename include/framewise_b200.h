@@ -124,6 +124,12 @@ int framewise_b200_adamw(const framewise_b200_tensor* tensors, int64_t count, in
                          int32_t state_bits, double lr, double beta1, double beta2, double eps,
                          double weight_decay, int64_t step, framewise_b200_stream_t stream);
 
+/* The same step; but where a parameter is not its master copy rounded, the program has changed it since (a model loaded,
+ * weights clipped), and the copy starts from the parameter's value.  Parameters without a copy: as above. */
+int framewise_b200_adamw_follow(const framewise_b200_tensor* tensors, int64_t count, int32_t dtype,
+                                int32_t state_bits, double lr, double beta1, double beta2, double eps,
+                                double weight_decay, int64_t step, framewise_b200_stream_t stream);
+
 /* 8-bit states to the values that they stand for: the codes in exp_avg / exp_avg_sq to f32 in param / master
  * (the second moment itself, not its root); other fields are ignored. */
 int framewise_b200_adamw_decode(const framewise_b200_tensor* tensors, int64_t count, framewise_b200_stream_t stream);
