@@ -46,6 +46,11 @@ int dtype_of(const Tensor& x, const char* name) {
 // values where they are: a view that holds them negated or conjugated is copied
 Tensor plain(const Tensor& x) { return x.is_neg() ? x.resolve_neg() : x; }
 
+// There are no forward-mode derivatives: a tensor that carries one is refused, for its tangent would be lost.
+void check_no_tangent(const Tensor& x, const char* name) {
+    TORCH_CHECK(!x.defined() || !x._fw_grad(/*level=*/0).defined(), "framewise: there are no forward-mode derivatives (of ", name, ")");
+}
+
 // (B,T) labels and (B,) lengths of a call; labels of one dimension are a batch of one
 struct Positions {
     int64_t B, T;
@@ -146,6 +151,7 @@ struct LinearCrossEntropyBackward : public torch::autograd::Node {
     }
     torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
         TORCH_CHECK(!torch::GradMode::is_enabled(), "framewise: there are no gradients of these gradients");
+        check_no_tangent(grads[0], "gradients");
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
         const Tensor w = weight.unpack();
         TORCH_CHECK(saved.defined(), "framewise: the graph has been freed");
@@ -171,6 +177,9 @@ struct LinearCrossEntropyBackward : public torch::autograd::Node {
 Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& targets, const OptTensor& bias,
                             const OptTensor& seq_lens, int64_t ignore_index) {
     dtype_of(hidden, "hidden");
+    check_no_tangent(hidden, "hidden");
+    check_no_tangent(weight, "weight");
+    if (bias.has_value()) check_no_tangent(*bias, "bias");
     const bool train = torch::GradMode::is_enabled() &&
                        (hidden.requires_grad() || weight.requires_grad() || (bias.has_value() && bias->requires_grad()));
     c10::cuda::CUDAGuard guard(hidden.device());
@@ -217,6 +226,7 @@ struct LabelEmbeddingBackward : public torch::autograd::Node {
     }
     torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
         TORCH_CHECK(!torch::GradMode::is_enabled(), "framewise: there are no gradients of these gradients");
+        check_no_tangent(grads[0], "gradients");
         if (!grads[0].defined()) return {Tensor()};
         const Tensor t = labels.unpack(), n = has_lens ? lens.unpack() : Tensor();
         c10::cuda::CUDAGuard guard(t.device());
@@ -234,6 +244,7 @@ struct LabelEmbeddingBackward : public torch::autograd::Node {
 
 Tensor label_embedding(const Tensor& labels, const Tensor& weight, double scale, const OptTensor& seq_lens, int64_t ignore_index) {
     dtype_of(weight, "weight");
+    check_no_tangent(weight, "weight");
     c10::cuda::CUDAGuard guard(weight.device());
     if (!torch::GradMode::is_enabled() || !weight.requires_grad())
         return embed_forward(weight, labels, Positions(labels, seq_lens, weight), scale, ignore_index);

@@ -64,3 +64,33 @@ def test_a_step_moves_the_versions_of_what_it_writes(fw, cuda, bits):
         m, v = torch.zeros(300, device=cuda), torch.zeros(300, device=cuda)
     fw.adamw_step([q], [torch.ones(300, device=cuda)], [m], [v], step=1)
     assert bool((q < 1).all())
+
+
+@pytest.mark.parametrize("train", [False, True])
+def test_forward_mode_derivatives_are_refused(fw, cuda, train):
+    """There are none; a tangent is not lost in silence."""
+    import torch.autograd.forward_ad as fwd
+
+    h, w, t = layer(cuda, torch.float32)
+    h, b = h.detach(), torch.zeros(90, device=cuda)
+
+    def dual(x):
+        return fwd.make_dual(x.detach().requires_grad_(train), torch.ones_like(x))
+
+    with fwd.dual_level():
+        for call in (lambda: fw.linear_cross_entropy(dual(h), w, t), lambda: fw.linear_cross_entropy(h, dual(w), t),
+                     lambda: fw.linear_cross_entropy(h, w, t, bias=dual(b)), lambda: fw.label_embedding(t, dual(w))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        # of the incoming gradients
+        for out, leaf in ((lambda x: fw.linear_cross_entropy(x, w, t), h), (lambda x: fw.label_embedding(t, x), w)):
+            x = leaf.clone().requires_grad_()
+            y = out(x)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, x, fwd.make_dual(torch.ones_like(y), torch.ones_like(y)))
+        # tensors without a tangent pass
+        assert bool(fw.linear_cross_entropy(h, w, t).isfinite().all())
+    for transform in (lambda: torch.func.jvp(lambda x: fw.linear_cross_entropy(x, w, t), (h,), (h,)),
+                      lambda: torch.func.vmap(lambda x: fw.label_embedding(t, x))(w[None])):
+        with pytest.raises(RuntimeError):
+            transform()
