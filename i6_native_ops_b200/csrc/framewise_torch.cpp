@@ -81,12 +81,6 @@ struct Positions {
 struct CeCall {
     framewise_b200_ce_shape shape = {};
     size_t saved = 0, forward = 0, backward = 0;
-
-    // One buffer: what is kept, then scratch, the backward pass's as well where that is small (an allocation less there).
-    static constexpr size_t kSmall = (size_t)32 << 20;
-    size_t work_at() const { return (saved + 255) / 256 * 256; }
-    bool   work_kept() const { return shape.train && backward <= kSmall; }
-    size_t buffer() const { return work_at() + (work_kept() ? std::max(forward, backward) : forward); }
 };
 
 struct CeInputs {
@@ -125,50 +119,54 @@ CeInputs ce_inputs(const Tensor& hidden_in, const Tensor& weight_in, const OptTe
     return in;
 }
 
-// (loss, what the backward pass needs)
+// (loss, what the backward pass needs: that alone, for the graph holds it, and hooks may carry it elsewhere and back)
 std::pair<Tensor, Tensor> ce_forward(const CeInputs& in, const Tensor& targets) {
+    const bool   apart = in.call.shape.train;  // without gradients scratch follows in the same buffer
+    const size_t kept  = (in.call.saved + 255) / 256 * 256;
     Tensor loss  = torch::empty(targets.sizes(), in.hidden.options().dtype(torch::kFloat32));
-    Tensor saved = bytes(in.call.buffer(), in.hidden);
-    char* const kept = static_cast<char*>(saved.data_ptr());
+    Tensor saved = bytes(apart ? in.call.saved : kept + in.call.forward, in.hidden);
+    Tensor work  = apart ? bytes(in.call.forward, in.hidden) : Tensor();
+    char* const at = static_cast<char*>(saved.data_ptr());
     check_status(framewise_b200_ce_forward(&in.call.shape, in.hidden.data_ptr(), in.weight.data_ptr(),
                                            in.bias.defined() ? in.bias.data_ptr() : nullptr, in.at.labels.data_ptr(), in.at.lens_ptr(),
-                                           loss.data_ptr<float>(), kept, in.call.saved, kept + in.call.work_at(), in.call.forward, stream_of()));
+                                           loss.data_ptr<float>(), at, in.call.saved, apart ? work.data_ptr() : at + kept, in.call.forward,
+                                           stream_of()));
     return {loss, saved};
 }
 
 // The node of the graph that a call leaves behind.  (A node of its own, rather than torch::autograd::Function: that packs
 // sizes into a dictionary, some ten microseconds a step.)
 struct LinearCrossEntropyBackward : public torch::autograd::Node {
-    torch::autograd::SavedVariable weight;  // a change of it before the backward pass is noticed
-    Tensor  saved;
+    torch::autograd::SavedVariable weight, saved;  // a change of the weight before the backward pass is noticed
     CeCall  call;
     bool    flat = false;
 
     std::string name() const override { return "LinearCrossEntropyBackward"; }
     void release_variables() override {
         weight.reset_data();
-        saved.reset();
+        saved.reset_data();
     }
     torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
         TORCH_CHECK(!torch::GradMode::is_enabled(), "framewise: there are no gradients of these gradients");
         check_no_tangent(grads[0], "gradients");
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
-        const Tensor w = weight.unpack();
-        TORCH_CHECK(saved.defined(), "framewise: the graph has been freed");
-        c10::cuda::CUDAGuard guard(w.device());
+        const Tensor w = weight.unpack(), kept = saved.unpack();
         const auto& s = call.shape;
+        TORCH_CHECK(w.is_cuda() && w.device() == kept.device() && w.is_contiguous() && w.dim() == 2 && w.size(0) == s.V && w.size(1) == s.D &&
+                        w.scalar_type() == (s.dtype == FRAMEWISE_B200_F32 ? torch::kFloat32 : torch::kBFloat16) && kept.is_contiguous() &&
+                        kept.scalar_type() == torch::kUInt8 && (size_t)kept.numel() >= call.saved,
+                    "framewise: saved-tensor hooks must give back what they were given");
+        c10::cuda::CUDAGuard guard(w.device());
         Tensor g = plain(grads[0]);
         if (g.scalar_type() != torch::kFloat32) g = g.to(torch::kFloat32);
-        Tensor dh, dw, db, work;
-        if (!call.work_kept()) work = bytes(call.backward, w);
-        char* const kept = static_cast<char*>(saved.data_ptr());
+        Tensor dh, dw, db, work = bytes(call.backward, w);
         const auto options = w.options().requires_grad(false);
         if (task_should_compute_output(0)) dh = flat ? torch::empty({s.T, s.D}, options) : torch::empty({s.B, s.T, s.D}, options);
         if (task_should_compute_output(1)) dw = torch::empty({s.V, s.D}, options);
         if (s.has_bias && task_should_compute_output(2)) db = torch::empty({s.V}, options);
         auto ptr = [](const Tensor& x) { return x.defined() ? x.data_ptr() : nullptr; };
         check_status(framewise_b200_ce_backward(&s, w.data_ptr(), g.data_ptr<float>(), flat ? 0 : g.stride(0), g.stride(-1), ptr(dh), ptr(dw),
-                                                ptr(db), kept, call.saved, call.work_kept() ? kept + call.work_at() : work.data_ptr(), call.backward,
+                                                ptr(db), kept.data_ptr(), call.saved, work.data_ptr(), call.backward,
                                                 stream_of()));
         return {dh, dw, db};
     }
@@ -184,16 +182,18 @@ Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Te
                        (hidden.requires_grad() || weight.requires_grad() || (bias.has_value() && bias->requires_grad()));
     c10::cuda::CUDAGuard guard(hidden.device());
     if (!train) return ce_forward(ce_inputs(hidden, weight, bias, targets, seq_lens, ignore_index, false), targets).first;
-    Tensor loss;
+    Tensor loss, w, saved;
     std::shared_ptr<LinearCrossEntropyBackward> node(new LinearCrossEntropyBackward(), torch::autograd::deleteNode);
     {
         at::AutoDispatchBelowADInplaceOrView below;
         const CeInputs in = ce_inputs(hidden, weight, bias, targets, seq_lens, ignore_index, true);
-        std::tie(loss, node->saved) = ce_forward(in, targets);
-        node->weight = torch::autograd::SavedVariable(in.weight, false);
-        node->call   = in.call;
-        node->flat   = targets.dim() == 1;
+        std::tie(loss, saved) = ce_forward(in, targets);
+        w          = in.weight;
+        node->call = in.call;
+        node->flat = targets.dim() == 1;
     }
+    node->weight = torch::autograd::SavedVariable(w, false);  // outside of the guard: hooks may run
+    node->saved  = torch::autograd::SavedVariable(saved, false);
     node->set_next_edges(torch::autograd::collect_next_edges(hidden, weight, bias.has_value() ? *bias : Tensor()));
     torch::autograd::set_history(loss, node);
     return loss;
@@ -229,6 +229,10 @@ struct LabelEmbeddingBackward : public torch::autograd::Node {
         check_no_tangent(grads[0], "gradients");
         if (!grads[0].defined()) return {Tensor()};
         const Tensor t = labels.unpack(), n = has_lens ? lens.unpack() : Tensor();
+        TORCH_CHECK(t.is_cuda() && t.is_contiguous() && t.numel() == B * T && (t.scalar_type() == torch::kInt32 || t.scalar_type() == torch::kInt64) &&
+                        t.device() == grads[0].device() &&
+                        (!has_lens || (n.device() == t.device() && n.is_contiguous() && n.numel() == B && n.scalar_type() == torch::kInt32)),
+                    "framewise: saved-tensor hooks must give back what they were given");
         c10::cuda::CUDAGuard guard(t.device());
         Tensor g = plain(grads[0]);
         if (g.stride(-1) != 1) g = g.contiguous();
@@ -248,17 +252,18 @@ Tensor label_embedding(const Tensor& labels, const Tensor& weight, double scale,
     c10::cuda::CUDAGuard guard(weight.device());
     if (!torch::GradMode::is_enabled() || !weight.requires_grad())
         return embed_forward(weight, labels, Positions(labels, seq_lens, weight), scale, ignore_index);
-    Tensor out;
+    Tensor out, t, n;
     std::shared_ptr<LabelEmbeddingBackward> node(new LabelEmbeddingBackward(), torch::autograd::deleteNode);
     {
         at::AutoDispatchBelowADInplaceOrView below;
         const Positions at(labels, seq_lens, weight);
         out = embed_forward(weight, labels, at, scale, ignore_index);
-        node->labels = torch::autograd::SavedVariable(at.labels, false);
-        if ((node->has_lens = at.lens.defined())) node->lens = torch::autograd::SavedVariable(at.lens, false);
+        t = at.labels, n = at.lens;
         node->flat = labels.dim() == 1, node->B = at.B, node->T = at.T, node->V = weight.size(0), node->D = weight.size(1);
         node->ignore_index = ignore_index, node->scale = scale;
     }
+    node->labels = torch::autograd::SavedVariable(t, false);
+    if ((node->has_lens = n.defined())) node->lens = torch::autograd::SavedVariable(n, false);
     node->set_next_edges(torch::autograd::collect_next_edges(weight));
     torch::autograd::set_history(out, node);
     return out;

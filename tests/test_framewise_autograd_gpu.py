@@ -1,6 +1,7 @@
 """What autograd has to know of the framewise operators: that the optimizer changed a tensor, what a graph keeps."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +95,70 @@ def test_forward_mode_derivatives_are_refused(fw, cuda, train):
                       lambda: torch.func.vmap(lambda x: fw.label_embedding(t, x))(w[None])):
         with pytest.raises(RuntimeError):
             transform()
+
+
+def gradients(fw, h, w, t, twice=False):
+    x, y = h.detach().requires_grad_(), w.detach().requires_grad_()
+    loss = fw.linear_cross_entropy(x, y, t).sum()
+    out = torch.autograd.grad(loss, (x, y), retain_graph=twice)
+    return (out, torch.autograd.grad(loss, (x, y))) if twice else out
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_saved_tensor_hooks_see_all_that_is_kept(fw, cuda, dtype):
+    """What the backward pass needs can be carried to the host and back; nothing of it stays on the device meanwhile."""
+    h, w, t = layer(cuda, dtype, B=8, T=200, V=300, D=256)
+    want = gradients(fw, h, w, t)
+    with torch.autograd.graph.save_on_cpu():
+        got = gradients(fw, h, w, t)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # a graph whose tensors are on the host holds the loss and little else
+    x, y = h.detach().requires_grad_(), w.detach().requires_grad_()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with torch.autograd.graph.save_on_cpu():
+        loss = fw.linear_cross_entropy(x, y, t)
+    assert torch.cuda.memory_allocated() - before <= loss.numel() * 4 + 65536
+    loss.sum().backward()
+    assert torch.equal(x.grad, want[0]) and torch.equal(y.grad, want[1])
+    # the embedding's labels and lengths as well
+    lens = torch.full((8,), 150, dtype=torch.int32, device=cuda)
+    y.grad = None
+    with torch.autograd.graph.save_on_cpu():
+        out = fw.label_embedding(t, y, seq_lens=lens)
+    out.backward(torch.ones_like(out))
+    z = w.detach().requires_grad_()
+    fw.label_embedding(t, z, seq_lens=lens).backward(torch.ones_like(out))
+    assert torch.equal(y.grad, z.grad)
+
+
+def test_what_hooks_give_back_is_looked_at(fw, cuda):
+    h, w, t = layer(cuda, torch.float32)
+    for spoil in (lambda x: x.cpu(), lambda x: x[:1], lambda x: x.double()):
+        for call in (lambda: fw.linear_cross_entropy(h, w.requires_grad_(), t), lambda: fw.label_embedding(t, w.requires_grad_())):
+            with torch.autograd.graph.saved_tensors_hooks(lambda x: x, spoil):
+                out = call()
+            with pytest.raises(RuntimeError, match="hooks"):
+                out.sum().backward()
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_checkpoints(fw, cuda, reentrant):
+    h, w, t = layer(cuda, torch.bfloat16)
+    want = gradients(fw, h, w, t)
+    x, y = h.detach().requires_grad_(), w.detach().requires_grad_()
+    loss = torch.utils.checkpoint.checkpoint(lambda a, b: fw.linear_cross_entropy(a * 1, b, t), x, y, use_reentrant=reentrant)
+    loss.sum().backward()
+    assert torch.equal(x.grad, want[0]) and torch.equal(y.grad, want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_two_backward_passes_over_one_graph(fw, cuda, dtype):
+    h, w, t = layer(cuda, dtype)
+    first, second = gradients(fw, h, w, t, twice=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    x = h.detach().requires_grad_()
+    loss = fw.linear_cross_entropy(x, w.detach(), t).sum()
+    loss.backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        loss.backward()
