@@ -162,3 +162,27 @@ def test_two_backward_passes_over_one_graph(fw, cuda, dtype):
     loss.backward()
     with pytest.raises(RuntimeError, match="second time"):
         loss.backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("sizes", [(3, 40, 90, 64), (2, 700, 1000, 300), (5, 300, 41, 256), (30, 400, 12001, 40)])
+def test_gradients_are_nan_throughout_where_a_wait_ran_out(fw, cuda, dtype, sizes):
+    """The mark that a wait ran out, the second word of what is kept, is set on the way from the forward to the backward
+    pass: no finite value may be left, whatever CTA writes last."""
+    B, T, V, D = sizes
+    h, w, t = layer(cuda, dtype, B, T, V, D)
+    h, w, b = h.detach().requires_grad_(), w.requires_grad_(), torch.zeros(V, dtype=dtype, device=cuda).requires_grad_()
+    t[0, 3] = -100
+
+    def mark(x):
+        if x.dtype == torch.uint8:
+            x = x.clone()
+            assert int(x[:8].view(torch.int32)[0]) == B * T - 1 and int(x[:8].view(torch.int32)[1]) == 0
+            x[:8].view(torch.int32)[1] = 1
+        return x
+
+    for _ in range(3):
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, mark):
+            loss = fw.linear_cross_entropy(h, w, t, bias=b)
+        for g in torch.autograd.grad(loss.sum(), (h, w, b)):
+            assert bool(g.isnan().all())
