@@ -225,7 +225,7 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
     p->weight       = s.take<__nv_bfloat16>(p->copy_weight ? p->parts * p->V * p->pitch : 0);
     p->saved_bytes  = s.used;
     Parts f(forward);
-    p->part   = f.take<float2>((workers + mt) * ce::Layout<ce::kLogits, 1, 1>::kGroups * tile);
+    p->part   = f.take<float2>((workers + mt) * ce::Layout<ce::kLogits, 1, 1, false>::kGroups * tile);
     p->target = f.take<float>(rows);
     p->forward_bytes = f.used;
     Parts b(backward);
@@ -239,10 +239,10 @@ int ce_plan(const framewise_b200_ce_shape* sh, void* saved, void* forward, void*
     return FRAMEWISE_B200_OK;
 }
 
-template <int KIND, int kPair, int PARTS>
+template <int KIND, int kPair, int PARTS, bool LONG = false>
 int launch_tiles(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const ce::Params& p, int workers, cudaStream_t stream) {
-    using L = ce::Layout<KIND, kPair, PARTS>;
-    auto kernel = ce::k_ce_tiles<KIND, kPair, PARTS>;
+    using L = ce::Layout<KIND, kPair, PARTS, LONG>;
+    auto kernel = ce::k_ce_tiles<KIND, kPair, PARTS, LONG>;
     static std::atomic<uint64_t> allowed{0};
     FW_DO(allow_shared(kernel, L::kBytes, allowed));
     cudaLaunchConfig_t c = {};
@@ -288,14 +288,15 @@ int ce_forward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* hidd
     ce::Params q = {};
     q.head = p.head, q.V = (int)p.V, q.D = (int)p.D, q.wide = p.wide_v;
     q.bias = p.bias, q.label = p.row_label, q.part = p.part, q.target = p.target;
-    FW_DO(launch_tiles<ce::kLogits, kPair, PARTS>(a, b, a, q, workers, stream));
+    FW_DO((p.D > ce::kLong ? launch_tiles<ce::kLogits, kPair, PARTS, true> : launch_tiles<ce::kLogits, kPair, PARTS>)(a, b, a, q, workers, stream));
     const int nt = (int)((p.V + p.wide_v - 1) / p.wide_v);
     auto join = [&](auto* kernel, int64_t lanes) {
         kernel<<<(unsigned)((p.N * lanes + 255) / 256), 256, 0, stream>>>(p.head, nt, tile, workers, p.part, p.target, p.row_label, p.row_position,
                                                                        loss, sh.train ? p.stats : nullptr);
     };
-    if (p.N > 4096) join(ce::k_join_rows<4>, 4);
-    else join(ce::k_join_rows<32>, 32);
+    constexpr int kGroups = ce::Layout<ce::kLogits, kPair, PARTS, false>::kGroups, kLongGroups = ce::Layout<ce::kLogits, kPair, PARTS, true>::kGroups;
+    if (p.N > 4096) p.D > ce::kLong ? join(ce::k_join_rows<4, kLongGroups>, 4) : join(ce::k_join_rows<4, kGroups>, 4);
+    else p.D > ce::kLong ? join(ce::k_join_rows<32, kLongGroups>, 32) : join(ce::k_join_rows<32, kGroups>, 32);
     FW_LAUNCHED();
     return FRAMEWISE_B200_OK;
 }
@@ -334,7 +335,8 @@ int ce_backward(const framewise_b200_ce_shape& sh, const CePlan& p, const X* wei
         ce::After after = {};
         g.row0 = c * p.chunk, g.add = c > 0;
         g.wide = p.wide_v;
-        FW_DO(launch_tiles<ce::kGradients, kPair, Q_PARTS>(x_k, w_k, q_out, g, workers, stream));
+        FW_DO((D > ce::kLong ? launch_tiles<ce::kGradients, kPair, Q_PARTS, true> : launch_tiles<ce::kGradients, kPair, Q_PARTS>)(x_k, w_k, q_out, g,
+                                                                                                                           workers, stream));
         g.wide = p.wide_d;
         if (grad_hidden) {
             g.out = grad_hidden, g.out_grain = grain(grad_hidden), g.pieces = p.pieces;
