@@ -205,8 +205,7 @@ class AdamW(torch.optim.Optimizer):
                 state = self.state[p]
                 if not state:
                     state.update(self._fresh(p, group["state_bits"]))
-                state["step"] += 1
-                calls.setdefault((p.device, p.dtype, state["step"]), []).append(p)
+                calls.setdefault((p.device, p.dtype, state["step"] + 1), []).append(p)
             for (_, dtype, step), params in calls.items():
                 states = [self.state[p] for p in params]
                 pick = lambda name: [s[name] for s in states]  # noqa: E731
@@ -215,6 +214,8 @@ class AdamW(torch.optim.Optimizer):
                                 pick("exp_avg"), pick("exp_avg_sq"), pick("exp_avg_steps") if eight else [],
                                 pick("exp_avg_sq_steps") if eight else [], float(group["lr"]), float(group["betas"][0]),
                                 float(group["betas"][1]), float(group["eps"]), float(group["weight_decay"]), int(step), True)
+                for s in states:  # a call that was refused has not taken place
+                    s["step"] = step
         return loss
 
 

@@ -102,3 +102,26 @@ def test_the_step_itself_takes_either(fw, cuda, bits):
         for a, b in zip(*out):
             assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num())
         assert bool(out[0][1][5].isnan()) and bool((out[0][1][9:12] > p[9:12].float() + 0.5).all()) != follow
+
+
+def test_a_refused_step_does_not_count(fw, cuda):
+    """A gradient that the step cannot take: an error, and nothing has happened, the count of steps included."""
+    p = [torch.nn.Parameter(torch.ones(6, 4, device=cuda)) for _ in range(2)]
+    o = fw.AdamW(p, lr=1e-2)
+    for x in p:
+        x.grad = torch.ones_like(x)
+    o.step()
+    p[1].grad = torch.ones(6, 4, device=cuda).to_sparse()
+    before = [x.detach().clone() for x in p]
+    with pytest.raises(RuntimeError):
+        o.step()
+    assert [o.state[x]["step"] for x in p] == [1, 1] and all(torch.equal(a, b) for a, b in zip(p, before))
+    p[1].grad = torch.ones(6, 4, device=cuda)
+    o.step()
+    q = [torch.nn.Parameter(torch.ones(6, 4, device=cuda)) for _ in range(2)]
+    o2 = fw.AdamW(q, lr=1e-2)
+    for _ in range(2):
+        for x in q:
+            x.grad = torch.ones_like(x)
+        o2.step()
+    assert all(torch.equal(a, b) for a, b in zip(p, q))
