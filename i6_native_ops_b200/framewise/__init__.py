@@ -77,9 +77,13 @@ def linear_cross_entropy(
 
     The (N, V) logits are never in memory: forward they stay on the SM, backward they are formed again and the
     gradients' left factor is held for some thousand rows at a time.  Sums are formed in 32 bits in a fixed order
-    (logits by 1024 of the width at most, then added up); the products of float32 inputs keep 24 bits.  Backward needs ``weight`` unchanged.  Derivatives are those of backward
-    passes and of the first order; others are refused.  What backward needs (the rows that count, for float32 in three
-    parts of 16 bits, and then the weight likewise) is saved as one tensor of bytes that saved-tensor hooks see."""
+    (logits by 1024 of the width at most, then added up); the products of float32 inputs keep 24 bits.  bfloat16: the
+    left factor is held in 8 bits (16 for up to 256 positions), so gradients are some 1.4 times as far from exact ones as
+    their own rounding alone, those of ``hidden`` twice where the rows of ``weight`` have most in common.
+
+    Backward needs ``weight`` unchanged.  Derivatives are those of backward passes and of the first order; others are
+    refused.  What backward needs (the rows that count, for float32 in three parts of 16 bits, and then the weight
+    likewise) is saved as one tensor of bytes that saved-tensor hooks see."""
     return core.linear_cross_entropy(hidden, weight, targets, bias, _lengths(seq_lens, targets), int(ignore_index))
 
 

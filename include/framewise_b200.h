@@ -68,8 +68,9 @@ int framewise_b200_ce_forward(const framewise_b200_ce_shape* shape, const void* 
  *     q = grad_loss (softmax(z) - onehot(target));  grad_hidden = q . weight,  grad_weight = q^T . hidden,
  *     grad_bias = sum of q.
  * The logits are computed again, q is held for some thousand rows at a time: in bf16 for bf16 inputs (8 bits of
- * each value, as the gradients themselves have; 16 bits for up to 256 rows), in three bf16 parts for f32.  Outputs are dense; a NULL output
- * is not computed.  Sums are formed in a fixed order: equal calls give equal bits. */
+ * each value, as the gradients themselves have, which are then some 1.4 times as far from exact ones as their own rounding;
+ * 16 bits for up to 256 positions), in three bf16 parts for f32.  Outputs are dense; a NULL output is not computed.  Sums
+ * are formed in a fixed order: equal calls give equal bits. */
 int framewise_b200_ce_backward(const framewise_b200_ce_shape* shape, const void* weight,
                                const float* grad_loss, int64_t grad_stride_b, int64_t grad_stride_t,
                                void* grad_hidden, void* grad_weight, void* grad_bias,
