@@ -187,13 +187,23 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, but codes, moments and copies keep their own types (torch would turn them into the parameters')."""
-        super().load_state_dict(state_dict)
+        seen = {}  # what earlier hooks have made of the states; later ones see them with their types
+        hooks = (self.register_load_state_dict_pre_hook(lambda _, given: seen.update(given)),
+                 self.register_load_state_dict_post_hook(lambda _: self._take_states(seen), prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _take_states(self, state_dict: dict) -> None:
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(ids, params):
             if i in state_dict["state"]:
-                self.state[p] = {k: v.to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
-                                 for k, v in state_dict["state"][i].items()}
+                state = {k: v.to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
+                         for k, v in state_dict["state"][i].items()}
+                self.state[p] = state
 
     @torch.no_grad()
     def step(self, closure=None):

@@ -125,3 +125,34 @@ def test_a_refused_step_does_not_count(fw, cuda):
             x.grad = torch.ones_like(x)
         o2.step()
     assert all(torch.equal(a, b) for a, b in zip(p, q))
+
+
+def trained(fw, cuda, dtype, bits, steps=3):
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    p = torch.nn.Parameter(torch.randn(40, 30, device=cuda, generator=gen).to(dtype))
+    o = fw.AdamW([p], state_bits=bits, **HYPER)
+    for _ in range(steps):
+        p.grad = torch.randn(40, 30, device=cuda, generator=gen).to(dtype)
+        o.step()
+    return p, o
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_states_that_hooks_change_on_the_way_in(fw, cuda, bits):
+    """A hook before loading that gives another dict is heard; one after loading sees the states as they will be."""
+    p, o = trained(fw, cuda, torch.bfloat16, bits)
+    q = torch.nn.Parameter(p.detach().clone())
+    o2 = fw.AdamW([q], state_bits=bits, **HYPER)
+
+    def later(_, given):
+        return {**given, "state": {i: {**s, "step": s["step"] + 100} for i, s in given["state"].items()}}
+
+    types = []
+    o2.register_load_state_dict_pre_hook(later)
+    o2.register_load_state_dict_post_hook(lambda opt: types.append({k: v.dtype for k, v in opt.state[q].items() if k != "step"}))
+    o2.load_state_dict(o.state_dict())
+    assert o2.state[q]["step"] == 103
+    assert types == [{k: v.dtype for k, v in o.state[p].items() if k != "step"}]
+    assert all(torch.equal(v, o2.state[q][k]) for k, v in o.state[p].items() if k != "step")
+    o2.load_state_dict(o.state_dict())  # the call's own hooks have gone, the program's stay
+    assert o2.state[q]["step"] == 103 and len(types) == 2
