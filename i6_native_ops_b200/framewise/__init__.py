@@ -182,11 +182,16 @@ class AdamW(torch.optim.Optimizer):
             for name in ("exp_avg", "exp_avg_sq"):
                 state[name] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
         if p.dtype != torch.float32:
-            state["master"] = p.detach().to(torch.float32, memory_format=torch.contiguous_format)
+            state["master"] = self._copy(p)
         return state
 
+    @staticmethod
+    def _copy(p: torch.Tensor) -> torch.Tensor:
+        return p.detach().to(torch.float32, memory_format=torch.contiguous_format)
+
     def load_state_dict(self, state_dict):
-        """As torch's, but codes, moments and copies keep their own types (torch would turn them into the parameters')."""
+        """As torch's, but codes, moments and copies keep their own types (torch would turn them into the parameters').
+        bfloat16 parameters whose states come from float32 ones start a copy of their own."""
         seen = {}  # what earlier hooks have made of the states; later ones see them with their types
         hooks = (self.register_load_state_dict_pre_hook(lambda _, given: seen.update(given)),
                  self.register_load_state_dict_post_hook(lambda _: self._take_states(seen), prepend=True))
@@ -203,6 +208,8 @@ class AdamW(torch.optim.Optimizer):
             if i in state_dict["state"]:
                 state = {k: v.to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
                          for k, v in state_dict["state"][i].items()}
+                if state and p.dtype != torch.float32 and "master" not in state:
+                    state["master"] = self._copy(p)
                 self.state[p] = state
 
     @torch.no_grad()

@@ -156,3 +156,18 @@ def test_states_that_hooks_change_on_the_way_in(fw, cuda, bits):
     assert all(torch.equal(v, o2.state[q][k]) for k, v in o.state[p].items() if k != "step")
     o2.load_state_dict(o.state_dict())  # the call's own hooks have gone, the program's stay
     assert o2.state[q]["step"] == 103 and len(types) == 2
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_states_of_float32_parameters_for_bfloat16_ones(fw, cuda, bits):
+    p, o = trained(fw, cuda, torch.float32, bits)
+    q = torch.nn.Parameter(p.detach().bfloat16())
+    o2 = fw.AdamW([q], state_bits=bits, **HYPER)
+    o2.load_state_dict(o.state_dict())
+    before = q.detach().float()
+    q.grad = torch.ones_like(q)
+    o2.step()
+    s = o2.state[q]
+    assert s["step"] == 4 and torch.equal(s["master"].bfloat16(), q.detach())
+    move = (s["master"] - before).abs()
+    assert bool((move > 0).any()) and bool((move <= 0.1).all())
