@@ -25,8 +25,13 @@ EXT_DIR = os.path.join(PKG, "fbw", "_build")
 EXT = os.path.join(EXT_DIR, "fbw_core.so")
 VIT_DIR = os.path.join(PKG, "fast_viterbi", "_build")
 VIT_EXT = os.path.join(VIT_DIR, "fast_viterbi_core.so")
-# framewise_b200.cu and what it includes
-FW_SOURCES = ("framewise_b200.cu", "linear_ce_b200.inc", "embedding_b200.inc", "adamw_b200.inc", "tensor_core.h")
+# the sources of libframewise_b200.so, each with what it includes
+FW_SOURCES = {
+    "framewise_b200.cu": ("linear_ce_b200.inc", "embedding_b200.inc", "adamw_b200.inc"),
+    "label_scores_b200.cu": (),
+}
+FW_HEADERS = ("framewise_host.h", "tensor_core.h")
+FW_OBJECTS = os.path.join(PKG, "framewise", "_build", "objects")
 FW_LIB = os.path.join(PKG, "libframewise_b200.so")
 FW_DIR = os.path.join(PKG, "framewise", "_build")
 FW_EXT = os.path.join(FW_DIR, "framewise_core.so")
@@ -48,8 +53,9 @@ def build_lib(force: bool = False, verbose: bool = False) -> str:
     src = os.path.join(PKG, "csrc", "fbw_b200.cu")
     csrc = os.path.join(PKG, "csrc")
     # the .inc files are included by fbw_b200.cu; host_fill.cpp is the library's one host-only source
+    framewise = {*FW_SOURCES, *(f for included in FW_SOURCES.values() for f in included)}
     host_src = os.path.join(csrc, "host_fill.cpp")
-    deps = [os.path.join(csrc, f) for f in os.listdir(csrc) if f.endswith((".cu", ".inc")) and f not in FW_SOURCES]
+    deps = [os.path.join(csrc, f) for f in os.listdir(csrc) if f.endswith((".cu", ".inc")) and f not in framewise]
     deps += [host_src, *(os.path.join(csrc, f) for f in ("host_fill.h", "scaled.h", "sweep_shapes.h"))]
     hdr = os.path.join(INCLUDE, "fbw_b200.h")
     if not force and _newer(LIB, deps + [hdr]):
@@ -66,15 +72,25 @@ def build_lib(force: bool = False, verbose: bool = False) -> str:
 
 def build_framewise_lib(force: bool = False, verbose: bool = False) -> str:
     csrc = os.path.join(PKG, "csrc")
-    deps = [os.path.join(csrc, f) for f in FW_SOURCES] + [os.path.join(INCLUDE, "framewise_b200.h")]
-    if not force and _newer(FW_LIB, deps):
-        return FW_LIB
     nvcc = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "bin", "nvcc")
-    cmd = [nvcc, *NVCC_FLAGS, "-Xlinker", "-soname=libframewise_b200.so", "-I", INCLUDE, "-o", FW_LIB, deps[0]]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd))
-    subprocess.run(cmd, check=True)
+    os.makedirs(FW_OBJECTS, exist_ok=True)
+    objects, running = [], []
+    for source, included in FW_SOURCES.items():  # each by itself, side by side
+        deps = [os.path.join(csrc, f) for f in (source, *included, *FW_HEADERS)] + [os.path.join(INCLUDE, "framewise_b200.h")]
+        objects.append(os.path.join(FW_OBJECTS, source + ".o"))
+        if not force and _newer(objects[-1], deps):
+            continue
+        cmd = [nvcc, *(f for f in NVCC_FLAGS if f != "-shared"), "-I", INCLUDE, "-c", "-o", objects[-1], deps[0]]
+        if verbose:
+            cmd.insert(1, "-Xptxas=-v")
+            print(" ".join(cmd))
+        running.append((cmd, subprocess.Popen(cmd)))
+    for cmd, process in running:
+        if process.wait() != 0:
+            raise subprocess.CalledProcessError(process.returncode, cmd)
+    if not force and not running and _newer(FW_LIB, objects):
+        return FW_LIB
+    subprocess.run([nvcc, *NVCC_FLAGS, "-Xlinker", "-soname=libframewise_b200.so", "-o", FW_LIB, *objects], check=True)
     return FW_LIB
 
 

@@ -269,9 +269,123 @@ Tensor label_embedding(const Tensor& labels, const Tensor& weight, double scale,
     return out;
 }
 
-// ------------------------------------------------------------------------------------------ AdamW
+// ------------------------------------------------------------------------------------------ label scores
 
 using Tensors = std::vector<Tensor>;
+
+struct ScoresInputs {
+    Tensor    logits;
+    Positions at;
+    framewise_b200_scores_shape shape = {};
+};
+
+ScoresInputs scores_inputs(const Tensor& logits_in, const Tensor& labels, int64_t top, const OptTensor& seq_lens, int64_t ignore_index) {
+    const int dtype = dtype_of(logits_in, "logits");
+    TORCH_CHECK(logits_in.dim() == labels.dim() + 1, "logits must have one dimension more than labels");
+    for (int64_t d = 0; d < labels.dim(); ++d) TORCH_CHECK(logits_in.size(d) == labels.size(d), "logits must have shape (*labels.shape, V)");
+    const int64_t V = logits_in.size(-1);
+    TORCH_CHECK(V > 0, "logits must have classes");
+    TORCH_CHECK(top >= 0 && top <= std::min<int64_t>(V, 32), "top must be in 0..min(V, 32)");
+    ScoresInputs in{plain(logits_in), Positions(labels, seq_lens, logits_in)};
+    if (V > 1 && in.logits.stride(-1) != 1) in.logits = in.logits.contiguous();
+    auto& s = in.shape;
+    s.B = in.at.B, s.T = in.at.T, s.V = V, s.top = (int32_t)top, s.ignore_index = ignore_index, s.dtype = dtype, s.labels64 = in.at.wide;
+    s.logits_stride_b = labels.dim() == 2 ? in.logits.stride(0) : 0;
+    s.logits_stride_t = in.logits.stride(-2);
+    return in;
+}
+
+// log probabilities, entropies, the alternatives' log probabilities and labels; `kept` (undefined: not kept) for the backward pass
+Tensors scores_forward(const ScoresInputs& in, const Tensor& labels, Tensor* kept) {
+    const auto options = in.logits.options().dtype(torch::kFloat32);
+    auto shape = labels.sizes().vec();
+    Tensor log_probs = torch::empty(shape, options), entropy = torch::empty(shape, options);
+    shape.push_back(in.shape.top);
+    Tensor top_log_probs = torch::empty(shape, options), top_labels = torch::empty(shape, labels.options());
+    if (kept) *kept = bytes((size_t)(in.at.B * in.at.T) * 16, in.logits);
+    check_status(framewise_b200_scores_forward(&in.shape, in.logits.data_ptr(), in.at.labels.data_ptr(), in.at.lens_ptr(), log_probs.data_ptr<float>(),
+                                               entropy.data_ptr<float>(), top_log_probs.data_ptr<float>(), top_labels.data_ptr(),
+                                               kept ? kept->data_ptr() : nullptr, stream_of()));
+    return {log_probs, entropy, top_log_probs, top_labels};
+}
+
+struct LabelScoresBackward : public torch::autograd::Node {
+    torch::autograd::SavedVariable logits, labels, lens, top_labels, kept;  // a change of the logits in between is noticed
+    framewise_b200_scores_shape shape = {};
+    bool has_lens = false, flat = false;
+
+    std::string name() const override { return "LabelScoresBackward"; }
+    void release_variables() override {
+        for (auto* x : {&logits, &labels, &lens, &top_labels, &kept}) x->reset_data();
+    }
+    torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+        TORCH_CHECK(!torch::GradMode::is_enabled(), "framewise: there are no gradients of these gradients");
+        for (const Tensor& g : grads) check_no_tangent(g, "gradients");
+        if (!grads[0].defined() && !grads[1].defined() && !grads[2].defined()) return {Tensor()};
+        const Tensor z = logits.unpack(), t = labels.unpack(), n = has_lens ? lens.unpack() : Tensor(), best = top_labels.unpack(), k = kept.unpack();
+        const auto&  s = shape;
+        const auto   label_type = s.labels64 ? torch::kInt64 : torch::kInt32;
+        TORCH_CHECK(z.is_cuda() && z.scalar_type() == (s.dtype == FRAMEWISE_B200_F32 ? torch::kFloat32 : torch::kBFloat16) && z.numel() == s.B * s.T * s.V &&
+                        z.dim() == (flat ? 2 : 3) && z.size(-1) == s.V && (s.V == 1 || z.stride(-1) == 1) && t.device() == z.device() && t.is_contiguous() &&
+                        t.numel() == s.B * s.T && t.scalar_type() == label_type && best.device() == z.device() && best.is_contiguous() &&
+                        best.numel() == s.B * s.T * s.top && best.scalar_type() == label_type && k.device() == z.device() && k.is_contiguous() &&
+                        k.scalar_type() == torch::kUInt8 && k.numel() >= 16 * s.B * s.T &&
+                        (!has_lens || (n.device() == z.device() && n.is_contiguous() && n.numel() == s.B && n.scalar_type() == torch::kInt32)),
+                    "framewise: saved-tensor hooks must give back what they were given");
+        c10::cuda::CUDAGuard guard(z.device());
+        framewise_b200_scores_shape with = s;
+        with.logits_stride_b = flat ? 0 : z.stride(0), with.logits_stride_t = z.stride(-2);  // hooks may have laid them out anew
+        Tensor g[3];
+        for (int i = 0; i < 3; ++i) {
+            if (!grads[i].defined()) continue;
+            g[i] = plain(grads[i]);
+            if (g[i].scalar_type() != torch::kFloat32) g[i] = g[i].to(torch::kFloat32);
+        }
+        framewise_b200_scores_grads in = {};
+        auto strides = [&](const Tensor& x, int64_t& b, int64_t& t) { b = flat ? 0 : x.stride(0), t = x.stride(flat ? 0 : 1); };
+        if (g[0].defined()) in.log_probs = g[0].data_ptr<float>(), strides(g[0], in.log_probs_stride_b, in.log_probs_stride_t);
+        if (g[1].defined()) in.entropy = g[1].data_ptr<float>(), strides(g[1], in.entropy_stride_b, in.entropy_stride_t);
+        if (g[2].defined() && s.top > 0) {
+            in.top_log_probs = g[2].data_ptr<float>(), strides(g[2], in.top_stride_b, in.top_stride_t);
+            in.top_stride_k = g[2].stride(-1);
+        }
+        Tensor dz = torch::empty(z.sizes(), z.options().requires_grad(false).memory_format(torch::MemoryFormat::Contiguous));
+        check_status(framewise_b200_scores_backward(&with, z.data_ptr(), t.data_ptr(), n.defined() ? n.data_ptr<int32_t>() : nullptr, best.data_ptr(),
+                                                    k.data_ptr(), &in, dz.data_ptr(), stream_of()));
+        return {dz};
+    }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> label_scores(const Tensor& logits, const Tensor& labels, int64_t top, const OptTensor& seq_lens,
+                                                        int64_t ignore_index) {
+    dtype_of(logits, "logits");
+    check_no_tangent(logits, "logits");
+    c10::cuda::CUDAGuard guard(logits.device());
+    Tensors out;
+    if (!torch::GradMode::is_enabled() || !logits.requires_grad()) {
+        out = scores_forward(scores_inputs(logits, labels, top, seq_lens, ignore_index), labels, nullptr);
+        return {out[0], out[1], out[2], out[3]};
+    }
+    Tensor z, t, n, kept;
+    std::shared_ptr<LabelScoresBackward> node(new LabelScoresBackward(), torch::autograd::deleteNode);
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const ScoresInputs in = scores_inputs(logits, labels, top, seq_lens, ignore_index);
+        out = scores_forward(in, labels, &kept);
+        z = in.logits, t = in.at.labels, n = in.at.lens;
+        node->shape = in.shape, node->flat = labels.dim() == 1;
+    }
+    node->logits     = torch::autograd::SavedVariable(z, false);  // outside of the guard: hooks may run
+    node->labels     = torch::autograd::SavedVariable(t, false);
+    node->top_labels = torch::autograd::SavedVariable(out[3], false);
+    node->kept       = torch::autograd::SavedVariable(kept, false);
+    if ((node->has_lens = n.defined())) node->lens = torch::autograd::SavedVariable(n, false);
+    node->set_next_edges(torch::autograd::collect_next_edges(logits));
+    torch::autograd::set_history(torch::autograd::variable_list{out[0], out[1], out[2]}, node);
+    return {out[0], out[1], out[2], out[3]};
+}
+
+// ------------------------------------------------------------------------------------------ AdamW
 
 void check_state(const Tensor& x, const Tensor& p, torch::ScalarType dtype, const char* name) {
     TORCH_CHECK(x.device() == p.device() && x.scalar_type() == dtype && x.is_contiguous() && x.sizes() == p.sizes(), name,
@@ -369,6 +483,7 @@ std::pair<Tensors, Tensors> adamw_values(const Tensors& exp_avg, const Tensors& 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("linear_cross_entropy", &linear_cross_entropy);
     m.def("label_embedding", &label_embedding);
+    m.def("label_scores", &label_scores);
     m.def("adamw_step", &adamw_step);
     m.def("adamw_values", &adamw_values);
     m.attr("state_block") = FRAMEWISE_B200_STATE_BLOCK;

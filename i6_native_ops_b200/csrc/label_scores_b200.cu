@@ -1,0 +1,515 @@
+// label_scores_b200.cu -- what a program reads off distributions over the classes that are in memory, behind the C ABI of
+// include/framewise_b200.h: log probabilities of given labels, entropies, the best alternatives, and their gradient.
+//
+// With z a row of V logits, t its label, m = max z, s = sum 2^d, d = (z - m) log2 e:
+//     log p = ln 2 (d - log2 s);  entropy = ln 2 (log2 s - (sum 2^d d) / s)
+//     alternatives: the `top` largest of z, equal ones by their index
+//     dz = g (onehot(t) - p) - g_H p (log p + entropy) + sum_j g_j (onehot(top_j) - p)
+// The forward pass meets each logit once and keeps of a row its maximum, log2 s and entropy; the backward pass meets it once
+// more and writes the gradient.  (The maximum is kept apart from log2 s: their sum would round off what lies near one.)
+#include "framewise_b200.h"
+#include "framewise_host.h"
+#include "tensor_core.h"
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cfloat>
+
+namespace {
+
+using namespace framewise_host;
+using namespace tensor_core;
+
+constexpr int   kMostTop  = 32;      // alternatives: one per lane
+constexpr int   kWarps    = 8;       // per CTA
+constexpr int   kMostTeam = 64;      // warps that share a row: up to 8 CTAs
+constexpr int   kAhead    = 4;       // vectors of 8 logits that a lane has under way
+constexpr float kLog2e    = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kNever    = -200.f;  // of an exponent of 2: zero in 32 bits
+
+struct Rows {  // where the rows are and which count
+    int64_t        N;
+    int            T, V, top, team;  // team: warps per row, a power of two
+    int64_t        stride_b, stride_t;
+    const void*    labels;
+    const int32_t* lens;
+    int64_t        ignore;
+};
+
+template <typename L>
+__device__ __forceinline__ bool counted(const Rows& r, int64_t n, int64_t& label) {
+    label = static_cast<const L*>(r.labels)[n];
+    return (r.lens == nullptr || (int)((uint32_t)n % (uint32_t)r.T) < r.lens[(uint32_t)n / (uint32_t)r.T]) && label != r.ignore;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// 8 logits in a row, once (32 bytes aligned for f32, 16 for bf16)
+__device__ __forceinline__ void load8(const float* x, float (&v)[8]) {
+    asm volatile("ld.global.L1::no_allocate.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "l"(x));
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* x, float (&v)[8]) {
+    uint32_t w[4];
+    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(x));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+__device__ __forceinline__ float value(float x) { return x; }
+__device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// A row in vectors of 8 whose addresses are aligned: the first begins `ahead` places before the row.  Places outside of the
+// row are not read and hold -inf, which changes no sum.
+template <typename X>
+struct Row {
+    const X* x;
+    int      V, ahead, steps;  // steps: of 32 vectors
+    __device__ Row(const X* x, int V) : x(x), V(V) {
+        ahead = (int)(reinterpret_cast<uintptr_t>(x) / sizeof(X) % 8);
+        steps = ((V + ahead + 7) / 8 + 31) / 32;
+    }
+    __device__ int first(int step, int lane) const { return (step * 32 + lane) * 8 - ahead; }
+    __device__ void load(int at, float (&v)[8]) const {
+        if (at >= 0 && at + 8 <= V) {
+            load8(x + at, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = at + i >= 0 && at + i < V ? value(x[at + i]) : -INFINITY;
+        }
+    }
+};
+
+// Larger values have larger keys, equal ones those of the lower index; NaN is the largest value.  0: no value.
+__device__ __forceinline__ uint64_t key_of(float v, int index) {
+    const uint32_t u = __float_as_uint(v + 0.f);  // one zero
+    const uint32_t o = v != v ? 0xffffffffu : (u >> 31) ? ~u : u | 0x80000000u;
+    return (uint64_t)o << 32 | (uint32_t)~index;
+}
+__device__ __forceinline__ float value_of(uint64_t key) {
+    const uint32_t o = (uint32_t)(key >> 32);
+    return o == 0xffffffffu ? __uint_as_float(0x7fffffffu) : __uint_as_float((o >> 31) ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ int index_of(uint64_t key) { return (int)~(uint32_t)key; }
+
+__device__ __forceinline__ uint64_t keep(uint64_t a, uint64_t b, bool larger) { return (a > b) == larger ? a : b; }
+
+// Networks of Batcher's over the lanes: `key` in falling order; a falling `list` and the 32 largest of it and `more` (falling).
+__device__ __forceinline__ uint64_t sorted(uint64_t key, int lane) {
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+        for (int j = k >> 1; j > 0; j >>= 1)
+            key = keep(key, __shfl_xor_sync(0xffffffffu, key, j), ((lane & j) == 0) == ((lane & k) == 0));
+    return key;
+}
+__device__ __forceinline__ uint64_t joined(uint64_t list, uint64_t more, int lane) {
+    list = max(list, __shfl_sync(0xffffffffu, more, 31 - lane));
+#pragma unroll
+    for (int j = 16; j > 0; j >>= 1) list = keep(list, __shfl_xor_sync(0xffffffffu, list, j), (lane & j) == 0);
+    return list;
+}
+
+struct Sums {  // of a part of a row: maximum, sum of 2^d, sum of 2^d d
+    float m, s, t;
+};
+__device__ __forceinline__ void rescale(Sums& a, float m) {
+    const float d = max_nan((a.m - m) * kLog2e, kNever), c = exp2_approx(d);
+    a.t = c * (a.t + a.s * d);
+    a.s = c * a.s;
+    a.m = m;
+}
+__device__ __forceinline__ Sums joined(Sums a, Sums b) {
+    const float m = max_nan(a.m, b.m);
+    rescale(a, m), rescale(b, m);
+    return {m, a.s + b.s, a.t + b.t};
+}
+
+// The 32 largest that a warp has met, a lane each, and those that wait to be sorted in: more than 32 never wait, so that a
+// row in rising order costs a network per 32 of its values.
+struct Best {
+    uint64_t  list;
+    uint64_t* wait;  // of this warp, 64 of them
+    int       count, top;
+    float     least;  // the list's last that counts: only larger values come in
+    bool      full, sure;  // sure: nothing can come in any more (NaN throughout)
+    __device__ Best(uint64_t* wait, int top) : list(0), wait(wait), count(0), top(top), least(-INFINITY), full(false), sure(false) {}
+    __device__ void sort_in(int lane) {
+        __syncwarp();
+        const uint64_t key = lane < min(count, 32) ? wait[lane] : 0, rest = lane + 32 < count ? wait[lane + 32] : 0;
+        __syncwarp();
+        list = joined(list, sorted(key, lane), lane);
+        count = max(0, count - 32);
+        if (lane < count) wait[lane] = rest;
+        const uint64_t last = __shfl_sync(0xffffffffu, list, top - 1);
+        full  = last != 0;
+        sure  = (uint32_t)(last >> 32) == 0xffffffffu;
+        least = full ? value_of(last) : -INFINITY;
+        __syncwarp();
+    }
+    // 8 values a lane, the first of index `at`; `most`: their maximum.  What the list holds when a step begins has lower
+    // indices than the step's values: equal ones stay out.  Within the step they come in any order, and equal ones come in.
+    __device__ void meet(const float (&v)[8], float most, int at, int V, float from, int lane) {
+        const bool  before = full;
+        const float floor  = least;
+        if (before && sure) return;
+        if (!__any_sync(0xffffffffu, before ? !(most <= floor) : !(most < from))) return;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool in = at + i >= 0 && at + i < V && (before ? !(v[i] <= floor) : !(v[i] < from)) && !(v[i] < least);
+            const uint32_t lanes = __ballot_sync(0xffffffffu, in);
+            if (!lanes) continue;
+            if (in) wait[count + __popc(lanes & ((1u << lane) - 1))] = key_of(v[i], at + i);
+            count += __popc(lanes);
+            if (count >= 32) sort_in(lane);
+        }
+    }
+    __device__ void finish(int lane) {
+        while (count > 0) sort_in(lane);
+    }
+};
+
+// The `top`-th largest of the lanes' values: at least as many of a row's are no smaller.
+__device__ __forceinline__ float nth_of_lanes(float v, int top, int lane) {
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            const float o = __shfl_xor_sync(0xffffffffu, v, j);
+            v = ((lane & j) == 0) == ((lane & k) == 0) ? fmaxf(v, o) : fminf(v, o);
+        }
+    return __shfl_sync(0xffffffffu, v, top - 1);
+}
+
+struct Scored {
+    float*  log_prob;
+    float*  entropy;
+    float*  top_log_prob;
+    void*   top_label;
+    float4* kept;  // or null: maximum, log2 s, entropy
+};
+
+// A row per team of r.team warps (1 to 8 of a CTA; 16 to 64: all of 2 to 8 CTAs of a cluster), which take its steps of 256
+// logits in turn.
+template <typename X, typename L, bool TOP>
+__global__ void __launch_bounds__(kWarps * 32) k_label_scores(const X* __restrict__ z, const Rows r, const Scored out) {
+    __shared__ Sums     part[kWarps];
+    __shared__ uint64_t best[TOP ? kWarps : 1][32];
+    __shared__ uint64_t waiting[TOP ? kWarps : 1][64];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int ctas = r.team > kWarps ? r.team / kWarps : 1, in_cta_team = min(r.team, kWarps);
+    const int rank = ctas > 1 ? (int)(blockIdx.x % ctas) : 0;
+    const int64_t n = ctas > 1 ? (int64_t)(blockIdx.x / ctas) : (int64_t)blockIdx.x * (kWarps / r.team) + warp / r.team;
+    const int member = rank * kWarps + warp % in_cta_team;
+    int64_t label = 0;
+    const bool inside = n < r.N, counts = inside && counted<L>(r, n, label);
+    const X* const x = counts ? z + (int64_t)((uint32_t)n / (uint32_t)r.T) * r.stride_b + (int64_t)((uint32_t)n % (uint32_t)r.T) * r.stride_t : z;
+
+    Sums a = {-FLT_MAX, 0.f, 0.f};
+    Best b(TOP ? waiting[warp] : nullptr, r.top);
+    if (counts) {
+        const Row<X> row(x, r.V);
+        float from = -INFINITY;  // smaller values than this are not among the best
+        for (int step = member; step < row.steps; step += r.team * kAhead) {
+            float v[kAhead][8];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int s = step + i * r.team;
+                if (s < row.steps) {
+                    row.load(row.first(s, lane), v[i]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[i][j] = -INFINITY;
+                }
+            }
+            float most[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                most[i] = v[i][0];
+#pragma unroll
+                for (int j = 1; j < 8; ++j) most[i] = max_nan(most[i], v[i][j]);
+            }
+            float all = max_nan(max_nan(most[0], most[1]), max_nan(most[2], most[3]));
+            static_assert(kAhead == 4, "");
+            if constexpr (TOP) {
+                if (step == member) from = nth_of_lanes(all != all ? INFINITY : all, r.top, lane);
+                if (__any_sync(0xffffffffu, b.full ? !b.sure && !(all <= b.least) : !(all < from))) {
+#pragma unroll
+                    for (int i = 0; i < kAhead; ++i)
+                        if (step + i * r.team < row.steps) b.meet(v[i], most[i], row.first(step + i * r.team, lane), r.V, from, lane);
+                }
+            }
+            const float m = max_nan(a.m, all);
+            rescale(a, m);
+            const float2 off = make_float2(-m, -m), scale = make_float2(kLog2e, kLog2e);
+            float2 s = make_float2(0.f, 0.f), t = s;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    float2 d = mul2(add2(make_float2(v[i][j], v[i][j + 1]), off), scale);
+                    d = make_float2(max_nan(d.x, kNever), max_nan(d.y, kNever));
+                    const float2 e = make_float2(exp2_approx(d.x), exp2_approx(d.y));
+                    s = add2(s, e);
+                    t = add2(t, mul2(e, d));
+                }
+            a.s += s.x + s.y;
+            a.t += t.x + t.y;
+        }
+#pragma unroll
+        for (int j = 16; j > 0; j >>= 1) a = joined(a, {__shfl_xor_sync(0xffffffffu, a.m, j), __shfl_xor_sync(0xffffffffu, a.s, j), __shfl_xor_sync(0xffffffffu, a.t, j)});
+        if constexpr (TOP) b.finish(lane);
+    }
+    // the team's parts, pairs of warps at a time
+    if (r.team > 1) {
+        if (lane == 0) part[warp] = a;
+        if (TOP) best[warp][lane] = b.list;
+        for (int j = 1; j < in_cta_team; j <<= 1) {
+            __syncthreads();
+            if ((warp & (2 * j - 1)) == 0) {
+                a = joined(a, part[warp + j]);
+                if (lane == 0) part[warp] = a;
+                if constexpr (TOP) {
+                    b.list = joined(b.list, best[warp + j][lane], lane);
+                    best[warp][lane] = b.list;
+                }
+            }
+        }
+        if (ctas > 1) {
+            cluster_sync();
+            if (rank == 0 && warp == 0) {
+                for (int j = 1; j < ctas; ++j) {
+                    const uint32_t from = in_cta(smem_addr(&part[0]), j);
+                    Sums o;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.m) : "r"(from) : "memory");
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.s) : "r"(from + 4) : "memory");
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.t) : "r"(from + 8) : "memory");
+                    a = joined(a, o);
+                    if constexpr (TOP) {
+                        uint64_t key;
+                        asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(key) : "r"(in_cta(smem_addr(&best[0][lane]), j)) : "memory");
+                        b.list = joined(b.list, key, lane);
+                    }
+                }
+            }
+            cluster_sync();  // what is read from a CTA is there until it has been
+        }
+    }
+    if (member != 0 || !inside) return;
+    // a row without a class that is possible has log probabilities of -inf and no entropy
+    const float log2_s = log2f(a.s), entropy = a.s == 0.f ? 0.f : kLn2 * (log2_s - a.t / a.s);
+    auto log_prob = [&](float v) { return a.s == 0.f ? -INFINITY : (v - a.m) - kLn2 * log2_s; };
+    if (lane == 0) {
+        out.log_prob[n] = !counts ? 0.f : label < 0 || label >= r.V ? __uint_as_float(0x7fffffffu) : log_prob(value(x[label]));
+        out.entropy[n]  = counts ? entropy : 0.f;
+        if (out.kept) out.kept[n] = make_float4(a.m, log2_s, entropy, 0.f);
+    }
+    if (TOP && lane < r.top) {
+        out.top_log_prob[n * r.top + lane] = counts ? log_prob(value_of(b.list)) : 0.f;
+        static_cast<L*>(out.top_label)[n * r.top + lane] = counts ? (L)index_of(b.list) : (L)r.ignore;
+    }
+}
+
+struct Incoming {  // strides in elements; null: none
+    const float *log_prob, *entropy, *top;
+    int64_t log_prob_b, log_prob_t, entropy_b, entropy_t, top_b, top_t, top_k;
+    const void*   top_label;
+    const float4* kept;
+};
+
+__device__ __forceinline__ void store8(float* to, const float (&v)[8]) {
+    asm volatile("st.global.L1::no_allocate.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
+                 "f"(v[5]), "f"(v[6]), "f"(v[7])
+                 : "memory");
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* to, const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
+    asm volatile("st.global.L1::no_allocate.v4.b32 [%0], {%1,%2,%3,%4};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+__device__ __forceinline__ void put(float* to, float v) { *to = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* to, float v) { *to = __float2bfloat16_rn(v); }
+
+// The gradient: a row per team as above, in steps that are aligned where it is written (`even`: and where it is read).
+template <typename X, typename L>
+__global__ void __launch_bounds__(kWarps * 32) k_label_scores_back(const X* __restrict__ z, const Rows r, const Incoming in, X* __restrict__ dz) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t all = (int64_t)blockIdx.x * kWarps + warp, n = all / r.team;
+    const int member = (int)(all % r.team);
+    if (n >= r.N) return;
+    const int64_t seq = (uint32_t)n / (uint32_t)r.T, at_t = (uint32_t)n % (uint32_t)r.T;
+    X* const to = dz + n * r.V;
+    const Row<X> row(to, r.V);
+    int64_t label = 0;
+    const bool   counts = counted<L>(r, n, label);
+    const float4 kept   = counts ? in.kept[n] : make_float4(0.f, -INFINITY, 0.f, 0.f);
+    float g_top = 0.f;  // of this lane's alternative
+    int   alternative = -1;
+    if (counts && in.top && lane < r.top) {
+        g_top = in.top[seq * in.top_b + at_t * in.top_t + lane * in.top_k];
+        alternative = (int)static_cast<const L*>(in.top_label)[n * r.top + lane];
+    }
+    const float g = counts && in.log_prob ? in.log_prob[seq * in.log_prob_b + at_t * in.log_prob_t] : 0.f;
+    const float h = counts && in.entropy ? in.entropy[seq * in.entropy_b + at_t * in.entropy_t] : 0.f;
+    float total = g_top;
+#pragma unroll
+    for (int j = 16; j > 0; j >>= 1) total += __shfl_xor_sync(0xffffffffu, total, j);
+    total += g;
+    // a value's gradient is p (c0 + c1 log2 p)
+    float c0 = -total - h * kept.z;
+    const float c1 = -h * kLn2;
+    if (counts && in.log_prob && (label < 0 || label >= r.V)) c0 = __uint_as_float(0x7fffffffu);
+    if (kept.y == -INFINITY) {  // does not count, or no class is possible
+        const float none = c0 != c0 ? c0 : 0.f;
+        const float v[8] = {none, none, none, none, none, none, none, none};
+        for (int step = member; step < row.steps; step += r.team) {
+            const int at = row.first(step, lane);
+            if (at >= 0 && at + 8 <= r.V) {
+                store8(to + at, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (at + i >= 0 && at + i < r.V) put(to + at + i, none);
+            }
+        }
+        return;
+    }
+    const X* const x = z + seq * r.stride_b + at_t * r.stride_t;
+    const bool even = (reinterpret_cast<uintptr_t>(x) / sizeof(X)) % 8 == row.ahead;
+    const Row<X> from(x, r.V);
+    auto gradient = [&](float v) {
+        const float l = max_nan((v - kept.x) * kLog2e - kept.y, kNever);  // log2 p
+        return exp2_approx(l) * (c0 + c1 * l);
+    };
+    for (int step = member; step < row.steps; step += r.team * kAhead) {
+        float v[kAhead][8];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int s = step + i * r.team, at = row.first(s, lane);
+            if (s >= row.steps) continue;
+            if (even) {
+                from.load(at, v[i]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] = at + j >= 0 && at + j < r.V ? value(x[at + j]) : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int s = step + i * r.team, at = row.first(s, lane);
+            if (s >= row.steps) continue;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = gradient(v[i][j]);
+            if (at >= 0 && at + 8 <= r.V) {
+                store8(to + at, v[i]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (at + j >= 0 && at + j < r.V) put(to + at + j, v[i][j]);
+            }
+        }
+    }
+    // The label and the alternatives: by the warp that wrote their places.
+    __syncwarp();
+    auto mine = [&](int index) { return (index + row.ahead) / 256 % r.team == member; };
+    const bool listed = __any_sync(0xffffffffu, alternative >= 0 && alternative == label);
+    if (alternative >= 0 && mine(alternative)) put(to + alternative, gradient(value(x[alternative])) + g_top + (alternative == label ? g : 0.f));
+    if (lane == 0 && !listed && label >= 0 && label < r.V && mine((int)label)) put(to + label, gradient(value(x[label])) + g);
+}
+
+// Warps per row: enough to fill the SMs, a step each at least.  (See the launches' comment for what was measured.)
+int team_of(int64_t N, int64_t V, int most) {
+    const int64_t want = (int64_t)sm_count() * 16;
+    int team = 1;
+    while (team < most && N * team < want && team * 256 < V) team *= 2;
+    return team;
+}
+
+bool sizes_ok(const framewise_b200_scores_shape* s) {
+    const int64_t kMost = (int64_t)1 << 31;
+    return s && s->B >= 0 && s->T >= 0 && s->V >= 1 && s->B < kMost && s->T < kMost && s->B * s->T < kMost && s->V < kMost / 16 && s->top >= 0 &&
+           s->top <= kMostTop && s->top <= s->V && (s->dtype == FRAMEWISE_B200_F32 || s->dtype == FRAMEWISE_B200_BF16);
+}
+
+Rows rows_of(const framewise_b200_scores_shape& s, const void* labels, const int32_t* lens, int most_team) {
+    Rows r = {};
+    r.N = s.B * s.T, r.T = (int)s.T, r.V = (int)s.V, r.top = s.top, r.team = team_of(r.N, s.V, most_team);
+    r.stride_b = s.logits_stride_b, r.stride_t = s.logits_stride_t;
+    r.labels = labels, r.lens = lens, r.ignore = s.ignore_index;
+    return r;
+}
+
+template <typename X, typename L, bool TOP>
+int forward(const Rows& r, const X* z, const Scored& out, cudaStream_t stream) {
+    const int ctas = r.team > kWarps ? r.team / kWarps : 1;
+    const int64_t grid = ctas > 1 ? r.N * ctas : (r.N + kWarps / r.team - 1) / (kWarps / r.team);
+    cudaLaunchConfig_t c = {};
+    c.gridDim  = dim3((unsigned)grid);
+    c.blockDim = dim3(kWarps * 32);
+    c.stream   = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = ctas, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    c.attrs    = at;
+    c.numAttrs = ctas > 1 ? 1 : 0;
+    FW_TRY(cudaLaunchKernelEx(&c, k_label_scores<X, L, TOP>, z, r, out));
+    FW_LAUNCHED();
+    return FRAMEWISE_B200_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int framewise_b200_scores_forward(const framewise_b200_scores_shape* shape, const void* logits, const void* labels, const int32_t* seq_lens,
+                                  float* log_probs, float* entropy, float* top_log_probs, void* top_labels, void* kept,
+                                  framewise_b200_stream_t stream) {
+    if (!sizes_ok(shape)) return FRAMEWISE_B200_BAD_ARGUMENT;
+    if (shape->B * shape->T == 0) return FRAMEWISE_B200_OK;
+    if (!logits || !labels || !log_probs || !entropy || (shape->top > 0 && (!top_log_probs || !top_labels)) || reinterpret_cast<uintptr_t>(kept) % 16 != 0)
+        return FRAMEWISE_B200_BAD_ARGUMENT;
+    const Rows   r   = rows_of(*shape, labels, seq_lens, kMostTeam);
+    const Scored out = {log_probs, entropy, top_log_probs, top_labels, static_cast<float4*>(kept)};
+    auto go = [&](auto x, auto l) {
+        using X = decltype(x);
+        using L = decltype(l);
+        return shape->top > 0 ? forward<X, L, true>(r, (const X*)logits, out, stream) : forward<X, L, false>(r, (const X*)logits, out, stream);
+    };
+    if (shape->dtype == FRAMEWISE_B200_F32) return shape->labels64 ? go(float(), int64_t()) : go(float(), int32_t());
+    return shape->labels64 ? go(__nv_bfloat16(), int64_t()) : go(__nv_bfloat16(), int32_t());
+}
+
+int framewise_b200_scores_backward(const framewise_b200_scores_shape* shape, const void* logits, const void* labels, const int32_t* seq_lens,
+                                   const void* top_labels, const void* kept, const framewise_b200_scores_grads* grads, void* grad_logits,
+                                   framewise_b200_stream_t stream) {
+    if (!sizes_ok(shape)) return FRAMEWISE_B200_BAD_ARGUMENT;
+    if (shape->B * shape->T == 0) return FRAMEWISE_B200_OK;
+    if (!logits || !labels || !kept || !grads || !grad_logits || reinterpret_cast<uintptr_t>(kept) % 16 != 0 ||
+        (grads->top_log_probs && shape->top > 0 && !top_labels))
+        return FRAMEWISE_B200_BAD_ARGUMENT;
+    const Rows r = rows_of(*shape, labels, seq_lens, 1 << 16);
+    Incoming   in = {};
+    in.log_prob = grads->log_probs, in.log_prob_b = grads->log_probs_stride_b, in.log_prob_t = grads->log_probs_stride_t;
+    in.entropy = grads->entropy, in.entropy_b = grads->entropy_stride_b, in.entropy_t = grads->entropy_stride_t;
+    in.top = shape->top > 0 ? grads->top_log_probs : nullptr, in.top_b = grads->top_stride_b, in.top_t = grads->top_stride_t, in.top_k = grads->top_stride_k;
+    in.top_label = top_labels, in.kept = static_cast<const float4*>(kept);
+    const unsigned grid = (unsigned)((r.N * r.team + kWarps - 1) / kWarps);
+    auto go = [&](auto x, auto l) -> int {
+        using X = decltype(x);
+        using L = decltype(l);
+        k_label_scores_back<X, L><<<grid, kWarps * 32, 0, stream>>>((const X*)logits, r, in, (X*)grad_logits);
+        FW_LAUNCHED();
+        return FRAMEWISE_B200_OK;
+    };
+    if (shape->dtype == FRAMEWISE_B200_F32) return shape->labels64 ? go(float(), int64_t()) : go(float(), int32_t());
+    return shape->labels64 ? go(__nv_bfloat16(), int64_t()) : go(__nv_bfloat16(), int32_t());
+}
+
+}  // extern "C"

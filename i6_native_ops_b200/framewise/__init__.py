@@ -5,6 +5,7 @@ them with an output layer over thousands of classes, an embedding of label conte
 
   :func:`linear_cross_entropy`  output layer and softmax cross entropy in one, without logits in memory
   :func:`label_embedding`       scaled embedding of labels (and its gradient)
+  :func:`label_scores`          log probabilities of given labels, entropies and the best classes, off logits in memory
   :class:`AdamW`                AdamW over all parameters at once, states in 32 or 8 bits; :func:`adamw_step`,
                                 :func:`adamw_values`, the step itself and what 8-bit states stand for
 
@@ -17,7 +18,7 @@ from __future__ import annotations
 import ctypes
 import importlib.util
 import os
-from typing import List, Optional, Sequence, Tuple, Union
+from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -103,6 +104,43 @@ def label_embedding(
         in 32 bits, in a fixed order (equal calls give equal bits).  A label outside 0..V-1 at a position that counts
         gives NaN, in its row and in the whole gradient."""
     return core.label_embedding(labels, weight, float(scale), _lengths(seq_lens, labels), int(ignore_index))
+
+
+class LabelScores(NamedTuple):
+    """What :func:`label_scores` returns."""
+
+    log_probs: torch.Tensor
+    entropy: torch.Tensor
+    top_log_probs: torch.Tensor
+    top_labels: torch.Tensor
+
+
+def label_scores(
+    logits: torch.Tensor,
+    labels: torch.Tensor,
+    top: int = 0,
+    seq_lens: Optional[torch.Tensor] = None,
+    ignore_index: int = -100,
+) -> LabelScores:
+    """Log probabilities of given labels under ``softmax(logits)``, its entropy and its best classes, position by
+    position.
+
+    :param logits: (B, T, V) or (N, V) float32 or bfloat16 (CUDA), such as the ``log_probs`` that ``fbw_loss`` and
+        ``align_viterbi`` take; any strides, read in place where the last dimension is dense.  A class of -inf has
+        probability 0.
+    :param labels: (B, T) or (N,) int32 or int64, such as an alignment
+    :param top: how many of the best classes are returned, at most 32
+    :param seq_lens: (B,) int32 lengths, or a (T, B) index mask
+    :param ignore_index: labels of positions that are left out
+    :return: ``log_probs`` and ``entropy``, float32 in the shape of ``labels``; ``top_log_probs`` and ``top_labels``, (..., top):
+        the largest logits in falling order, equal ones by their class (NaN is the largest), labels in the dtype of
+        ``labels``.  Positions past their length or left out have 0 and the ignored label, and their logits are never read.
+
+    A position whose logits are all -inf has log probabilities of -inf, entropy 0 and a gradient of 0; one with NaN or +inf
+    has NaN.  A label outside 0..V-1 at a position that counts gives NaN, there and in that position's gradient.
+    Everything is formed in 32 bits.  ``logits`` get gradients from the three float results, each position's in one pass,
+    rounded once; they must not change before the backward pass.  Derivatives are of the first order, by backward passes."""
+    return LabelScores(*core.label_scores(logits, labels, int(top), _lengths(seq_lens, labels), int(ignore_index)))
 
 
 State = Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]
@@ -240,4 +278,4 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
 
-__all__ = ["core", "linear_cross_entropy", "label_embedding", "adamw_step", "adamw_values", "AdamW"]
+__all__ = ["core", "linear_cross_entropy", "label_embedding", "LabelScores", "label_scores", "adamw_step", "adamw_values", "AdamW"]

@@ -135,6 +135,43 @@ int framewise_b200_adamw_follow(const framewise_b200_tensor* tensors, int64_t co
  * (the second moment itself, not its root); other fields are ignored. */
 int framewise_b200_adamw_decode(const framewise_b200_tensor* tensors, int64_t count, framewise_b200_stream_t stream);
 
+/* Sizes and types of one call on distributions over V classes that are in memory.  B*T below 2^31, V below 2^27. */
+typedef struct {
+    int64_t B, T, V;
+    int64_t logits_stride_b, logits_stride_t; /* in elements; the last dimension of `logits` is dense */
+    int64_t ignore_index;
+    int32_t dtype;    /* of logits and their gradient          */
+    int32_t labels64; /* labels and top_labels are int64 (else int32) */
+    int32_t top;      /* alternatives: 0 .. min(V, 32)         */
+} framewise_b200_scores_shape;
+
+/* For z = logits[b,t,:] and log p = z - log sum_v exp z[v]:
+ *     log_probs[b,t] = log p[label];  entropy[b,t] = - sum_v p log p  (classes of z = -inf add nothing);
+ *     top_labels[b,t,:], top_log_probs[b,t,:]: the `top` largest of z in falling order, equal ones by their index (NaN is
+ *     the largest), and their log p.
+ * Positions that do not count: 0, and `ignore_index` as labels.  A row of -inf alone: log probabilities -inf, entropy 0.
+ * A row with NaN or +inf: NaN.  logits (B,T,V), labels (B,T) dense, outputs dense, f32.  `kept`: 16 B T bytes, 16-byte
+ * aligned, for the backward pass, or NULL. */
+int framewise_b200_scores_forward(const framewise_b200_scores_shape* shape, const void* logits, const void* labels,
+                                  const int32_t* seq_lens, float* log_probs, float* entropy, float* top_log_probs,
+                                  void* top_labels, void* kept, framewise_b200_stream_t stream);
+
+/* Incoming gradients, f32, with strides in elements (0 allowed); NULL: none. */
+typedef struct {
+    const float* log_probs;
+    const float* entropy;
+    const float* top_log_probs;
+    int64_t log_probs_stride_b, log_probs_stride_t, entropy_stride_b, entropy_stride_t;
+    int64_t top_stride_b, top_stride_t, top_stride_k;
+} framewise_b200_scores_grads;
+
+/* grad_logits (B,T,V) dense: g (onehot(label) - p) - g_H p (log p + entropy) + sum_j g_j (onehot(top_labels[j]) - p), in 32
+ * bits, rounded once; zeros at positions that do not count and in rows of -inf alone. */
+int framewise_b200_scores_backward(const framewise_b200_scores_shape* shape, const void* logits, const void* labels,
+                                   const int32_t* seq_lens, const void* top_labels, const void* kept,
+                                   const framewise_b200_scores_grads* grads, void* grad_logits,
+                                   framewise_b200_stream_t stream);
+
 /* Number of kernels of this library launched by this process so far. */
 int64_t framewise_b200_launch_count(void);
 
