@@ -29,6 +29,7 @@ VIT_EXT = os.path.join(VIT_DIR, "fast_viterbi_core.so")
 FW_SOURCES = {
     "framewise_b200.cu": ("linear_ce_b200.inc", "embedding_b200.inc", "adamw_b200.inc"),
     "label_scores_b200.cu": (),
+    "muon_b200.cu": (),
 }
 FW_HEADERS = ("framewise_host.h", "tensor_core.h")
 FW_OBJECTS = os.path.join(PKG, "framewise", "_build", "objects")

@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 
 #include <algorithm>
+#include <cmath>
 #include <memory>
 #include <string>
 #include <tuple>
@@ -478,6 +479,78 @@ std::pair<Tensors, Tensors> adamw_values(const Tensors& exp_avg, const Tensors& 
     return {m, v};
 }
 
+// ------------------------------------------------------------------------------------------ Muon
+
+// coefficients: three per step
+void check_coefficients(const std::vector<double>& coefficients) {
+    TORCH_CHECK(!coefficients.empty() && coefficients.size() % 3 == 0 && coefficients.size() <= 300, "steps must be in 1..100, of three coefficients each");
+    for (double c : coefficients) TORCH_CHECK(std::isfinite(c), "coefficients must be finite");
+}
+
+void check_muon_status(int status, const char* sizes) {
+    TORCH_CHECK(status != FRAMEWISE_B200_BAD_ARGUMENT, "coefficients must keep singular values below 10^6, and ", sizes);
+    check_status(status);
+}
+
+Tensor orthogonalize(const Tensor& x_in, const std::vector<double>& coefficients, double eps) {
+    const int dtype = dtype_of(x_in, "x");
+    check_no_tangent(x_in, "x");
+    TORCH_CHECK(!torch::GradMode::is_enabled() || !x_in.requires_grad(), "framewise: orthogonalize has no gradient: detach x");
+    TORCH_CHECK(x_in.dim() >= 2, "x must have shape (..., rows, cols)");
+    TORCH_CHECK(eps >= 1e-37, "eps must be positive");
+    check_coefficients(coefficients);
+    c10::cuda::CUDAGuard guard(x_in.device());
+    const Tensor  x = plain(x_in).contiguous();
+    Tensor        out = torch::empty(x.sizes(), x.options().requires_grad(false).memory_format(torch::MemoryFormat::Contiguous));
+    const int64_t rows = x.size(-2), cols = x.size(-1), count = x.numel() > 0 ? x.numel() / (rows * cols) : 0;
+    const size_t  need = framewise_b200_orthogonalize_bytes(count, rows, cols, dtype);
+    TORCH_CHECK(need > 0, "x is too large");
+    Tensor work = bytes(need, x);
+    check_muon_status(framewise_b200_orthogonalize(count, rows, cols, dtype, x.data_ptr(), out.data_ptr(), coefficients.data(),
+                                                   (int32_t)(coefficients.size() / 3), eps, work.data_ptr(), need, stream_of()),
+                      "x must not be too large");
+    return out;
+}
+
+// master: empty, or one per parameter; follow: the copies take over what has been changed in the parameters.
+void muon_step(const Tensors& params, const Tensors& grads, const Tensors& momentum, const Tensors& master, double lr, double beta, bool nesterov,
+               double weight_decay, bool match_rms, const std::vector<double>& coefficients, double eps, bool follow) {
+    const size_t n = params.size();
+    TORCH_CHECK(grads.size() == n && momentum.size() == n && (master.empty() || master.size() == n), "Muon: the lists must have one entry per parameter");
+    TORCH_CHECK(lr >= 0 && weight_decay >= 0 && beta >= 0 && beta < 1 && eps >= 1e-37,
+                "Muon: lr and weight_decay must not be negative, beta must be in [0, 1), eps positive");
+    check_coefficients(coefficients);
+    if (n == 0) return;
+    const int dtype = dtype_of(params[0], "parameters");
+    TORCH_CHECK(master.empty() || dtype != FRAMEWISE_B200_F32, "Muon: float32 parameters need no copies");
+    c10::cuda::CUDAGuard guard(params[0].device());
+    Tensors kept;  // gradients that had to be copied
+    std::vector<framewise_b200_matrix> list(n);
+    for (size_t i = 0; i < n; ++i) {
+        const Tensor& p = params[i];
+        TORCH_CHECK(p.device() == params[0].device() && p.scalar_type() == params[0].scalar_type(), "Muon: parameters of one call must share device and dtype");
+        TORCH_CHECK(p.dim() == 2, "Muon: parameters must be matrices");
+        TORCH_CHECK(p.is_contiguous() && !p.is_neg(), "Muon: parameters must be contiguous");
+        TORCH_CHECK(grads[i].layout() == torch::kStrided && grads[i].device() == p.device() && grads[i].scalar_type() == p.scalar_type() && grads[i].sizes() == p.sizes(),
+                    "Muon: a gradient must be dense, with the shape, device and dtype of its parameter");
+        Tensor g = grads[i];
+        if (!g.is_contiguous() || g.is_neg()) {
+            g = plain(g).contiguous();
+            kept.push_back(g);
+        }
+        check_state(momentum[i], p, torch::kFloat32, "momentum");
+        if (!master.empty()) check_state(master[i], p, torch::kFloat32, "master");
+        list[i] = {p.data_ptr(), g.data_ptr(), momentum[i].data_ptr<float>(), master.empty() ? nullptr : master[i].data_ptr<float>(), p.size(0), p.size(1)};
+    }
+    const size_t need = framewise_b200_muon_bytes(list.data(), (int64_t)n, dtype);
+    TORCH_CHECK(need > 0, "Muon: a parameter is too large");
+    Tensor work = bytes(need, params[0]);
+    check_muon_status(framewise_b200_muon(list.data(), (int64_t)n, dtype, lr, beta, nesterov, weight_decay, match_rms, coefficients.data(),
+                                          (int32_t)(coefficients.size() / 3), eps, follow, work.data_ptr(), need, stream_of()),
+                      "parameters must not be too large");
+    for (const Tensors* const x : {&params, &master, &momentum}) written(*x);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -486,6 +559,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("label_scores", &label_scores);
     m.def("adamw_step", &adamw_step);
     m.def("adamw_values", &adamw_values);
+    m.def("orthogonalize", &orthogonalize);
+    m.def("muon_step", &muon_step);
     m.attr("state_block") = FRAMEWISE_B200_STATE_BLOCK;
     m.def("launch_count", []() { return framewise_b200_launch_count(); });
 }

@@ -1,0 +1,789 @@
+// muon_b200.cu -- orthogonalisation of matrices by Newton-Schulz products and the Muon step that uses it, behind the C ABI
+// of include/framewise_b200.h.
+//
+// With U (m,n), m <= n (the others lie transposed), X = U / max(|U|, eps) and per step, for coefficients a, b, c:
+//     A = X X^T;   B = b A + c A A;   X = a X + B X
+// which makes of each singular value s the value s (a + b s^2 + c s^4): after some steps they are all near one.
+// Per step 2 m n m + 2 m m m + 2 m m n operations, of which half of the first two are not needed, for A and B are symmetric.
+//
+// X is held in 32 bits; the products' operands are rounded from it to fp16: one part (11 bits) for bf16 matrices, two parts
+// (22 bits, three products) for f32 ones.  a X is added in 32 bits, outside of the products: small singular values are those that
+// grow, by a factor of a step, and an error that a product made of X would grow with them.  What B's and A's roundings do is
+// a change of the factor B, small for small singular values, and does not grow.  fp16 rather than bf16: as fast, eight times
+// finer, and all operands are bounded, so that powers of two (from the coefficients, for any matrix) keep them in its range.
+#include "framewise_b200.h"
+#include "framewise_host.h"
+#include "tensor_core.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+#include <vector>
+
+namespace {
+
+using namespace framewise_host;
+using namespace tensor_core;
+
+constexpr int kMostMatrices = 256;   // of a chain of launches
+constexpr int kSlots        = 24;    // matrices in a launch's arguments
+constexpr int kChunk        = 16384; // values per CTA of the pass over gradients
+constexpr int kRowsPerCta   = 128;   // of a tile: the lanes of tensor memory
+constexpr int kWide         = 256;   // columns of a tile at most: two accumulators fill tensor memory
+constexpr int kDepth        = 64;    // K per stage
+constexpr int kSegment      = 4;     // f32: stages after which an accumulator is added up in registers, for tensor cores cut
+                                     // off what they add, at 2^-24 of the sum a step, and never round it up
+constexpr int kMostStages   = 8;
+constexpr int kEpilogue     = 8;     // warps that finish tiles
+constexpr int kThreads      = 64 + 32 * kEpilogue;
+constexpr int kShared       = 232448 - 2048;  // dynamic; the rest: the static arrays
+constexpr uint64_t kPatience = 4000000000ull;  // nanoseconds after which a wait gives up; they end within microseconds
+
+// A matrix of a chain.  Its parts of the workspace are in panels of 64 columns, in which the rows follow each other: a row of
+// fp16 is 128 bytes there, a tensor copy's line.
+struct Entry {
+    const void* grad;
+    float*      momentum;   // or null: grad is what is made orthogonal
+    void*       param;      // or the result
+    float*      master;     // or null
+    double*     partial;    // sums of squares of the chunks
+    float*      x[2];       // X, before and after a step
+    int64_t     operand[2]; // its fp16 parts, as rows of 128 bytes of the workspace
+    int64_t     gram, factor; // A and B, likewise
+    int         rows, cols; // of the parameter
+    int         m, n, mp, panels;  // m <= n; rows of a panel (multiple of 128), panels of X
+    int         chunks, first_chunk, first_block, first_sym, first_apply;  // where its work begins in each launch
+    float       rate;
+};
+
+struct Slots {
+    int   count, base;
+    Entry* table;
+    Entry entry[kSlots];
+};
+
+// Which matrix a unit of work belongs to: the last whose first is not past it.
+template <typename F>
+__device__ __forceinline__ int find(int count, int unit, F&& first) {
+    int lo = 0, hi = count;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (first(mid) <= unit) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ float value(float x) { return x; }
+__device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void put(float* to, float v) { *to = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* to, float v) { *to = __float2bfloat16_rn(v); }
+
+struct Rates {
+    float keep, beta, nesterov;  // 1 - beta; nesterov: 0 or 1
+    float eps, decay;            // decay: 1 - lr weight_decay
+    int   follow;
+};
+
+// what is made orthogonal, from the gradient and the new momentum
+__device__ __forceinline__ float direction(float g, float v, const Rates& r) { return r.nesterov != 0.f ? g + (v - g) * r.beta : v; }
+
+// Momentum, and the sum of squares of each chunk in 64 bits (so that no square leaves the range); writes the table down.
+template <typename X>
+__global__ void __launch_bounds__(256) k_muon_collect(const __grid_constant__ Slots s, const Rates r) {
+    const int  e = find(s.count, blockIdx.x + s.entry[0].first_chunk, [&](int i) { return s.entry[i].first_chunk; });
+    const Entry& m = s.entry[e];
+    const int  chunk = blockIdx.x + s.entry[0].first_chunk - m.first_chunk;
+    if (chunk == 0) {
+        const int* from = reinterpret_cast<const int*>(&m);
+        int*       to   = reinterpret_cast<int*>(s.table + s.base + e);
+        for (int i = threadIdx.x; i < (int)(sizeof(Entry) / 4); i += 256) to[i] = from[i];
+    }
+    const int64_t all = (int64_t)m.rows * m.cols, begin = (int64_t)chunk * kChunk, end = min(all, begin + kChunk);
+    const X* const g = static_cast<const X*>(m.grad);
+    double sum = 0.0;
+    for (int64_t i = begin + threadIdx.x; i < end; i += 256) {
+        float u = value(g[i]);
+        if (m.momentum) {
+            const float v0 = m.momentum[i], v = v0 + (u - v0) * r.keep;
+            m.momentum[i] = v;
+            u = direction(u, v, r);
+        }
+        sum += (double)u * (double)u;
+    }
+#pragma unroll
+    for (int j = 16; j > 0; j >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, j);
+    __shared__ double part[8];
+    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 8; ++i) sum += part[i];
+        m.partial[chunk] = sum;
+    }
+}
+
+// fp16 parts of a value that has been brought into range
+template <int PARTS>
+__device__ __forceinline__ void split(float v, __half (&h)[PARTS]) {
+    h[0] = __float2half_rn(v);
+    if (PARTS == 2) h[PARTS - 1] = __float2half_rn(v - __half2float(h[0]));
+}
+
+// X = U / max(|U|, eps) in 32 bits and as operands: a CTA per 64 columns and rows, zeros where there are none.
+template <typename X, int PARTS>
+__global__ void __launch_bounds__(256) k_muon_begin(const Entry* __restrict__ table, int count, const Rates r, float scale, __half* work) {
+    __shared__ double part[8];
+    __shared__ float  tile[64][65];
+    const int   e = find(count, blockIdx.x, [&](int i) { return table[i].first_block; });
+    const Entry& m = table[e];
+    const int block = blockIdx.x - m.first_block, panel = block / (m.mp / 64), row0 = block % (m.mp / 64) * 64;
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < m.chunks; i += 256) sum += m.partial[i];
+#pragma unroll
+    for (int j = 16; j > 0; j >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, j);
+    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = sum;
+    const X* const g = static_cast<const X*>(m.grad);
+    const bool tall = m.rows > m.cols;
+    for (int i = threadIdx.x; i < 4096; i += 256) {  // neighbours in memory first
+        const int c = i % 64, l = i / 64;
+        const int row = row0 + (tall ? c : l), col = panel * 64 + (tall ? l : c);
+        float u = 0.f;
+        if (row < m.m && col < m.n) {
+            const int64_t at = tall ? (int64_t)col * m.cols + row : (int64_t)row * m.cols + col;
+            u = value(g[at]);
+            if (m.momentum) u = direction(u, m.momentum[at], r);
+        }
+        if (tall) tile[c][l] = u;
+        else tile[l][c] = u;
+    }
+    __syncthreads();
+    sum = part[0];
+    for (int i = 1; i < 8; ++i) sum += part[i];
+    // |U| may be past the range of 32 bits (or below): 64 bits up to the quotient
+    const double by = 1.0 / fmax(sqrt(sum), (double)r.eps);
+    const bool   far = !(by < 1e30);
+    const float  by32 = (float)by;
+    const int64_t at0 = ((int64_t)panel * m.mp + row0) * 64, plane = (int64_t)m.panels * m.mp * 64;
+    __half* const op = work + m.operand[0] * 64;
+    for (int i = threadIdx.x; i < 4096; i += 256) {
+        const float u = tile[i / 64][i % 64], x = far ? (float)(u * by) : u * by32;
+        m.x[0][at0 + i] = x;
+        __half h[PARTS];
+        split<PARTS>(x * scale, h);
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) op[p * plane + at0 + i] = h[p];
+    }
+}
+
+// p = p decay - rate X, or the result X itself: a CTA per 64 columns and rows of X.
+template <typename X>
+__global__ void __launch_bounds__(256) k_muon_finish(const Entry* __restrict__ table, int count, const Rates r, int last, const int* failed) {
+    __shared__ float tile[64][65];
+    const int   e = find(count, blockIdx.x, [&](int i) { return table[i].first_block; });
+    const Entry& m = table[e];
+    const int block = blockIdx.x - m.first_block, panel = block / (m.mp / 64), row0 = block % (m.mp / 64) * 64;
+    const float* const x = m.x[last] + ((int64_t)panel * m.mp + row0) * 64;
+    const bool none = *failed != 0;
+    for (int i = threadIdx.x; i < 4096; i += 256) tile[i / 64][i % 64] = none ? __uint_as_float(0x7fffffffu) : x[i];
+    __syncthreads();
+    const bool tall = m.rows > m.cols;
+    X* const p = static_cast<X*>(m.param);
+    for (int i = threadIdx.x; i < 4096; i += 256) {
+        const int c = i % 64, l = i / 64;
+        const int row = row0 + (tall ? c : l), col = panel * 64 + (tall ? l : c);
+        if (row >= m.m || col >= m.n) continue;
+        const int64_t at = tall ? (int64_t)col * m.cols + row : (int64_t)row * m.cols + col;
+        float o = tall ? tile[c][l] : tile[l][c];
+        if (m.momentum) {
+            float was = value(p[at]);
+            if (m.master) {
+                const float held = m.master[at];
+                X rounded;
+                put(&rounded, held);
+                // a copy of which the parameter is not the rounded value has been left behind by the program
+                if (!r.follow || value(rounded) == was || (was != was && held != held)) was = held;
+            }
+            o = was * r.decay - m.rate * o;
+            if (m.master) m.master[at] = o;
+        }
+        put(p + at, o);
+    }
+}
+
+// ------------------------------------------------------------------------------------------ products
+
+enum Kind { kGram = 0, kSquare = 1, kApply = 2 };
+
+struct Params {
+    const Entry* table;
+    int     count, tiles, wide, stages;
+    int     from;        // which X a step starts from
+    __half* work;
+    int*    failed;      // a wait ran out
+    float   product;     // factor of the finished sums
+    float   old;         // kSquare: of A; kApply: a
+    float   scale;       // kApply: of the operands
+    int     last;        // kApply: no operands are needed any more
+};
+
+// fp16 operands, f32 sums
+__host__ __device__ constexpr uint32_t half_kind(int m, int n, bool b_mn) {
+    return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+// Tiles of 128 rows by up to 256 columns.  kGram: A = X X^T; kSquare: b A + c A A; of both the tiles on and above the diagonal,
+// what lies above it is written to both places.  kApply: a X + B X.
+template <int KIND, int PARTS>
+__global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constant__ CUtensorMap map, const Params p) {
+    constexpr bool kBMn = KIND == kApply;       // the second operand's rows lie along K
+    constexpr bool kSegments = PARTS == 2;
+    extern __shared__ char shared_raw[];
+    __shared__ int firsts[kMostMatrices];
+    __shared__ uint64_t bars_at[2 * kMostStages + 6];
+    __shared__ uint32_t slot_at;
+    __shared__ volatile int give_up;
+    const uint32_t base = (smem_addr(shared_raw) + 1023u) & ~1023u;
+    const uint32_t full = smem_addr(bars_at), empty = full + 8 * kMostStages, done = empty + 8 * kMostStages, freed = done + 16, drained = freed + 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int part_b = p.wide * kDepth * 2, part_a = kRowsPerCta * kDepth * 2, stage_bytes = PARTS * (part_a + part_b);
+
+    for (int i = threadIdx.x; i < p.count; i += kThreads) firsts[i] = KIND == kApply ? p.table[i].first_apply : p.table[i].first_sym;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; ++s) bar_init(full + 8 * s, 1), bar_init(empty + 8 * s, 1);
+        for (int i = 0; i < 2; ++i) bar_init(done + 8 * i, 1), bar_init(freed + 8 * i, kEpilogue);
+        bar_init(drained, 1);
+        give_up = 0;
+        bar_init_fence();
+        prefetch_map(&map);
+    }
+    if (warp == 1) tmem_alloc<1>(smem_addr(&slot_at), 512);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *const_cast<volatile uint32_t*>(&slot_at);
+
+    auto bounded = [&](uint32_t bar, uint32_t parity, bool heed) -> bool {
+        uint64_t since = 0;
+        for (int i = 1;; ++i) {
+            if (bar_try(bar, parity)) return true;
+            if (i % 64) continue;
+            uint64_t now;
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+            if (since == 0) since = now;
+            if (now - since > kPatience || (heed && give_up)) return false;
+        }
+    };
+    auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+        if (bounded(bar, parity, true)) return true;
+        give_up = 1;
+        atomicExch(p.failed, 1);
+        return false;
+    };
+
+    // Tile u: its matrix, and the first row and column.  Symmetric results: rows of tiles from the diagonal on.
+    struct Tile {
+        int e, row, col, depth;
+    };
+    auto tile_at = [&](int u) -> Tile {
+        Tile t;
+        t.e = find(p.count, u, [&](int i) { return firsts[i]; });
+        const Entry& m = p.table[t.e];
+        int at = u - firsts[t.e];
+        if (KIND == kApply) {
+            const int nt = (m.panels * 64 + p.wide - 1) / p.wide;
+            t.row = at / nt * kRowsPerCta, t.col = at % nt * p.wide;
+        } else {
+            const int nt = (m.mp + p.wide - 1) / p.wide;
+            int row = 0;
+            for (;; ++row) {
+                const int first = row * kRowsPerCta / p.wide, tiles = nt - first;
+                if (at < tiles) {
+                    t.col = (first + at) * p.wide;
+                    break;
+                }
+                at -= tiles;
+            }
+            t.row = row * kRowsPerCta;
+        }
+        t.depth = KIND == kGram ? m.panels : (m.m + 63) / 64;
+        return t;
+    };
+
+    if (warp == 0 && lane == 0) {  // ---- copies
+        int      stage = 0, issued = 0;
+        uint32_t phase = 0;
+        bool     ok = true;
+        for (int u = blockIdx.x; u < p.tiles && ok; u += gridDim.x) {
+            const Tile t = tile_at(u);
+            const Entry m = p.table[t.e];
+            // rows of 128 bytes: where panel k of the first operand begins, and the second's
+            const int64_t x0 = m.operand[p.from], x_plane = (int64_t)m.panels * m.mp, s_plane = (int64_t)(m.mp / 64) * m.mp;
+            const int64_t a0 = KIND == kGram ? x0 : KIND == kSquare ? m.gram : m.factor, b0 = KIND == kSquare ? m.gram : x0;
+            const int64_t a_plane = KIND == kGram ? x_plane : s_plane, b_plane = KIND == kSquare ? s_plane : x_plane;
+            // columns of the tile that there are, in units of 64
+            const int limit = KIND == kApply ? m.panels * 64 : m.mp, have = min(p.wide, limit - t.col) / 64;
+            for (int k = 0; k < t.depth; ++k) {
+                ok = wait(empty + 8 * stage, phase ^ 1);
+                if (!ok) break;
+                const uint32_t a = base + stage * stage_bytes, b = a + PARTS * part_a, bar = full + 8 * stage;
+                bar_expect(bar, PARTS * (part_a + have * 8192));
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q) {
+                    const int64_t a_at = a0 + q * a_plane + (int64_t)k * m.mp + t.row;
+                    load_box<1>(a + q * part_a, &map, bar, 0, (int)a_at, 0);
+                    load_box<1>(a + q * part_a + 8192, &map, bar, 0, (int)a_at + 64, 0);
+                    for (int j = 0; j < have; ++j) {
+                        const int64_t b_at = b0 + q * b_plane + (kBMn ? (int64_t)(t.col / 64 + j) * m.mp + k * 64 : (int64_t)k * m.mp + t.col + j * 64);
+                        load_box<1>(b + q * part_b + j * 8192, &map, bar, 0, (int)b_at, 0);
+                    }
+                }
+                ++issued;
+                if (++stage == p.stages) stage = 0, phase ^= 1;
+            }
+        }
+        // the last stages are handed back before the CTA ends; where a wait ran out, copies in flight end first
+        for (int i = 0; ok && i < p.stages && i < issued; ++i) {
+            ok = wait(empty + 8 * stage, phase ^ 1);
+            if (ok && ++stage == p.stages) stage = 0, phase ^= 1;
+        }
+        if (give_up) {
+            for (int i = 0; i < p.stages && i < issued; ++i) {
+                if (--stage < 0) stage = p.stages - 1, phase ^= 1;
+                bounded(full + 8 * stage, phase, false);
+            }
+        }
+    } else if (warp == 1 && lane == 0) {  // ---- products
+        int      stage = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool     ok = true;
+        for (int u = blockIdx.x; u < p.tiles && ok; u += gridDim.x) {
+            const Tile t = tile_at(u);
+            const Entry m = p.table[t.e];
+            const int limit = KIND == kApply ? m.panels * 64 : m.mp;
+            const uint32_t kind = half_kind(kRowsPerCta, min(p.wide, limit - t.col), kBMn);
+            for (int k0 = 0; k0 < t.depth && ok; k0 += kSegments ? kSegment : t.depth) {
+                ok = wait(freed + 8 * acc, acc_phase ^ 1);
+                if (!ok) break;
+                fence_after();
+                const uint32_t d = tmem + acc * kWide;
+                const int k1 = kSegments ? min(t.depth, k0 + kSegment) : t.depth;
+                for (int k = k0; k < k1; ++k) {
+                    ok = wait(full + 8 * stage, phase);
+                    if (!ok) break;
+                    fence_after();
+                    const uint32_t a = base + stage * stage_bytes, b = a + PARTS * part_a;
+#pragma unroll
+                    for (int q = PARTS == 2 ? 0 : 2; q < 3; ++q) {  // of two parts: the small products first
+                        const uint32_t aq = q == 0 ? a + part_a : a, bq = q == 1 ? b + part_b : b;
+#pragma unroll
+                        for (int i = 0; i < kDepth / 16; ++i)
+                            product<1>(d, operand(aq + i * 32, 8192), operand(bq + i * (kBMn ? 2048 : 32), 8192), kind,
+                                       k > k0 || q > (PARTS == 2 ? 0 : 2) || i > 0);
+                    }
+                    products_commit<1>(empty + 8 * stage);
+                    if (++stage == p.stages) stage = 0, phase ^= 1;
+                }
+                products_commit<1>(done + 8 * acc);
+                if (++acc == 2) acc = 0, acc_phase ^= 1;
+            }
+        }
+        if (!ok) {  // products under way still read shared memory
+            products_commit<1>(drained);
+            bounded(drained, 0, false);
+        }
+    } else if (warp >= 2) {  // ---- finished tiles: a row a lane
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        const int half_wide = p.wide / 2;
+        int      acc = 0;
+        uint32_t acc_phase = 0;
+        bool     ok = true;
+        for (int u = blockIdx.x; u < p.tiles && ok; u += gridDim.x) {
+            const Tile t = tile_at(u);
+            const Entry m = p.table[t.e];
+            const int row = t.row + quarter * 32 + lane, col0 = t.col + half * half_wide;
+            const int limit = KIND == kApply ? m.panels * 64 : m.mp;
+            const int64_t s_plane = (int64_t)(m.mp / 64) * m.mp * 64, x_plane = (int64_t)m.panels * m.mp * 64;
+            auto finish = [&](float* v, int c) {  // 32 columns
+                const int col = col0 + c;
+                if (col >= limit) return;
+                const int64_t at = ((int64_t)(col / 64) * m.mp + row) * 64 + col % 64;
+                if (KIND == kApply) {
+                    const float4* const was = reinterpret_cast<const float4*>(m.x[p.from] + at);
+                    float4* const to = reinterpret_cast<float4*>(m.x[p.from ^ 1] + at);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float4 x = was[j];
+                        v[4 * j] = fmaf(p.old, x.x, v[4 * j] * p.product), v[4 * j + 1] = fmaf(p.old, x.y, v[4 * j + 1] * p.product);
+                        v[4 * j + 2] = fmaf(p.old, x.z, v[4 * j + 2] * p.product), v[4 * j + 3] = fmaf(p.old, x.w, v[4 * j + 3] * p.product);
+                        to[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                    }
+                    if (p.last) return;
+                } else if (row / 128 > col / 128) {
+                    return;  // below the diagonal
+                }
+                __half* const to = p.work + (KIND == kGram ? m.gram : KIND == kSquare ? m.factor : m.operand[p.from ^ 1]) * 64;
+                const int64_t plane = KIND == kApply ? x_plane : s_plane;
+                if (KIND == kSquare) {
+                    const uint4* const a0 = reinterpret_cast<const uint4*>(p.work + m.gram * 64 + at);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint4 w = a0[j];
+                        uint4 w1 = make_uint4(0, 0, 0, 0);
+                        if (PARTS == 2) w1 = *reinterpret_cast<const uint4*>(p.work + m.gram * 64 + plane + at + 8 * j);
+                        const uint32_t hi[4] = {w.x, w.y, w.z, w.w}, lo[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float2 a = __half22float2(reinterpret_cast<const __half2&>(hi[i]));
+                            if (PARTS == 2) {
+                                const float2 l = __half22float2(reinterpret_cast<const __half2&>(lo[i]));
+                                a.x += l.x, a.y += l.y;
+                            }
+                            v[8 * j + 2 * i]     = fmaf(p.old, a.x, v[8 * j + 2 * i] * p.product);
+                            v[8 * j + 2 * i + 1] = fmaf(p.old, a.y, v[8 * j + 2 * i + 1] * p.product);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] *= KIND == kApply ? p.scale : p.product;
+                }
+                const bool mirror = KIND != kApply && col / 128 > row / 128;
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+                        w[j] = reinterpret_cast<const uint32_t&>(h);
+                        if (q + 1 < PARTS) {
+                            const float2 back = __half22float2(h);
+                            v[2 * j] -= back.x, v[2 * j + 1] -= back.y;
+                        }
+                    }
+                    uint4* const o = reinterpret_cast<uint4*>(to + q * plane + at);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+                    if (mirror) {
+                        __half* const under = to + q * plane + ((int64_t)(row / 64) * m.mp + col) * 64 + row % 64;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const __half2 h = reinterpret_cast<const __half2&>(w[j]);
+                            under[(2 * j) * 64] = h.x, under[(2 * j + 1) * 64] = h.y;
+                        }
+                    }
+                }
+            };
+            float total[kSegments ? kWide / 2 : 1];
+            if constexpr (kSegments) {
+#pragma unroll
+                for (int j = 0; j < kWide / 2; ++j) total[j] = 0.f;
+            }
+            for (int k0 = 0; k0 < t.depth; k0 += kSegments ? kSegment : t.depth) {
+                ok = __all_sync(0xffffffffu, wait(done + 8 * acc, acc_phase));
+                if (!ok) break;
+                fence_after();
+                const uint32_t acc_at = tmem + ((uint32_t)(quarter * 32) << 16) + acc * kWide + half * half_wide;
+#pragma unroll
+                for (int c = 0; c < kWide / 2; c += 32) {
+                    if (c < half_wide && col0 + c < limit) {
+                        float2 pairs[16];
+                        float* const v = reinterpret_cast<float*>(pairs);
+                        tmem_load32(acc_at + c, pairs);
+                        tmem_loaded(pairs);
+                        if constexpr (kSegments) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) total[c + j] += v[j];
+                        } else {
+                            finish(v, c);
+                        }
+                    }
+                }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(freed + 8 * acc);
+                if (++acc == 2) acc = 0, acc_phase ^= 1;
+            }
+            if (!ok) break;
+            if constexpr (kSegments) {
+#pragma unroll
+                for (int c = 0; c < kWide / 2; c += 32)
+                    if (c < half_wide) finish(total + c, c);
+            }
+        }
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 1) tmem_free<1>(tmem, 512);
+}
+
+// ------------------------------------------------------------------------------------------ host side
+
+struct Matrix {
+    void*       param;
+    const void* grad;
+    float*      momentum;
+    float*      master;
+    int64_t     rows, cols;
+    double      rate;
+};
+
+// Powers of two that bring the operands of each step into the range of fp16, for singular values of at most one before.
+struct Step {
+    float a, b, c;
+    int   x, gram, factor;  // exponents
+};
+
+bool steps_of(const double* abc, int count, std::vector<Step>* steps) {
+    double most = 1.0 + 1.0 / 1024;  // of the singular values; the first are at most one but for roundings
+    auto exponent = [](double bound) { return bound > 0 ? 15 - std::max(-60, (int)std::ceil(std::log2(bound))) : 15; };
+    for (int i = 0; i < count; ++i) {
+        const double a = abc[3 * i], b = abc[3 * i + 1], c = abc[3 * i + 2];
+        if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
+        double factor = 0, next = 0;
+        for (int j = 0; j <= 4096; ++j) {
+            const double s = most * j / 4096, f = b * s * s + c * s * s * s * s;
+            factor = std::max(factor, std::fabs(f)), next = std::max(next, std::fabs(s * (a + f)));
+        }
+        factor *= 1.01, next *= 1.01;
+        Step s = {(float)a, (float)b, (float)c, exponent(most), exponent(most * most), exponent(factor)};
+        steps->push_back(s);
+        if (!(next < 1e6)) return false;
+        most = std::max(next, 1e-6);
+    }
+    return true;
+}
+
+struct Chain {  // matrices of a chain of launches, and what its workspace holds
+    std::vector<Entry> entry;
+    Entry*   table;
+    int32_t* failed;
+    int64_t  chunks, blocks;
+    size_t   bytes;
+};
+
+Chain chain_of(const Matrix* matrices, int64_t count, int parts, void* work) {
+    Chain c;
+    Parts w(work);
+    c.failed = w.take<int32_t>(64);
+    c.table  = w.take<Entry>(count);
+    c.chunks = c.blocks = 0;
+    c.entry.resize(count);
+    for (int64_t i = 0; i < count; ++i) {
+        Entry& e = c.entry[i];
+        const Matrix& m = matrices[i];
+        e = {};
+        e.grad = m.grad, e.momentum = m.momentum, e.param = m.param, e.master = m.master, e.rate = (float)m.rate;
+        e.rows = (int)m.rows, e.cols = (int)m.cols;
+        e.m = std::min(e.rows, e.cols), e.n = std::max(e.rows, e.cols);
+        e.mp = (int)up(e.m, kRowsPerCta), e.panels = (int)((e.n + 63) / 64);
+        e.chunks = (int)((m.rows * m.cols + kChunk - 1) / kChunk);
+        e.first_chunk = (int)c.chunks, e.first_block = (int)c.blocks;
+        c.chunks += e.chunks, c.blocks += (int64_t)e.panels * (e.mp / 64);
+        e.partial = w.take<double>(e.chunks);
+        const int64_t values = (int64_t)e.panels * e.mp * 64;
+        for (int j = 0; j < 2; ++j) e.x[j] = w.take<float>(values);
+        for (int j = 0; j < 2; ++j) {
+            e.operand[j] = (int64_t)(w.used / 128);
+            w.take<__half>(parts * values);
+        }
+        for (int64_t* at : {&e.gram, &e.factor}) {
+            *at = (int64_t)(w.used / 128);
+            w.take<__half>((int64_t)parts * e.mp * e.mp);
+        }
+    }
+    c.bytes = w.used;
+    return c;
+}
+
+// How many of the matrices, from the first on, go together: as many as some hundred megabytes hold.
+constexpr size_t kChainBytes = (size_t)1 << 30;
+int64_t together(const Matrix* matrices, int64_t count, int parts) {
+    size_t bytes = 0;
+    int64_t i = 0;
+    for (; i < count && i < kMostMatrices; ++i) {
+        const int64_t m = std::min(matrices[i].rows, matrices[i].cols), n = std::max(matrices[i].rows, matrices[i].cols);
+        const size_t more = (size_t)up(m, 128) * ((size_t)up(n, 64) * (8 + 4 * parts) + (size_t)up(m, 128) * 4 * parts);
+        if (i > 0 && bytes + more > kChainBytes) break;
+        bytes += more;
+    }
+    return i;
+}
+
+bool matrices_ok(const Matrix* m, int64_t count) {
+    for (int64_t i = 0; i < count; ++i) {
+        const int64_t rows = m[i].rows, cols = m[i].cols;
+        // rows of the workspace are counted in 32 bits
+        if (rows < 1 || cols < 1 || rows >= ((int64_t)1 << 30) || cols >= ((int64_t)1 << 30) || up(std::min(rows, cols), 128) > ((int64_t)1 << 20) ||
+            (double)up(std::min(rows, cols), 128) * up(std::max(rows, cols), 64) >= 1e10)
+            return false;
+    }
+    return true;
+}
+
+template <int KIND, int PARTS>
+int launch(const CUtensorMap& map, const Params& p, int grid, cudaStream_t stream) {
+    auto kernel = k_muon_tiles<KIND, PARTS>;
+    static std::atomic<uint64_t> allowed{0};
+    FW_DO(allow_shared(kernel, kShared, allowed));
+    kernel<<<grid, kThreads, kShared, stream>>>(map, p);
+    FW_LAUNCHED();
+    return FRAMEWISE_B200_OK;
+}
+
+template <typename X>
+int run_chain(Chain& c, const Rates& rates, const std::vector<Step>& steps, char* work, cudaStream_t stream) {
+    constexpr int PARTS = sizeof(X) == 4 ? 2 : 1;
+    const int sms = sm_count(), count = (int)c.entry.size();
+    if (sms < 1) return FRAMEWISE_B200_CUDA_ERROR;
+    // tiles as wide as leaves all SMs something to do
+    auto lay = [&](int wide, bool apply, bool write) {
+        int64_t tiles = 0;
+        for (Entry& e : c.entry) {
+            if (write) (apply ? e.first_apply : e.first_sym) = (int)tiles;
+            const int mt = e.mp / kRowsPerCta, nt = ((apply ? e.panels * 64 : e.mp) + wide - 1) / wide;
+            if (apply) tiles += (int64_t)mt * nt;
+            else for (int r = 0; r < mt; ++r) tiles += nt - r * kRowsPerCta / wide;
+        }
+        return tiles;
+    };
+    auto width = [&](bool apply) {
+        int wide = kWide;
+        while (wide > 64 && lay(wide, apply, false) < sms) wide /= 2;
+        return wide;
+    };
+    const int     wide_sym = width(false), wide_apply = width(true);
+    const int64_t sym = lay(wide_sym, false, true), apply = lay(wide_apply, true, true);
+    if (sym >= INT32_MAX || apply >= INT32_MAX || c.chunks >= INT32_MAX || c.blocks >= INT32_MAX || c.bytes / 128 >= INT32_MAX) return FRAMEWISE_B200_BAD_ARGUMENT;
+    FW_DO(bind_device());
+    CUtensorMap map;
+    const int64_t lines = (int64_t)(c.bytes / 128);
+    if (!map_of(&map, work, false, 64, lines, 1, 64, lines * 64, 64, 64)) return FRAMEWISE_B200_TENSOR_MAP;
+    FW_TRY(cudaMemsetAsync(c.failed, 0, 4, stream));
+    for (int i = 0; i < count; i += kSlots) {
+        Slots s;
+        s.count = std::min(kSlots, count - i), s.base = i, s.table = c.table;
+        int64_t chunks = 0;
+        for (int j = 0; j < s.count; ++j) s.entry[j] = c.entry[i + j], chunks += s.entry[j].chunks;
+        k_muon_collect<X><<<(unsigned)chunks, 256, 0, stream>>>(s, rates);
+        FW_LAUNCHED();
+    }
+    __half* const halves = reinterpret_cast<__half*>(work);
+    k_muon_begin<X, PARTS><<<(unsigned)c.blocks, 256, 0, stream>>>(c.table, count, rates, std::ldexp(1.f, steps[0].x), halves);
+    FW_LAUNCHED();
+    auto stages = [&](int wide) { return std::min(kMostStages, (kShared - 1024) / (PARTS * (kRowsPerCta + wide) * kDepth * 2)); };
+    Params p = {};
+    p.table = c.table, p.count = count, p.work = halves, p.failed = c.failed;
+    const int grid_sym = (int)std::min<int64_t>(sym, sms), grid_apply = (int)std::min<int64_t>(apply, sms);
+    for (size_t i = 0; i < steps.size(); ++i) {
+        const Step& s = steps[i];
+        p.from = (int)(i & 1), p.tiles = (int)sym, p.wide = wide_sym, p.stages = stages(wide_sym), p.last = 0;
+        p.product = std::ldexp(1.f, s.gram - 2 * s.x);
+        FW_DO(launch<kGram, PARTS>(map, p, grid_sym, stream));
+        p.product = std::ldexp(s.c, s.factor - 2 * s.gram), p.old = std::ldexp(s.b, s.factor - s.gram);
+        FW_DO(launch<kSquare, PARTS>(map, p, grid_sym, stream));
+        p.tiles = (int)apply, p.wide = wide_apply, p.stages = stages(wide_apply);
+        p.product = std::ldexp(1.f, -s.factor - s.x), p.old = s.a, p.last = i + 1 == steps.size();
+        p.scale = p.last ? 0.f : std::ldexp(1.f, steps[i + 1].x);
+        FW_DO(launch<kApply, PARTS>(map, p, grid_apply, stream));
+    }
+    k_muon_finish<X><<<(unsigned)c.blocks, 256, 0, stream>>>(c.table, count, rates, (int)(steps.size() & 1), c.failed);
+    FW_LAUNCHED();
+    return FRAMEWISE_B200_OK;
+}
+
+size_t bytes_for(const std::vector<Matrix>& list, int parts) {
+    size_t most = 256;
+    for (size_t i = 0; i < list.size();) {
+        const int64_t n = together(list.data() + i, (int64_t)(list.size() - i), parts);
+        most = std::max(most, chain_of(list.data() + i, n, parts, nullptr).bytes);
+        i += n;
+    }
+    return most;
+}
+
+int run(const std::vector<Matrix>& list, int dtype, const Rates& rates, const double* coefficients, int steps, void* work, size_t work_bytes,
+        cudaStream_t stream) {
+    if (list.empty()) return FRAMEWISE_B200_OK;
+    const int parts = dtype == FRAMEWISE_B200_F32 ? 2 : 1;
+    std::vector<Step> plan;
+    if (!work || misaligned(work) || !coefficients || steps < 1 || steps > 100 || !steps_of(coefficients, steps, &plan)) return FRAMEWISE_B200_BAD_ARGUMENT;
+    if (work_bytes < bytes_for(list, parts)) return FRAMEWISE_B200_WORKSPACE;
+    for (size_t i = 0; i < list.size();) {
+        const int64_t n = together(list.data() + i, (int64_t)(list.size() - i), parts);
+        Chain c = chain_of(list.data() + i, n, parts, work);
+        FW_DO(dtype == FRAMEWISE_B200_F32 ? run_chain<float>(c, rates, plan, static_cast<char*>(work), stream)
+                                          : run_chain<__nv_bfloat16>(c, rates, plan, static_cast<char*>(work), stream));
+        i += n;
+    }
+    return FRAMEWISE_B200_OK;
+}
+
+bool dtype_ok(int dtype) { return dtype == FRAMEWISE_B200_F32 || dtype == FRAMEWISE_B200_BF16; }
+
+// the matrices of a Muon step; those without values are passed over
+int muon_list(const framewise_b200_matrix* matrices, int64_t count, double lr, int adjust, std::vector<Matrix>* list) {
+    if (count < 0 || (count > 0 && !matrices)) return FRAMEWISE_B200_BAD_ARGUMENT;
+    for (int64_t i = 0; i < count; ++i) {
+        const framewise_b200_matrix& m = matrices[i];
+        if (m.rows < 0 || m.cols < 0) return FRAMEWISE_B200_BAD_ARGUMENT;
+        if (m.rows == 0 || m.cols == 0) continue;
+        const double by = adjust ? 0.2 * std::sqrt((double)std::max(m.rows, m.cols)) : std::sqrt(std::max(1.0, (double)m.rows / m.cols));
+        list->push_back({m.param, m.grad, m.momentum, m.master, m.rows, m.cols, lr * by});
+    }
+    return matrices_ok(list->data(), (int64_t)list->size()) ? FRAMEWISE_B200_OK : FRAMEWISE_B200_BAD_ARGUMENT;
+}
+
+std::vector<Matrix> batch_list(int64_t count, int64_t rows, int64_t cols, int dtype, const void* x, void* out) {
+    std::vector<Matrix> list;
+    const int64_t bytes = rows * cols * (dtype == FRAMEWISE_B200_F32 ? 4 : 2);
+    for (int64_t i = 0; i < count; ++i)
+        list.push_back({out ? static_cast<char*>(out) + i * bytes : nullptr, x ? static_cast<const char*>(x) + i * bytes : nullptr, nullptr, nullptr, rows, cols, 0.0});
+    return list;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t framewise_b200_muon_bytes(const framewise_b200_matrix* matrices, int64_t count, int32_t dtype) {
+    std::vector<Matrix> list;
+    if (!dtype_ok(dtype) || muon_list(matrices, count, 0.0, 0, &list) != FRAMEWISE_B200_OK) return 0;
+    return bytes_for(list, dtype == FRAMEWISE_B200_F32 ? 2 : 1);
+}
+
+int framewise_b200_muon(const framewise_b200_matrix* matrices, int64_t count, int32_t dtype, double lr, double beta, int32_t nesterov,
+                        double weight_decay, int32_t match_rms, const double* coefficients, int32_t steps, double eps, int32_t follow,
+                        void* work, size_t work_bytes, framewise_b200_stream_t stream) {
+    std::vector<Matrix> list;
+    if (!dtype_ok(dtype) || !(eps > 0)) return FRAMEWISE_B200_BAD_ARGUMENT;
+    FW_DO(muon_list(matrices, count, lr, match_rms, &list));
+    for (const Matrix& m : list)
+        if (!m.param || !m.grad || !m.momentum || (m.master && dtype == FRAMEWISE_B200_F32)) return FRAMEWISE_B200_BAD_ARGUMENT;
+    const Rates rates = {(float)(1 - beta), (float)beta, nesterov ? 1.f : 0.f, (float)eps, (float)(1 - lr * weight_decay), follow};
+    return run(list, dtype, rates, coefficients, steps, work, work_bytes, stream);
+}
+
+size_t framewise_b200_orthogonalize_bytes(int64_t count, int64_t rows, int64_t cols, int32_t dtype) {
+    if (!dtype_ok(dtype) || count < 0 || rows < 0 || cols < 0) return 0;
+    if (count == 0 || rows == 0 || cols == 0) return 256;
+    const std::vector<Matrix> list = batch_list(std::min<int64_t>(count, kMostMatrices), rows, cols, dtype, nullptr, nullptr);
+    return matrices_ok(list.data(), (int64_t)list.size()) ? bytes_for(list, dtype == FRAMEWISE_B200_F32 ? 2 : 1) : 0;
+}
+
+int framewise_b200_orthogonalize(int64_t count, int64_t rows, int64_t cols, int32_t dtype, const void* x, void* out, const double* coefficients,
+                                 int32_t steps, double eps, void* work, size_t work_bytes, framewise_b200_stream_t stream) {
+    if (!dtype_ok(dtype) || count < 0 || rows < 0 || cols < 0 || !(eps > 0)) return FRAMEWISE_B200_BAD_ARGUMENT;
+    if (count == 0 || rows == 0 || cols == 0) return FRAMEWISE_B200_OK;
+    if (!x || !out) return FRAMEWISE_B200_BAD_ARGUMENT;
+    const std::vector<Matrix> list = batch_list(count, rows, cols, dtype, x, out);
+    if (!matrices_ok(list.data(), (int64_t)list.size())) return FRAMEWISE_B200_BAD_ARGUMENT;
+    const Rates rates = {0.f, 0.f, 0.f, (float)eps, 1.f, 0};
+    return run(list, dtype, rates, coefficients, steps, work, work_bytes, stream);
+}
+
+}  // extern "C"

@@ -8,6 +8,8 @@ them with an output layer over thousands of classes, an embedding of label conte
   :func:`label_scores`          log probabilities of given labels, entropies and the best classes, off logits in memory
   :class:`AdamW`                AdamW over all parameters at once, states in 32 or 8 bits; :func:`adamw_step`,
                                 :func:`adamw_values`, the step itself and what 8-bit states stand for
+  :class:`Muon`                 Muon for hidden layers' matrices, all of them in a launch per product; :func:`muon_step`,
+                                :func:`orthogonalize`, the step itself and its Newton-Schulz products
 
 No counterpart in the reference, which ends at losses on log probabilities.  The native extension is required:
 importing this module fails if it is not built (``python -m i6_native_ops_b200.build``); there is no CPU or
@@ -192,7 +194,38 @@ def adamw_values(exp_avg: Sequence[State], exp_avg_sq: Sequence[State]) -> Tuple
     return core.adamw_values(m, m_steps, v, v_steps)
 
 
-class AdamW(torch.optim.Optimizer):
+class _Optimizer(torch.optim.Optimizer):
+    """States keep their own types when they are loaded."""
+
+    @staticmethod
+    def _copy(p: torch.Tensor) -> torch.Tensor:
+        return p.detach().to(torch.float32, memory_format=torch.contiguous_format)
+
+    def load_state_dict(self, state_dict):
+        """As torch's, but codes, moments and copies keep their own types (torch would turn them into the parameters').
+        bfloat16 parameters whose states come from float32 ones start a copy of their own."""
+        seen = {}  # what earlier hooks have made of the states; later ones see them with their types
+        hooks = (self.register_load_state_dict_pre_hook(lambda _, given: seen.update(given)),
+                 self.register_load_state_dict_post_hook(lambda _: self._take_states(seen), prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _take_states(self, state_dict: dict) -> None:
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(ids, params):
+            if i in state_dict["state"]:
+                state = {k: v.to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
+                         for k, v in state_dict["state"][i].items()}
+                if state and p.dtype != torch.float32 and "master" not in state:
+                    state["master"] = self._copy(p)
+                self.state[p] = state
+
+
+class AdamW(_Optimizer):
     """AdamW whose step takes all parameters of a group in one launch or a few.
 
     ``state_bits=8`` holds the moments in 8 bits (2 bytes a parameter instead of 8): per 256 values a step and quadratic
@@ -223,33 +256,6 @@ class AdamW(torch.optim.Optimizer):
             state["master"] = self._copy(p)
         return state
 
-    @staticmethod
-    def _copy(p: torch.Tensor) -> torch.Tensor:
-        return p.detach().to(torch.float32, memory_format=torch.contiguous_format)
-
-    def load_state_dict(self, state_dict):
-        """As torch's, but codes, moments and copies keep their own types (torch would turn them into the parameters').
-        bfloat16 parameters whose states come from float32 ones start a copy of their own."""
-        seen = {}  # what earlier hooks have made of the states; later ones see them with their types
-        hooks = (self.register_load_state_dict_pre_hook(lambda _, given: seen.update(given)),
-                 self.register_load_state_dict_post_hook(lambda _: self._take_states(seen), prepend=True))
-        try:
-            super().load_state_dict(state_dict)
-        finally:
-            for hook in hooks:
-                hook.remove()
-
-    def _take_states(self, state_dict: dict) -> None:
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        for i, p in zip(ids, params):
-            if i in state_dict["state"]:
-                state = {k: v.to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
-                         for k, v in state_dict["state"][i].items()}
-                if state and p.dtype != torch.float32 and "master" not in state:
-                    state["master"] = self._copy(p)
-                self.state[p] = state
-
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -278,4 +284,121 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
 
-__all__ = ["core", "linear_cross_entropy", "label_embedding", "LabelScores", "label_scores", "adamw_step", "adamw_values", "AdamW"]
+Triple = Tuple[float, float, float]
+COEFFICIENTS: Triple = (3.4445, -4.7750, 2.0315)
+
+
+def _flat(coefficients: Union[Triple, Sequence[Triple]], steps: int) -> List[float]:
+    """Three numbers per step, from those of one step or of all."""
+    rows = [tuple(c) for c in coefficients] if isinstance(coefficients[0], (tuple, list)) else [tuple(coefficients)] * int(steps)
+    if len(rows) != steps or any(len(r) != 3 for r in rows):
+        raise RuntimeError("coefficients must be three numbers, or three for each of the steps")
+    return [float(c) for r in rows for c in r]
+
+
+def _match_rms(adjust_lr: Optional[str]) -> bool:
+    if adjust_lr not in (None, "original", "match_rms_adamw"):
+        raise ValueError('adjust_lr must be "original" or "match_rms_adamw"')
+    return adjust_lr == "match_rms_adamw"
+
+
+def orthogonalize(
+    x: torch.Tensor,
+    steps: int = 5,
+    coefficients: Union[Triple, Sequence[Triple]] = COEFFICIENTS,
+    eps: float = 1e-7,
+) -> torch.Tensor:
+    """Matrices with singular values near one and the singular vectors of ``x``, by Newton-Schulz products: ``X = x /
+    max(|x|, eps)`` (Frobenius norm), then ``steps`` times ``A = X X^T; X = a X + (b A + c A A) X``, matrices with more
+    rows than columns the other way round.
+
+    :param x: (..., rows, cols) float32 or bfloat16 (CUDA)
+    :param coefficients: (a, b, c) of every step, or one such triple per step.  Those that let singular values grow past
+        10^6 are refused
+    :return: the same shape and dtype; there is no gradient.  X is held in 32 bits; the operands of the products have 11
+        bits for bfloat16 matrices and 22 for float32 ones, sums are formed in 32 bits in a fixed order.  A matrix with NaN or
+        an infinity becomes NaN, one of zeros stays as it is."""
+    return core.orthogonalize(x, _flat(coefficients, steps), float(eps))
+
+
+def muon_step(
+    params: Sequence[torch.Tensor],
+    grads: Sequence[torch.Tensor],
+    momentum: Sequence[torch.Tensor],
+    lr: float = 1e-3,
+    beta: float = 0.95,
+    nesterov: bool = True,
+    weight_decay: float = 0.1,
+    steps: int = 5,
+    coefficients: Union[Triple, Sequence[Triple]] = COEFFICIENTS,
+    eps: float = 1e-7,
+    adjust_lr: Optional[str] = None,
+    master: Optional[Sequence[torch.Tensor]] = None,
+    follow: bool = False,
+) -> None:
+    """One step of Muon over a list of matrices, in place: ``v += (1 - beta) (g - v)``, ``u = g + beta (v - g)`` (without
+    ``nesterov``: ``v``), ``p = p (1 - lr weight_decay) - lr s orthogonalize(u)``.  All matrices, of whatever shapes, go
+    through each product in one launch (256 of them, as far as a gigabyte of scratch holds them).  As after any operation in
+    place, graphs that saved a parameter before refuse their backward pass.
+
+    :param params: contiguous CUDA matrices, all float32 or all bfloat16
+    :param momentum: per parameter a float32 tensor of its shape
+    :param adjust_lr: ``"original"`` (or None): ``s = sqrt(max(1, rows / cols))``; ``"match_rms_adamw"``: ``s = 0.2
+        sqrt(max(rows, cols))``
+    :param master: float32 copies of bfloat16 parameters, updated in place of them; they then get their rounded values
+    :param follow: a copy of which its parameter is not the rounded value starts from the parameter, as for
+        :func:`adamw_step`"""
+    core.muon_step(list(params), list(grads), list(momentum), [] if master is None else list(master), float(lr), float(beta), bool(nesterov),
+                   float(weight_decay), _match_rms(adjust_lr), _flat(coefficients, steps), float(eps), bool(follow))
+
+
+class Muon(_Optimizer):
+    """Muon for the matrices of a model's hidden layers: momentum, made orthogonal, as the update.  (Embeddings, output
+    layers and vectors are for :class:`AdamW`.)
+
+    Parameters have to be matrices.  bfloat16 parameters get a float32 copy that the steps accumulate in
+    (``state["master"]``); values that the program changes between steps are taken over from the parameter.  Parameters
+    without a gradient are passed over.  The arguments are those of :func:`muon_step`."""
+
+    def __init__(self, params, lr: float = 1e-3, beta: float = 0.95, nesterov: bool = True, weight_decay: float = 0.1, steps: int = 5,
+                 coefficients: Union[Triple, Sequence[Triple]] = COEFFICIENTS, eps: float = 1e-7, adjust_lr: Optional[str] = None):
+        _flat(coefficients, steps)
+        _match_rms(adjust_lr)
+        super().__init__(params, dict(lr=lr, beta=beta, nesterov=nesterov, weight_decay=weight_decay, steps=steps, coefficients=coefficients,
+                                      eps=eps, adjust_lr=adjust_lr))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() != 2:
+                self.param_groups.pop()
+                raise ValueError(f"Muon takes matrices, got a parameter of shape {tuple(p.shape)}")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            calls = {}  # parameters of one device and dtype go together
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                state = self.state[p]
+                if not state:
+                    state["momentum"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                    if p.dtype != torch.float32:
+                        state["master"] = self._copy(p)
+                calls.setdefault((p.device, p.dtype), []).append(p)
+            for (_, dtype), params in calls.items():
+                states = [self.state[p] for p in params]
+                muon_step(params, [p.grad for p in params], [s["momentum"] for s in states], lr=group["lr"], beta=group["beta"],
+                          nesterov=group["nesterov"], weight_decay=group["weight_decay"], steps=group["steps"],
+                          coefficients=group["coefficients"], eps=group["eps"], adjust_lr=group["adjust_lr"],
+                          master=None if dtype == torch.float32 else [s["master"] for s in states], follow=True)
+        return loss
+
+
+__all__ = ["core", "linear_cross_entropy", "label_embedding", "LabelScores", "label_scores", "adamw_step", "adamw_values", "AdamW",
+           "orthogonalize", "muon_step", "Muon"]

@@ -1,6 +1,7 @@
 /* framewise_b200.h -- C ABI of the operators of framewise training on B200 (sm_100a): output layer with
- * softmax cross entropy, label embedding, AdamW.  They follow an alignment or a label sequence: a network
- * is trained on one class per frame (the (B,T) result of fbw_b200_viterbi) or on label sequences.
+ * softmax cross entropy, label embedding, scores of labels off logits, AdamW, Muon.  They follow an alignment or a
+ * label sequence: a network is trained on one class per frame (the (B,T) result of fbw_b200_viterbi) or on label
+ * sequences.
  * No counterpart in the reference, which ends at the losses on log probabilities.
  *
  * All pointers are DEVICE pointers unless a comment says host.  Sizes are 64-bit.  No call allocates
@@ -171,6 +172,38 @@ int framewise_b200_scores_backward(const framewise_b200_scores_shape* shape, con
                                    const int32_t* seq_lens, const void* top_labels, const void* kept,
                                    const framewise_b200_scores_grads* grads, void* grad_logits,
                                    framewise_b200_stream_t stream);
+
+/* Orthogonalisation by Newton-Schulz products.  For X = x / max(|x|, eps) (Frobenius norm; matrices with more rows than
+ * columns lie transposed) and each of `steps` triples (a, b, c) of `coefficients` (HOST array of 3 steps values):
+ *     A = X X^T;  X = a X + (b A + c A A) X
+ * X is held in 32 bits; the products' operands are rounded to 11 bits for bf16 matrices, 22 for f32 ones, the sums are
+ * formed in 32 bits in a fixed order: equal calls give equal bits.  `count` dense matrices of rows x cols one after another,
+ * out likewise (may be x).  A matrix with NaN or an infinity becomes NaN; zeros stay zeros.  Coefficients that let a
+ * singular value grow past 10^6 are refused.  The result of _bytes is 0 for sizes past the limits. */
+size_t framewise_b200_orthogonalize_bytes(int64_t count, int64_t rows, int64_t cols, int32_t dtype);
+int framewise_b200_orthogonalize(int64_t count, int64_t rows, int64_t cols, int32_t dtype, const void* x, void* out,
+                                 const double* coefficients, int32_t steps, double eps, void* work, size_t work_bytes,
+                                 framewise_b200_stream_t stream);
+
+/* One matrix of a Muon step: param and grad of rows x cols (`dtype`), momentum (f32), dense; master: f32, or NULL. */
+typedef struct {
+    void*       param;
+    const void* grad;
+    float*      momentum;
+    float*      master;
+    int64_t     rows, cols;
+} framewise_b200_matrix;
+
+/* A step of Muon over `count` matrices (HOST array):
+ *     v = v + (g - v) (1 - beta);   u = nesterov ? g + (v - g) beta : v;   o = u orthogonalised as above
+ *     x = x (1 - lr weight_decay) - lr s o,   s = sqrt(max(1, rows / cols)), or match_rms: 0.2 sqrt(max(rows, cols))
+ * x being the master copy where there is one (the parameter is then x rounded once); follow: a copy of which its parameter
+ * is not the rounded value starts from the parameter.  All matrices go through each product in one launch. */
+size_t framewise_b200_muon_bytes(const framewise_b200_matrix* matrices, int64_t count, int32_t dtype);
+int framewise_b200_muon(const framewise_b200_matrix* matrices, int64_t count, int32_t dtype, double lr, double beta,
+                        int32_t nesterov, double weight_decay, int32_t match_rms, const double* coefficients,
+                        int32_t steps, double eps, int32_t follow, void* work, size_t work_bytes,
+                        framewise_b200_stream_t stream);
 
 /* Number of kernels of this library launched by this process so far. */
 int64_t framewise_b200_launch_count(void);
