@@ -11,6 +11,10 @@
 // grow, by a factor of a step, and an error that a product made of X would grow with them.  What B's and A's roundings do is
 // a change of the factor B, small for small singular values, and does not grow.  fp16 rather than bf16: as fast, eight times
 // finer, and all operands are bounded, so that powers of two (from the coefficients, for any matrix) keep them in its range.
+// Once singular values are near one, B is near (b + c) times the identity and undoes most of a X.  So a multiple t of the
+// identity is taken from B and added to a, where it costs no rounding: t = b s^2 + c s^4 for the singular value s that all
+// would have if they were equal (1 / sqrt(m) at first; a matrix below eps, which stays small, has small t).  Errors of bf16 results besides their own rounding: 64 x 256 0.93e-3 of the norm
+// (1.9e-3 without), 512 x 2048 0.6e-3 (1.3e-3); the rounding alone is 1.66e-3.
 #include "framewise_b200.h"
 #include "framewise_host.h"
 #include "tensor_core.h"
@@ -35,8 +39,9 @@ constexpr int kChunk        = 16384; // values per CTA of the pass over gradient
 constexpr int kRowsPerCta   = 128;   // of a tile: the lanes of tensor memory
 constexpr int kWide         = 256;   // columns of a tile at most: two accumulators fill tensor memory
 constexpr int kDepth        = 64;    // K per stage
-constexpr int kSegment      = 4;     // f32: stages after which an accumulator is added up in registers, for tensor cores cut
-                                     // off what they add, at 2^-24 of the sum a step, and never round it up
+constexpr int kSegment      = 1;     // f32: stages after which an accumulator is added up in registers, for tensor cores cut
+                                     // off what they add, at 2^-24 of the sum a step, and never round it up: 6 x 500 x 2001 is off
+                                     // by 5.1e-6 of its norm with 4, by 2.0e-6 with 1 (plain 32 bits: 2.7e-6)
 constexpr int kMostStages   = 8;
 constexpr int kEpilogue     = 8;     // warps that finish tiles
 constexpr int kThreads      = 64 + 32 * kEpilogue;
@@ -51,6 +56,7 @@ struct Entry {
     void*       param;      // or the result
     float*      master;     // or null
     double*     partial;    // sums of squares of the chunks
+    float*      shift;      // per step: the multiple of the identity that B does without
     float*      x[2];       // X, before and after a step
     int64_t     operand[2]; // its fp16 parts, as rows of 128 bytes of the workspace
     int64_t     gram, factor; // A and B, likewise
@@ -58,6 +64,12 @@ struct Entry {
     int         m, n, mp, panels;  // m <= n; rows of a panel (multiple of 128), panels of X
     int         chunks, first_chunk, first_block, first_sym, first_apply;  // where its work begins in each launch
     float       rate;
+};
+
+constexpr int kMostSteps = 100;
+struct Steps {
+    int   count;
+    float abc[3 * kMostSteps];
 };
 
 struct Slots {
@@ -135,7 +147,7 @@ __device__ __forceinline__ void split(float v, __half (&h)[PARTS]) {
 
 // X = U / max(|U|, eps) in 32 bits and as operands: a CTA per 64 columns and rows, zeros where there are none.
 template <typename X, int PARTS>
-__global__ void __launch_bounds__(256) k_muon_begin(const Entry* __restrict__ table, int count, const Rates r, float scale, __half* work) {
+__global__ void __launch_bounds__(256) k_muon_begin(const Entry* __restrict__ table, int count, const Rates r, float scale, __half* work, const __grid_constant__ Steps steps) {
     __shared__ double part[8];
     __shared__ float  tile[64][65];
     const int   e = find(count, blockIdx.x, [&](int i) { return table[i].first_block; });
@@ -166,6 +178,14 @@ __global__ void __launch_bounds__(256) k_muon_begin(const Entry* __restrict__ ta
     // |U| may be past the range of 32 bits (or below): 64 bits up to the quotient
     const double by = 1.0 / fmax(sqrt(sum), (double)r.eps);
     const bool   far = !(by < 1e30);
+    if (block == 0 && threadIdx.x == 0) {
+        float one = (float)(fmin(1.0, sqrt(sum) * by) * rsqrt((double)m.m));  // all singular values, if they are equal
+        for (int i = 0; i < steps.count; ++i) {
+            const float square = one * one, t = square * (steps.abc[3 * i + 1] + steps.abc[3 * i + 2] * square);
+            m.shift[i] = t;
+            one *= steps.abc[3 * i] + t;
+        }
+    }
     const float  by32 = (float)by;
     const int64_t at0 = ((int64_t)panel * m.mp + row0) * 64, plane = (int64_t)m.panels * m.mp * 64;
     __half* const op = work + m.operand[0] * 64;
@@ -221,12 +241,12 @@ enum Kind { kGram = 0, kSquare = 1, kApply = 2 };
 struct Params {
     const Entry* table;
     int     count, tiles, wide, stages;
-    int     from;        // which X a step starts from
+    int     from, step;  // from: which X it starts from
     __half* work;
     int*    failed;      // a wait ran out
     float   product;     // factor of the finished sums
     float   old;         // kSquare: of A; kApply: a
-    float   scale;       // kApply: of the operands
+    float   scale;       // kSquare: of B; kApply: of the operands
     int     last;        // kApply: no operands are needed any more
 };
 
@@ -407,6 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
             const int row = t.row + quarter * 32 + lane, col0 = t.col + half * half_wide;
             const int limit = KIND == kApply ? m.panels * 64 : m.mp;
             const int64_t s_plane = (int64_t)(m.mp / 64) * m.mp * 64, x_plane = (int64_t)m.panels * m.mp * 64;
+            const float shift = KIND == kGram ? 0.f : m.shift[p.step], old = KIND == kApply ? p.old + shift : p.old;
             auto finish = [&](float* v, int c) {  // 32 columns
                 const int col = col0 + c;
                 if (col >= limit) return;
@@ -417,8 +438,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const float4 x = was[j];
-                        v[4 * j] = fmaf(p.old, x.x, v[4 * j] * p.product), v[4 * j + 1] = fmaf(p.old, x.y, v[4 * j + 1] * p.product);
-                        v[4 * j + 2] = fmaf(p.old, x.z, v[4 * j + 2] * p.product), v[4 * j + 3] = fmaf(p.old, x.w, v[4 * j + 3] * p.product);
+                        v[4 * j] = fmaf(old, x.x, v[4 * j] * p.product), v[4 * j + 1] = fmaf(old, x.y, v[4 * j + 1] * p.product);
+                        v[4 * j + 2] = fmaf(old, x.z, v[4 * j + 2] * p.product), v[4 * j + 3] = fmaf(old, x.w, v[4 * j + 3] * p.product);
                         to[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
                     }
                     if (p.last) return;
@@ -442,9 +463,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                                 const float2 l = __half22float2(reinterpret_cast<const __half2&>(lo[i]));
                                 a.x += l.x, a.y += l.y;
                             }
-                            v[8 * j + 2 * i]     = fmaf(p.old, a.x, v[8 * j + 2 * i] * p.product);
-                            v[8 * j + 2 * i + 1] = fmaf(p.old, a.y, v[8 * j + 2 * i + 1] * p.product);
+                            v[8 * j + 2 * i]     = fmaf(old, a.x, v[8 * j + 2 * i] * p.product);
+                            v[8 * j + 2 * i + 1] = fmaf(old, a.y, v[8 * j + 2 * i + 1] * p.product);
                         }
+                    }
+                    const int hit = row - col;  // the diagonal's place among these columns
+                    if (hit >= 0 && hit < 32) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] -= j == hit ? shift * p.scale : 0.f;
                     }
                 } else {
 #pragma unroll
@@ -544,12 +570,13 @@ bool steps_of(const double* abc, int count, std::vector<Step>* steps) {
     for (int i = 0; i < count; ++i) {
         const double a = abc[3 * i], b = abc[3 * i + 1], c = abc[3 * i + 2];
         if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
-        double factor = 0, next = 0;
+        double low = 0, high = 0, next = 0;  // of B, less any of its own values
         for (int j = 0; j <= 4096; ++j) {
             const double s = most * j / 4096, f = b * s * s + c * s * s * s * s;
-            factor = std::max(factor, std::fabs(f)), next = std::max(next, std::fabs(s * (a + f)));
+            low = std::min(low, f), high = std::max(high, f), next = std::max(next, std::fabs(s * (a + f)));
         }
-        factor *= 1.01, next *= 1.01;
+        const double factor = 1.01 * (high - low);
+        next *= 1.01;
         Step s = {(float)a, (float)b, (float)c, exponent(most), exponent(most * most), exponent(factor)};
         steps->push_back(s);
         if (!(next < 1e6)) return false;
@@ -566,7 +593,7 @@ struct Chain {  // matrices of a chain of launches, and what its workspace holds
     size_t   bytes;
 };
 
-Chain chain_of(const Matrix* matrices, int64_t count, int parts, void* work) {
+Chain chain_of(const Matrix* matrices, int64_t count, int parts, int steps, void* work) {
     Chain c;
     Parts w(work);
     c.failed = w.take<int32_t>(64);
@@ -585,6 +612,7 @@ Chain chain_of(const Matrix* matrices, int64_t count, int parts, void* work) {
         e.first_chunk = (int)c.chunks, e.first_block = (int)c.blocks;
         c.chunks += e.chunks, c.blocks += (int64_t)e.panels * (e.mp / 64);
         e.partial = w.take<double>(e.chunks);
+        e.shift   = w.take<float>(steps);
         const int64_t values = (int64_t)e.panels * e.mp * 64;
         for (int j = 0; j < 2; ++j) e.x[j] = w.take<float>(values);
         for (int j = 0; j < 2; ++j) {
@@ -664,6 +692,9 @@ int run_chain(Chain& c, const Rates& rates, const std::vector<Step>& steps, char
     const int64_t lines = (int64_t)(c.bytes / 128);
     if (!map_of(&map, work, false, 64, lines, 1, 64, lines * 64, 64, 64)) return FRAMEWISE_B200_TENSOR_MAP;
     FW_TRY(cudaMemsetAsync(c.failed, 0, 4, stream));
+    Steps abc;
+    abc.count = (int)steps.size();
+    for (size_t i = 0; i < steps.size(); ++i) abc.abc[3 * i] = steps[i].a, abc.abc[3 * i + 1] = steps[i].b, abc.abc[3 * i + 2] = steps[i].c;
     for (int i = 0; i < count; i += kSlots) {
         Slots s;
         s.count = std::min(kSlots, count - i), s.base = i, s.table = c.table;
@@ -673,7 +704,7 @@ int run_chain(Chain& c, const Rates& rates, const std::vector<Step>& steps, char
         FW_LAUNCHED();
     }
     __half* const halves = reinterpret_cast<__half*>(work);
-    k_muon_begin<X, PARTS><<<(unsigned)c.blocks, 256, 0, stream>>>(c.table, count, rates, std::ldexp(1.f, steps[0].x), halves);
+    k_muon_begin<X, PARTS><<<(unsigned)c.blocks, 256, 0, stream>>>(c.table, count, rates, std::ldexp(1.f, steps[0].x), halves, abc);
     FW_LAUNCHED();
     auto stages = [&](int wide) { return std::min(kMostStages, (kShared - 1024) / (PARTS * (kRowsPerCta + wide) * kDepth * 2)); };
     Params p = {};
@@ -681,10 +712,10 @@ int run_chain(Chain& c, const Rates& rates, const std::vector<Step>& steps, char
     const int grid_sym = (int)std::min<int64_t>(sym, sms), grid_apply = (int)std::min<int64_t>(apply, sms);
     for (size_t i = 0; i < steps.size(); ++i) {
         const Step& s = steps[i];
-        p.from = (int)(i & 1), p.tiles = (int)sym, p.wide = wide_sym, p.stages = stages(wide_sym), p.last = 0;
+        p.step = (int)i, p.from = (int)(i & 1), p.tiles = (int)sym, p.wide = wide_sym, p.stages = stages(wide_sym), p.last = 0;
         p.product = std::ldexp(1.f, s.gram - 2 * s.x);
         FW_DO(launch<kGram, PARTS>(map, p, grid_sym, stream));
-        p.product = std::ldexp(s.c, s.factor - 2 * s.gram), p.old = std::ldexp(s.b, s.factor - s.gram);
+        p.product = std::ldexp(s.c, s.factor - 2 * s.gram), p.old = std::ldexp(s.b, s.factor - s.gram), p.scale = std::ldexp(1.f, s.factor);
         FW_DO(launch<kSquare, PARTS>(map, p, grid_sym, stream));
         p.tiles = (int)apply, p.wide = wide_apply, p.stages = stages(wide_apply);
         p.product = std::ldexp(1.f, -s.factor - s.x), p.old = s.a, p.last = i + 1 == steps.size();
@@ -697,10 +728,11 @@ int run_chain(Chain& c, const Rates& rates, const std::vector<Step>& steps, char
 }
 
 size_t bytes_for(const std::vector<Matrix>& list, int parts) {
+    // (room for the most steps, so that it does not depend on them)
     size_t most = 256;
     for (size_t i = 0; i < list.size();) {
         const int64_t n = together(list.data() + i, (int64_t)(list.size() - i), parts);
-        most = std::max(most, chain_of(list.data() + i, n, parts, nullptr).bytes);
+        most = std::max(most, chain_of(list.data() + i, n, parts, kMostSteps, nullptr).bytes);
         i += n;
     }
     return most;
@@ -711,11 +743,11 @@ int run(const std::vector<Matrix>& list, int dtype, const Rates& rates, const do
     if (list.empty()) return FRAMEWISE_B200_OK;
     const int parts = dtype == FRAMEWISE_B200_F32 ? 2 : 1;
     std::vector<Step> plan;
-    if (!work || misaligned(work) || !coefficients || steps < 1 || steps > 100 || !steps_of(coefficients, steps, &plan)) return FRAMEWISE_B200_BAD_ARGUMENT;
+    if (!work || misaligned(work) || !coefficients || steps < 1 || steps > kMostSteps || !steps_of(coefficients, steps, &plan)) return FRAMEWISE_B200_BAD_ARGUMENT;
     if (work_bytes < bytes_for(list, parts)) return FRAMEWISE_B200_WORKSPACE;
     for (size_t i = 0; i < list.size();) {
         const int64_t n = together(list.data() + i, (int64_t)(list.size() - i), parts);
-        Chain c = chain_of(list.data() + i, n, parts, work);
+        Chain c = chain_of(list.data() + i, n, parts, kMostSteps, work);
         FW_DO(dtype == FRAMEWISE_B200_F32 ? run_chain<float>(c, rates, plan, static_cast<char*>(work), stream)
                                           : run_chain<__nv_bfloat16>(c, rates, plan, static_cast<char*>(work), stream));
         i += n;
