@@ -25,7 +25,9 @@ using namespace tensor_core;
 constexpr int   kMostTop  = 32;      // alternatives: one per lane
 constexpr int   kWarps    = 8;       // per CTA
 constexpr int   kMostTeam = 64;      // warps that share a row: up to 8 CTAs
-constexpr int   kAhead    = 4;       // vectors of 8 logits that a lane has under way
+constexpr int   kAhead    = 4;       // vectors of 8 logits that a lane has under way: a block
+constexpr int   kCells    = 16;      // blocks between looks for the best
+constexpr int   kFew      = 8;       // alternatives that the lanes' largest cells alone single out well
 constexpr float kLog2e    = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNever    = -200.f;  // of an exponent of 2: zero in 32 bits
 
@@ -50,38 +52,79 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one is
     return d;
 }
 
-// 8 logits in a row, once (32 bytes aligned for f32, 16 for bf16)
-__device__ __forceinline__ void load8(const float* x, float (&v)[8]) {
-    asm volatile("ld.global.L1::no_allocate.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
-                 : "l"(x));
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
-__device__ __forceinline__ void load8(const __nv_bfloat16* x, float (&v)[8]) {
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+    return d;
+}
+
+// 8 logits in a row, as they are in memory (aligned: 32 bytes for f32, 16 for bf16)
+template <typename X>
+struct Raw;
+template <>
+struct Raw<float> {
+    float w[8];
+    __device__ __forceinline__ void load(const float* x) {
+        asm volatile("ld.global.L1::no_allocate.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=f"(w[0]), "=f"(w[1]), "=f"(w[2]), "=f"(w[3]), "=f"(w[4]), "=f"(w[5]), "=f"(w[6]), "=f"(w[7])
+                     : "l"(x));
+    }
+    __device__ __forceinline__ void set(int i, const float* x) { w[i] = x ? *x : -INFINITY; }
+    __device__ __forceinline__ float get(int i) const { return w[i]; }
+};
+template <>
+struct Raw<__nv_bfloat16> {
     uint32_t w[4];
-    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(x));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-}
+    __device__ __forceinline__ void load(const __nv_bfloat16* x) {
+        asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(x));
+    }
+    __device__ __forceinline__ void set(int i, const __nv_bfloat16* x) {
+        const uint32_t v = x ? *reinterpret_cast<const uint16_t*>(x) : 0xff80u;  // -inf
+        w[i / 2] = i % 2 ? (w[i / 2] & 0xffffu) | v << 16 : v;
+    }
+    __device__ __forceinline__ float get(int i) const { return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); }
+};
 __device__ __forceinline__ float value(float x) { return x; }
 __device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// A row in vectors of 8 whose addresses are aligned: the first begins `ahead` places before the row.  Places outside of the
-// row are not read and hold -inf, which changes no sum.
+// A row in vectors of 8, 32 of them a step.  The vectors' addresses are aligned: the first begins `ahead` places before the row.
+// Places outside of the row are not read and hold -inf, which changes no sum.
 template <typename X>
 struct Row {
     const X* x;
-    int      V, ahead, steps;  // steps: of 32 vectors
+    int      V, ahead, steps;
     __device__ Row(const X* x, int V) : x(x), V(V) {
         ahead = (int)(reinterpret_cast<uintptr_t>(x) / sizeof(X) % 8);
         steps = ((V + ahead + 7) / 8 + 31) / 32;
     }
-    __device__ int first(int step, int lane) const { return (step * 32 + lane) * 8 - ahead; }
-    __device__ void load(int at, float (&v)[8]) const {
-        if (at >= 0 && at + 8 <= V) {
-            load8(x + at, v);
+    __device__ __forceinline__ int first(int step, int lane) const { return (step * 32 + lane) * 8 - ahead; }
+    // A block: kAhead steps, `team` apart.
+    __device__ __forceinline__ bool inside(int step, int team) const {
+        return step * 256 >= ahead && (step + (kAhead - 1) * team + 1) * 256 - ahead <= V;
+    }
+    __device__ __forceinline__ void load(int step, int team, int lane, Raw<X> (&v)[kAhead], bool aligned = true) const {
+        if (aligned && inside(step, team)) {
+            const X* const from = x + first(step, lane);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) v[i].load(from + (int64_t)i * team * 256);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = at + i >= 0 && at + i < V ? value(x[at + i]) : -INFINITY;
+            for (int i = 0; i < kAhead; ++i) {
+                const int at = first(step + i * team, lane);
+                if (aligned && at >= 0 && at + 8 <= V) {
+                    v[i].load(x + at);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[i].set(j, at + j >= 0 && at + j < V ? x + at + j : nullptr);
+                }
+            }
         }
     }
 };
@@ -131,52 +174,8 @@ __device__ __forceinline__ Sums joined(Sums a, Sums b) {
     return {m, a.s + b.s, a.t + b.t};
 }
 
-// The 32 largest that a warp has met, a lane each, and those that wait to be sorted in: more than 32 never wait, so that a
-// row in rising order costs a network per 32 of its values.
-struct Best {
-    uint64_t  list;
-    uint64_t* wait;  // of this warp, 64 of them
-    int       count, top;
-    float     least;  // the list's last that counts: only larger values come in
-    bool      full, sure;  // sure: nothing can come in any more (NaN throughout)
-    __device__ Best(uint64_t* wait, int top) : list(0), wait(wait), count(0), top(top), least(-INFINITY), full(false), sure(false) {}
-    __device__ void sort_in(int lane) {
-        __syncwarp();
-        const uint64_t key = lane < min(count, 32) ? wait[lane] : 0, rest = lane + 32 < count ? wait[lane + 32] : 0;
-        __syncwarp();
-        list = joined(list, sorted(key, lane), lane);
-        count = max(0, count - 32);
-        if (lane < count) wait[lane] = rest;
-        const uint64_t last = __shfl_sync(0xffffffffu, list, top - 1);
-        full  = last != 0;
-        sure  = (uint32_t)(last >> 32) == 0xffffffffu;
-        least = full ? value_of(last) : -INFINITY;
-        __syncwarp();
-    }
-    // 8 values a lane, the first of index `at`; `most`: their maximum.  What the list holds when a step begins has lower
-    // indices than the step's values: equal ones stay out.  Within the step they come in any order, and equal ones come in.
-    __device__ void meet(const float (&v)[8], float most, int at, int V, float from, int lane) {
-        const bool  before = full;
-        const float floor  = least;
-        if (before && sure) return;
-        if (!__any_sync(0xffffffffu, before ? !(most <= floor) : !(most < from))) return;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const bool in = at + i >= 0 && at + i < V && (before ? !(v[i] <= floor) : !(v[i] < from)) && !(v[i] < least);
-            const uint32_t lanes = __ballot_sync(0xffffffffu, in);
-            if (!lanes) continue;
-            if (in) wait[count + __popc(lanes & ((1u << lane) - 1))] = key_of(v[i], at + i);
-            count += __popc(lanes);
-            if (count >= 32) sort_in(lane);
-        }
-    }
-    __device__ void finish(int lane) {
-        while (count > 0) sort_in(lane);
-    }
-};
-
-// The `top`-th largest of the lanes' values: at least as many of a row's are no smaller.
-__device__ __forceinline__ float nth_of_lanes(float v, int top, int lane) {
+// The lanes' values in falling order.
+__device__ __forceinline__ float falling(float v, int lane) {
 #pragma unroll
     for (int k = 2; k <= 32; k <<= 1)
 #pragma unroll
@@ -184,8 +183,102 @@ __device__ __forceinline__ float nth_of_lanes(float v, int top, int lane) {
             const float o = __shfl_xor_sync(0xffffffffu, v, j);
             v = ((lane & j) == 0) == ((lane & k) == 0) ? fmaxf(v, o) : fminf(v, o);
         }
-    return __shfl_sync(0xffffffffu, v, top - 1);
+    return v;
 }
+
+// What a warp needs to find a row's best.
+struct Room {
+    float    cell[kCells][32];
+    uint16_t near[kCells * 32];
+    uint64_t wait[64];
+};
+
+// The best that a warp has met.  While the sums are formed only the maximum of each cell, the 32 values that a lane has of a
+// block, is written down.  After kCells blocks, or at the row's end, those cells are read again whose maximum is no smaller
+// than the `top`-th largest of the lanes' maxima: some more than `top` of them.  (Looking at each value while the sums are formed,
+// against the list so far: 26 instructions a value for the whole kernel, 20000 x 12001 f32 with 8 alternatives 664 us; 219 this way,
+// and 148 without alternatives.)
+struct Best {
+    uint64_t list;    // the 32 largest so far, a lane each, in falling order
+    Room&    room;
+    int      count, top;
+    float    least;   // the last of the list that counts
+    bool     full;
+    __device__ Best(Room& room, int top) : list(0), room(room), count(0), top(top), least(-INFINITY), full(false) {}
+    // those that wait; more than 32 never do, so that a row in rising order costs a network per 32 of its values
+    __device__ void sort_in(int lane) {
+        __syncwarp();
+        const uint64_t key = lane < min(count, 32) ? room.wait[lane] : 0, rest = lane + 32 < count ? room.wait[lane + 32] : 0;
+        __syncwarp();
+        list  = joined(list, sorted(key, lane), lane);
+        count = max(0, count - 32);
+        if (lane < count) room.wait[lane] = rest;
+        const uint64_t last = __shfl_sync(0xffffffffu, list, top - 1);
+        full  = last != 0;
+        least = full ? value_of(last) : -INFINITY;
+        __syncwarp();
+    }
+    template <typename X>
+    __device__ void look(const Row<X>& row, int step, int team, int blocks, int lane) {  // the first block's first step
+        __syncwarp();
+        float most = -INFINITY, second = -INFINITY;
+        for (int b = 0; b < blocks; ++b) {
+            float c = room.cell[b][lane];
+            c = c != c ? INFINITY : c;
+            second = fmaxf(second, fminf(most, c)), most = fmaxf(most, c);
+        }
+        // The `top`-th largest of the lanes' maxima, or of their two largest cells: as many cells' are no smaller.
+        float order = falling(most, lane);
+        if (top > kFew) {
+            order = fmaxf(order, __shfl_sync(0xffffffffu, falling(second, lane), 31 - lane));
+#pragma unroll
+            for (int j = 16; j > 0; j >>= 1) {
+                const float o = __shfl_xor_sync(0xffffffffu, order, j);
+                order = (lane & j) == 0 ? fmaxf(order, o) : fminf(order, o);
+            }
+        }
+        const float from = __shfl_sync(0xffffffffu, order, top - 1);
+        int cells = 0;
+        for (int b = 0; b < blocks; ++b) {
+            const float    c = room.cell[b][lane];
+            const bool     in = !(c < from) && !(full && c <= least);
+            const uint32_t lanes = __ballot_sync(0xffffffffu, in);
+            if (in) room.near[cells + __popc(lanes & ((1u << lane) - 1))] = (uint16_t)(b * 32 + lane);
+            cells += __popc(lanes);
+        }
+        __syncwarp();
+        // What the list holds when a block begins has lower indices than the block's values: equal ones stay out.  Within a block
+        // they come in any order, and equal ones come in.  (NaN: nothing is larger, and `least` is as large.)
+        int   block = -1;
+        bool  before = false;
+        float floor = -INFINITY;
+        constexpr int kLoads = 12;
+        for (int i = 0; i < cells; i += kLoads) {
+            float v[kLoads];
+#pragma unroll
+            for (int q = 0; q < kLoads; ++q) {
+                v[q] = -INFINITY;
+                if (i + q >= cells) continue;
+                const int cell = room.near[i + q], at = row.first(step + (cell / 32 * kAhead + lane / 8) * team, cell % 32) + lane % 8;
+                const float c = room.cell[cell / 32][cell % 32];
+                if (cell / 32 != block && full && (c <= least || least != least)) continue;  // has been overtaken
+                if (at >= 0 && at < row.V) v[q] = value(row.x[at]);
+            }
+#pragma unroll
+            for (int q = 0; q < kLoads; ++q) {
+                if (i + q >= cells) break;
+                const int cell = room.near[i + q], at = row.first(step + (cell / 32 * kAhead + lane / 8) * team, cell % 32) + lane % 8;
+                if (cell / 32 != block) block = cell / 32, before = full, floor = least;
+                const bool in = at >= 0 && at < row.V && !(v[q] < from) && !(before && (v[q] <= floor || floor != floor)) && !(v[q] < least);
+                const uint32_t lanes = __ballot_sync(0xffffffffu, in);
+                if (in) room.wait[count + __popc(lanes & ((1u << lane) - 1))] = key_of(v[q], at);
+                count += __popc(lanes);
+                if (count >= 32) sort_in(lane);
+            }
+        }
+        while (count > 0) sort_in(lane);
+    }
+};
 
 struct Scored {
     float*  log_prob;
@@ -198,10 +291,10 @@ struct Scored {
 // A row per team of r.team warps (1 to 8 of a CTA; 16 to 64: all of 2 to 8 CTAs of a cluster), which take its steps of 256
 // logits in turn.
 template <typename X, typename L, bool TOP>
-__global__ void __launch_bounds__(kWarps * 32) k_label_scores(const X* __restrict__ z, const Rows r, const Scored out) {
+__global__ void __launch_bounds__(kWarps * 32, sizeof(X) == 4 && !TOP ? 4 : 3) k_label_scores(const X* __restrict__ z, const Rows r, const Scored out) {
     __shared__ Sums     part[kWarps];
     __shared__ uint64_t best[TOP ? kWarps : 1][32];
-    __shared__ uint64_t waiting[TOP ? kWarps : 1][64];
+    __shared__ Room     room[TOP ? kWarps : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int ctas = r.team > kWarps ? r.team / kWarps : 1, in_cta_team = min(r.team, kWarps);
     const int rank = ctas > 1 ? (int)(blockIdx.x % ctas) : 0;
@@ -211,40 +304,30 @@ __global__ void __launch_bounds__(kWarps * 32) k_label_scores(const X* __restric
     const bool inside = n < r.N, counts = inside && counted<L>(r, n, label);
     const X* const x = counts ? z + (int64_t)((uint32_t)n / (uint32_t)r.T) * r.stride_b + (int64_t)((uint32_t)n % (uint32_t)r.T) * r.stride_t : z;
 
+    float at_label = __uint_as_float(0x7fffffffu);  // NaN outside of the vocabulary
+    if (counts && member == 0 && lane == 0 && label >= 0 && label < r.V) at_label = value(x[label]);
     Sums a = {-FLT_MAX, 0.f, 0.f};
-    Best b(TOP ? waiting[warp] : nullptr, r.top);
+    Best b(room[TOP ? warp : 0], r.top);
     if (counts) {
         const Row<X> row(x, r.V);
-        float from = -INFINITY;  // smaller values than this are not among the best
-        for (int step = member; step < row.steps; step += r.team * kAhead) {
-            float v[kAhead][8];
+        constexpr bool kEarly = sizeof(X) == 2;  // the next block is loaded before this one is worked on
+        Raw<X> v[kAhead], next[kEarly ? kAhead : 1];
+        const int hop = r.team * kAhead;
+        int blocks = 0, looked = member;
+        if (member < row.steps) row.load(member, r.team, lane, v);
+        for (int step = member; step < row.steps; step += hop) {
+            const bool more = step + hop < row.steps;
+            if constexpr (kEarly)
+                if (more) row.load(step + hop, r.team, lane, next);
+            float all = max_nan(v[0].get(0), v[0].get(1), v[0].get(2)), other = max_nan(v[0].get(3), v[0].get(4), v[0].get(5));
+            all = max_nan(all, v[0].get(6), v[0].get(7));
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const int s = step + i * r.team;
-                if (s < row.steps) {
-                    row.load(row.first(s, lane), v[i]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[i][j] = -INFINITY;
-                }
+            for (int i = 1; i < kAhead; ++i) {
+                all   = max_nan(max_nan(all, v[i].get(0), v[i].get(1)), v[i].get(2), v[i].get(3));
+                other = max_nan(max_nan(other, v[i].get(4), v[i].get(5)), v[i].get(6), v[i].get(7));
             }
-            float most[kAhead];
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                most[i] = v[i][0];
-#pragma unroll
-                for (int j = 1; j < 8; ++j) most[i] = max_nan(most[i], v[i][j]);
-            }
-            float all = max_nan(max_nan(most[0], most[1]), max_nan(most[2], most[3]));
-            static_assert(kAhead == 4, "");
-            if constexpr (TOP) {
-                if (step == member) from = nth_of_lanes(all != all ? INFINITY : all, r.top, lane);
-                if (__any_sync(0xffffffffu, b.full ? !b.sure && !(all <= b.least) : !(all < from))) {
-#pragma unroll
-                    for (int i = 0; i < kAhead; ++i)
-                        if (step + i * r.team < row.steps) b.meet(v[i], most[i], row.first(step + i * r.team, lane), r.V, from, lane);
-                }
-            }
+            all = max_nan(all, other);
+            if (TOP) room[warp].cell[blocks][lane] = all;
             const float m = max_nan(a.m, all);
             rescale(a, m);
             const float2 off = make_float2(-m, -m), scale = make_float2(kLog2e, kLog2e);
@@ -253,18 +336,29 @@ __global__ void __launch_bounds__(kWarps * 32) k_label_scores(const X* __restric
             for (int i = 0; i < kAhead; ++i)
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
-                    float2 d = mul2(add2(make_float2(v[i][j], v[i][j + 1]), off), scale);
+                    float2 d = mul2(add2(make_float2(v[i].get(j), v[i].get(j + 1)), off), scale);
                     d = make_float2(max_nan(d.x, kNever), max_nan(d.y, kNever));
                     const float2 e = make_float2(exp2_approx(d.x), exp2_approx(d.y));
                     s = add2(s, e);
-                    t = add2(t, mul2(e, d));
+                    t = fma2(e, d, t);
                 }
             a.s += s.x + s.y;
             a.t += t.x + t.y;
+            if (TOP && (++blocks == kCells || !more)) {
+                b.look(row, looked, r.team, blocks, lane);
+                blocks = 0, looked = step + hop;
+            }
+            if (more) {
+                if constexpr (kEarly) {
+#pragma unroll
+                    for (int i = 0; i < kAhead; ++i) v[i] = next[i];
+                } else {
+                    row.load(step + hop, r.team, lane, v);
+                }
+            }
         }
 #pragma unroll
         for (int j = 16; j > 0; j >>= 1) a = joined(a, {__shfl_xor_sync(0xffffffffu, a.m, j), __shfl_xor_sync(0xffffffffu, a.s, j), __shfl_xor_sync(0xffffffffu, a.t, j)});
-        if constexpr (TOP) b.finish(lane);
     }
     // the team's parts, pairs of warps at a time
     if (r.team > 1) {
@@ -306,7 +400,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_label_scores(const X* __restric
     const float log2_s = log2f(a.s), entropy = a.s == 0.f ? 0.f : kLn2 * (log2_s - a.t / a.s);
     auto log_prob = [&](float v) { return a.s == 0.f ? -INFINITY : (v - a.m) - kLn2 * log2_s; };
     if (lane == 0) {
-        out.log_prob[n] = !counts ? 0.f : label < 0 || label >= r.V ? __uint_as_float(0x7fffffffu) : log_prob(value(x[label]));
+        out.log_prob[n] = !counts ? 0.f : at_label != at_label ? at_label : log_prob(at_label);
         out.entropy[n]  = counts ? entropy : 0.f;
         if (out.kept) out.kept[n] = make_float4(a.m, log2_s, entropy, 0.f);
     }
@@ -339,7 +433,7 @@ __device__ __forceinline__ void put(__nv_bfloat16* to, float v) { *to = __float2
 
 // The gradient: a row per team as above, in steps that are aligned where it is written (`even`: and where it is read).
 template <typename X, typename L>
-__global__ void __launch_bounds__(kWarps * 32) k_label_scores_back(const X* __restrict__ z, const Rows r, const Incoming in, X* __restrict__ dz) {
+__global__ void __launch_bounds__(kWarps * 32, sizeof(X) == 4 ? 4 : 3) k_label_scores_back(const X* __restrict__ z, const Rows r, const Incoming in, X* __restrict__ dz) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t all = (int64_t)blockIdx.x * kWarps + warp, n = all / r.team;
     const int member = (int)(all % r.team);
@@ -382,37 +476,50 @@ __global__ void __launch_bounds__(kWarps * 32) k_label_scores_back(const X* __re
         return;
     }
     const X* const x = z + seq * r.stride_b + at_t * r.stride_t;
+    // read by vectors where they are aligned in the logits as in the gradient
     const bool even = (reinterpret_cast<uintptr_t>(x) / sizeof(X)) % 8 == row.ahead;
-    const Row<X> from(x, r.V);
-    auto gradient = [&](float v) {
-        const float l = max_nan((v - kept.x) * kLog2e - kept.y, kNever);  // log2 p
-        return exp2_approx(l) * (c0 + c1 * l);
+    Row<X> from(x, r.V);
+    from.ahead = row.ahead, from.steps = row.steps;
+    const float2 off = make_float2(-kept.x, -kept.x), scale = make_float2(kLog2e, kLog2e), log2_s = make_float2(-kept.y, -kept.y);
+    const float2 c0s = make_float2(c0, c0), c1s = make_float2(c1, c1);
+    auto gradients = [&](float2 v) {
+        float2 l = fma2(add2(v, off), scale, log2_s);  // log2 p
+        l = make_float2(max_nan(l.x, kNever), max_nan(l.y, kNever));
+        return mul2(make_float2(exp2_approx(l.x), exp2_approx(l.y)), fma2(c1s, l, c0s));
     };
-    for (int step = member; step < row.steps; step += r.team * kAhead) {
-        float v[kAhead][8];
+    auto gradient = [&](float v) { return gradients(make_float2(v, v)).x; };
+    constexpr bool kEarly = sizeof(X) == 2;
+    Raw<X> v[kAhead], next[kEarly ? kAhead : 1];
+    const int hop = r.team * kAhead;
+    if (member < row.steps) from.load(member, r.team, lane, v, even);
+    for (int step = member; step < row.steps; step += hop) {
+        const bool more = step + hop < row.steps;
+        if constexpr (kEarly)
+            if (more) from.load(step + hop, r.team, lane, next, even);
+        const bool inside = row.inside(step, r.team);
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const int s = step + i * r.team, at = row.first(s, lane);
-            if (s >= row.steps) continue;
-            if (even) {
-                from.load(at, v[i]);
-            } else {
+            float out[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] = at + j >= 0 && at + j < r.V ? value(x[at + j]) : -INFINITY;
+            for (int j = 0; j < 8; j += 2) {
+                const float2 g2 = gradients(make_float2(v[i].get(j), v[i].get(j + 1)));
+                out[j] = g2.x, out[j + 1] = g2.y;
             }
-        }
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const int s = step + i * r.team, at = row.first(s, lane);
-            if (s >= row.steps) continue;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = gradient(v[i][j]);
-            if (at >= 0 && at + 8 <= r.V) {
-                store8(to + at, v[i]);
+            const int at = row.first(step + i * r.team, lane);
+            if (inside || (at >= 0 && at + 8 <= r.V)) {
+                store8(to + at, out);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (at + j >= 0 && at + j < r.V) put(to + at + j, v[i][j]);
+                    if (at + j >= 0 && at + j < r.V) put(to + at + j, out[j]);
+            }
+        }
+        if (more) {
+            if constexpr (kEarly) {
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) v[i] = next[i];
+            } else {
+                from.load(step + hop, r.team, lane, v, even);
             }
         }
     }
