@@ -48,8 +48,9 @@ constexpr int kThreads      = 64 + 32 * kEpilogue;
 constexpr int kShared       = 232448 - 2048;  // dynamic; the rest: the static arrays
 constexpr uint64_t kPatience = 4000000000ull;  // nanoseconds after which a wait gives up; they end within microseconds
 
-// A matrix of a chain.  Its parts of the workspace are in panels of 64 columns, in which the rows follow each other: a row of
-// fp16 is 128 bytes there, a tensor copy's line.
+// A matrix of a chain.  Operands lie in panels of 64 columns of fp16, in which the rows follow each other: a row is 128 bytes
+// there, a tensor copy's line.  X itself is met by warps whose lanes have a row each: squares of 32 x 32 values, in which four
+// columns of 32 rows, 512 bytes, follow each other (see place).
 struct Entry {
     const void* grad;
     float*      momentum;   // or null: grad is what is made orthogonal
@@ -95,14 +96,51 @@ __device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162floa
 __device__ __forceinline__ void put(float* to, float v) { *to = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* to, float v) { *to = __float2bfloat16_rn(v); }
 
+// Where a value of X lies.
+__device__ __forceinline__ int64_t place(int mp, int row, int col) {
+    return ((int64_t)(col / 32) * (mp / 32) + row / 32) * 1024 + col % 32 / 4 * 128 + row % 32 * 4 + col % 4;
+}
+
 struct Rates {
     float keep, beta, nesterov;  // 1 - beta; nesterov: 0 or 1
     float eps, decay;            // decay: 1 - lr weight_decay
     int   follow;
 };
 
+// The nearest fp16 numbers of two values, which keep what is left of them.
+__device__ __forceinline__ uint32_t part_of(float2& v) {
+    const __half2 h = __floats2half2_rn(v.x, v.y);
+    const float2  back = __half22float2(h);
+    v.x -= back.x, v.y -= back.y;
+    return reinterpret_cast<const uint32_t&>(h);
+}
+
 // what is made orthogonal, from the gradient and the new momentum
 __device__ __forceinline__ float direction(float g, float v, const Rates& r) { return r.nesterov != 0.f ? g + (v - g) * r.beta : v; }
+
+// four values in a row; `wide`: aligned for one access, else as many as there are (`left`)
+__device__ __forceinline__ void load4(const float* x, bool wide, int left, float (&v)[4]) {
+    if (wide) {
+        const float4 a = *reinterpret_cast<const float4*>(x);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = i < left ? x[i] : 0.f;
+    }
+}
+__device__ __forceinline__ void load4(const __nv_bfloat16* x, bool wide, int left, float (&v)[4]) {
+    if (wide) {
+        const uint2 a = *reinterpret_cast<const uint2*>(x);
+        v[0] = __uint_as_float(a.x << 16), v[1] = __uint_as_float(a.x & 0xffff0000u), v[2] = __uint_as_float(a.y << 16), v[3] = __uint_as_float(a.y & 0xffff0000u);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = i < left ? value(x[i]) : 0.f;
+    }
+}
+template <typename X>
+__device__ __forceinline__ bool aligned4(const X* g, const float* v) {
+    return reinterpret_cast<uintptr_t>(g) % (4 * sizeof(X)) == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0;
+}
 
 // Momentum, and the sum of squares of each chunk in 64 bits (so that no square leaves the range); writes the table down.
 template <typename X>
@@ -115,17 +153,44 @@ __global__ void __launch_bounds__(256) k_muon_collect(const __grid_constant__ Sl
         int*       to   = reinterpret_cast<int*>(s.table + s.base + e);
         for (int i = threadIdx.x; i < (int)(sizeof(Entry) / 4); i += 256) to[i] = from[i];
     }
-    const int64_t all = (int64_t)m.rows * m.cols, begin = (int64_t)chunk * kChunk, end = min(all, begin + kChunk);
-    const X* const g = static_cast<const X*>(m.grad);
+    const int64_t begin = (int64_t)chunk * kChunk;
+    const int     left = (int)min((int64_t)m.rows * m.cols - begin, (int64_t)kChunk);
+    const X* const g = static_cast<const X*>(m.grad) + begin;
+    float* const   v = m.momentum ? m.momentum + begin : nullptr;
+    const bool wide = aligned4(g, v);
     double sum = 0.0;
-    for (int64_t i = begin + threadIdx.x; i < end; i += 256) {
-        float u = value(g[i]);
-        if (m.momentum) {
-            const float v0 = m.momentum[i], v = v0 + (u - v0) * r.keep;
-            m.momentum[i] = v;
-            u = direction(u, v, r);
+    constexpr int kAhead = 4;
+    for (int i0 = threadIdx.x * 4; i0 < left; i0 += 1024 * kAhead) {
+        float u[kAhead][4], old[kAhead][4];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const int i = i0 + a * 1024;
+            if (i >= left) continue;
+            load4(g + i, wide && i + 4 <= left, left - i, u[a]);
+            if (v) load4(v + i, wide && i + 4 <= left, left - i, old[a]);
         }
-        sum += (double)u * (double)u;
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const int i = i0 + a * 1024;
+            if (i >= left) continue;
+            if (v) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    old[a][j] += (u[a][j] - old[a][j]) * r.keep;
+                    u[a][j] = direction(u[a][j], old[a][j], r);
+                }
+                if (wide && i + 4 <= left) {
+                    *reinterpret_cast<float4*>(v + i) = make_float4(old[a][0], old[a][1], old[a][2], old[a][3]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (i + j < left) v[i + j] = old[a][j];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (i + j < left) sum += (double)u[a][j] * (double)u[a][j];
+        }
     }
 #pragma unroll
     for (int j = 16; j > 0; j >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, j);
@@ -138,13 +203,6 @@ __global__ void __launch_bounds__(256) k_muon_collect(const __grid_constant__ Sl
     }
 }
 
-// fp16 parts of a value that has been brought into range
-template <int PARTS>
-__device__ __forceinline__ void split(float v, __half (&h)[PARTS]) {
-    h[0] = __float2half_rn(v);
-    if (PARTS == 2) h[PARTS - 1] = __float2half_rn(v - __half2float(h[0]));
-}
-
 // X = U / max(|U|, eps) in 32 bits and as operands: a CTA per 64 columns and rows, zeros where there are none.
 template <typename X, int PARTS>
 __global__ void __launch_bounds__(256) k_muon_begin(const Entry* __restrict__ table, int count, const Rates r, float scale, __half* work, const __grid_constant__ Steps steps) {
@@ -153,31 +211,42 @@ __global__ void __launch_bounds__(256) k_muon_begin(const Entry* __restrict__ ta
     const int   e = find(count, blockIdx.x, [&](int i) { return table[i].first_block; });
     const Entry& m = table[e];
     const int block = blockIdx.x - m.first_block, panel = block / (m.mp / 64), row0 = block % (m.mp / 64) * 64;
+    const X* const     g = static_cast<const X*>(m.grad);
+    const float* const v = m.momentum;
+    const bool tall = m.rows > m.cols;
+    // neighbours in memory first: `line` of U as it lies, four values from `at` on
+    const int  lines = tall ? m.n : m.m, line0 = tall ? panel * 64 : row0, col0 = tall ? row0 : panel * 64;
+    const bool wide = aligned4(g, v) && m.cols % 4 == 0;
+    float u[4][4], mom[4][4];
+    const int at = threadIdx.x % 16 * 4, l0 = threadIdx.x / 16, left = m.cols - col0 - at;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int line = line0 + l0 + i * 16;
+        const bool some = line < lines && left > 0;
+        const int64_t from = some ? (int64_t)line * m.cols + col0 + at : 0;
+        load4(g + from, some && wide, some ? left : 0, u[i]);
+        if (v) load4(v + from, some && wide, some ? left : 0, mom[i]);
+    }
     double sum = 0.0;
     for (int i = threadIdx.x; i < m.chunks; i += 256) sum += m.partial[i];
 #pragma unroll
     for (int j = 16; j > 0; j >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, j);
     if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = sum;
-    const X* const g = static_cast<const X*>(m.grad);
-    const bool tall = m.rows > m.cols;
-    for (int i = threadIdx.x; i < 4096; i += 256) {  // neighbours in memory first
-        const int c = i % 64, l = i / 64;
-        const int row = row0 + (tall ? c : l), col = panel * 64 + (tall ? l : c);
-        float u = 0.f;
-        if (row < m.m && col < m.n) {
-            const int64_t at = tall ? (int64_t)col * m.cols + row : (int64_t)row * m.cols + col;
-            u = value(g[at]);
-            if (m.momentum) u = direction(u, m.momentum[at], r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float x = v ? direction(u[i][j], mom[i][j], r) : u[i][j];
+            if (tall) tile[at + j][l0 + i * 16] = x;
+            else tile[l0 + i * 16][at + j] = x;
         }
-        if (tall) tile[c][l] = u;
-        else tile[l][c] = u;
-    }
     __syncthreads();
     sum = part[0];
     for (int i = 1; i < 8; ++i) sum += part[i];
     // |U| may be past the range of 32 bits (or below): 64 bits up to the quotient
     const double by = 1.0 / fmax(sqrt(sum), (double)r.eps);
     const bool   far = !(by < 1e30);
+    const float  by32 = (float)by;
     if (block == 0 && threadIdx.x == 0) {
         float one = (float)(fmin(1.0, sqrt(sum) * by) * rsqrt((double)m.m));  // all singular values, if they are equal
         for (int i = 0; i < steps.count; ++i) {
@@ -186,57 +255,35 @@ __global__ void __launch_bounds__(256) k_muon_begin(const Entry* __restrict__ ta
             one *= steps.abc[3 * i] + t;
         }
     }
-    const float  by32 = (float)by;
-    const int64_t at0 = ((int64_t)panel * m.mp + row0) * 64, plane = (int64_t)m.panels * m.mp * 64;
-    __half* const op = work + m.operand[0] * 64;
-    for (int i = threadIdx.x; i < 4096; i += 256) {
-        const float u = tile[i / 64][i % 64], x = far ? (float)(u * by) : u * by32;
-        m.x[0][at0 + i] = x;
-        __half h[PARTS];
-        split<PARTS>(x * scale, h);
+    auto x_of = [&](int row, int col) {
+        const float x = tile[row][col];
+        return far ? (float)(x * by) : x * by32;
+    };
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) op[p * plane + at0 + i] = h[p];
+    for (int i = 0; i < 4; ++i) {  // a warp: 32 rows of four columns, 512 bytes of X
+        const int row = (threadIdx.x / 32 & 1) * 32 + threadIdx.x % 32, col = (threadIdx.x / 64 + i * 4) * 4;
+        *reinterpret_cast<float4*>(m.x[0] + place(m.mp, row0 + row, panel * 64 + col)) = make_float4(x_of(row, col), x_of(row, col + 1), x_of(row, col + 2), x_of(row, col + 3));
     }
-}
-
-// p = p decay - rate X, or the result X itself: a CTA per 64 columns and rows of X.
-template <typename X>
-__global__ void __launch_bounds__(256) k_muon_finish(const Entry* __restrict__ table, int count, const Rates r, int last, const int* failed) {
-    __shared__ float tile[64][65];
-    const int   e = find(count, blockIdx.x, [&](int i) { return table[i].first_block; });
-    const Entry& m = table[e];
-    const int block = blockIdx.x - m.first_block, panel = block / (m.mp / 64), row0 = block % (m.mp / 64) * 64;
-    const float* const x = m.x[last] + ((int64_t)panel * m.mp + row0) * 64;
-    const bool none = *failed != 0;
-    for (int i = threadIdx.x; i < 4096; i += 256) tile[i / 64][i % 64] = none ? __uint_as_float(0x7fffffffu) : x[i];
-    __syncthreads();
-    const bool tall = m.rows > m.cols;
-    X* const p = static_cast<X*>(m.param);
-    for (int i = threadIdx.x; i < 4096; i += 256) {
-        const int c = i % 64, l = i / 64;
-        const int row = row0 + (tall ? c : l), col = panel * 64 + (tall ? l : c);
-        if (row >= m.m || col >= m.n) continue;
-        const int64_t at = tall ? (int64_t)col * m.cols + row : (int64_t)row * m.cols + col;
-        float o = tall ? tile[c][l] : tile[l][c];
-        if (m.momentum) {
-            float was = value(p[at]);
-            if (m.master) {
-                const float held = m.master[at];
-                X rounded;
-                put(&rounded, held);
-                // a copy of which the parameter is not the rounded value has been left behind by the program
-                if (!r.follow || value(rounded) == was || (was != was && held != held)) was = held;
-            }
-            o = was * r.decay - m.rate * o;
-            if (m.master) m.master[at] = o;
+    __half* const op = work + m.operand[0] * 64 + ((int64_t)panel * m.mp + row0) * 64;
+    const int64_t plane = (int64_t)m.panels * m.mp * 64;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // a row's 128 bytes by eight lanes
+        const int row = threadIdx.x / 8 + i * 32, col = threadIdx.x % 8 * 8;
+        uint32_t w[PARTS][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float2 x = make_float2(x_of(row, col + 2 * j) * scale, x_of(row, col + 2 * j + 1) * scale);
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) w[q][j] = part_of(x);
         }
-        put(p + at, o);
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) *reinterpret_cast<uint4*>(op + q * plane + row * 64 + col) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
     }
 }
 
 // ------------------------------------------------------------------------------------------ products
 
-enum Kind { kGram = 0, kSquare = 1, kApply = 2 };
+enum Kind { kGram = 0, kSquare = 1, kApply = 2, kLast = 3 };
 
 struct Params {
     const Entry* table;
@@ -247,7 +294,7 @@ struct Params {
     float   product;     // factor of the finished sums
     float   old;         // kSquare: of A; kApply: a
     float   scale;       // kSquare: of B; kApply: of the operands
-    int     last;        // kApply: no operands are needed any more
+    Rates   rates;       // kLast
 };
 
 // fp16 operands, f32 sums
@@ -255,23 +302,102 @@ __host__ __device__ constexpr uint32_t half_kind(int m, int n, bool b_mn) {
     return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+__device__ __forceinline__ void load_sector(const __half* x, uint32_t* w) {
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(x)
+                 : "memory");
+}
+__device__ __forceinline__ void store_sector(__half* x, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(x), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]),
+                 "r"(w[7])
+                 : "memory");
+}
+
+// p = p decay - rate X, or the result X itself, for a row a lane and 32 columns of X.  Matrices that lie are turned in shared
+// memory first (32 rows of 33 words of this warp's), so that neighbouring lanes always have neighbouring values in memory.
+constexpr int kTurn = 32 * 33 * 4;
+template <int PARTS>
+__device__ __forceinline__ void update(const Entry& m, const Rates& r, float* v, int row, int col, char* turn, int lane) {
+    using X = std::conditional_t<PARTS == 2, float, __nv_bfloat16>;
+    const bool tall = m.rows > m.cols;
+    float* const t = reinterpret_cast<float*>(turn);
+    if (!tall) {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) t[lane * 33 + j] = v[j];
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = t[j * 33 + lane];
+    }
+    // value j of a lane: line j of 32, place `at` of it
+    const int line0 = tall ? col : row - lane, at = tall ? row : col + lane, lines = min(32, m.rows - line0);
+    if (at >= m.cols) return;
+    const int64_t first = (int64_t)line0 * m.cols + at;
+    X* const p = static_cast<X*>(m.param) + first;
+    if (!m.momentum) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (j < lines) put(p + (int64_t)j * m.cols, v[j]);
+        return;
+    }
+    float* const master = m.master ? m.master + first : nullptr;
+#pragma unroll
+    for (int j0 = 0; j0 < 32; j0 += 8) {
+        float was[8], held[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            was[j] = j0 + j < lines ? value(p[(int64_t)(j0 + j) * m.cols]) : 0.f;
+            held[j] = master && j0 + j < lines ? master[(int64_t)(j0 + j) * m.cols] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (j0 + j >= lines) continue;
+            if (master) {
+                X rounded;
+                put(&rounded, held[j]);
+                // a copy of which the parameter is not the rounded value has been left behind by the program
+                if (!r.follow || value(rounded) == was[j] || (was[j] != was[j] && held[j] != held[j])) was[j] = held[j];
+            }
+            const float now = was[j] * r.decay - m.rate * v[j0 + j];
+            if (master) master[(int64_t)(j0 + j) * m.cols] = now;
+            put(p + (int64_t)(j0 + j) * m.cols, now);
+        }
+    }
+}
+
+// After a wait ran out the results are NaN.
+template <typename X>
+__global__ void __launch_bounds__(256) k_muon_check(const Entry* __restrict__ table, int count, const int* failed) {
+    if (*failed == 0) return;
+    for (int e = 0; e < count; ++e) {
+        const Entry& m = table[e];
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)m.rows * m.cols; i += (int64_t)gridDim.x * 256) {
+            put(static_cast<X*>(m.param) + i, __uint_as_float(0x7fffffffu));
+            if (m.master) m.master[i] = __uint_as_float(0x7fffffffu);
+        }
+    }
+}
+
 // Tiles of 128 rows by up to 256 columns.  kGram: A = X X^T; kSquare: b A + c A A; of both the tiles on and above the diagonal,
-// what lies above it is written to both places.  kApply: a X + B X.
+// what lies above it is written to both places.  kApply: a X + B X.  kLast: likewise, and the parameters' update.
 template <int KIND, int PARTS>
 __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constant__ CUtensorMap map, const Params p) {
-    constexpr bool kBMn = KIND == kApply;       // the second operand's rows lie along K
+    constexpr bool kApplies = KIND == kApply || KIND == kLast;
+    constexpr bool kBMn = kApplies;             // the second operand's rows lie along K
     constexpr bool kSegments = PARTS == 2;
     extern __shared__ char shared_raw[];
     __shared__ int firsts[kMostMatrices];
     __shared__ uint64_t bars_at[2 * kMostStages + 6];
     __shared__ uint32_t slot_at;
     __shared__ volatile int give_up;
-    const uint32_t base = (smem_addr(shared_raw) + 1023u) & ~1023u;
     const uint32_t full = smem_addr(bars_at), empty = full + 8 * kMostStages, done = empty + 8 * kMostStages, freed = done + 16, drained = freed + 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kTurns = KIND == kLast ? kEpilogue * kTurn : 0;
+    const uint32_t base = (smem_addr(shared_raw) + kTurns + 1023u) & ~1023u;
     const int part_b = p.wide * kDepth * 2, part_a = kRowsPerCta * kDepth * 2, stage_bytes = PARTS * (part_a + part_b);
 
-    for (int i = threadIdx.x; i < p.count; i += kThreads) firsts[i] = KIND == kApply ? p.table[i].first_apply : p.table[i].first_sym;
+    for (int i = threadIdx.x; i < p.count; i += kThreads) firsts[i] = kApplies ? p.table[i].first_apply : p.table[i].first_sym;
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) bar_init(full + 8 * s, 1), bar_init(empty + 8 * s, 1);
         for (int i = 0; i < 2; ++i) bar_init(done + 8 * i, 1), bar_init(freed + 8 * i, kEpilogue);
@@ -313,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
         t.e = find(p.count, u, [&](int i) { return firsts[i]; });
         const Entry& m = p.table[t.e];
         int at = u - firsts[t.e];
-        if (KIND == kApply) {
+        if (kApplies) {
             const int nt = (m.panels * 64 + p.wide - 1) / p.wide;
             t.row = at / nt * kRowsPerCta, t.col = at % nt * p.wide;
         } else {
@@ -341,11 +467,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
             const Tile t = tile_at(u);
             const Entry m = p.table[t.e];
             // rows of 128 bytes: where panel k of the first operand begins, and the second's
-            const int64_t x0 = m.operand[p.from], x_plane = (int64_t)m.panels * m.mp, s_plane = (int64_t)(m.mp / 64) * m.mp;
+            const int64_t x0 = p.from ? m.operand[1] : m.operand[0], x_plane = (int64_t)m.panels * m.mp, s_plane = (int64_t)(m.mp / 64) * m.mp;
             const int64_t a0 = KIND == kGram ? x0 : KIND == kSquare ? m.gram : m.factor, b0 = KIND == kSquare ? m.gram : x0;
             const int64_t a_plane = KIND == kGram ? x_plane : s_plane, b_plane = KIND == kSquare ? s_plane : x_plane;
             // columns of the tile that there are, in units of 64
-            const int limit = KIND == kApply ? m.panels * 64 : m.mp, have = min(p.wide, limit - t.col) / 64;
+            const int limit = kApplies ? m.panels * 64 : m.mp, have = min(p.wide, limit - t.col) / 64;
             for (int k = 0; k < t.depth; ++k) {
                 ok = wait(empty + 8 * stage, phase ^ 1);
                 if (!ok) break;
@@ -383,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
         for (int u = blockIdx.x; u < p.tiles && ok; u += gridDim.x) {
             const Tile t = tile_at(u);
             const Entry m = p.table[t.e];
-            const int limit = KIND == kApply ? m.panels * 64 : m.mp;
+            const int limit = kApplies ? m.panels * 64 : m.mp;
             const uint32_t kind = half_kind(kRowsPerCta, min(p.wide, limit - t.col), kBMn);
             for (int k0 = 0; k0 < t.depth && ok; k0 += kSegments ? kSegment : t.depth) {
                 ok = wait(freed + 8 * acc, acc_phase ^ 1);
@@ -425,46 +551,54 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
             const Tile t = tile_at(u);
             const Entry m = p.table[t.e];
             const int row = t.row + quarter * 32 + lane, col0 = t.col + half * half_wide;
-            const int limit = KIND == kApply ? m.panels * 64 : m.mp;
+            const int limit = kApplies ? m.panels * 64 : m.mp;
             const int64_t s_plane = (int64_t)(m.mp / 64) * m.mp * 64, x_plane = (int64_t)m.panels * m.mp * 64;
-            const float shift = KIND == kGram ? 0.f : m.shift[p.step], old = KIND == kApply ? p.old + shift : p.old;
-            auto finish = [&](float* v, int c) {  // 32 columns
+            const float shift = KIND == kGram ? 0.f : m.shift[p.step], old = kApplies ? p.old + shift : p.old;
+            const int64_t at0 = kApplies ? place(m.mp, row, col0) : 0;
+            const float* const x_from = p.from ? m.x[1] : m.x[0];
+            float* const       x_to   = p.from ? m.x[0] : m.x[1];
+            const int64_t      target = KIND == kGram ? m.gram : KIND == kSquare ? m.factor : p.from ? m.operand[0] : m.operand[1];
+            auto load_x = [&](int c, float4 (&x)[8]) {  // 32 columns of X
+                if (col0 + c >= limit) return;
+                const float4* const from = reinterpret_cast<const float4*>(x_from + at0 + (int64_t)(c / 32) * m.mp * 32);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = from[j * 32];
+            };
+            auto finish = [&](float* v, int c, const float4 (&x)[8]) {  // 32 columns
                 const int col = col0 + c;
                 if (col >= limit) return;
-                const int64_t at = ((int64_t)(col / 64) * m.mp + row) * 64 + col % 64;
-                if (KIND == kApply) {
-                    const float4* const was = reinterpret_cast<const float4*>(m.x[p.from] + at);
-                    float4* const to = reinterpret_cast<float4*>(m.x[p.from ^ 1] + at);
+                if (kApplies) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float4 x = was[j];
-                        v[4 * j] = fmaf(old, x.x, v[4 * j] * p.product), v[4 * j + 1] = fmaf(old, x.y, v[4 * j + 1] * p.product);
-                        v[4 * j + 2] = fmaf(old, x.z, v[4 * j + 2] * p.product), v[4 * j + 3] = fmaf(old, x.w, v[4 * j + 3] * p.product);
-                        to[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                        v[4 * j] = fmaf(old, x[j].x, v[4 * j] * p.product), v[4 * j + 1] = fmaf(old, x[j].y, v[4 * j + 1] * p.product);
+                        v[4 * j + 2] = fmaf(old, x[j].z, v[4 * j + 2] * p.product), v[4 * j + 3] = fmaf(old, x[j].w, v[4 * j + 3] * p.product);
                     }
-                    if (p.last) return;
+                }
+                if constexpr (KIND == kLast) {
+                    update<PARTS>(m, p.rates, v, row, col, shared_raw + (warp - 2) * kTurn, lane);
+                    __syncwarp();
+                    return;
+                }
+                if (KIND == kApply) {
+                    float4* const to = reinterpret_cast<float4*>(x_to + at0 + (int64_t)(c / 32) * m.mp * 32);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) to[j * 32] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
                 } else if (row / 128 > col / 128) {
                     return;  // below the diagonal
                 }
-                __half* const to = p.work + (KIND == kGram ? m.gram : KIND == kSquare ? m.factor : m.operand[p.from ^ 1]) * 64;
+                const int64_t at = ((int64_t)(col / 64) * m.mp + row) * 64 + col % 64;
+                __half* const to = p.work + target * 64;
                 const int64_t plane = KIND == kApply ? x_plane : s_plane;
                 if (KIND == kSquare) {
-                    const uint4* const a0 = reinterpret_cast<const uint4*>(p.work + m.gram * 64 + at);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint4 w = a0[j];
-                        uint4 w1 = make_uint4(0, 0, 0, 0);
-                        if (PARTS == 2) w1 = *reinterpret_cast<const uint4*>(p.work + m.gram * 64 + plane + at + 8 * j);
-                        const uint32_t hi[4] = {w.x, w.y, w.z, w.w}, lo[4] = {w1.x, w1.y, w1.z, w1.w};
+                    for (int q = PARTS - 1; q >= 0; --q) {
+                        uint32_t w[16];
+                        load_sector(p.work + m.gram * 64 + q * plane + at, w), load_sector(p.work + m.gram * 64 + q * plane + at + 16, w + 8);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float2 a = __half22float2(reinterpret_cast<const __half2&>(hi[i]));
-                            if (PARTS == 2) {
-                                const float2 l = __half22float2(reinterpret_cast<const __half2&>(lo[i]));
-                                a.x += l.x, a.y += l.y;
-                            }
-                            v[8 * j + 2 * i]     = fmaf(old, a.x, v[8 * j + 2 * i] * p.product);
-                            v[8 * j + 2 * i + 1] = fmaf(old, a.y, v[8 * j + 2 * i + 1] * p.product);
+                        for (int j = 0; j < 16; ++j) {
+                            const float2 a = __half22float2(reinterpret_cast<const __half2&>(w[j]));
+                            v[2 * j] = fmaf(old, a.x, q == PARTS - 1 ? v[2 * j] * p.product : v[2 * j]);
+                            v[2 * j + 1] = fmaf(old, a.y, q == PARTS - 1 ? v[2 * j + 1] * p.product : v[2 * j + 1]);
                         }
                     }
                     const int hit = row - col;  // the diagonal's place among these columns
@@ -482,16 +616,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                     uint32_t w[16];
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-                        w[j] = reinterpret_cast<const uint32_t&>(h);
-                        if (q + 1 < PARTS) {
-                            const float2 back = __half22float2(h);
-                            v[2 * j] -= back.x, v[2 * j + 1] -= back.y;
-                        }
+                        float2 two = make_float2(v[2 * j], v[2 * j + 1]);
+                        w[j] = part_of(two);
+                        v[2 * j] = two.x, v[2 * j + 1] = two.y;
                     }
-                    uint4* const o = reinterpret_cast<uint4*>(to + q * plane + at);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) o[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+                    store_sector(to + q * plane + at, w), store_sector(to + q * plane + at + 16, w + 8);
                     if (mirror) {
                         __half* const under = to + q * plane + ((int64_t)(row / 64) * m.mp + col) * 64 + row % 64;
 #pragma unroll
@@ -502,6 +631,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                     }
                 }
             };
+            float4 x_of[kApplies && !kSegments ? 2 : 1][8];
+            if (kApplies && !kSegments) load_x(0, x_of[0]);  // ahead of the sums
             float total[kSegments ? kWide / 2 : 1];
             if constexpr (kSegments) {
 #pragma unroll
@@ -523,7 +654,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
 #pragma unroll
                             for (int j = 0; j < 32; ++j) total[c + j] += v[j];
                         } else {
-                            finish(v, c);
+                            if (kApplies && c + 32 < half_wide) load_x(c + 32, x_of[kApplies ? (c / 32 + 1) & 1 : 0]);
+                            finish(v, c, x_of[kApplies ? c / 32 & 1 : 0]);
+                            __syncwarp();
                         }
                     }
                 }
@@ -535,8 +668,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
             if (!ok) break;
             if constexpr (kSegments) {
 #pragma unroll
-                for (int c = 0; c < kWide / 2; c += 32)
-                    if (c < half_wide) finish(total + c, c);
+                for (int c = 0; c < kWide / 2; c += 32) {
+                    if (c >= half_wide) continue;
+                    if (kApplies) load_x(c, x_of[0]);
+                    finish(total + c, c, x_of[0]);
+                }
             }
         }
     }
@@ -706,23 +842,23 @@ int run_chain(Chain& c, const Rates& rates, const std::vector<Step>& steps, char
     __half* const halves = reinterpret_cast<__half*>(work);
     k_muon_begin<X, PARTS><<<(unsigned)c.blocks, 256, 0, stream>>>(c.table, count, rates, std::ldexp(1.f, steps[0].x), halves, abc);
     FW_LAUNCHED();
-    auto stages = [&](int wide) { return std::min(kMostStages, (kShared - 1024) / (PARTS * (kRowsPerCta + wide) * kDepth * 2)); };
+    auto stages = [&](int wide, int other) { return std::min(kMostStages, (kShared - 1024 - other) / (PARTS * (kRowsPerCta + wide) * kDepth * 2)); };
     Params p = {};
     p.table = c.table, p.count = count, p.work = halves, p.failed = c.failed;
     const int grid_sym = (int)std::min<int64_t>(sym, sms), grid_apply = (int)std::min<int64_t>(apply, sms);
     for (size_t i = 0; i < steps.size(); ++i) {
         const Step& s = steps[i];
-        p.step = (int)i, p.from = (int)(i & 1), p.tiles = (int)sym, p.wide = wide_sym, p.stages = stages(wide_sym), p.last = 0;
+        p.step = (int)i, p.from = (int)(i & 1), p.tiles = (int)sym, p.wide = wide_sym, p.stages = stages(wide_sym, 0);
         p.product = std::ldexp(1.f, s.gram - 2 * s.x);
         FW_DO(launch<kGram, PARTS>(map, p, grid_sym, stream));
         p.product = std::ldexp(s.c, s.factor - 2 * s.gram), p.old = std::ldexp(s.b, s.factor - s.gram), p.scale = std::ldexp(1.f, s.factor);
         FW_DO(launch<kSquare, PARTS>(map, p, grid_sym, stream));
-        p.tiles = (int)apply, p.wide = wide_apply, p.stages = stages(wide_apply);
-        p.product = std::ldexp(1.f, -s.factor - s.x), p.old = s.a, p.last = i + 1 == steps.size();
-        p.scale = p.last ? 0.f : std::ldexp(1.f, steps[i + 1].x);
-        FW_DO(launch<kApply, PARTS>(map, p, grid_apply, stream));
+        const bool last = i + 1 == steps.size();
+        p.tiles = (int)apply, p.wide = wide_apply, p.stages = stages(wide_apply, last ? kEpilogue * kTurn : 0);
+        p.product = std::ldexp(1.f, -s.factor - s.x), p.old = s.a, p.scale = last ? 0.f : std::ldexp(1.f, steps[i + 1].x), p.rates = rates;
+        FW_DO((last ? launch<kLast, PARTS> : launch<kApply, PARTS>)(map, p, grid_apply, stream));
     }
-    k_muon_finish<X><<<(unsigned)c.blocks, 256, 0, stream>>>(c.table, count, rates, (int)(steps.size() & 1), c.failed);
+    k_muon_check<X><<<sms, 256, 0, stream>>>(c.table, count, c.failed);
     FW_LAUNCHED();
     return FRAMEWISE_B200_OK;
 }
