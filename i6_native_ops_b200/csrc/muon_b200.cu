@@ -26,6 +26,7 @@
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
+#include <utility>
 #include <vector>
 
 namespace {
@@ -37,7 +38,8 @@ constexpr int kMostMatrices = 256;   // of a chain of launches
 constexpr int kSlots        = 24;    // matrices in a launch's arguments
 constexpr int kChunk        = 16384; // values per CTA of the pass over gradients
 constexpr int kRowsPerCta   = 128;   // of a tile: the lanes of tensor memory
-constexpr int kWide         = 256;   // columns of a tile at most: two accumulators fill tensor memory
+constexpr int kColumns      = 512;   // of tensor memory: a ring of accumulators
+constexpr int kMostAccs     = 8;
 constexpr int kDepth        = 64;    // K per stage
 constexpr int kSegment      = 1;     // f32: stages after which an accumulator is added up in registers, for tensor cores cut
                                      // off what they add, at 2^-24 of the sum a step, and never round it up: 6 x 500 x 2001 is off
@@ -115,6 +117,11 @@ __device__ __forceinline__ uint32_t part_of(float2& v) {
     return reinterpret_cast<const uint32_t&>(h);
 }
 
+// Launches of a chain follow each other without a gap: the next one's CTAs come when this one's leave, and wait for
+// all of it to be done before they read or write memory.
+__device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void former_is_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // what is made orthogonal, from the gradient and the new momentum
 __device__ __forceinline__ float direction(float g, float v, const Rates& r) { return r.nesterov != 0.f ? g + (v - g) * r.beta : v; }
 
@@ -153,6 +160,7 @@ __global__ void __launch_bounds__(256) k_muon_collect(const __grid_constant__ Sl
         int*       to   = reinterpret_cast<int*>(s.table + s.base + e);
         for (int i = threadIdx.x; i < (int)(sizeof(Entry) / 4); i += 256) to[i] = from[i];
     }
+    next_may_start();
     const int64_t begin = (int64_t)chunk * kChunk;
     const int     left = (int)min((int64_t)m.rows * m.cols - begin, (int64_t)kChunk);
     const X* const g = static_cast<const X*>(m.grad) + begin;
@@ -208,6 +216,8 @@ template <typename X, int PARTS>
 __global__ void __launch_bounds__(256) k_muon_begin(const Entry* __restrict__ table, int count, const Rates r, float scale, __half* work, const __grid_constant__ Steps steps) {
     __shared__ double part[8];
     __shared__ float  tile[64][65];
+    next_may_start();
+    former_is_done();
     const int   e = find(count, blockIdx.x, [&](int i) { return table[i].first_block; });
     const Entry& m = table[e];
     const int block = blockIdx.x - m.first_block, panel = block / (m.mp / 64), row0 = block % (m.mp / 64) * 64;
@@ -297,6 +307,9 @@ struct Params {
     Rates   rates;       // kLast
 };
 
+// Columns of a tile at most.  f32: the sums of its segments have to fit the registers of those who add them up.
+__host__ __device__ constexpr int most_wide(int parts) { return parts == 2 ? 128 : 256; }
+
 // fp16 operands, f32 sums
 __host__ __device__ constexpr uint32_t half_kind(int m, int n, bool b_mn) {
     return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
@@ -314,61 +327,68 @@ __device__ __forceinline__ void store_sector(__half* x, const uint32_t* w) {
                  : "memory");
 }
 
-// p = p decay - rate X, or the result X itself, for a row a lane and 32 columns of X.  Matrices that lie are turned in shared
-// memory first (32 rows of 33 words of this warp's), so that neighbouring lanes always have neighbouring values in memory.
+// p = p decay - rate X, or the result X itself, for a row a lane and 32 columns of X.  They go through shared memory (32 rows of 33
+// words of this warp's), so that neighbouring lanes have neighbouring values in memory whichever way the parameter lies, and
+// so that the code is a loop: written out for 32 values it did not fit the instruction cache (4 x 2048 x 8192 bf16: 515 us a launch).
 constexpr int kTurn = 32 * 33 * 4;
+template <typename X, int USE>  // 0: the result, 1: parameters, 2: parameters and their copies
+__device__ __forceinline__ void update_lines(const float* t, X* p, float* copy, int lines, int64_t pitch, const Rates& r, float rate) {
+    constexpr int kAtOnce = 16;
+#pragma unroll 1
+    for (int j0 = 0; j0 < 32; j0 += kAtOnce) {
+        X     was[kAtOnce];
+        float held[kAtOnce];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            if (USE >= 1 && j0 + j < lines) was[j] = p[j * pitch];
+            if (USE == 2 && j0 + j < lines) held[j] = copy[j * pitch];
+        }
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            float now = t[(j0 + j) * 33];
+            if (USE >= 1) {
+                float old = value(was[j]);
+                if (USE == 2) {
+                    X rounded;
+                    put(&rounded, held[j]);
+                    // a copy of which the parameter is not the rounded value has been left behind by the program
+                    if (!r.follow || value(rounded) == old || (old != old && held[j] != held[j])) old = held[j];
+                }
+                now = old * r.decay - rate * now;
+            }
+            if (j0 + j < lines) {
+                if (USE == 2) copy[j * pitch] = now;
+                put(p + j * pitch, now);
+            }
+        }
+        p += kAtOnce * pitch;
+        if (USE == 2) copy += kAtOnce * pitch;
+    }
+}
 template <int PARTS>
-__device__ __forceinline__ void update(const Entry& m, const Rates& r, float* v, int row, int col, char* turn, int lane) {
+__device__ __forceinline__ void update(const Entry& m, const Rates& r, const float* v, int row, int col, char* turn, int lane) {
     using X = std::conditional_t<PARTS == 2, float, __nv_bfloat16>;
     const bool tall = m.rows > m.cols;
     float* const t = reinterpret_cast<float*>(turn);
-    if (!tall) {
-        __syncwarp();
+    const int own = tall ? lane : lane * 33, step = tall ? 33 : 1;
+    __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) t[lane * 33 + j] = v[j];
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = t[j * 33 + lane];
-    }
-    // value j of a lane: line j of 32, place `at` of it
-    const int line0 = tall ? col : row - lane, at = tall ? row : col + lane, lines = min(32, m.rows - line0);
-    if (at >= m.cols) return;
+    for (int j = 0; j < 32; ++j) t[own + j * step] = v[j];
+    __syncwarp();
+    // line j of 32, place `at` of it
+    const int line0 = tall ? col : row - lane, at = tall ? row : col + lane, lines = at < m.cols ? min(32, m.rows - line0) : 0;
     const int64_t first = (int64_t)line0 * m.cols + at;
     X* const p = static_cast<X*>(m.param) + first;
-    if (!m.momentum) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < lines) put(p + (int64_t)j * m.cols, v[j]);
-        return;
-    }
-    float* const master = m.master ? m.master + first : nullptr;
-#pragma unroll
-    for (int j0 = 0; j0 < 32; j0 += 8) {
-        float was[8], held[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            was[j] = j0 + j < lines ? value(p[(int64_t)(j0 + j) * m.cols]) : 0.f;
-            held[j] = master && j0 + j < lines ? master[(int64_t)(j0 + j) * m.cols] : 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (j0 + j >= lines) continue;
-            if (master) {
-                X rounded;
-                put(&rounded, held[j]);
-                // a copy of which the parameter is not the rounded value has been left behind by the program
-                if (!r.follow || value(rounded) == was[j] || (was[j] != was[j] && held[j] != held[j])) was[j] = held[j];
-            }
-            const float now = was[j] * r.decay - m.rate * v[j0 + j];
-            if (master) master[(int64_t)(j0 + j) * m.cols] = now;
-            put(p + (int64_t)(j0 + j) * m.cols, now);
-        }
-    }
+    if (!m.momentum) update_lines<X, 0>(t + lane, p, nullptr, lines, m.cols, r, m.rate);
+    else if (!m.master) update_lines<X, 1>(t + lane, p, nullptr, lines, m.cols, r, m.rate);
+    else update_lines<X, 2>(t + lane, p, m.master + first, lines, m.cols, r, m.rate);
+    __syncwarp();
 }
 
 // After a wait ran out the results are NaN.
 template <typename X>
 __global__ void __launch_bounds__(256) k_muon_check(const Entry* __restrict__ table, int count, const int* failed) {
+    former_is_done();
     if (*failed == 0) return;
     for (int e = 0; e < count; ++e) {
         const Entry& m = table[e];
@@ -381,34 +401,41 @@ __global__ void __launch_bounds__(256) k_muon_check(const Entry* __restrict__ ta
 
 // Tiles of 128 rows by up to 256 columns.  kGram: A = X X^T; kSquare: b A + c A A; of both the tiles on and above the diagonal,
 // what lies above it is written to both places.  kApply: a X + B X.  kLast: likewise, and the parameters' update.
-template <int KIND, int PARTS>
+// CG: CTAs per tile (2: of 256 rows, each CTA with 128 of them and half of the second operand).
+template <int KIND, int PARTS, int CG>
 __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constant__ CUtensorMap map, const Params p) {
     constexpr bool kApplies = KIND == kApply || KIND == kLast;
     constexpr bool kBMn = kApplies;             // the second operand's rows lie along K
     constexpr bool kSegments = PARTS == 2;
+    constexpr int  kWide = most_wide(PARTS), kTile = kRowsPerCta * CG;
     extern __shared__ char shared_raw[];
     __shared__ int firsts[kMostMatrices];
-    __shared__ uint64_t bars_at[2 * kMostStages + 6];
+    __shared__ uint64_t bars_at[2 * kMostStages + 2 * kMostAccs + 1];
     __shared__ uint32_t slot_at;
     __shared__ volatile int give_up;
-    const uint32_t full = smem_addr(bars_at), empty = full + 8 * kMostStages, done = empty + 8 * kMostStages, freed = done + 16, drained = freed + 16;
+    const uint32_t full = smem_addr(bars_at), empty = full + 8 * kMostStages, done = empty + 8 * kMostStages, freed = done + 8 * kMostAccs,
+                   drained = freed + 8 * kMostAccs;
+    const int rank = CG == 2 ? (int)cluster_rank() : 0, worker = blockIdx.x / CG, workers = gridDim.x / CG, accs = min(kMostAccs, kColumns / p.wide);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int kTurns = KIND == kLast ? kEpilogue * kTurn : 0;
     const uint32_t base = (smem_addr(shared_raw) + kTurns + 1023u) & ~1023u;
-    const int part_b = p.wide * kDepth * 2, part_a = kRowsPerCta * kDepth * 2, stage_bytes = PARTS * (part_a + part_b);
+    const int part_b = p.wide / CG * kDepth * 2, part_a = kRowsPerCta * kDepth * 2, stage_bytes = PARTS * (part_a + part_b);
 
-    for (int i = threadIdx.x; i < p.count; i += kThreads) firsts[i] = kApplies ? p.table[i].first_apply : p.table[i].first_sym;
+    next_may_start();
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) bar_init(full + 8 * s, 1), bar_init(empty + 8 * s, 1);
-        for (int i = 0; i < 2; ++i) bar_init(done + 8 * i, 1), bar_init(freed + 8 * i, kEpilogue);
+        for (int i = 0; i < accs; ++i) bar_init(done + 8 * i, 1), bar_init(freed + 8 * i, kEpilogue * CG);
         bar_init(drained, 1);
         give_up = 0;
         bar_init_fence();
         prefetch_map(&map);
     }
-    if (warp == 1) tmem_alloc<1>(smem_addr(&slot_at), 512);
+    if (warp == 1) tmem_alloc<CG>(smem_addr(&slot_at), kColumns);
+    former_is_done();
+    for (int i = threadIdx.x; i < p.count; i += kThreads) firsts[i] = kApplies ? p.table[i].first_apply : p.table[i].first_sym;
     fence_before();
     __syncthreads();
+    if (CG == 2) cluster_sync();
     fence_after();
     const uint32_t tmem = *const_cast<volatile uint32_t*>(&slot_at);
 
@@ -440,20 +467,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
         const Entry& m = p.table[t.e];
         int at = u - firsts[t.e];
         if (kApplies) {
-            const int nt = (m.panels * 64 + p.wide - 1) / p.wide;
-            t.row = at / nt * kRowsPerCta, t.col = at % nt * p.wide;
+            // a column after the other: its part of X is met by all rows at once, B stays near
+            const int mt = m.mp / kTile;
+            t.row = at % mt * kTile, t.col = at / mt * p.wide;
         } else {
             const int nt = (m.mp + p.wide - 1) / p.wide;
             int row = 0;
             for (;; ++row) {
-                const int first = row * kRowsPerCta / p.wide, tiles = nt - first;
+                const int first = row * kTile / p.wide, tiles = nt - first;
                 if (at < tiles) {
                     t.col = (first + at) * p.wide;
                     break;
                 }
                 at -= tiles;
             }
-            t.row = row * kRowsPerCta;
+            t.row = row * kTile;
         }
         t.depth = KIND == kGram ? m.panels : (m.m + 63) / 64;
         return t;
@@ -463,28 +491,28 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
         int      stage = 0, issued = 0;
         uint32_t phase = 0;
         bool     ok = true;
-        for (int u = blockIdx.x; u < p.tiles && ok; u += gridDim.x) {
+        for (int u = worker; u < p.tiles && ok; u += workers) {
             const Tile t = tile_at(u);
             const Entry m = p.table[t.e];
             // rows of 128 bytes: where panel k of the first operand begins, and the second's
             const int64_t x0 = p.from ? m.operand[1] : m.operand[0], x_plane = (int64_t)m.panels * m.mp, s_plane = (int64_t)(m.mp / 64) * m.mp;
             const int64_t a0 = KIND == kGram ? x0 : KIND == kSquare ? m.gram : m.factor, b0 = KIND == kSquare ? m.gram : x0;
             const int64_t a_plane = KIND == kGram ? x_plane : s_plane, b_plane = KIND == kSquare ? s_plane : x_plane;
-            // columns of the tile that there are, in units of 64
-            const int limit = kApplies ? m.panels * 64 : m.mp, have = min(p.wide, limit - t.col) / 64;
+            // columns of the tile that there are and are this CTA's, in units of 64
+            const int limit = kApplies ? m.panels * 64 : m.mp, have = min(p.wide, limit - t.col) / (64 * CG), from = t.col + rank * have * 64;
             for (int k = 0; k < t.depth; ++k) {
                 ok = wait(empty + 8 * stage, phase ^ 1);
                 if (!ok) break;
-                const uint32_t a = base + stage * stage_bytes, b = a + PARTS * part_a, bar = full + 8 * stage;
-                bar_expect(bar, PARTS * (part_a + have * 8192));
+                const uint32_t a = base + stage * stage_bytes, b = a + PARTS * part_a, bar = CG == 2 ? in_cta(full + 8 * stage, 0) : full + 8 * stage;
+                if (rank == 0) bar_expect(full + 8 * stage, CG * PARTS * (part_a + have * 8192));
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q) {
-                    const int64_t a_at = a0 + q * a_plane + (int64_t)k * m.mp + t.row;
-                    load_box<1>(a + q * part_a, &map, bar, 0, (int)a_at, 0);
-                    load_box<1>(a + q * part_a + 8192, &map, bar, 0, (int)a_at + 64, 0);
+                    const int64_t a_at = a0 + q * a_plane + (int64_t)k * m.mp + t.row + rank * kRowsPerCta;
+                    load_box<CG>(a + q * part_a, &map, bar, 0, (int)a_at, 0);
+                    load_box<CG>(a + q * part_a + 8192, &map, bar, 0, (int)a_at + 64, 0);
                     for (int j = 0; j < have; ++j) {
-                        const int64_t b_at = b0 + q * b_plane + (kBMn ? (int64_t)(t.col / 64 + j) * m.mp + k * 64 : (int64_t)k * m.mp + t.col + j * 64);
-                        load_box<1>(b + q * part_b + j * 8192, &map, bar, 0, (int)b_at, 0);
+                        const int64_t b_at = b0 + q * b_plane + (kBMn ? (int64_t)(from / 64 + j) * m.mp + k * 64 : (int64_t)k * m.mp + from + j * 64);
+                        load_box<CG>(b + q * part_b + j * 8192, &map, bar, 0, (int)b_at, 0);
                     }
                 }
                 ++issued;
@@ -496,26 +524,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
             ok = wait(empty + 8 * stage, phase ^ 1);
             if (ok && ++stage == p.stages) stage = 0, phase ^= 1;
         }
-        if (give_up) {
+        if (give_up && rank == 0) {
             for (int i = 0; i < p.stages && i < issued; ++i) {
                 if (--stage < 0) stage = p.stages - 1, phase ^= 1;
                 bounded(full + 8 * stage, phase, false);
             }
         }
-    } else if (warp == 1 && lane == 0) {  // ---- products
+    } else if (warp == 1 && lane == 0 && rank == 0) {  // ---- products
         int      stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool     ok = true;
-        for (int u = blockIdx.x; u < p.tiles && ok; u += gridDim.x) {
+        for (int u = worker; u < p.tiles && ok; u += workers) {
             const Tile t = tile_at(u);
             const Entry m = p.table[t.e];
             const int limit = kApplies ? m.panels * 64 : m.mp;
-            const uint32_t kind = half_kind(kRowsPerCta, min(p.wide, limit - t.col), kBMn);
+            const uint32_t kind = half_kind(kTile, min(p.wide, limit - t.col), kBMn);
             for (int k0 = 0; k0 < t.depth && ok; k0 += kSegments ? kSegment : t.depth) {
                 ok = wait(freed + 8 * acc, acc_phase ^ 1);
                 if (!ok) break;
                 fence_after();
-                const uint32_t d = tmem + acc * kWide;
+                const uint32_t d = tmem + acc * p.wide;
                 const int k1 = kSegments ? min(t.depth, k0 + kSegment) : t.depth;
                 for (int k = k0; k < k1; ++k) {
                     ok = wait(full + 8 * stage, phase);
@@ -527,30 +555,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                         const uint32_t aq = q == 0 ? a + part_a : a, bq = q == 1 ? b + part_b : b;
 #pragma unroll
                         for (int i = 0; i < kDepth / 16; ++i)
-                            product<1>(d, operand(aq + i * 32, 8192), operand(bq + i * (kBMn ? 2048 : 32), 8192), kind,
+                            product<CG>(d, operand(aq + i * 32, 8192), operand(bq + i * (kBMn ? 2048 : 32), 8192), kind,
                                        k > k0 || q > (PARTS == 2 ? 0 : 2) || i > 0);
                     }
-                    products_commit<1>(empty + 8 * stage);
+                    products_commit<CG>(empty + 8 * stage);
                     if (++stage == p.stages) stage = 0, phase ^= 1;
                 }
-                products_commit<1>(done + 8 * acc);
-                if (++acc == 2) acc = 0, acc_phase ^= 1;
+                products_commit<CG>(done + 8 * acc);
+                if (++acc == accs) acc = 0, acc_phase ^= 1;
             }
         }
         if (!ok) {  // products under way still read shared memory
-            products_commit<1>(drained);
+            products_commit<CG>(drained);
             bounded(drained, 0, false);
         }
     } else if (warp >= 2) {  // ---- finished tiles: a row a lane
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         const int half_wide = p.wide / 2;
+        const uint32_t freed0 = CG == 2 ? in_cta(freed, 0) : freed;
         int      acc = 0;
         uint32_t acc_phase = 0;
         bool     ok = true;
-        for (int u = blockIdx.x; u < p.tiles && ok; u += gridDim.x) {
+        for (int u = worker; u < p.tiles && ok; u += workers) {
             const Tile t = tile_at(u);
             const Entry m = p.table[t.e];
-            const int row = t.row + quarter * 32 + lane, col0 = t.col + half * half_wide;
+            const int row = t.row + rank * kRowsPerCta + quarter * 32 + lane, col0 = t.col + half * half_wide;
             const int limit = kApplies ? m.panels * 64 : m.mp;
             const int64_t s_plane = (int64_t)(m.mp / 64) * m.mp * 64, x_plane = (int64_t)m.panels * m.mp * 64;
             const float shift = KIND == kGram ? 0.f : m.shift[p.step], old = kApplies ? p.old + shift : p.old;
@@ -631,8 +660,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                     }
                 }
             };
-            float4 x_of[kApplies && !kSegments ? 2 : 1][8];
-            if (kApplies && !kSegments) load_x(0, x_of[0]);  // ahead of the sums
+            constexpr int kBuffers = kApplies ? 2 : 1;
+            float4 x_of[kBuffers][8];
+            if (kApplies) load_x(0, x_of[0]);  // ahead of the sums
+            if (kApplies && kSegments && half_wide > 32) load_x(32, x_of[kBuffers - 1]);
             float total[kSegments ? kWide / 2 : 1];
             if constexpr (kSegments) {
 #pragma unroll
@@ -642,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                 ok = __all_sync(0xffffffffu, wait(done + 8 * acc, acc_phase));
                 if (!ok) break;
                 fence_after();
-                const uint32_t acc_at = tmem + ((uint32_t)(quarter * 32) << 16) + acc * kWide + half * half_wide;
+                const uint32_t acc_at = tmem + ((uint32_t)(quarter * 32) << 16) + acc * p.wide + half * half_wide;
 #pragma unroll
                 for (int c = 0; c < kWide / 2; c += 32) {
                     if (c < half_wide && col0 + c < limit) {
@@ -654,24 +685,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
 #pragma unroll
                             for (int j = 0; j < 32; ++j) total[c + j] += v[j];
                         } else {
-                            if (kApplies && c + 32 < half_wide) load_x(c + 32, x_of[kApplies ? (c / 32 + 1) & 1 : 0]);
-                            finish(v, c, x_of[kApplies ? c / 32 & 1 : 0]);
+                            if (kBuffers == 2 && c + 32 < half_wide) load_x(c + 32, x_of[(c / 32 + 1) % kBuffers]);
+                            finish(v, c, x_of[c / 32 % kBuffers]);
                             __syncwarp();
                         }
                     }
                 }
                 fence_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive(freed + 8 * acc);
-                if (++acc == 2) acc = 0, acc_phase ^= 1;
+                if (lane == 0) bar_arrive(freed0 + 8 * acc);
+                if (++acc == accs) acc = 0, acc_phase ^= 1;
             }
             if (!ok) break;
             if constexpr (kSegments) {
 #pragma unroll
                 for (int c = 0; c < kWide / 2; c += 32) {
                     if (c >= half_wide) continue;
-                    if (kApplies) load_x(c, x_of[0]);
-                    finish(total + c, c, x_of[0]);
+                    finish(total + c, c, x_of[c / 32 % kBuffers]);
+                    __syncwarp();
                 }
             }
         }
@@ -679,8 +710,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
     __syncwarp();
     fence_before();
     __syncthreads();
+    if (CG == 2) cluster_sync();
     fence_after();
-    if (warp == 1) tmem_free<1>(tmem, 512);
+    if (warp == 1) tmem_free<CG>(tmem, kColumns);
 }
 
 // ------------------------------------------------------------------------------------------ host side
@@ -726,6 +758,7 @@ struct Chain {  // matrices of a chain of launches, and what its workspace holds
     Entry*   table;
     int32_t* failed;
     int64_t  chunks, blocks;
+    bool     pairs;  // tiles of pairs of CTAs are possible
     size_t   bytes;
 };
 
@@ -736,6 +769,13 @@ Chain chain_of(const Matrix* matrices, int64_t count, int parts, int steps, void
     c.table  = w.take<Entry>(count);
     c.chunks = c.blocks = 0;
     c.entry.resize(count);
+    // pairs of CTAs take 256 rows: where that pads little
+    double padded = 0, least = 0;
+    for (int64_t i = 0; i < count; ++i) {
+        const int64_t m = std::min(matrices[i].rows, matrices[i].cols), n = std::max(matrices[i].rows, matrices[i].cols);
+        least += (double)up(m, 128) * up(n, 64) * m, padded += (double)up(m, 256) * up(n, 128) * m;
+    }
+    c.pairs = padded <= 1.1 * least;
     for (int64_t i = 0; i < count; ++i) {
         Entry& e = c.entry[i];
         const Matrix& m = matrices[i];
@@ -743,7 +783,7 @@ Chain chain_of(const Matrix* matrices, int64_t count, int parts, int steps, void
         e.grad = m.grad, e.momentum = m.momentum, e.param = m.param, e.master = m.master, e.rate = (float)m.rate;
         e.rows = (int)m.rows, e.cols = (int)m.cols;
         e.m = std::min(e.rows, e.cols), e.n = std::max(e.rows, e.cols);
-        e.mp = (int)up(e.m, kRowsPerCta), e.panels = (int)((e.n + 63) / 64);
+        e.mp = (int)up(e.m, c.pairs ? 256 : 128), e.panels = (int)(up(e.n, c.pairs ? 128 : 64) / 64);
         e.chunks = (int)((m.rows * m.cols + kChunk - 1) / kChunk);
         e.first_chunk = (int)c.chunks, e.first_block = (int)c.blocks;
         c.chunks += e.chunks, c.blocks += (int64_t)e.panels * (e.mp / 64);
@@ -771,7 +811,7 @@ int64_t together(const Matrix* matrices, int64_t count, int parts) {
     int64_t i = 0;
     for (; i < count && i < kMostMatrices; ++i) {
         const int64_t m = std::min(matrices[i].rows, matrices[i].cols), n = std::max(matrices[i].rows, matrices[i].cols);
-        const size_t more = (size_t)up(m, 128) * ((size_t)up(n, 64) * (8 + 4 * parts) + (size_t)up(m, 128) * 4 * parts);
+        const size_t more = (size_t)up(m, 256) * ((size_t)up(n, 128) * (8 + 4 * parts) + (size_t)up(m, 256) * 4 * parts);
         if (i > 0 && bytes + more > kChainBytes) break;
         bytes += more;
     }
@@ -782,47 +822,72 @@ bool matrices_ok(const Matrix* m, int64_t count) {
     for (int64_t i = 0; i < count; ++i) {
         const int64_t rows = m[i].rows, cols = m[i].cols;
         // rows of the workspace are counted in 32 bits
-        if (rows < 1 || cols < 1 || rows >= ((int64_t)1 << 30) || cols >= ((int64_t)1 << 30) || up(std::min(rows, cols), 128) > ((int64_t)1 << 20) ||
-            (double)up(std::min(rows, cols), 128) * up(std::max(rows, cols), 64) >= 1e10)
+        if (rows < 1 || cols < 1 || rows >= ((int64_t)1 << 30) || cols >= ((int64_t)1 << 30) || up(std::min(rows, cols), 256) > ((int64_t)1 << 20) ||
+            (double)up(std::min(rows, cols), 256) * up(std::max(rows, cols), 128) >= 1e10)
             return false;
     }
     return true;
 }
 
-template <int KIND, int PARTS>
-int launch(const CUtensorMap& map, const Params& p, int grid, cudaStream_t stream) {
-    auto kernel = k_muon_tiles<KIND, PARTS>;
-    static std::atomic<uint64_t> allowed{0};
-    FW_DO(allow_shared(kernel, kShared, allowed));
-    kernel<<<grid, kThreads, kShared, stream>>>(map, p);
+// A launch of the chain, which may begin before the former has ended (see former_is_done), with CTAs in clusters of `cluster`.
+template <typename... P, typename... A>
+int follow(void (*kernel)(P...), int64_t grid, int threads, int shared, int cluster, cudaStream_t stream, A&&... args) {
+    cudaLaunchConfig_t c = {};
+    c.gridDim          = dim3((unsigned)grid);
+    c.blockDim         = dim3(threads);
+    c.dynamicSmemBytes = shared;
+    c.stream           = stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
+    c.attrs    = at;
+    c.numAttrs = cluster > 1 ? 2 : 1;
+    FW_TRY(cudaLaunchKernelEx(&c, kernel, std::forward<A>(args)...));
     FW_LAUNCHED();
     return FRAMEWISE_B200_OK;
+}
+
+template <int KIND, int PARTS, int CG>
+int launch(const CUtensorMap& map, const Params& p, int sms, cudaStream_t stream) {
+    auto kernel = k_muon_tiles<KIND, PARTS, CG>;
+    static std::atomic<uint64_t> allowed{0};
+    FW_DO(allow_shared(kernel, kShared, allowed));
+    return follow(kernel, std::min(p.tiles, sms / CG) * CG, kThreads, kShared, CG, stream, map, p);
 }
 
 template <typename X>
 int run_chain(Chain& c, const Rates& rates, const std::vector<Step>& steps, char* work, cudaStream_t stream) {
     constexpr int PARTS = sizeof(X) == 4 ? 2 : 1;
     const int sms = sm_count(), count = (int)c.entry.size();
-    if (sms < 1) return FRAMEWISE_B200_CUDA_ERROR;
-    // tiles as wide as leaves all SMs something to do
-    auto lay = [&](int wide, bool apply, bool write) {
+    if (sms < 2) return FRAMEWISE_B200_CUDA_ERROR;
+    struct Shape {
+        int     pair, wide;
+        int64_t tiles;
+    };
+    auto lay = [&](int pair, int wide, bool apply, bool write) {
         int64_t tiles = 0;
+        const int rows = kRowsPerCta * pair;
         for (Entry& e : c.entry) {
             if (write) (apply ? e.first_apply : e.first_sym) = (int)tiles;
-            const int mt = e.mp / kRowsPerCta, nt = ((apply ? e.panels * 64 : e.mp) + wide - 1) / wide;
+            const int mt = e.mp / rows, nt = ((apply ? e.panels * 64 : e.mp) + wide - 1) / wide;
             if (apply) tiles += (int64_t)mt * nt;
-            else for (int r = 0; r < mt; ++r) tiles += nt - r * kRowsPerCta / wide;
+            else for (int r = 0; r < mt; ++r) tiles += nt - r * rows / wide;
         }
         return tiles;
     };
-    auto width = [&](bool apply) {
-        int wide = kWide;
-        while (wide > 64 && lay(wide, apply, false) < sms) wide /= 2;
-        return wide;
+    // pairs of CTAs where there are tiles for all of them; else tiles as wide as leaves all SMs something to do
+    auto shape = [&](bool apply) {
+        Shape s = {1, most_wide(PARTS), 0};
+        if (c.pairs && lay(2, s.wide, apply, false) >= sms / 2) s.pair = 2;
+        else while (s.wide > 64 && lay(1, s.wide, apply, false) < sms) s.wide /= 2;
+        s.tiles = lay(s.pair, s.wide, apply, true);
+        return s;
     };
-    const int     wide_sym = width(false), wide_apply = width(true);
-    const int64_t sym = lay(wide_sym, false, true), apply = lay(wide_apply, true, true);
-    if (sym >= INT32_MAX || apply >= INT32_MAX || c.chunks >= INT32_MAX || c.blocks >= INT32_MAX || c.bytes / 128 >= INT32_MAX) return FRAMEWISE_B200_BAD_ARGUMENT;
+    const Shape sym = shape(false), apply = shape(true);
+    if (sym.tiles >= INT32_MAX || apply.tiles >= INT32_MAX || c.chunks >= INT32_MAX || c.blocks >= INT32_MAX || c.bytes / 128 >= INT32_MAX)
+        return FRAMEWISE_B200_BAD_ARGUMENT;
     FW_DO(bind_device());
     CUtensorMap map;
     const int64_t lines = (int64_t)(c.bytes / 128);
@@ -840,27 +905,29 @@ int run_chain(Chain& c, const Rates& rates, const std::vector<Step>& steps, char
         FW_LAUNCHED();
     }
     __half* const halves = reinterpret_cast<__half*>(work);
-    k_muon_begin<X, PARTS><<<(unsigned)c.blocks, 256, 0, stream>>>(c.table, count, rates, std::ldexp(1.f, steps[0].x), halves, abc);
-    FW_LAUNCHED();
-    auto stages = [&](int wide, int other) { return std::min(kMostStages, (kShared - 1024 - other) / (PARTS * (kRowsPerCta + wide) * kDepth * 2)); };
+    FW_DO(follow(k_muon_begin<X, PARTS>, c.blocks, 256, 0, 1, stream, (const Entry*)c.table, count, rates, std::ldexp(1.f, steps[0].x), halves, abc));
+    auto go = [&](auto kind, const Shape& sh, Params& p) {
+        constexpr int KIND = decltype(kind)::value;
+        const int other = KIND == kLast ? kEpilogue * kTurn : 0;
+        p.tiles = (int)sh.tiles, p.wide = sh.wide;
+        p.stages = std::min(kMostStages, (kShared - 1024 - other) / (PARTS * (kRowsPerCta + sh.wide / sh.pair) * kDepth * 2));
+        return sh.pair == 2 ? launch<KIND, PARTS, 2>(map, p, sms, stream) : launch<KIND, PARTS, 1>(map, p, sms, stream);
+    };
     Params p = {};
-    p.table = c.table, p.count = count, p.work = halves, p.failed = c.failed;
-    const int grid_sym = (int)std::min<int64_t>(sym, sms), grid_apply = (int)std::min<int64_t>(apply, sms);
+    p.table = c.table, p.count = count, p.work = halves, p.failed = c.failed, p.rates = rates;
     for (size_t i = 0; i < steps.size(); ++i) {
         const Step& s = steps[i];
-        p.step = (int)i, p.from = (int)(i & 1), p.tiles = (int)sym, p.wide = wide_sym, p.stages = stages(wide_sym, 0);
+        p.step = (int)i, p.from = (int)(i & 1);
         p.product = std::ldexp(1.f, s.gram - 2 * s.x);
-        FW_DO(launch<kGram, PARTS>(map, p, grid_sym, stream));
+        FW_DO(go(std::integral_constant<int, kGram>(), sym, p));
         p.product = std::ldexp(s.c, s.factor - 2 * s.gram), p.old = std::ldexp(s.b, s.factor - s.gram), p.scale = std::ldexp(1.f, s.factor);
-        FW_DO(launch<kSquare, PARTS>(map, p, grid_sym, stream));
+        FW_DO(go(std::integral_constant<int, kSquare>(), sym, p));
         const bool last = i + 1 == steps.size();
-        p.tiles = (int)apply, p.wide = wide_apply, p.stages = stages(wide_apply, last ? kEpilogue * kTurn : 0);
-        p.product = std::ldexp(1.f, -s.factor - s.x), p.old = s.a, p.scale = last ? 0.f : std::ldexp(1.f, steps[i + 1].x), p.rates = rates;
-        FW_DO((last ? launch<kLast, PARTS> : launch<kApply, PARTS>)(map, p, grid_apply, stream));
+        p.product = std::ldexp(1.f, -s.factor - s.x), p.old = s.a, p.scale = last ? 0.f : std::ldexp(1.f, steps[i + 1].x);
+        if (last) FW_DO(go(std::integral_constant<int, kLast>(), apply, p));
+        else FW_DO(go(std::integral_constant<int, kApply>(), apply, p));
     }
-    k_muon_check<X><<<sms, 256, 0, stream>>>(c.table, count, c.failed);
-    FW_LAUNCHED();
-    return FRAMEWISE_B200_OK;
+    return follow(k_muon_check<X>, sms, 256, 0, 1, stream, (const Entry*)c.table, count, (const int*)c.failed);
 }
 
 size_t bytes_for(const std::vector<Matrix>& list, int parts) {
