@@ -105,15 +105,15 @@ inline EncodeTiled encode_tiled() {
     return f;
 }
 
-// planes x rows x cols, rows `pitch` elements apart, read or written in boxes of box_cols x box_rows
+// planes x rows x cols, rows `pitch` elements apart, read or written in boxes of box_cols x box_rows (of box_planes planes)
 inline bool map_of(CUtensorMap* map, const void* base, bool f32, int64_t cols, int64_t rows, int64_t planes, int64_t pitch, int64_t plane,
-            int box_cols, int box_rows) {
+                   int box_cols, int box_rows, int box_planes = 1) {
     const EncodeTiled f = encode_tiled();
     if (!f) return false;
     const int64_t    size = f32 ? 4 : 2;
     const cuuint64_t dims[3]    = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
     const cuuint64_t strides[2] = {(cuuint64_t)(pitch * size), (cuuint64_t)(plane * size)};
-    const cuuint32_t box[3]     = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
+    const cuuint32_t box[3]     = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, (cuuint32_t)box_planes};
     const cuuint32_t step[3]    = {1, 1, 1};
     const int row_bytes = box_cols * (int)size;
     return f(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims,

@@ -50,8 +50,9 @@ constexpr int kThreads      = 64 + 32 * kEpilogue;
 constexpr int kShared       = 232448 - 2048;  // dynamic; the rest: the static arrays
 constexpr uint64_t kPatience = 4000000000ull;  // nanoseconds after which a wait gives up; they end within microseconds
 
-// A matrix of a chain.  Operands lie in panels of 64 columns of fp16, in which the rows follow each other: a row is 128 bytes
-// there, a tensor copy's line.  X itself is met by warps whose lanes have a row each: squares of 32 x 32 values, in which four
+// A matrix of a chain.  Operands lie in units of 128 rows by 64 columns of fp16, 16 KB, a row of units after the other: one
+// tensor copy brings 128 rows of 64 columns, or 64 rows of 128.  (With panels of 64 columns, and copies of 64 by 64, the thread that
+// asks for them held up the products.)  X itself is met by warps whose lanes have a row each: squares of 32 x 32 values, in which four
 // columns of 32 rows, 512 bytes, follow each other (see place).
 struct Entry {
     const void* grad;
@@ -61,10 +62,10 @@ struct Entry {
     double*     partial;    // sums of squares of the chunks
     float*      shift;      // per step: the multiple of the identity that B does without
     float*      x[2];       // X, before and after a step
-    int64_t     operand[2]; // its fp16 parts, as rows of 128 bytes of the workspace
-    int64_t     gram, factor; // A and B, likewise
+    int         operand[2]; // its fp16 parts, as units of the workspace
+    int         gram, factor; // A and B, likewise
     int         rows, cols; // of the parameter
-    int         m, n, mp, panels;  // m <= n; rows of a panel (multiple of 128), panels of X
+    int         m, n, mp, panels;  // m <= n; rows (a multiple of 128) and units of a row of X
     int         chunks, first_chunk, first_block, first_sym, first_apply;  // where its work begins in each launch
     float       rate;
 };
@@ -101,6 +102,12 @@ __device__ __forceinline__ void put(__nv_bfloat16* to, float v) { *to = __float2
 // Where a value of X lies.
 __device__ __forceinline__ int64_t place(int mp, int row, int col) {
     return ((int64_t)(col / 32) * (mp / 32) + row / 32) * 1024 + col % 32 / 4 * 128 + row % 32 * 4 + col % 4;
+}
+
+// Where an operand's value lies in its units, `panels` of them a row.
+constexpr int kUnit = 128 * 64;
+__device__ __forceinline__ int64_t in_units(int panels, int row, int col) {
+    return ((int64_t)(row / 128) * panels + col / 64) * kUnit + row % 128 * 64 + col % 64;
 }
 
 struct Rates {
@@ -274,7 +281,7 @@ __global__ void __launch_bounds__(256) k_muon_begin(const Entry* __restrict__ ta
         const int row = (threadIdx.x / 32 & 1) * 32 + threadIdx.x % 32, col = (threadIdx.x / 64 + i * 4) * 4;
         *reinterpret_cast<float4*>(m.x[0] + place(m.mp, row0 + row, panel * 64 + col)) = make_float4(x_of(row, col), x_of(row, col + 1), x_of(row, col + 2), x_of(row, col + 3));
     }
-    __half* const op = work + m.operand[0] * 64 + ((int64_t)panel * m.mp + row0) * 64;
+    __half* const op = work + (int64_t)m.operand[0] * kUnit + in_units(m.panels, row0, panel * 64);
     const int64_t plane = (int64_t)m.panels * m.mp * 64;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {  // a row's 128 bytes by eight lanes
@@ -298,6 +305,7 @@ enum Kind { kGram = 0, kSquare = 1, kApply = 2, kLast = 3 };
 struct Params {
     const Entry* table;
     int     count, tiles, wide, stages;
+    int     span;        // columns of the second operand that a copy brings
     int     from, step;  // from: which X it starts from
     __half* work;
     int*    failed;      // a wait ran out
@@ -403,7 +411,7 @@ __global__ void __launch_bounds__(256) k_muon_check(const Entry* __restrict__ ta
 // what lies above it is written to both places.  kApply: a X + B X.  kLast: likewise, and the parameters' update.
 // CG: CTAs per tile (2: of 256 rows, each CTA with 128 of them and half of the second operand).
 template <int KIND, int PARTS, int CG>
-__global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constant__ CUtensorMap map, const Params p) {
+__global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
     constexpr bool kApplies = KIND == kApply || KIND == kLast;
     constexpr bool kBMn = kApplies;             // the second operand's rows lie along K
     constexpr bool kSegments = PARTS == 2;
@@ -428,7 +436,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
         bar_init(drained, 1);
         give_up = 0;
         bar_init_fence();
-        prefetch_map(&map);
+        prefetch_map(&map_a);
+        prefetch_map(&map_b);
     }
     if (warp == 1) tmem_alloc<CG>(smem_addr(&slot_at), kColumns);
     former_is_done();
@@ -494,25 +503,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
         for (int u = worker; u < p.tiles && ok; u += workers) {
             const Tile t = tile_at(u);
             const Entry m = p.table[t.e];
-            // rows of 128 bytes: where panel k of the first operand begins, and the second's
-            const int64_t x0 = p.from ? m.operand[1] : m.operand[0], x_plane = (int64_t)m.panels * m.mp, s_plane = (int64_t)(m.mp / 64) * m.mp;
-            const int64_t a0 = KIND == kGram ? x0 : KIND == kSquare ? m.gram : m.factor, b0 = KIND == kSquare ? m.gram : x0;
-            const int64_t a_plane = KIND == kGram ? x_plane : s_plane, b_plane = KIND == kSquare ? s_plane : x_plane;
-            // columns of the tile that there are and are this CTA's, in units of 64
-            const int limit = kApplies ? m.panels * 64 : m.mp, have = min(p.wide, limit - t.col) / (64 * CG), from = t.col + rank * have * 64;
+            // units: where the operands begin, and those of their second parts
+            const int x0 = p.from ? m.operand[1] : m.operand[0], x_part = m.mp / 128 * m.panels, s_row = m.mp / 64, s_part = m.mp / 128 * s_row;
+            const int a0 = KIND == kGram ? x0 : KIND == kSquare ? m.gram : m.factor, b0 = KIND == kSquare ? m.gram : x0;
+            const int a_part = KIND == kGram ? x_part : s_part, b_part = KIND == kSquare ? s_part : x_part, b_row = KIND == kSquare ? s_row : m.panels;
+            const int a_first = a0 + (t.row / 128 + rank) * (KIND == kGram ? m.panels : s_row);
+            // columns of the tile that there are and are this CTA's
+            const int limit = kApplies ? m.panels * 64 : m.mp, have = min(p.wide, limit - t.col) / CG, from = t.col + rank * have;
+            const int copies = (have + p.span - 1) / p.span, span_bytes = p.span * kDepth * 2;
             for (int k = 0; k < t.depth; ++k) {
                 ok = wait(empty + 8 * stage, phase ^ 1);
                 if (!ok) break;
                 const uint32_t a = base + stage * stage_bytes, b = a + PARTS * part_a, bar = CG == 2 ? in_cta(full + 8 * stage, 0) : full + 8 * stage;
-                if (rank == 0) bar_expect(full + 8 * stage, CG * PARTS * (part_a + have * 8192));
+                if (rank == 0) bar_expect(full + 8 * stage, CG * PARTS * (part_a + copies * span_bytes));
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q) {
-                    const int64_t a_at = a0 + q * a_plane + (int64_t)k * m.mp + t.row + rank * kRowsPerCta;
-                    load_box<CG>(a + q * part_a, &map, bar, 0, (int)a_at, 0);
-                    load_box<CG>(a + q * part_a + 8192, &map, bar, 0, (int)a_at + 64, 0);
-                    for (int j = 0; j < have; ++j) {
-                        const int64_t b_at = b0 + q * b_plane + (kBMn ? (int64_t)(from / 64 + j) * m.mp + k * 64 : (int64_t)k * m.mp + from + j * 64);
-                        load_box<CG>(b + q * part_b + j * 8192, &map, bar, 0, (int)b_at, 0);
+                    load_box<CG>(a + q * part_a, &map_a, bar, 0, 0, a_first + q * a_part + k);
+                    for (int j = 0; j < copies; ++j) {
+                        const int col = from + j * p.span;
+                        if (kBMn) load_box<CG>(b + q * part_b + j * span_bytes, &map_b, bar, 0, k % 2 * 64, b0 + q * b_part + k / 2 * b_row + col / 64);
+                        else load_box<CG>(b + q * part_b + j * span_bytes, &map_b, bar, 0, col % 128, b0 + q * b_part + col / 128 * b_row + k);
                     }
                 }
                 ++issued;
@@ -581,12 +591,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
             const Entry m = p.table[t.e];
             const int row = t.row + rank * kRowsPerCta + quarter * 32 + lane, col0 = t.col + half * half_wide;
             const int limit = kApplies ? m.panels * 64 : m.mp;
-            const int64_t s_plane = (int64_t)(m.mp / 64) * m.mp * 64, x_plane = (int64_t)m.panels * m.mp * 64;
+            const int64_t s_plane = (int64_t)m.mp * m.mp, x_plane = (int64_t)m.panels * m.mp * 64;
             const float shift = KIND == kGram ? 0.f : m.shift[p.step], old = kApplies ? p.old + shift : p.old;
             const int64_t at0 = kApplies ? place(m.mp, row, col0) : 0;
             const float* const x_from = p.from ? m.x[1] : m.x[0];
             float* const       x_to   = p.from ? m.x[0] : m.x[1];
-            const int64_t      target = KIND == kGram ? m.gram : KIND == kSquare ? m.factor : p.from ? m.operand[0] : m.operand[1];
+            const int          target = KIND == kGram ? m.gram : KIND == kSquare ? m.factor : p.from ? m.operand[0] : m.operand[1];
             auto load_x = [&](int c, float4 (&x)[8]) {  // 32 columns of X
                 if (col0 + c >= limit) return;
                 const float4* const from = reinterpret_cast<const float4*>(x_from + at0 + (int64_t)(c / 32) * m.mp * 32);
@@ -615,14 +625,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                 } else if (row / 128 > col / 128) {
                     return;  // below the diagonal
                 }
-                const int64_t at = ((int64_t)(col / 64) * m.mp + row) * 64 + col % 64;
-                __half* const to = p.work + target * 64;
+                const int64_t at = in_units(kApplies ? m.panels : m.mp / 64, row, col);
+                __half* const to = p.work + (int64_t)target * kUnit;
                 const int64_t plane = KIND == kApply ? x_plane : s_plane;
                 if (KIND == kSquare) {
 #pragma unroll
                     for (int q = PARTS - 1; q >= 0; --q) {
                         uint32_t w[16];
-                        load_sector(p.work + m.gram * 64 + q * plane + at, w), load_sector(p.work + m.gram * 64 + q * plane + at + 16, w + 8);
+                        load_sector(p.work + (int64_t)m.gram * kUnit + q * plane + at, w), load_sector(p.work + (int64_t)m.gram * kUnit + q * plane + at + 16, w + 8);
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
                             const float2 a = __half22float2(reinterpret_cast<const __half2&>(w[j]));
@@ -651,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                     }
                     store_sector(to + q * plane + at, w), store_sector(to + q * plane + at + 16, w + 8);
                     if (mirror) {
-                        __half* const under = to + q * plane + ((int64_t)(row / 64) * m.mp + col) * 64 + row % 64;
+                        __half* const under = to + q * plane + in_units(m.mp / 64, col, row);
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
                             const __half2 h = reinterpret_cast<const __half2&>(w[j]);
@@ -791,16 +801,15 @@ Chain chain_of(const Matrix* matrices, int64_t count, int parts, int steps, void
         e.shift   = w.take<float>(steps);
         const int64_t values = (int64_t)e.panels * e.mp * 64;
         for (int j = 0; j < 2; ++j) e.x[j] = w.take<float>(values);
-        for (int j = 0; j < 2; ++j) {
-            e.operand[j] = (int64_t)(w.used / 128);
-            w.take<__half>(parts * values);
-        }
-        for (int64_t* at : {&e.gram, &e.factor}) {
-            *at = (int64_t)(w.used / 128);
-            w.take<__half>((int64_t)parts * e.mp * e.mp);
-        }
+        auto units = [&](int* at, int64_t halves) {
+            w.used = (size_t)up((int64_t)w.used, kUnit * 2);
+            *at = (int)(w.used / (kUnit * 2));
+            w.take<__half>(halves);
+        };
+        for (int& at : e.operand) units(&at, parts * values);
+        units(&e.gram, (int64_t)parts * e.mp * e.mp), units(&e.factor, (int64_t)parts * e.mp * e.mp);
     }
-    c.bytes = w.used;
+    c.bytes = (size_t)up((int64_t)w.used, kUnit * 2);
     return c;
 }
 
@@ -850,11 +859,11 @@ int follow(void (*kernel)(P...), int64_t grid, int threads, int shared, int clus
 }
 
 template <int KIND, int PARTS, int CG>
-int launch(const CUtensorMap& map, const Params& p, int sms, cudaStream_t stream) {
+int launch(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int sms, cudaStream_t stream) {
     auto kernel = k_muon_tiles<KIND, PARTS, CG>;
     static std::atomic<uint64_t> allowed{0};
     FW_DO(allow_shared(kernel, kShared, allowed));
-    return follow(kernel, std::min(p.tiles, sms / CG) * CG, kThreads, kShared, CG, stream, map, p);
+    return follow(kernel, std::min(p.tiles, sms / CG) * CG, kThreads, kShared, CG, stream, a, b, p);
 }
 
 template <typename X>
@@ -886,12 +895,15 @@ int run_chain(Chain& c, const Rates& rates, const std::vector<Step>& steps, char
         return s;
     };
     const Shape sym = shape(false), apply = shape(true);
-    if (sym.tiles >= INT32_MAX || apply.tiles >= INT32_MAX || c.chunks >= INT32_MAX || c.blocks >= INT32_MAX || c.bytes / 128 >= INT32_MAX)
+    if (sym.tiles >= INT32_MAX || apply.tiles >= INT32_MAX || c.chunks >= INT32_MAX || c.blocks >= INT32_MAX || c.bytes / (kUnit * 2) >= INT32_MAX)
         return FRAMEWISE_B200_BAD_ARGUMENT;
     FW_DO(bind_device());
-    CUtensorMap map;
-    const int64_t lines = (int64_t)(c.bytes / 128);
-    if (!map_of(&map, work, false, 64, lines, 1, 64, lines * 64, 64, 64)) return FRAMEWISE_B200_TENSOR_MAP;
+    // 128 rows of a unit; 64 of them; 64 rows of two units
+    CUtensorMap tall, square, two;
+    const int64_t units = (int64_t)(c.bytes / (kUnit * 2));
+    if (!map_of(&tall, work, false, 64, 128, units, 64, kUnit, 64, 128) || !map_of(&square, work, false, 64, 128, units, 64, kUnit, 64, 64) ||
+        !map_of(&two, work, false, 64, 128, units, 64, kUnit, 64, 64, 2))
+        return FRAMEWISE_B200_TENSOR_MAP;
     FW_TRY(cudaMemsetAsync(c.failed, 0, 4, stream));
     Steps abc;
     abc.count = (int)steps.size();
@@ -911,7 +923,9 @@ int run_chain(Chain& c, const Rates& rates, const std::vector<Step>& steps, char
         const int other = KIND == kLast ? kEpilogue * kTurn : 0;
         p.tiles = (int)sh.tiles, p.wide = sh.wide;
         p.stages = std::min(kMostStages, (kShared - 1024 - other) / (PARTS * (kRowsPerCta + sh.wide / sh.pair) * kDepth * 2));
-        return sh.pair == 2 ? launch<KIND, PARTS, 2>(map, p, sms, stream) : launch<KIND, PARTS, 1>(map, p, sms, stream);
+        p.span = std::min(128, sh.wide / sh.pair);
+        const CUtensorMap& b = p.span == 64 ? square : KIND == kApply || KIND == kLast ? two : tall;
+        return sh.pair == 2 ? launch<KIND, PARTS, 2>(tall, b, p, sms, stream) : launch<KIND, PARTS, 1>(tall, b, p, sms, stream);
     };
     Params p = {};
     p.table = c.table, p.count = count, p.work = halves, p.failed = c.failed, p.rates = rates;
