@@ -38,12 +38,14 @@ constexpr int kMostMatrices = 256;   // of a chain of launches
 constexpr int kSlots        = 24;    // matrices in a launch's arguments
 constexpr int kChunk        = 16384; // values per CTA of the pass over gradients
 constexpr int kRowsPerCta   = 128;   // of a tile: the lanes of tensor memory
+constexpr int kMostWide     = 256;   // columns of a tile at most
 constexpr int kColumns      = 512;   // of tensor memory: a ring of accumulators
 constexpr int kMostAccs     = 8;
 constexpr int kDepth        = 64;    // K per stage
-constexpr int kSegment      = 1;     // f32: stages after which an accumulator is added up in registers, for tensor cores cut
-                                     // off what they add, at 2^-24 of the sum a step, and never round it up: 6 x 500 x 2001 is off
-                                     // by 5.1e-6 of its norm with 4, by 2.0e-6 with 1 (plain 32 bits: 2.7e-6)
+constexpr int kSegment      = 2;     // f32: stages after which an accumulator is added up in registers, for tensor cores cut
+                                     // off what they add, at 2^-24 of the sum a step, and never round it up.  A segment's small
+                                     // products come first, so that eight steps of it count: 6 x 500 x 2001 is off by SEGERR of
+                                     // its norm (plain 32 bits: 2.7e-6; segments of four stages, stage by stage: 5.1e-6)
 constexpr int kMostStages   = 8;
 constexpr int kEpilogue     = 8;     // warps that finish tiles
 constexpr int kThreads      = 64 + 32 * kEpilogue;
@@ -315,9 +317,6 @@ struct Params {
     Rates   rates;       // kLast
 };
 
-// Columns of a tile at most.  f32: the sums of its segments have to fit the registers of those who add them up.
-__host__ __device__ constexpr int most_wide(int parts) { return parts == 2 ? 128 : 256; }
-
 // fp16 operands, f32 sums
 __host__ __device__ constexpr uint32_t half_kind(int m, int n, bool b_mn) {
     return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
@@ -335,61 +334,79 @@ __device__ __forceinline__ void store_sector(__half* x, const uint32_t* w) {
                  : "memory");
 }
 
-// p = p decay - rate X, or the result X itself, for a row a lane and 32 columns of X.  They go through shared memory (32 rows of 33
+// p = p decay - rate X, or the result X itself, for a row a lane and 32 columns of X.  They go through shared memory (32 rows of 32
 // words of this warp's), so that neighbouring lanes have neighbouring values in memory whichever way the parameter lies, and
 // so that the code is a loop: written out for 32 values it did not fit the instruction cache (4 x 2048 x 8192 bf16: 515 us a launch).
-constexpr int kTurn = 32 * 33 * 4;
-template <typename X, int USE>  // 0: the result, 1: parameters, 2: parameters and their copies
-__device__ __forceinline__ void update_lines(const float* t, X* p, float* copy, int lines, int64_t pitch, const Rates& r, float rate) {
-    constexpr int kAtOnce = 16;
-#pragma unroll 1
-    for (int j0 = 0; j0 < 32; j0 += kAtOnce) {
-        X     was[kAtOnce];
-        float held[kAtOnce];
+constexpr int kTurn = 32 * 32 * 4;
+// Line 0 of the 32 that a warp meets, and the place of them that is this lane's: those lines that there are.
+struct Lines {
+    int64_t first;
+    int     count;
+    __device__ __forceinline__ Lines(const Entry& m, int row, int col, int lane) {
+        const bool tall = m.rows > m.cols;
+        const int  line = tall ? col : row - lane, at = tall ? row : col + lane;
+        first = (int64_t)line * m.cols + at, count = at < m.cols ? min(32, m.rows - line) : 0;
+    }
+};
+template <typename X>
+__device__ __forceinline__ void load_parameters(const Entry& m, int row, int col, int lane, X (&was)[32]) {
+    const Lines at(m, row, col, lane);
+    const X*    p = static_cast<const X*>(m.param) + at.first;
+    if (m.momentum) {
 #pragma unroll
-        for (int j = 0; j < kAtOnce; ++j) {
-            if (USE >= 1 && j0 + j < lines) was[j] = p[j * pitch];
-            if (USE == 2 && j0 + j < lines) held[j] = copy[j * pitch];
-        }
-#pragma unroll
-        for (int j = 0; j < kAtOnce; ++j) {
-            float now = t[(j0 + j) * 33];
-            if (USE >= 1) {
-                float old = value(was[j]);
-                if (USE == 2) {
-                    X rounded;
-                    put(&rounded, held[j]);
-                    // a copy of which the parameter is not the rounded value has been left behind by the program
-                    if (!r.follow || value(rounded) == old || (old != old && held[j] != held[j])) old = held[j];
-                }
-                now = old * r.decay - rate * now;
-            }
-            if (j0 + j < lines) {
-                if (USE == 2) copy[j * pitch] = now;
-                put(p + j * pitch, now);
-            }
-        }
-        p += kAtOnce * pitch;
-        if (USE == 2) copy += kAtOnce * pitch;
+        for (int j = 0; j < 32; ++j, p += m.cols)
+            if (j < at.count) was[j] = *p;
     }
 }
-template <int PARTS>
-__device__ __forceinline__ void update(const Entry& m, const Rates& r, const float* v, int row, int col, char* turn, int lane) {
-    using X = std::conditional_t<PARTS == 2, float, __nv_bfloat16>;
+template <bool EARLY, typename X>  // EARLY: `was` holds the parameters
+__device__ __forceinline__ void update(const Entry& m, const Rates& r, const float* v, int row, int col, char* turn, int lane, const X* was) {
     const bool tall = m.rows > m.cols;
     float* const t = reinterpret_cast<float*>(turn);
-    const int own = tall ? lane : lane * 33, step = tall ? 33 : 1;
     __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 32; ++j) t[own + j * step] = v[j];
+    for (int j = 0; j < 32; ++j) t[tall ? j * 32 + (lane ^ j) : lane * 32 + (j ^ lane)] = v[j];
     __syncwarp();
-    // line j of 32, place `at` of it
-    const int line0 = tall ? col : row - lane, at = tall ? row : col + lane, lines = at < m.cols ? min(32, m.rows - line0) : 0;
-    const int64_t first = (int64_t)line0 * m.cols + at;
-    X* const p = static_cast<X*>(m.param) + first;
-    if (!m.momentum) update_lines<X, 0>(t + lane, p, nullptr, lines, m.cols, r, m.rate);
-    else if (!m.master) update_lines<X, 1>(t + lane, p, nullptr, lines, m.cols, r, m.rate);
-    else update_lines<X, 2>(t + lane, p, m.master + first, lines, m.cols, r, m.rate);
+    auto x = [&](int j) { return t[j * 32 + (lane ^ j)]; };
+    const Lines at(m, row, col, lane);
+    X* p = static_cast<X*>(m.param) + at.first;
+    if (!m.momentum) {
+#pragma unroll 8
+        for (int j = 0; j < 32; ++j, p += m.cols)
+            if (j < at.count) put(p, x(j));
+    } else if (!m.master) {
+        if constexpr (EARLY) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j, p += m.cols)
+                if (j < at.count) put(p, value(was[j]) * r.decay - m.rate * x(j));
+        } else {
+            constexpr int kAtOnce = 16;
+#pragma unroll 1
+            for (int j0 = 0; j0 < 32; j0 += kAtOnce) {
+                X now[kAtOnce];
+                const X* from = p;
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j, from += m.cols)
+                    if (j0 + j < at.count) now[j] = *from;
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j, p += m.cols)
+                    if (j0 + j < at.count) put(p, value(now[j]) * r.decay - m.rate * x(j0 + j));
+            }
+        }
+    } else {
+        float* copy = m.master + at.first;
+#pragma unroll 4
+        for (int j = 0; j < 32; ++j, p += m.cols, copy += m.cols) {
+            if (j >= at.count) continue;
+            const float held = *copy, old = value(*p);
+            X rounded;
+            put(&rounded, held);
+            // a copy of which the parameter is not the rounded value has been left behind by the program
+            const bool left = r.follow && !(value(rounded) == old || (old != old && held != held));
+            const float now = (left ? old : held) * r.decay - m.rate * x(j);
+            *copy = now;
+            put(p, now);
+        }
+    }
     __syncwarp();
 }
 
@@ -415,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
     constexpr bool kApplies = KIND == kApply || KIND == kLast;
     constexpr bool kBMn = kApplies;             // the second operand's rows lie along K
     constexpr bool kSegments = PARTS == 2;
-    constexpr int  kWide = most_wide(PARTS), kTile = kRowsPerCta * CG;
+    constexpr int  kTile = kRowsPerCta * CG;
     extern __shared__ char shared_raw[];
     __shared__ int firsts[kMostMatrices];
     __shared__ uint64_t bars_at[2 * kMostStages + 2 * kMostAccs + 1];
@@ -554,22 +571,45 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                 if (!ok) break;
                 fence_after();
                 const uint32_t d = tmem + acc * p.wide;
-                const int k1 = kSegments ? min(t.depth, k0 + kSegment) : t.depth;
-                for (int k = k0; k < k1; ++k) {
-                    ok = wait(full + 8 * stage, phase);
-                    if (!ok) break;
-                    fence_after();
-                    const uint32_t a = base + stage * stage_bytes, b = a + PARTS * part_a;
+                if constexpr (kSegments) {  // the small products of all stages, then the large ones
+                    const int some = min(kSegment, t.depth - k0);
+                    for (int large = 0; large < 2 && ok; ++large) {
+                        int      at = stage;
+                        uint32_t at_phase = phase;
+                        for (int k = 0; k < some; ++k) {
+                            if (!large) {
+                                ok = wait(full + 8 * at, at_phase);
+                                if (!ok) break;
+                                fence_after();
+                            }
+                            const uint32_t a = base + at * stage_bytes, b = a + PARTS * part_a;
 #pragma unroll
-                    for (int q = PARTS == 2 ? 0 : 2; q < 3; ++q) {  // of two parts: the small products first
-                        const uint32_t aq = q == 0 ? a + part_a : a, bq = q == 1 ? b + part_b : b;
+                            for (int q = 0; q < 2; ++q) {
+                                if (large && q == 1) continue;
+                                const uint32_t aq = !large && q == 0 ? a + part_a : a, bq = !large && q == 1 ? b + part_b : b;
+#pragma unroll
+                                for (int i = 0; i < kDepth / 16; ++i)
+                                    product<CG>(d, operand(aq + i * 32, 8192), operand(bq + i * (kBMn ? 2048 : 32), 8192), kind,
+                                                large || k > 0 || q > 0 || i > 0);
+                            }
+                            if (large) products_commit<CG>(empty + 8 * at);
+                            if (++at == p.stages) at = 0, at_phase ^= 1;
+                        }
+                        if (large) stage = at, phase = at_phase;
+                    }
+                    if (!ok) break;
+                } else {
+                    for (int k = 0; k < t.depth; ++k) {
+                        ok = wait(full + 8 * stage, phase);
+                        if (!ok) break;
+                        fence_after();
+                        const uint32_t a = base + stage * stage_bytes, b = a + part_a;
 #pragma unroll
                         for (int i = 0; i < kDepth / 16; ++i)
-                            product<CG>(d, operand(aq + i * 32, 8192), operand(bq + i * (kBMn ? 2048 : 32), 8192), kind,
-                                       k > k0 || q > (PARTS == 2 ? 0 : 2) || i > 0);
+                            product<CG>(d, operand(a + i * 32, 8192), operand(b + i * (kBMn ? 2048 : 32), 8192), kind, k > 0 || i > 0);
+                        products_commit<CG>(empty + 8 * stage);
+                        if (++stage == p.stages) stage = 0, phase ^= 1;
                     }
-                    products_commit<CG>(empty + 8 * stage);
-                    if (++stage == p.stages) stage = 0, phase ^= 1;
                 }
                 products_commit<CG>(done + 8 * acc);
                 if (++acc == accs) acc = 0, acc_phase ^= 1;
@@ -603,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = from[j * 32];
             };
-            auto finish = [&](float* v, int c, const float4 (&x)[8]) {  // 32 columns
+            auto finish = [&](float* v, int c, const float4 (&x)[8], auto* was) {  // 32 columns
                 const int col = col0 + c;
                 if (col >= limit) return;
                 if (kApplies) {
@@ -614,8 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                     }
                 }
                 if constexpr (KIND == kLast) {
-                    update<PARTS>(m, p.rates, v, row, col, shared_raw + (warp - 2) * kTurn, lane);
-                    __syncwarp();
+                    update<!kSegments>(m, p.rates, v, row, col, shared_raw + (warp - 2) * kTurn, lane, was);
                     return;
                 }
                 if (KIND == kApply) {
@@ -670,36 +709,52 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                     }
                 }
             };
-            constexpr int kBuffers = kApplies ? 2 : 1;
+            constexpr int kBuffers = KIND == kApply && !kSegments ? 2 : 1;
             float4 x_of[kBuffers][8];
-            if (kApplies) load_x(0, x_of[0]);  // ahead of the sums
-            if (kApplies && kSegments && half_wide > 32) load_x(32, x_of[kBuffers - 1]);
-            float total[kSegments ? kWide / 2 : 1];
+            if (KIND == kApply && !kSegments) load_x(0, x_of[0]);  // ahead of the sums
+            using X = std::conditional_t<PARTS == 2, float, __nv_bfloat16>;
+            X was[KIND == kLast && !kSegments ? 32 : 1];
+            float total[kSegments ? kMostWide / 2 : 1];
             if constexpr (kSegments) {
 #pragma unroll
-                for (int j = 0; j < kWide / 2; ++j) total[j] = 0.f;
+                for (int j = 0; j < kMostWide / 2; ++j) total[j] = 0.f;
             }
             for (int k0 = 0; k0 < t.depth; k0 += kSegments ? kSegment : t.depth) {
                 ok = __all_sync(0xffffffffu, wait(done + 8 * acc, acc_phase));
                 if (!ok) break;
                 fence_after();
                 const uint32_t acc_at = tmem + ((uint32_t)(quarter * 32) << 16) + acc * p.wide + half * half_wide;
+                auto columns = [&](int c, auto buffer) {
+                    constexpr int kBuffer = decltype(buffer)::value;
+                    float2 pairs[16];
+                    float* const v = reinterpret_cast<float*>(pairs);
+                    if constexpr (KIND == kLast && !kSegments) load_x(c, x_of[0]), load_parameters(m, row, col0 + c, lane, was);
+                    tmem_load32(acc_at + c, pairs);
+                    tmem_loaded(pairs);
+                    if constexpr (kBuffers == 2)
+                        if (c + 32 < half_wide) load_x(c + 32, x_of[kBuffer ^ 1]);
+                    finish(v, c, x_of[kBuffer], was);
+                    __syncwarp();
+                };
+                if constexpr (kSegments) {
 #pragma unroll
-                for (int c = 0; c < kWide / 2; c += 32) {
-                    if (c < half_wide && col0 + c < limit) {
+                    for (int c = 0; c < kMostWide / 2; c += 32) {
+                        if (c >= half_wide || col0 + c >= limit) continue;
                         float2 pairs[16];
-                        float* const v = reinterpret_cast<float*>(pairs);
+                        const float* const v = reinterpret_cast<const float*>(pairs);
                         tmem_load32(acc_at + c, pairs);
                         tmem_loaded(pairs);
-                        if constexpr (kSegments) {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) total[c + j] += v[j];
-                        } else {
-                            if (kBuffers == 2 && c + 32 < half_wide) load_x(c + 32, x_of[(c / 32 + 1) % kBuffers]);
-                            finish(v, c, x_of[c / 32 % kBuffers]);
-                            __syncwarp();
-                        }
+                        for (int j = 0; j < 32; ++j) total[c + j] += v[j];
                     }
+                } else if constexpr (kBuffers == 2) {
+                    for (int c = 0; c < half_wide && col0 + c < limit; c += 64) {
+                        columns(c, std::integral_constant<int, 0>());
+                        if (c + 32 < half_wide && col0 + c + 32 < limit) columns(c + 32, std::integral_constant<int, 1>());
+                    }
+                } else {
+#pragma unroll 1
+                    for (int c = 0; c < half_wide && col0 + c < limit; c += 32) columns(c, std::integral_constant<int, 0>());
                 }
                 fence_before();
                 __syncwarp();
@@ -709,9 +764,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
             if (!ok) break;
             if constexpr (kSegments) {
 #pragma unroll
-                for (int c = 0; c < kWide / 2; c += 32) {
+                for (int c = 0; c < kMostWide / 2; c += 32) {
                     if (c >= half_wide) continue;
-                    finish(total + c, c, x_of[c / 32 % kBuffers]);
+                    if (kApplies) load_x(c, x_of[0]);
+                    finish(total + c, c, x_of[0], was);
                     __syncwarp();
                 }
             }
@@ -886,13 +942,22 @@ int run_chain(Chain& c, const Rates& rates, const std::vector<Step>& steps, char
         }
         return tiles;
     };
-    // pairs of CTAs where there are tiles for all of them; else tiles as wide as leaves all SMs something to do
+    // The shape of the tiles whose time is the shortest by this count: clocks of a stage of 64 of K by what the products take or what
+    // a CTA can be fed (48 bytes a clock, measured), some thousand clocks a tile for what does not overlap, and whole rounds.
     auto shape = [&](bool apply) {
-        Shape s = {1, most_wide(PARTS), 0};
-        if (c.pairs && lay(2, s.wide, apply, false) >= sms / 2) s.pair = 2;
-        else while (s.wide > 64 && lay(1, s.wide, apply, false) < sms) s.wide /= 2;
-        s.tiles = lay(s.pair, s.wide, apply, true);
-        return s;
+        Shape  best = {1, 64, 0};
+        double least = 1e300;
+        for (int pair = 1; pair <= (c.pairs ? 2 : 1); ++pair)
+            for (int wide = 64 * pair; wide <= kMostWide; wide *= 2) {
+                const double products = wide * 2.0 * (PARTS == 2 ? 3 : 1), fed = PARTS * (kRowsPerCta + wide / pair) * kDepth * 2 / 48.0;
+                const int64_t tiles = lay(pair, wide, apply, false), workers = sms / pair;
+                double stages = 0;
+                for (const Entry& e : c.entry) stages = std::max(stages, (double)(apply ? (e.m + 63) / 64 : e.panels));
+                const double time = (double)((tiles + workers - 1) / workers) * (stages * std::max(products, fed) + 3000);
+                if (time < least) least = time, best = {pair, wide, tiles};
+            }
+        lay(best.pair, best.wide, apply, true);
+        return best;
     };
     const Shape sym = shape(false), apply = shape(true);
     if (sym.tiles >= INT32_MAX || apply.tiles >= INT32_MAX || c.chunks >= INT32_MAX || c.blocks >= INT32_MAX || c.bytes / (kUnit * 2) >= INT32_MAX)
