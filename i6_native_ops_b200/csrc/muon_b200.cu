@@ -41,12 +41,12 @@ constexpr int kRowsPerCta   = 128;   // of a tile: the lanes of tensor memory
 constexpr int kMostWide     = 256;   // columns of a tile at most
 constexpr int kColumns      = 512;   // of tensor memory: a ring of accumulators
 constexpr int kMostAccs     = 8;
-constexpr int kDepth        = 64;    // K per stage
-constexpr int kSegment      = 2;     // f32: stages after which an accumulator is added up in registers, for tensor cores cut
+constexpr int kDepth        = 64;    // K per stage: one part of both operands
+constexpr int kSegment      = 2;     // f32: steps of 64 of K after which an accumulator is added up in registers, for tensor cores cut
                                      // off what they add, at 2^-24 of the sum a step, and never round it up.  A segment's small
                                      // products come first, so that eight steps of it count: 6 x 500 x 2001 is off by SEGERR of
                                      // its norm (plain 32 bits: 2.7e-6; segments of four stages, stage by stage: 5.1e-6)
-constexpr int kMostStages   = 8;
+constexpr int kMostStages   = 12;
 constexpr int kEpilogue     = 8;     // warps that finish tiles
 constexpr int kThreads      = 64 + 32 * kEpilogue;
 constexpr int kShared       = 232448 - 2048;  // dynamic; the rest: the static arrays
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int kTurns = KIND == kLast ? kEpilogue * kTurn : 0;
     const uint32_t base = (smem_addr(shared_raw) + kTurns + 1023u) & ~1023u;
-    const int part_b = p.wide / CG * kDepth * 2, part_a = kRowsPerCta * kDepth * 2, stage_bytes = PARTS * (part_a + part_b);
+    const int part_b = p.wide / CG * kDepth * 2, part_a = kRowsPerCta * kDepth * 2, stage_bytes = part_a + part_b;
 
     next_may_start();
     if (threadIdx.x == 0) {
@@ -528,22 +528,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
             // columns of the tile that there are and are this CTA's
             const int limit = kApplies ? m.panels * 64 : m.mp, have = min(p.wide, limit - t.col) / CG, from = t.col + rank * have;
             const int copies = (have + p.span - 1) / p.span, span_bytes = p.span * kDepth * 2;
-            for (int k = 0; k < t.depth; ++k) {
-                ok = wait(empty + 8 * stage, phase ^ 1);
-                if (!ok) break;
-                const uint32_t a = base + stage * stage_bytes, b = a + PARTS * part_a, bar = CG == 2 ? in_cta(full + 8 * stage, 0) : full + 8 * stage;
-                if (rank == 0) bar_expect(full + 8 * stage, CG * PARTS * (part_a + copies * span_bytes));
-#pragma unroll
-                for (int q = 0; q < PARTS; ++q) {
-                    load_box<CG>(a + q * part_a, &map_a, bar, 0, 0, a_first + q * a_part + k);
+            for (int k = 0; k < t.depth && ok; ++k) {
+                for (int q = PARTS - 1; q >= 0; --q) {  // the small part is met, and its stage free again, first
+                    ok = wait(empty + 8 * stage, phase ^ 1);
+                    if (!ok) break;
+                    const uint32_t a = base + stage * stage_bytes, b = a + part_a, bar = CG == 2 ? in_cta(full + 8 * stage, 0) : full + 8 * stage;
+                    if (rank == 0) bar_expect(full + 8 * stage, CG * (part_a + copies * span_bytes));
+                    load_box<CG>(a, &map_a, bar, 0, 0, a_first + q * a_part + k);
                     for (int j = 0; j < copies; ++j) {
                         const int col = from + j * p.span;
-                        if (kBMn) load_box<CG>(b + q * part_b + j * span_bytes, &map_b, bar, 0, k % 2 * 64, b0 + q * b_part + k / 2 * b_row + col / 64);
-                        else load_box<CG>(b + q * part_b + j * span_bytes, &map_b, bar, 0, col % 128, b0 + q * b_part + col / 128 * b_row + k);
+                        if (kBMn) load_box<CG>(b + j * span_bytes, &map_b, bar, 0, k % 2 * 64, b0 + q * b_part + k / 2 * b_row + col / 64);
+                        else load_box<CG>(b + j * span_bytes, &map_b, bar, 0, col % 128, b0 + q * b_part + col / 128 * b_row + k);
                     }
+                    ++issued;
+                    if (++stage == p.stages) stage = 0, phase ^= 1;
                 }
-                ++issued;
-                if (++stage == p.stages) stage = 0, phase ^= 1;
             }
         }
         // the last stages are handed back before the CTA ends; where a wait ran out, copies in flight end first
@@ -571,44 +570,49 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                 if (!ok) break;
                 fence_after();
                 const uint32_t d = tmem + acc * p.wide;
-                if constexpr (kSegments) {  // the small products of all stages, then the large ones
+                auto next = [&](int& at, uint32_t& at_phase) {
+                    if (++at == p.stages) at = 0, at_phase ^= 1;
+                };
+                auto multiply = [&](int stage_a, int stage_b, bool add) {
+                    const uint32_t a = base + stage_a * stage_bytes, b = base + stage_b * stage_bytes + part_a;
+#pragma unroll
+                    for (int i = 0; i < kDepth / 16; ++i)
+                        product<CG>(d, operand(a + i * 32, 8192), operand(b + i * (kBMn ? 2048 : 32), 8192), kind, add || i > 0);
+                };
+                auto arrived = [&](int at, uint32_t at_phase) {
+                    ok = ok && wait(full + 8 * at, at_phase);
+                    if (ok) fence_after();
+                    return ok;
+                };
+                if constexpr (kSegments) {  // the small products of all steps, then the large ones
+                    int large[kSegment] = {};
                     const int some = min(kSegment, t.depth - k0);
-                    for (int large = 0; large < 2 && ok; ++large) {
-                        int      at = stage;
-                        uint32_t at_phase = phase;
-                        for (int k = 0; k < some; ++k) {
-                            if (!large) {
-                                ok = wait(full + 8 * at, at_phase);
-                                if (!ok) break;
-                                fence_after();
-                            }
-                            const uint32_t a = base + at * stage_bytes, b = a + PARTS * part_a;
 #pragma unroll
-                            for (int q = 0; q < 2; ++q) {
-                                if (large && q == 1) continue;
-                                const uint32_t aq = !large && q == 0 ? a + part_a : a, bq = !large && q == 1 ? b + part_b : b;
-#pragma unroll
-                                for (int i = 0; i < kDepth / 16; ++i)
-                                    product<CG>(d, operand(aq + i * 32, 8192), operand(bq + i * (kBMn ? 2048 : 32), 8192), kind,
-                                                large || k > 0 || q > 0 || i > 0);
-                            }
-                            if (large) products_commit<CG>(empty + 8 * at);
-                            if (++at == p.stages) at = 0, at_phase ^= 1;
-                        }
-                        if (large) stage = at, phase = at_phase;
+                    for (int k = 0; k < kSegment; ++k) {
+                        if (k >= some) continue;
+                        const int low = stage;
+                        if (!arrived(stage, phase)) break;
+                        next(stage, phase);
+                        if (!arrived(stage, phase)) break;
+                        large[k] = stage;
+                        multiply(low, large[k], k > 0);
+                        multiply(large[k], low, true);
+                        products_commit<CG>(empty + 8 * low);
+                        next(stage, phase);
                     }
                     if (!ok) break;
+#pragma unroll
+                    for (int k = 0; k < kSegment; ++k) {
+                        if (k >= some) continue;
+                        multiply(large[k], large[k], true);
+                        products_commit<CG>(empty + 8 * large[k]);
+                    }
                 } else {
                     for (int k = 0; k < t.depth; ++k) {
-                        ok = wait(full + 8 * stage, phase);
-                        if (!ok) break;
-                        fence_after();
-                        const uint32_t a = base + stage * stage_bytes, b = a + part_a;
-#pragma unroll
-                        for (int i = 0; i < kDepth / 16; ++i)
-                            product<CG>(d, operand(a + i * 32, 8192), operand(b + i * (kBMn ? 2048 : 32), 8192), kind, k > 0 || i > 0);
+                        if (!arrived(stage, phase)) break;
+                        multiply(stage, stage, k > 0);
                         products_commit<CG>(empty + 8 * stage);
-                        if (++stage == p.stages) stage = 0, phase ^= 1;
+                        next(stage, phase);
                     }
                 }
                 products_commit<CG>(done + 8 * acc);
@@ -987,7 +991,7 @@ int run_chain(Chain& c, const Rates& rates, const std::vector<Step>& steps, char
         constexpr int KIND = decltype(kind)::value;
         const int other = KIND == kLast ? kEpilogue * kTurn : 0;
         p.tiles = (int)sh.tiles, p.wide = sh.wide;
-        p.stages = std::min(kMostStages, (kShared - 1024 - other) / (PARTS * (kRowsPerCta + sh.wide / sh.pair) * kDepth * 2));
+        p.stages = std::min(kMostStages, (kShared - 1024 - other) / ((kRowsPerCta + sh.wide / sh.pair) * kDepth * 2));
         p.span = std::min(128, sh.wide / sh.pair);
         const CUtensorMap& b = p.span == 64 ? square : KIND == kApply || KIND == kLast ? two : tall;
         return sh.pair == 2 ? launch<KIND, PARTS, 2>(tall, b, p, sms, stream) : launch<KIND, PARTS, 1>(tall, b, p, sms, stream);
