@@ -62,7 +62,7 @@ struct Entry {
     float*      master;     // or null
     double*     partial;    // sums of squares of the chunks
     float*      shift;      // per step: the multiple of the identity that B does without
-    float*      x[2];       // X, before and after a step
+    float*      x;          // X
     int         operand[2]; // its fp16 parts, as units of the workspace
     int         gram, factor; // A and B, likewise
     int         rows, cols; // of the parameter
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(256) k_muon_begin(const Entry* __restrict__ ta
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // a warp: 32 rows of four columns, 512 bytes of X
         const int row = (threadIdx.x / 32 & 1) * 32 + threadIdx.x % 32, col = (threadIdx.x / 64 + i * 4) * 4;
-        *reinterpret_cast<float4*>(m.x[0] + place(m.mp, row0 + row, panel * 64 + col)) = make_float4(x_of(row, col), x_of(row, col + 1), x_of(row, col + 2), x_of(row, col + 3));
+        *reinterpret_cast<float4*>(m.x + place(m.mp, row0 + row, panel * 64 + col)) = make_float4(x_of(row, col), x_of(row, col + 1), x_of(row, col + 2), x_of(row, col + 3));
     }
     __half* const op = work + (int64_t)m.operand[0] * kUnit + in_units(m.panels, row0, panel * 64);
     const int64_t plane = (int64_t)m.panels * m.mp * 64;
@@ -335,77 +335,141 @@ __device__ __forceinline__ void store_sector(__half* x, const uint32_t* w) {
                  : "memory");
 }
 
-// p = p decay - rate X, or the result X itself, for a row a lane and 32 columns of X.  They go through shared memory (32 rows of 32
-// words of this warp's), so that neighbouring lanes have neighbouring values in memory whichever way the parameter lies, and
-// so that the code is a loop: written out for 32 values it did not fit the instruction cache (4 x 2048 x 8192 bf16: 515 us a launch).
-constexpr int kTurn = 32 * 32 * 4;
-// Line 0 of the 32 that a warp meets, and the place of them that is this lane's: those lines that there are.
+constexpr int kTurn = 32 * 32 * 4;  // shared memory of a warp that finishes tiles: to turn 32 x 32 values
+
+// 32 rows, one a lane, of 32 fp16 numbers, to memory the other way round: `to` is where this lane's column goes, 64 bytes.
+__device__ __forceinline__ void store_turned(__half* to, const uint32_t (&w)[16], char* turn, int lane) {
+    uint32_t* const t = reinterpret_cast<uint32_t*>(turn);  // 16 words of two rows for each column
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {  // even lanes take column 2 j of their row and the next, odd ones column 2 j + 1 of theirs and the one before
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, w[j], 1);
+        const int col = 2 * j + (lane & 1);
+        t[col * 16 + ((lane / 8 ^ (col / 2 & 3)) * 4 + lane / 2 % 4)] = lane & 1 ? __byte_perm(other, w[j], 0x7632) : __byte_perm(w[j], other, 0x5410);
+    }
+    __syncwarp();
+    uint32_t o[16];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(o + 4 * j) = *reinterpret_cast<const uint4*>(t + lane * 16 + (j ^ (lane / 2 & 3)) * 4);
+    store_sector(to, o), store_sector(to + 16, o + 8);
+    __syncwarp();
+}
+
+// Parameters of 32 x 32 values of X, by lines of the parameter: line 0 of them, how many there are, and how many values of each.
 struct Lines {
     int64_t first;
-    int     count;
-    __device__ __forceinline__ Lines(const Entry& m, int row, int col, int lane) {
+    int     count, width;
+    __device__ __forceinline__ Lines(const Entry& m, int row0, int col0) {  // of X
         const bool tall = m.rows > m.cols;
-        const int  line = tall ? col : row - lane, at = tall ? row : col + lane;
-        first = (int64_t)line * m.cols + at, count = at < m.cols ? min(32, m.rows - line) : 0;
+        const int  line = tall ? col0 : row0, at = tall ? row0 : col0;
+        first = (int64_t)line * m.cols + at, count = max(0, min(32, m.rows - line)), width = max(0, min(32, m.cols - at));
+    }
+};
+
+// 16 bytes of parameters at a time
+template <typename X>
+struct Grain {
+    static constexpr int kValues = 16 / sizeof(X), kLanes = 32 / kValues, kLines = 32 / kLanes;  // lanes a line, lines at once
+    uint4 w;
+    __device__ __forceinline__ float get(int i) const {
+        const uint32_t* const u = reinterpret_cast<const uint32_t*>(&w);
+        return sizeof(X) == 4 ? __uint_as_float(u[i]) : __uint_as_float(i % 2 ? u[i / 2] & 0xffff0000u : u[i / 2] << 16);
+    }
+    __device__ __forceinline__ void set(const float (&v)[kValues]) {
+        uint32_t* const u = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(X) == 4) u[i] = __float_as_uint(v[i]);
+            else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
+        }
     }
 };
 template <typename X>
-__device__ __forceinline__ void load_parameters(const Entry& m, int row, int col, int lane, X (&was)[32]) {
-    const Lines at(m, row, col, lane);
-    const X*    p = static_cast<const X*>(m.param) + at.first;
-    if (m.momentum) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j, p += m.cols)
-            if (j < at.count) was[j] = *p;
-    }
+__device__ __forceinline__ bool by_grains(const Entry& m) {
+    return m.cols * sizeof(X) % 16 == 0 && (reinterpret_cast<uintptr_t>(m.param) | reinterpret_cast<uintptr_t>(m.master)) % 16 == 0;
 }
-template <bool EARLY, typename X>  // EARLY: `was` holds the parameters
-__device__ __forceinline__ void update(const Entry& m, const Rates& r, const float* v, int row, int col, char* turn, int lane, const X* was) {
+
+// The new value of a parameter; `held`: its copy, if there is one.
+template <typename X>
+__device__ __forceinline__ float updated(float old, float held, bool copied, float x, const Rates& r, float rate) {
+    if (copied) {
+        X rounded;
+        put(&rounded, held);
+        // a copy of which the parameter is not the rounded value has been left behind by the program
+        if (!r.follow || value(rounded) == old || (old != old && held != held)) old = held;
+    }
+    return old * r.decay - rate * x;
+}
+
+template <typename X>
+__device__ __forceinline__ void load_parameters(const Entry& m, const Lines& at, int lane, Grain<X> (&was)[32 / Grain<X>::kLines]) {
+    using G = Grain<X>;
+    const X* p = static_cast<const X*>(m.param) + at.first + (int64_t)(lane / G::kLanes) * m.cols + lane % G::kLanes * G::kValues;
+#pragma unroll
+    for (int i = 0; i < 32 / G::kLines; ++i, p += (int64_t)G::kLines * m.cols)
+        if (i * G::kLines + lane / G::kLanes < at.count && lane % G::kLanes * G::kValues < at.width) was[i].w = *reinterpret_cast<const uint4*>(p);
+}
+
+// p = p decay - rate X, or the result X itself, for 32 x 32 values of X, a row a lane.  They go through shared memory, so that
+// neighbouring lanes have neighbouring values in memory whichever way the parameter lies: 16 bytes a lane, where lines of the
+// parameter begin at multiples of that (`was`: loaded before), else a value a lane.  (A value a lane throughout: 27 to 32 us for a
+// tile of 128 x 256 bf16, GRAINS this way.)
+template <typename X>
+__device__ __forceinline__ void update(const Entry& m, const Rates& r, const float* v, const Lines& at, bool grains, char* turn, int lane,
+                                       const Grain<X> (&was)[32 / Grain<X>::kLines]) {
+    using G = Grain<X>;
     const bool tall = m.rows > m.cols;
     float* const t = reinterpret_cast<float*>(turn);
     __syncwarp();
+    if (tall) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) t[tall ? j * 32 + (lane ^ j) : lane * 32 + (j ^ lane)] = v[j];
-    __syncwarp();
-    auto x = [&](int j) { return t[j * 32 + (lane ^ j)]; };
-    const Lines at(m, row, col, lane);
-    X* p = static_cast<X*>(m.param) + at.first;
-    if (!m.momentum) {
-#pragma unroll 8
-        for (int j = 0; j < 32; ++j, p += m.cols)
-            if (j < at.count) put(p, x(j));
-    } else if (!m.master) {
-        if constexpr (EARLY) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j, p += m.cols)
-                if (j < at.count) put(p, value(was[j]) * r.decay - m.rate * x(j));
-        } else {
-            constexpr int kAtOnce = 16;
-#pragma unroll 1
-            for (int j0 = 0; j0 < 32; j0 += kAtOnce) {
-                X now[kAtOnce];
-                const X* from = p;
-#pragma unroll
-                for (int j = 0; j < kAtOnce; ++j, from += m.cols)
-                    if (j0 + j < at.count) now[j] = *from;
-#pragma unroll
-                for (int j = 0; j < kAtOnce; ++j, p += m.cols)
-                    if (j0 + j < at.count) put(p, value(now[j]) * r.decay - m.rate * x(j0 + j));
-            }
-        }
+        for (int j = 0; j < 32; ++j) t[j * 32 + (lane ^ (j & 7) << 2)] = v[j];
     } else {
-        float* copy = m.master + at.first;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) *reinterpret_cast<float4*>(t + lane * 32 + (j * 4 ^ (lane & 7) << 2)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    }
+    __syncwarp();
+    X* const p = static_cast<X*>(m.param) + at.first;
+    if (grains) {
+        const int l0 = lane / G::kLanes, c0 = lane % G::kLanes * G::kValues;
+#pragma unroll
+        for (int i = 0; i < 32 / G::kLines; ++i) {
+            const int line = i * G::kLines + l0;
+            if (line >= at.count || c0 >= at.width) continue;
+            float x[G::kValues];
+#pragma unroll
+            for (int j = 0; j < G::kValues; j += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(t + line * 32 + (c0 + j ^ (line & 7) << 2));
+                x[j] = f.x, x[j + 1] = f.y, x[j + 2] = f.z, x[j + 3] = f.w;
+            }
+            const int64_t to = (int64_t)line * m.cols + c0;
+            if (m.momentum) {
+                float* const copy = m.master ? m.master + at.first + to : nullptr;
+#pragma unroll
+                for (int j = 0; j < G::kValues; j += 4) {
+                    float4 held = copy ? *reinterpret_cast<const float4*>(copy + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    float* const h = reinterpret_cast<float*>(&held);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) h[k] = x[j + k] = updated<X>(was[i].get(j + k), h[k], copy != nullptr, x[j + k], r, m.rate);
+                    if (copy) *reinterpret_cast<float4*>(copy + j) = held;
+                }
+            }
+            G now;
+            now.set(x);
+            *reinterpret_cast<uint4*>(p + to) = now.w;
+        }
+    } else if (lane < at.width) {
 #pragma unroll 4
-        for (int j = 0; j < 32; ++j, p += m.cols, copy += m.cols) {
+        for (int j = 0; j < 32; ++j) {
             if (j >= at.count) continue;
-            const float held = *copy, old = value(*p);
-            X rounded;
-            put(&rounded, held);
-            // a copy of which the parameter is not the rounded value has been left behind by the program
-            const bool left = r.follow && !(value(rounded) == old || (old != old && held != held));
-            const float now = (left ? old : held) * r.decay - m.rate * x(j);
-            *copy = now;
-            put(p, now);
+            const int64_t to = (int64_t)j * m.cols + lane;
+            float x = t[j * 32 + (lane ^ (j & 7) << 2)];
+            if (m.momentum) {
+                float* const copy = m.master ? m.master + at.first + to : nullptr;
+                x = updated<X>(value(p[to]), copy ? *copy : 0.f, copy != nullptr, x, r, m.rate);
+                if (copy) *copy = x;
+            }
+            put(p + to, x);
         }
     }
     __syncwarp();
@@ -413,10 +477,11 @@ __device__ __forceinline__ void update(const Entry& m, const Rates& r, const flo
 
 template <typename X>
 __device__ __noinline__ void no_result(const Entry& m, int row, int col, int lane) {
-    const Lines at(m, row, col, lane);
-    for (int j = 0; j < at.count; ++j) {
-        put(static_cast<X*>(m.param) + at.first + (int64_t)j * m.cols, __uint_as_float(0x7fffffffu));
-        if (m.master) m.master[at.first + (int64_t)j * m.cols] = __uint_as_float(0x7fffffffu);
+    const Lines at(m, row - lane, col);
+    for (int j = 0; j < at.count && lane < at.width; ++j) {
+        const int64_t to = at.first + (int64_t)j * m.cols + lane;
+        put(static_cast<X*>(m.param) + to, __uint_as_float(0x7fffffffu));
+        if (m.master) m.master[to] = __uint_as_float(0x7fffffffu);
     }
 }
 
@@ -663,19 +728,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_chain(const __grid_constan
                 const int     panels = KIND == kApply ? m.panels : m.mp / 64;
                 const int64_t plane  = (int64_t)panels * m.mp * 64;
                 const bool    odd    = t.step & 1;
-                const float* const x_from = odd ? m.x[1] : m.x[0];
-                float* const       x_to   = odd ? m.x[0] : m.x[1];
                 __half* const to = p.work + (int64_t)(KIND == kGram ? m.gram : KIND == kSquare ? m.factor : odd ? m.operand[0] : m.operand[1]) * kUnit;
                 const __half* const a_from = p.work + (int64_t)m.gram * kUnit;
                 auto load_x = [&](int c, float4 (&x)[8]) {  // 32 columns of X
                     if (col0 + c >= limit) return;
-                    const float4* const from = reinterpret_cast<const float4*>(x_from + at0 + (int64_t)(c / 32) * m.mp * 32);
+                    const float4* const from = reinterpret_cast<const float4*>(m.x + at0 + (int64_t)(c / 32) * m.mp * 32);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) x[j] = __ldcg(from + j * 32);
                 };
-                constexpr int kBuffers = KIND == kApply && !kSegments ? 2 : 1;
+                constexpr int kBuffers = kApplies && !kSegments ? 2 : 1;
                 float4 x_of[kBuffers][8];
-                X      was[KIND == kLast && !kSegments ? 32 : 1];
+                Grain<X>   was[32 / Grain<X>::kLines];
+                const bool grains = KIND == kLast && by_grains<X>(m), early = grains && m.momentum;
                 auto finish = [&](float* v, int c, const float4 (&x)[8]) {  // 32 columns
                     const int col = col0 + c;
                     if (col >= limit) return;
@@ -688,11 +752,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_chain(const __grid_constan
                         if constexpr (kSegments) load_x(c + 32 < half_wide ? c + 32 : p.wide, x_of[0]);  // the next, meanwhile
                     }
                     if constexpr (KIND == kLast) {
-                        update<!kSegments>(m, p.rates, v, row, col, turn, lane, was);
+                        update<X>(m, p.rates, v, Lines(m, row - lane, col), grains, turn, lane, was);
+                        if (early && c + 32 < half_wide && col + 32 < limit) load_parameters<X>(m, Lines(m, row - lane, col + 32), lane, was);
                         return;
                     }
                     if constexpr (KIND == kApply) {
-                        float4* const x_at = reinterpret_cast<float4*>(x_to + at0 + (int64_t)(c / 32) * m.mp * 32);
+                        float4* const x_at = reinterpret_cast<float4*>(m.x + at0 + (int64_t)(c / 32) * m.mp * 32);
 #pragma unroll
                         for (int j = 0; j < 8; ++j) x_at[j * 32] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
                     } else if (row / 128 > col / 128) {
@@ -734,17 +799,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_chain(const __grid_constan
                             v[2 * j] = two.x, v[2 * j + 1] = two.y;
                         }
                         store_sector(to + q * plane + at, w), store_sector(to + q * plane + at + 16, w + 8);
-                        if (mirror) {
-                            __half* const under = to + q * plane + in_units(panels, col, row);
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                const __half2 h = reinterpret_cast<const __half2&>(w[j]);
-                                under[(2 * j) * 64] = h.x, under[(2 * j + 1) * 64] = h.y;
-                            }
-                        }
+                        if (mirror) store_turned(to + q * plane + in_units(panels, col + lane, row - lane), w, turn, lane);
                     }
                 };
-                if constexpr (kBuffers == 2) load_x(0, x_of[0]);  // ahead of the sums
+                if constexpr (kApplies && !kSegments) load_x(0, x_of[0]);  // ahead of the sums
+                if (KIND == kLast && early && col0 < limit) load_parameters<X>(m, Lines(m, row - lane, col0), lane, was);
                 [[maybe_unused]] float total[kSegments ? kMostWide / 2 : 1];
                 if constexpr (kSegments) {
 #pragma unroll
@@ -758,7 +817,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_chain(const __grid_constan
                     auto columns = [&](int c, auto buffer) {
                         constexpr int kBuffer = decltype(buffer)::value;
                         float2 pairs[16];
-                        if constexpr (KIND == kLast && !kSegments) load_x(c, x_of[0]), load_parameters(m, row, col0 + c, lane, was);
                         tmem_load32(acc_at + c, pairs);
                         tmem_loaded(pairs);
                         if constexpr (kBuffers == 2)
@@ -908,7 +966,7 @@ Chain chain_of(const Matrix* matrices, int64_t count, int parts, int steps, void
         e.partial = w.take<double>(e.chunks);
         e.shift   = w.take<float>(steps);
         const int64_t values = (int64_t)e.panels * e.mp * 64;
-        for (int j = 0; j < 2; ++j) e.x[j] = w.take<float>(values);
+        e.x = w.take<float>(values);
         auto units = [&](int* at, int64_t halves) {
             w.used = (size_t)up((int64_t)w.used, kUnit * 2);
             *at = (int)(w.used / (kUnit * 2));
@@ -928,7 +986,7 @@ int64_t together(const Matrix* matrices, int64_t count, int parts) {
     int64_t i = 0;
     for (; i < count && i < kMostMatrices; ++i) {
         const int64_t m = std::min(matrices[i].rows, matrices[i].cols), n = std::max(matrices[i].rows, matrices[i].cols);
-        const size_t more = (size_t)up(m, 256) * ((size_t)up(n, 128) * (8 + 4 * parts) + (size_t)up(m, 256) * 4 * parts);
+        const size_t more = (size_t)up(m, 256) * ((size_t)up(n, 128) * (4 + 4 * parts) + (size_t)up(m, 256) * 4 * parts);
         if (i > 0 && bytes + more > kChainBytes) break;
         bytes += more;
     }
