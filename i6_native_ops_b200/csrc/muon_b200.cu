@@ -34,7 +34,7 @@ namespace {
 using namespace framewise_host;
 using namespace tensor_core;
 
-constexpr int kMostMatrices = 96;    // of a chain
+constexpr int kMostMatrices = 256;   // of a chain of launches
 constexpr int kSlots        = 24;    // matrices in a launch's arguments
 constexpr int kChunk        = 16384; // values per CTA of the pass over gradients
 constexpr int kRowsPerCta   = 128;   // of a tile: the lanes of tensor memory
@@ -49,7 +49,8 @@ constexpr int kSegment      = 2;     // f32: steps of 64 of K after which an acc
 constexpr int kMostStages   = 12;
 constexpr int kEpilogue     = 8;     // warps that finish tiles
 constexpr int kThreads      = 64 + 32 * kEpilogue;
-constexpr int kShared       = 232448 - 1152;  // dynamic; the rest: the static arrays
+constexpr int kShared       = 232448 - 2048;  // dynamic; the rest: the static arrays
+constexpr uint64_t kPatience = 4000000000ull;  // nanoseconds after which a wait gives up; they end within microseconds
 
 // A matrix of a chain.  Operands lie in units of 128 rows by 64 columns of fp16, 16 KB, a row of units after the other: one
 // tensor copy brings 128 rows of 64 columns, or 64 rows of 128.  (With panels of 64 columns, and copies of 64 by 64, the thread that
@@ -62,13 +63,12 @@ struct Entry {
     float*      master;     // or null
     double*     partial;    // sums of squares of the chunks
     float*      shift;      // per step: the multiple of the identity that B does without
-    float*      x;          // X
+    float*      x[2];       // X, before and after a step
     int         operand[2]; // its fp16 parts, as units of the workspace
     int         gram, factor; // A and B, likewise
     int         rows, cols; // of the parameter
     int         m, n, mp, panels;  // m <= n; rows (a multiple of 128) and units of a row of X
-    int         chunks, first_chunk, first_block, first_sym, first_apply;  // where its work begins
-    int         sym, apply;   // its tiles
+    int         chunks, first_chunk, first_block, first_sym, first_apply;  // where its work begins in each launch
     float       rate;
 };
 
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(256) k_muon_begin(const Entry* __restrict__ ta
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // a warp: 32 rows of four columns, 512 bytes of X
         const int row = (threadIdx.x / 32 & 1) * 32 + threadIdx.x % 32, col = (threadIdx.x / 64 + i * 4) * 4;
-        *reinterpret_cast<float4*>(m.x + place(m.mp, row0 + row, panel * 64 + col)) = make_float4(x_of(row, col), x_of(row, col + 1), x_of(row, col + 2), x_of(row, col + 3));
+        *reinterpret_cast<float4*>(m.x[0] + place(m.mp, row0 + row, panel * 64 + col)) = make_float4(x_of(row, col), x_of(row, col + 1), x_of(row, col + 2), x_of(row, col + 3));
     }
     __half* const op = work + (int64_t)m.operand[0] * kUnit + in_units(m.panels, row0, panel * 64);
     const int64_t plane = (int64_t)m.panels * m.mp * 64;
@@ -306,22 +306,15 @@ enum Kind { kGram = 0, kSquare = 1, kApply = 2, kLast = 3 };
 
 struct Params {
     const Entry* table;
-    int*     done;        // per matrix: warps that have finished a tile of it
-    int*     failed;      // a wait ran out
-    __half*  work;
-    int      count, steps, wide, stages;
-    int      span;        // columns of the second operand that a copy brings
-    int      sym, apply;  // tiles of a symmetric product and of a X + B X
-    uint64_t patience;    // nanoseconds after which a wait gives up
-    Rates    rates;
-};
-
-// A step's factors: of the finished sums of the three products, of A in B, of t in B, of X beside t, and of the next operands.
-struct Factors {
-    float gram, square, of_gram, of_one, apply, a, operand;
-};
-struct AllFactors {
-    Factors step[kMostSteps];
+    int     count, tiles, wide, stages;
+    int     span;        // columns of the second operand that a copy brings
+    int     from, step;  // from: which X it starts from
+    __half* work;
+    int*    failed;      // a wait ran out
+    float   product;     // factor of the finished sums
+    float   old;         // kSquare: of A; kApply: a
+    float   scale;       // kSquare: of B; kApply: of the operands
+    Rates   rates;       // kLast
 };
 
 // fp16 operands, f32 sums
@@ -329,31 +322,19 @@ __host__ __device__ constexpr uint32_t half_kind(int m, int n, bool b_mn) {
     return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+__device__ __forceinline__ void load_sector(const __half* x, uint32_t* w) {
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(x)
+                 : "memory");
+}
 __device__ __forceinline__ void store_sector(__half* x, const uint32_t* w) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(x), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]),
                  "r"(w[7])
                  : "memory");
 }
 
-constexpr int kTurn = 32 * 32 * 4;  // shared memory of a warp that finishes tiles: to turn 32 x 32 values
-
-// 32 rows, one a lane, of 32 fp16 numbers, to memory the other way round: `to` is where this lane's column goes, 64 bytes.
-__device__ __forceinline__ void store_turned(__half* to, const uint32_t (&w)[16], char* turn, int lane) {
-    uint32_t* const t = reinterpret_cast<uint32_t*>(turn);  // 16 words of two rows for each column
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {  // even lanes take column 2 j of their row and the next, odd ones column 2 j + 1 of theirs and the one before
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, w[j], 1);
-        const int col = 2 * j + (lane & 1);
-        t[col * 16 + ((lane / 8 ^ (col / 2 & 3)) * 4 + lane / 2 % 4)] = lane & 1 ? __byte_perm(other, w[j], 0x7632) : __byte_perm(w[j], other, 0x5410);
-    }
-    __syncwarp();
-    uint32_t o[16];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(o + 4 * j) = *reinterpret_cast<const uint4*>(t + lane * 16 + (j ^ (lane / 2 & 3)) * 4);
-    store_sector(to, o), store_sector(to + 16, o + 8);
-    __syncwarp();
-}
+constexpr int kTurn = 32 * 32 * 4;  // shared memory of a warp that updates parameters: to turn 32 x 32 values
 
 // Parameters of 32 x 32 values of X, by lines of the parameter: line 0 of them, how many there are, and how many values of each.
 struct Lines {
@@ -401,22 +382,22 @@ __device__ __forceinline__ float updated(float old, float held, bool copied, flo
     return old * r.decay - rate * x;
 }
 
-template <typename X>
-__device__ __forceinline__ void load_parameters(const Entry& m, const Lines& at, int lane, Grain<X> (&was)[32 / Grain<X>::kLines]) {
+// FIRST to LAST: of the lane's grains
+template <typename X, int FIRST, int LAST, int N>
+__device__ __forceinline__ void load_parameters(const Entry& m, const Lines& at, int lane, Grain<X> (&was)[N]) {
     using G = Grain<X>;
-    const X* p = static_cast<const X*>(m.param) + at.first + (int64_t)(lane / G::kLanes) * m.cols + lane % G::kLanes * G::kValues;
+    const X* p = static_cast<const X*>(m.param) + at.first + (int64_t)(FIRST * G::kLines + lane / G::kLanes) * m.cols + lane % G::kLanes * G::kValues;
 #pragma unroll
-    for (int i = 0; i < 32 / G::kLines; ++i, p += (int64_t)G::kLines * m.cols)
-        if (i * G::kLines + lane / G::kLanes < at.count && lane % G::kLanes * G::kValues < at.width) was[i].w = *reinterpret_cast<const uint4*>(p);
+    for (int i = FIRST; i < LAST; ++i, p += (int64_t)G::kLines * m.cols)
+        if (i * G::kLines + lane / G::kLanes < at.count && lane % G::kLanes * G::kValues < at.width) was[i - FIRST].w = *reinterpret_cast<const uint4*>(p);
 }
 
 // p = p decay - rate X, or the result X itself, for 32 x 32 values of X, a row a lane.  They go through shared memory, so that
 // neighbouring lanes have neighbouring values in memory whichever way the parameter lies: 16 bytes a lane, where lines of the
-// parameter begin at multiples of that (`was`: loaded before), else a value a lane.  (A value a lane throughout: 27 to 32 us for a
-// tile of 128 x 256 bf16, GRAINS this way.)
-template <typename X>
-__device__ __forceinline__ void update(const Entry& m, const Rates& r, const float* v, const Lines& at, bool grains, char* turn, int lane,
-                                       const Grain<X> (&was)[32 / Grain<X>::kLines]) {
+// parameter begin at multiples of that (EARLY: `was` has been loaded before), else a value a lane.  (A value a lane throughout:
+// 71 us for the last product of 16 x 512 x 2048 bf16, 54 this way.)
+template <typename X, bool EARLY, int N>
+__device__ __forceinline__ void update(const Entry& m, const Rates& r, const float* v, const Lines& at, bool grains, char* turn, int lane, Grain<X> (&was)[N]) {
     using G = Grain<X>;
     const bool tall = m.rows > m.cols;
     float* const t = reinterpret_cast<float*>(turn);
@@ -430,33 +411,45 @@ __device__ __forceinline__ void update(const Entry& m, const Rates& r, const flo
     }
     __syncwarp();
     X* const p = static_cast<X*>(m.param) + at.first;
-    if (grains) {
-        const int l0 = lane / G::kLanes, c0 = lane % G::kLanes * G::kValues;
+    const int l0 = lane / G::kLanes, c0 = lane % G::kLanes * G::kValues;
+    auto store_grain = [&](int i, const G& old) {
+        const int line = i * G::kLines + l0;
+        if (line >= at.count || c0 >= at.width) return;
+        float x[G::kValues];
 #pragma unroll
-        for (int i = 0; i < 32 / G::kLines; ++i) {
-            const int line = i * G::kLines + l0;
-            if (line >= at.count || c0 >= at.width) continue;
-            float x[G::kValues];
+        for (int j = 0; j < G::kValues; j += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(t + line * 32 + (c0 + j ^ (line & 7) << 2));
+            x[j] = f.x, x[j + 1] = f.y, x[j + 2] = f.z, x[j + 3] = f.w;
+        }
+        const int64_t to = (int64_t)line * m.cols + c0;
+        if (m.momentum) {
+            float* const copy = m.master ? m.master + at.first + to : nullptr;
 #pragma unroll
             for (int j = 0; j < G::kValues; j += 4) {
-                const float4 f = *reinterpret_cast<const float4*>(t + line * 32 + (c0 + j ^ (line & 7) << 2));
-                x[j] = f.x, x[j + 1] = f.y, x[j + 2] = f.z, x[j + 3] = f.w;
-            }
-            const int64_t to = (int64_t)line * m.cols + c0;
-            if (m.momentum) {
-                float* const copy = m.master ? m.master + at.first + to : nullptr;
+                float4 held = copy ? *reinterpret_cast<const float4*>(copy + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+                float* const h = reinterpret_cast<float*>(&held);
 #pragma unroll
-                for (int j = 0; j < G::kValues; j += 4) {
-                    float4 held = copy ? *reinterpret_cast<const float4*>(copy + j) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    float* const h = reinterpret_cast<float*>(&held);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) h[k] = x[j + k] = updated<X>(was[i].get(j + k), h[k], copy != nullptr, x[j + k], r, m.rate);
-                    if (copy) *reinterpret_cast<float4*>(copy + j) = held;
-                }
+                for (int k = 0; k < 4; ++k) h[k] = x[j + k] = updated<X>(old.get(j + k), h[k], copy != nullptr, x[j + k], r, m.rate);
+                if (copy) *reinterpret_cast<float4*>(copy + j) = held;
             }
-            G now;
-            now.set(x);
-            *reinterpret_cast<uint4*>(p + to) = now.w;
+        }
+        G now;
+        now.set(x);
+        *reinterpret_cast<uint4*>(p + to) = now.w;
+    };
+    if (grains) {
+        constexpr int kAll = 32 / G::kLines;
+        if constexpr (EARLY) {
+#pragma unroll
+            for (int i = 0; i < kAll; ++i) store_grain(i, was[i]);
+        } else {
+#pragma unroll
+            for (int i0 = 0; i0 < kAll; i0 += N) {
+                if (m.momentum) i0 == 0 ? load_parameters<X, 0, N>(m, at, lane, was) : load_parameters<X, N, 2 * N>(m, at, lane, was);
+                static_assert(EARLY || kAll == 2 * N, "");
+#pragma unroll
+                for (int i = 0; i < N; ++i) store_grain(i0 + i, was[i]);
+            }
         }
     } else if (lane < at.width) {
 #pragma unroll 4
@@ -475,41 +468,31 @@ __device__ __forceinline__ void update(const Entry& m, const Rates& r, const flo
     __syncwarp();
 }
 
+// After a wait ran out the results are NaN.
 template <typename X>
-__device__ __noinline__ void no_result(const Entry& m, int row, int col, int lane) {
-    const Lines at(m, row - lane, col);
-    for (int j = 0; j < at.count && lane < at.width; ++j) {
-        const int64_t to = at.first + (int64_t)j * m.cols + lane;
-        put(static_cast<X*>(m.param) + to, __uint_as_float(0x7fffffffu));
-        if (m.master) m.master[to] = __uint_as_float(0x7fffffffu);
+__global__ void __launch_bounds__(256) k_muon_check(const Entry* __restrict__ table, int count, const int* failed) {
+    former_is_done();
+    if (*failed == 0) return;
+    for (int e = 0; e < count; ++e) {
+        const Entry& m = table[e];
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)m.rows * m.cols; i += (int64_t)gridDim.x * 256) {
+            put(static_cast<X*>(m.param) + i, __uint_as_float(0x7fffffffu));
+            if (m.master) m.master[i] = __uint_as_float(0x7fffffffu);
+        }
     }
 }
 
-__device__ __forceinline__ int load_acquire(const int* p) {
-    int v;
-    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-    return v;
-}
-__device__ __forceinline__ void add_release(int* p, int v) { asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory"); }
-// what was written by stores is seen by copies, and the other way round
-__device__ __forceinline__ void copies_and_stores() { asm volatile("fence.proxy.async.global;" ::: "memory"); }
-
-// All products of a chain, in one launch of CTAs that stay: tiles of 128 rows (CG 2: of 256 on a pair of CTAs, each with 128 of
-// them and half of the second operand) by up to 256 columns, in the order steps, products, matrices, dealt out in turn.
-//   kGram    A = X X^T       of both the tiles on and above the diagonal; what lies above it is written to both places
-//   kSquare  b A + c A A - t
-//   kApply   (a + t) X + B X; kLast: likewise, and the parameters' update
-// A tile waits for all tiles of its matrix's product before (`done` counts them), which are dealt out before it, so that the
-// waits end; no product waits for the other matrices, and none of them ends with idle SMs but the last.
-// One warp asks for copies, one for products, eight finish tiles, a row a lane.
-template <int PARTS, int CG>
-__global__ void __launch_bounds__(kThreads, 1) k_muon_chain(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_columns,
-                                                            const __grid_constant__ CUtensorMap map_two, const Params p, const __grid_constant__ AllFactors factors) {
-    using X = std::conditional_t<PARTS == 2, float, __nv_bfloat16>;
+// Tiles of 128 rows by up to 256 columns.  kGram: A = X X^T; kSquare: b A + c A A; of both the tiles on and above the diagonal,
+// what lies above it is written to both places.  kApply: a X + B X.  kLast: likewise, and the parameters' update.
+// CG: CTAs per tile (2: of 256 rows, each CTA with 128 of them and half of the second operand).
+template <int KIND, int PARTS, int CG>
+__global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
+    constexpr bool kApplies = KIND == kApply || KIND == kLast;
+    constexpr bool kBMn = kApplies;             // the second operand's rows lie along K
     constexpr bool kSegments = PARTS == 2;
     constexpr int  kTile = kRowsPerCta * CG;
     extern __shared__ char shared_raw[];
-    __shared__ int first_sym[kMostMatrices], first_apply[kMostMatrices];
+    __shared__ int firsts[kMostMatrices];
     __shared__ uint64_t bars_at[2 * kMostStages + 2 * kMostAccs + 1];
     __shared__ uint32_t slot_at;
     __shared__ volatile int give_up;
@@ -517,112 +500,103 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_chain(const __grid_constan
                    drained = freed + 8 * kMostAccs;
     const int rank = CG == 2 ? (int)cluster_rank() : 0, worker = blockIdx.x / CG, workers = gridDim.x / CG, accs = min(kMostAccs, kColumns / p.wide);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t base = (smem_addr(shared_raw) + kEpilogue * kTurn + 1023u) & ~1023u;
+    constexpr int kTurns = KIND == kLast ? kEpilogue * kTurn : 0;
+    const uint32_t base = (smem_addr(shared_raw) + kTurns + 1023u) & ~1023u;
     const int part_b = p.wide / CG * kDepth * 2, part_a = kRowsPerCta * kDepth * 2, stage_bytes = part_a + part_b;
 
-    for (int i = threadIdx.x; i < p.count; i += kThreads) first_sym[i] = p.table[i].first_sym, first_apply[i] = p.table[i].first_apply;
+    next_may_start();
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) bar_init(full + 8 * s, 1), bar_init(empty + 8 * s, 1);
         for (int i = 0; i < accs; ++i) bar_init(done + 8 * i, 1), bar_init(freed + 8 * i, kEpilogue * CG);
         bar_init(drained, 1);
         give_up = 0;
         bar_init_fence();
-        prefetch_map(&map_rows), prefetch_map(&map_columns), prefetch_map(&map_two);
+        prefetch_map(&map_a);
+        prefetch_map(&map_b);
     }
     if (warp == 1) tmem_alloc<CG>(smem_addr(&slot_at), kColumns);
+    former_is_done();
+    for (int i = threadIdx.x; i < p.count; i += kThreads) firsts[i] = kApplies ? p.table[i].first_apply : p.table[i].first_sym;
     fence_before();
     __syncthreads();
     if (CG == 2) cluster_sync();
     fence_after();
     const uint32_t tmem = *const_cast<volatile uint32_t*>(&slot_at);
 
-    // waits with a limit; `heed`: they also end when another of this CTA's has given up
-    auto within = [&](auto&& ready, bool heed) -> bool {
+    auto bounded = [&](uint32_t bar, uint32_t parity, bool heed) -> bool {
         uint64_t since = 0;
         for (int i = 1;; ++i) {
-            if (ready()) return true;
+            if (bar_try(bar, parity)) return true;
             if (i % 64) continue;
             uint64_t now;
             asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
             if (since == 0) since = now;
-            if (now - since > p.patience || (heed && give_up)) return false;
+            if (now - since > kPatience || (heed && give_up)) return false;
         }
     };
-    auto failed = [&]() {
+    auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+        if (bounded(bar, parity, true)) return true;
         give_up = 1;
         atomicExch(p.failed, 1);
-        __threadfence();
         return false;
     };
-    auto wait = [&](uint32_t bar, uint32_t parity) -> bool { return within([&] { return bar_try(bar, parity); }, true) || failed(); };
 
+    // Tile u: its matrix, and the first row and column.  Symmetric results: rows of tiles from the diagonal on.
     struct Tile {
-        int step, kind, e, row, col, depth, need;
+        int e, row, col, depth;
     };
-    const int per_step = 2 * p.sym + p.apply, tiles = per_step * p.steps;
     auto tile_at = [&](int u) -> Tile {
         Tile t;
-        t.step = u / per_step;
-        int at = u - t.step * per_step;
-        t.kind = at < p.sym ? kGram : at < 2 * p.sym ? kSquare : t.step + 1 < p.steps ? kApply : kLast;
-        const bool sym = t.kind <= kSquare;
-        if (t.kind == kSquare) at -= p.sym;
-        if (!sym) at -= 2 * p.sym;
-        const int* const firsts = sym ? first_sym : first_apply;
-        t.e = find(p.count, at, [&](int i) { return firsts[i]; });
-        at -= firsts[t.e];
+        t.e = find(p.count, u, [&](int i) { return firsts[i]; });
         const Entry& m = p.table[t.e];
-        if (sym) {  // rows of tiles from the diagonal on
+        int at = u - firsts[t.e];
+        if (kApplies) {
+            // a column after the other: its part of X is met by all rows at once, B stays near
+            const int mt = m.mp / kTile;
+            t.row = at % mt * kTile, t.col = at / mt * p.wide;
+        } else {
             const int nt = (m.mp + p.wide - 1) / p.wide;
             int row = 0;
             for (;; ++row) {
-                const int first = row * kTile / p.wide, some = nt - first;
-                if (at < some) {
+                const int first = row * kTile / p.wide, tiles = nt - first;
+                if (at < tiles) {
                     t.col = (first + at) * p.wide;
                     break;
                 }
-                at -= some;
+                at -= tiles;
             }
             t.row = row * kTile;
-        } else {  // a column after the other: its part of X is met by all rows at once, B stays near
-            const int mt = m.mp / kTile;
-            t.row = at % mt * kTile, t.col = at / mt * p.wide;
         }
-        t.depth = t.kind == kGram ? m.panels : (m.m + 63) / 64;
-        t.need  = (t.step * (2 * m.sym + m.apply) + (t.kind == kGram ? 0 : t.kind == kSquare ? m.sym : 2 * m.sym)) * CG * kEpilogue;
+        t.depth = KIND == kGram ? m.panels : (m.m + 63) / 64;
         return t;
     };
-    auto ready = [&](const Tile& t) -> bool { return t.need == 0 || within([&] { return load_acquire(p.done + t.e) >= t.need; }, true) || failed(); };
-    auto width_of = [&](const Tile& t, const Entry& m) { return min(p.wide, (t.kind >= kApply ? m.panels * 64 : m.mp) - t.col); };
 
     if (warp == 0 && lane == 0) {  // ---- copies
         int      stage = 0, issued = 0;
         uint32_t phase = 0;
         bool     ok = true;
-        for (int u = worker; u < tiles && ok; u += workers) {
+        for (int u = worker; u < p.tiles && ok; u += workers) {
             const Tile t = tile_at(u);
-            const Entry& m = p.table[t.e];
+            const Entry m = p.table[t.e];
             // units: where the operands begin, and those of their second parts
-            const bool gram = t.kind == kGram, square = t.kind == kSquare, applies = t.kind >= kApply;
-            const int x0 = t.step & 1 ? m.operand[1] : m.operand[0], x_part = m.mp / 128 * m.panels, s_row = m.mp / 64, s_part = m.mp / 128 * s_row;
-            const int a_part = gram ? x_part : s_part, b_part = square ? s_part : x_part, b_row = square ? s_row : m.panels;
-            const int a_first = (gram ? x0 : square ? m.gram : m.factor) + (t.row / 128 + rank) * (gram ? m.panels : s_row), b0 = square ? m.gram : x0;
-            const int have = width_of(t, m) / CG, from = t.col + rank * have;  // columns of the tile that are this CTA's
+            const int x0 = p.from ? m.operand[1] : m.operand[0], x_part = m.mp / 128 * m.panels, s_row = m.mp / 64, s_part = m.mp / 128 * s_row;
+            const int a0 = KIND == kGram ? x0 : KIND == kSquare ? m.gram : m.factor, b0 = KIND == kSquare ? m.gram : x0;
+            const int a_part = KIND == kGram ? x_part : s_part, b_part = KIND == kSquare ? s_part : x_part, b_row = KIND == kSquare ? s_row : m.panels;
+            const int a_first = a0 + (t.row / 128 + rank) * (KIND == kGram ? m.panels : s_row);
+            // columns of the tile that there are and are this CTA's
+            const int limit = kApplies ? m.panels * 64 : m.mp, have = min(p.wide, limit - t.col) / CG, from = t.col + rank * have;
             const int copies = (have + p.span - 1) / p.span, span_bytes = p.span * kDepth * 2;
-            const CUtensorMap* const map_b = applies ? &map_two : &map_columns;
-            ok = ready(t);
-            copies_and_stores();
             for (int k = 0; k < t.depth && ok; ++k) {
                 for (int q = PARTS - 1; q >= 0; --q) {  // the small part is met, and its stage free again, first
                     ok = wait(empty + 8 * stage, phase ^ 1);
                     if (!ok) break;
                     const uint32_t a = base + stage * stage_bytes, b = a + part_a, bar = CG == 2 ? in_cta(full + 8 * stage, 0) : full + 8 * stage;
                     if (rank == 0) bar_expect(full + 8 * stage, CG * (part_a + copies * span_bytes));
-                    load_box<CG>(a, &map_rows, bar, 0, 0, a_first + q * a_part + k);
+                    load_box<CG>(a, &map_a, bar, 0, 0, a_first + q * a_part + k);
                     for (int j = 0; j < copies; ++j) {
                         const int col = from + j * p.span;
-                        const int y = applies ? k % 2 * 64 : col % 128, z = b0 + q * b_part + (applies ? k / 2 * b_row + col / 64 : col / 128 * b_row + k);
-                        load_box<CG>(b + j * span_bytes, map_b, bar, 0, y, z);
+                        if (kBMn) load_box<CG>(b + j * span_bytes, &map_b, bar, 0, k % 2 * 64, b0 + q * b_part + k / 2 * b_row + col / 64);
+                        else load_box<CG>(b + j * span_bytes, &map_b, bar, 0, col % 128, b0 + q * b_part + col / 128 * b_row + k);
                     }
                     ++issued;
                     if (++stage == p.stages) stage = 0, phase ^= 1;
@@ -637,17 +611,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_chain(const __grid_constan
         if (give_up && rank == 0) {
             for (int i = 0; i < p.stages && i < issued; ++i) {
                 if (--stage < 0) stage = p.stages - 1, phase ^= 1;
-                within([&] { return bar_try(full + 8 * stage, phase); }, false);
+                bounded(full + 8 * stage, phase, false);
             }
         }
     } else if (warp == 1 && lane == 0 && rank == 0) {  // ---- products
         int      stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool     ok = true;
-        for (int u = worker; u < tiles && ok; u += workers) {
+        for (int u = worker; u < p.tiles && ok; u += workers) {
             const Tile t = tile_at(u);
-            const bool     b_mn = t.kind >= kApply;  // the second operand's rows lie along K
-            const uint32_t kind = half_kind(kTile, width_of(t, p.table[t.e]), b_mn), b_step = b_mn ? 2048 : 32;
+            const Entry m = p.table[t.e];
+            const int limit = kApplies ? m.panels * 64 : m.mp;
+            const uint32_t kind = half_kind(kTile, min(p.wide, limit - t.col), kBMn);
             for (int k0 = 0; k0 < t.depth && ok; k0 += kSegments ? kSegment : t.depth) {
                 ok = wait(freed + 8 * acc, acc_phase ^ 1);
                 if (!ok) break;
@@ -659,7 +634,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_chain(const __grid_constan
                 auto multiply = [&](int stage_a, int stage_b, bool add) {
                     const uint32_t a = base + stage_a * stage_bytes, b = base + stage_b * stage_bytes + part_a;
 #pragma unroll
-                    for (int i = 0; i < kDepth / 16; ++i) product<CG>(d, operand(a + i * 32, 8192), operand(b + i * b_step, 8192), kind, add || i > 0);
+                    for (int i = 0; i < kDepth / 16; ++i)
+                        product<CG>(d, operand(a + i * 32, 8192), operand(b + i * (kBMn ? 2048 : 32), 8192), kind, add || i > 0);
                 };
                 auto arrived = [&](int at, uint32_t at_phase) {
                     ok = ok && wait(full + 8 * at, at_phase);
@@ -703,182 +679,164 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_chain(const __grid_constan
         }
         if (!ok) {  // products under way still read shared memory
             products_commit<CG>(drained);
-            within([&] { return bar_try(drained, 0); }, false);
+            bounded(drained, 0, false);
         }
     } else if (warp >= 2) {  // ---- finished tiles: a row a lane
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         const int half_wide = p.wide / 2;
         const uint32_t freed0 = CG == 2 ? in_cta(freed, 0) : freed;
-        char* const turn = shared_raw + (warp - 2) * kTurn;
         int      acc = 0;
         uint32_t acc_phase = 0;
         bool     ok = true;
-        for (int u = worker; u < tiles; u += workers) {
+        for (int u = worker; u < p.tiles && ok; u += workers) {
             const Tile t = tile_at(u);
-            const Entry& m = p.table[t.e];
+            const Entry m = p.table[t.e];
             const int row = t.row + rank * kRowsPerCta + quarter * 32 + lane, col0 = t.col + half * half_wide;
-            const int limit = t.col + width_of(t, m);
-            if (ok && t.kind != kGram) ok = __all_sync(0xffffffffu, ready(t));  // X and A are read here as well
-            auto tile = [&](auto kind_of) {
-                constexpr int  KIND = decltype(kind_of)::value;
-                constexpr bool kApplies = KIND >= kApply;
-                const Factors& f = factors.step[t.step];
-                const float shift = KIND == kGram ? 0.f : m.shift[t.step], old = kApplies ? f.a + shift : f.of_gram;
-                const int64_t at0 = kApplies ? place(m.mp, row, col0) : 0;
-                const int     panels = KIND == kApply ? m.panels : m.mp / 64;
-                const int64_t plane  = (int64_t)panels * m.mp * 64;
-                const bool    odd    = t.step & 1;
-                __half* const to = p.work + (int64_t)(KIND == kGram ? m.gram : KIND == kSquare ? m.factor : odd ? m.operand[0] : m.operand[1]) * kUnit;
-                const __half* const a_from = p.work + (int64_t)m.gram * kUnit;
-                auto load_x = [&](int c, float4 (&x)[8]) {  // 32 columns of X
-                    if (col0 + c >= limit) return;
-                    const float4* const from = reinterpret_cast<const float4*>(m.x + at0 + (int64_t)(c / 32) * m.mp * 32);
+            const int limit = kApplies ? m.panels * 64 : m.mp;
+            const int64_t s_plane = (int64_t)m.mp * m.mp, x_plane = (int64_t)m.panels * m.mp * 64;
+            const float shift = KIND == kGram ? 0.f : m.shift[p.step], old = kApplies ? p.old + shift : p.old;
+            const int64_t at0 = kApplies ? place(m.mp, row, col0) : 0;
+            const float* const x_from = p.from ? m.x[1] : m.x[0];
+            float* const       x_to   = p.from ? m.x[0] : m.x[1];
+            const int          target = KIND == kGram ? m.gram : KIND == kSquare ? m.factor : p.from ? m.operand[0] : m.operand[1];
+            using X = std::conditional_t<PARTS == 2, float, __nv_bfloat16>;
+            // (f32: the sums need the registers; half of the parameters at a time)
+            constexpr int kGrains = 32 / Grain<X>::kLines / (kSegments ? 2 : 1);
+            Grain<X> was[kGrains];
+            const bool grains = KIND == kLast && by_grains<X>(m), early = grains && m.momentum && !kSegments;
+            auto load_x = [&](int c, float4 (&x)[8]) {  // 32 columns of X
+                if (col0 + c >= limit) return;
+                const float4* const from = reinterpret_cast<const float4*>(x_from + at0 + (int64_t)(c / 32) * m.mp * 32);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] = __ldcg(from + j * 32);
-                };
-                constexpr int kBuffers = kApplies && !kSegments ? 2 : 1;
-                float4 x_of[kBuffers][8];
-                Grain<X>   was[32 / Grain<X>::kLines];
-                const bool grains = KIND == kLast && by_grains<X>(m), early = grains && m.momentum;
-                auto finish = [&](float* v, int c, const float4 (&x)[8]) {  // 32 columns
-                    const int col = col0 + c;
-                    if (col >= limit) return;
-                    if constexpr (kApplies) {
+                for (int j = 0; j < 8; ++j) x[j] = from[j * 32];
+            };
+            auto finish = [&](float* v, int c, const float4 (&x)[8]) {  // 32 columns
+                const int col = col0 + c;
+                if (col >= limit) return;
+                if (kApplies) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            v[4 * j] = fmaf(old, x[j].x, v[4 * j] * f.apply), v[4 * j + 1] = fmaf(old, x[j].y, v[4 * j + 1] * f.apply);
-                            v[4 * j + 2] = fmaf(old, x[j].z, v[4 * j + 2] * f.apply), v[4 * j + 3] = fmaf(old, x[j].w, v[4 * j + 3] * f.apply);
-                        }
-                        if constexpr (kSegments) load_x(c + 32 < half_wide ? c + 32 : p.wide, x_of[0]);  // the next, meanwhile
+                    for (int j = 0; j < 8; ++j) {
+                        v[4 * j] = fmaf(old, x[j].x, v[4 * j] * p.product), v[4 * j + 1] = fmaf(old, x[j].y, v[4 * j + 1] * p.product);
+                        v[4 * j + 2] = fmaf(old, x[j].z, v[4 * j + 2] * p.product), v[4 * j + 3] = fmaf(old, x[j].w, v[4 * j + 3] * p.product);
                     }
-                    if constexpr (KIND == kLast) {
-                        update<X>(m, p.rates, v, Lines(m, row - lane, col), grains, turn, lane, was);
-                        if (early && c + 32 < half_wide && col + 32 < limit) load_parameters<X>(m, Lines(m, row - lane, col + 32), lane, was);
-                        return;
-                    }
-                    if constexpr (KIND == kApply) {
-                        float4* const x_at = reinterpret_cast<float4*>(m.x + at0 + (int64_t)(c / 32) * m.mp * 32);
+                }
+                if constexpr (KIND == kLast) {
+                    update<X, !kSegments>(m, p.rates, v, Lines(m, row - lane, col), grains, shared_raw + (warp - 2) * kTurn, lane, was);
+                    if (early && c + 32 < half_wide && col + 32 < limit) load_parameters<X, 0, kGrains>(m, Lines(m, row - lane, col + 32), lane, was);
+                    return;
+                }
+                if (KIND == kApply) {
+                    float4* const to = reinterpret_cast<float4*>(x_to + at0 + (int64_t)(c / 32) * m.mp * 32);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) x_at[j * 32] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-                    } else if (row / 128 > col / 128) {
-                        return;  // below the diagonal
-                    }
-                    const int64_t at = in_units(panels, row, col);
-                    if constexpr (KIND == kSquare) {
+                    for (int j = 0; j < 8; ++j) to[j * 32] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                } else if (row / 128 > col / 128) {
+                    return;  // below the diagonal
+                }
+                const int64_t at = in_units(kApplies ? m.panels : m.mp / 64, row, col);
+                __half* const to = p.work + (int64_t)target * kUnit;
+                const int64_t plane = KIND == kApply ? x_plane : s_plane;
+                if (KIND == kSquare) {
 #pragma unroll
-                        for (int q = PARTS - 1; q >= 0; --q) {
-                            uint4 w[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) w[j] = __ldcg(reinterpret_cast<const uint4*>(a_from + q * plane + at) + j);
-                            const uint32_t* const halves = reinterpret_cast<const uint32_t*>(w);
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                const float2 a = __half22float2(reinterpret_cast<const __half2&>(halves[j]));
-                                v[2 * j] = fmaf(old, a.x, q == PARTS - 1 ? v[2 * j] * f.square : v[2 * j]);
-                                v[2 * j + 1] = fmaf(old, a.y, q == PARTS - 1 ? v[2 * j + 1] * f.square : v[2 * j + 1]);
-                            }
-                        }
-                        const int hit = row - col;  // the diagonal's place among these columns
-                        if (hit >= 0 && hit < 32) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] -= j == hit ? shift * f.of_one : 0.f;
-                        }
-                        __syncwarp();
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] *= KIND == kApply ? f.operand : f.gram;
-                    }
-                    const bool mirror = KIND != kApply && col / 128 > row / 128;
-#pragma unroll
-                    for (int q = 0; q < PARTS; ++q) {
+                    for (int q = PARTS - 1; q >= 0; --q) {
                         uint32_t w[16];
+                        load_sector(p.work + (int64_t)m.gram * kUnit + q * plane + at, w), load_sector(p.work + (int64_t)m.gram * kUnit + q * plane + at + 16, w + 8);
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
-                            float2 two = make_float2(v[2 * j], v[2 * j + 1]);
-                            w[j] = part_of(two);
-                            v[2 * j] = two.x, v[2 * j + 1] = two.y;
+                            const float2 a = __half22float2(reinterpret_cast<const __half2&>(w[j]));
+                            v[2 * j] = fmaf(old, a.x, q == PARTS - 1 ? v[2 * j] * p.product : v[2 * j]);
+                            v[2 * j + 1] = fmaf(old, a.y, q == PARTS - 1 ? v[2 * j + 1] * p.product : v[2 * j + 1]);
                         }
-                        store_sector(to + q * plane + at, w), store_sector(to + q * plane + at + 16, w + 8);
-                        if (mirror) store_turned(to + q * plane + in_units(panels, col + lane, row - lane), w, turn, lane);
                     }
-                };
-                if constexpr (kApplies && !kSegments) load_x(0, x_of[0]);  // ahead of the sums
-                if (KIND == kLast && early && col0 < limit) load_parameters<X>(m, Lines(m, row - lane, col0), lane, was);
-                [[maybe_unused]] float total[kSegments ? kMostWide / 2 : 1];
-                if constexpr (kSegments) {
+                    const int hit = row - col;  // the diagonal's place among these columns
+                    if (hit >= 0 && hit < 32) {
 #pragma unroll
-                    for (int j = 0; j < kMostWide / 2; ++j) total[j] = 0.f;
+                        for (int j = 0; j < 32; ++j) v[j] -= j == hit ? shift * p.scale : 0.f;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] *= KIND == kApply ? p.scale : p.product;
                 }
-                for (int k0 = 0; k0 < t.depth; k0 += kSegments ? kSegment : t.depth) {
-                    ok = __all_sync(0xffffffffu, wait(done + 8 * acc, acc_phase));
-                    if (!ok) return;
-                    fence_after();
-                    const uint32_t acc_at = tmem + ((uint32_t)(quarter * 32) << 16) + acc * p.wide + half * half_wide;
-                    auto columns = [&](int c, auto buffer) {
-                        constexpr int kBuffer = decltype(buffer)::value;
-                        float2 pairs[16];
-                        tmem_load32(acc_at + c, pairs);
-                        tmem_loaded(pairs);
-                        if constexpr (kBuffers == 2)
-                            if (c + 32 < half_wide) load_x(c + 32, x_of[kBuffer ^ 1]);
-                        finish(reinterpret_cast<float*>(pairs), c, x_of[kBuffer]);
-                        __syncwarp();
-                    };
-                    if constexpr (kSegments) {
+                const bool mirror = KIND != kApply && col / 128 > row / 128;
 #pragma unroll
-                        for (int c = 0; c < kMostWide / 2; c += 32) {
-                            if (c >= half_wide || col0 + c >= limit) continue;
-                            float2 pairs[16];
-                            const float* const v = reinterpret_cast<const float*>(pairs);
-                            tmem_load32(acc_at + c, pairs);
-                            tmem_loaded(pairs);
+                for (int q = 0; q < PARTS; ++q) {
+                    uint32_t w[16];
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) total[c + j] += v[j];
+                    for (int j = 0; j < 16; ++j) {
+                        float2 two = make_float2(v[2 * j], v[2 * j + 1]);
+                        w[j] = part_of(two);
+                        v[2 * j] = two.x, v[2 * j + 1] = two.y;
+                    }
+                    store_sector(to + q * plane + at, w), store_sector(to + q * plane + at + 16, w + 8);
+                    if (mirror) {
+                        __half* const under = to + q * plane + in_units(m.mp / 64, col, row);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const __half2 h = reinterpret_cast<const __half2&>(w[j]);
+                            under[(2 * j) * 64] = h.x, under[(2 * j + 1) * 64] = h.y;
                         }
-                    } else if constexpr (kBuffers == 2) {
-                        for (int c = 0; c < half_wide && col0 + c < limit; c += 64) {
-                            columns(c, std::integral_constant<int, 0>());
-                            if (c + 32 < half_wide && col0 + c + 32 < limit) columns(c + 32, std::integral_constant<int, kBuffers - 1>());
-                        }
-                    } else {
-#pragma unroll 1
-                        for (int c = 0; c < half_wide && col0 + c < limit; c += 32) columns(c, std::integral_constant<int, 0>());
-                    }
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(freed0 + 8 * acc);
-                    if (++acc == accs) acc = 0, acc_phase ^= 1;
-                }
-                if constexpr (kSegments) {
-                    if (kApplies) load_x(0, x_of[0]);
-#pragma unroll
-                    for (int c = 0; c < kMostWide / 2; c += 32) {
-                        if (c >= half_wide) continue;
-                        finish(total + c, c, x_of[0]);
-                        __syncwarp();
-                    }
-                }
-                if (KIND != kLast) {  // the tile's part of this warp is there for all to see
-                    copies_and_stores();
-                    __syncwarp();
-                    if (lane == 0) {
-                        __threadfence();
-                        add_release(p.done + t.e, 1);
                     }
                 }
             };
-            // after a wait ran out, anywhere, the results are NaN
-            if (ok && t.kind == kLast && load_acquire(p.failed) != 0) ok = false;
-            ok = __all_sync(0xffffffffu, ok);
-            if (ok) {
-                if (t.kind == kGram) tile(std::integral_constant<int, kGram>());
-                else if (t.kind == kSquare) tile(std::integral_constant<int, kSquare>());
-                else if (t.kind == kApply) tile(std::integral_constant<int, kApply>());
-                else tile(std::integral_constant<int, kLast>());
+            constexpr int kBuffers = KIND == kApply && !kSegments ? 2 : 1;
+            float4 x_of[kBuffers][8];
+            if (KIND == kApply && !kSegments) load_x(0, x_of[0]);  // ahead of the sums
+            if (KIND == kLast && early && col0 < limit) load_parameters<X, 0, kGrains>(m, Lines(m, row - lane, col0), lane, was);
+            float total[kSegments ? kMostWide / 2 : 1];
+            if constexpr (kSegments) {
+#pragma unroll
+                for (int j = 0; j < kMostWide / 2; ++j) total[j] = 0.f;
             }
-            if (!ok && t.kind == kLast) {
-                give_up = 1;
-                for (int c = 0; c < half_wide && col0 + c < limit; c += 32) no_result<X>(m, row, col0 + c, lane);
+            for (int k0 = 0; k0 < t.depth; k0 += kSegments ? kSegment : t.depth) {
+                ok = __all_sync(0xffffffffu, wait(done + 8 * acc, acc_phase));
+                if (!ok) break;
+                fence_after();
+                const uint32_t acc_at = tmem + ((uint32_t)(quarter * 32) << 16) + acc * p.wide + half * half_wide;
+                auto columns = [&](int c, auto buffer) {
+                    constexpr int kBuffer = decltype(buffer)::value;
+                    float2 pairs[16];
+                    float* const v = reinterpret_cast<float*>(pairs);
+                    if constexpr (KIND == kLast && !kSegments) load_x(c, x_of[0]);
+                    tmem_load32(acc_at + c, pairs);
+                    tmem_loaded(pairs);
+                    if constexpr (kBuffers == 2)
+                        if (c + 32 < half_wide) load_x(c + 32, x_of[kBuffer ^ 1]);
+                    finish(v, c, x_of[kBuffer]);
+                    __syncwarp();
+                };
+                if constexpr (kSegments) {
+#pragma unroll
+                    for (int c = 0; c < kMostWide / 2; c += 32) {
+                        if (c >= half_wide || col0 + c >= limit) continue;
+                        float2 pairs[16];
+                        const float* const v = reinterpret_cast<const float*>(pairs);
+                        tmem_load32(acc_at + c, pairs);
+                        tmem_loaded(pairs);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) total[c + j] += v[j];
+                    }
+                } else if constexpr (kBuffers == 2) {
+                    for (int c = 0; c < half_wide && col0 + c < limit; c += 64) {
+                        columns(c, std::integral_constant<int, 0>());
+                        if (c + 32 < half_wide && col0 + c + 32 < limit) columns(c + 32, std::integral_constant<int, 1>());
+                    }
+                } else {
+#pragma unroll 1
+                    for (int c = 0; c < half_wide && col0 + c < limit; c += 32) columns(c, std::integral_constant<int, 0>());
+                }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(freed0 + 8 * acc);
+                if (++acc == accs) acc = 0, acc_phase ^= 1;
+            }
+            if (!ok) break;
+            if constexpr (kSegments) {
+#pragma unroll
+                for (int c = 0; c < kMostWide / 2; c += 32) {
+                    if (c >= half_wide) continue;
+                    if (kApplies) load_x(c, x_of[0]);
+                    finish(total + c, c, x_of[0]);
+                    __syncwarp();
+                }
             }
         }
     }
@@ -932,7 +890,6 @@ struct Chain {  // matrices of a chain of launches, and what its workspace holds
     std::vector<Entry> entry;
     Entry*   table;
     int32_t* failed;
-    int32_t* done;
     int64_t  chunks, blocks;
     bool     pairs;  // tiles of pairs of CTAs are possible
     size_t   bytes;
@@ -941,7 +898,7 @@ struct Chain {  // matrices of a chain of launches, and what its workspace holds
 Chain chain_of(const Matrix* matrices, int64_t count, int parts, int steps, void* work) {
     Chain c;
     Parts w(work);
-    c.failed = w.take<int32_t>(64 + count), c.done = c.failed + 64;
+    c.failed = w.take<int32_t>(64);
     c.table  = w.take<Entry>(count);
     c.chunks = c.blocks = 0;
     c.entry.resize(count);
@@ -966,7 +923,7 @@ Chain chain_of(const Matrix* matrices, int64_t count, int parts, int steps, void
         e.partial = w.take<double>(e.chunks);
         e.shift   = w.take<float>(steps);
         const int64_t values = (int64_t)e.panels * e.mp * 64;
-        e.x = w.take<float>(values);
+        for (int j = 0; j < 2; ++j) e.x[j] = w.take<float>(values);
         auto units = [&](int* at, int64_t halves) {
             w.used = (size_t)up((int64_t)w.used, kUnit * 2);
             *at = (int)(w.used / (kUnit * 2));
@@ -986,7 +943,7 @@ int64_t together(const Matrix* matrices, int64_t count, int parts) {
     int64_t i = 0;
     for (; i < count && i < kMostMatrices; ++i) {
         const int64_t m = std::min(matrices[i].rows, matrices[i].cols), n = std::max(matrices[i].rows, matrices[i].cols);
-        const size_t more = (size_t)up(m, 256) * ((size_t)up(n, 128) * (4 + 4 * parts) + (size_t)up(m, 256) * 4 * parts);
+        const size_t more = (size_t)up(m, 256) * ((size_t)up(n, 128) * (8 + 4 * parts) + (size_t)up(m, 256) * 4 * parts);
         if (i > 0 && bytes + more > kChainBytes) break;
         bytes += more;
     }
@@ -1024,48 +981,12 @@ int follow(void (*kernel)(P...), int64_t grid, int threads, int shared, int clus
     return FRAMEWISE_B200_OK;
 }
 
-// How many CTAs of a chain can be there at once: they wait for one another.
-template <int PARTS, int CG>
-int chain_grid() {
-    static std::atomic<int> known[kMostDevices];
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-    if (dev < kMostDevices && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
-    cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(sm_count() / CG * CG), c.blockDim = dim3(kThreads), c.dynamicSmemBytes = kShared;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = CG, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-    c.attrs = at, c.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, k_muon_chain<PARTS, CG>, &c) != cudaSuccess) return 0;
-    n = std::min(n, sm_count() / CG) * CG;
-    if (dev < kMostDevices) known[dev].store(n, std::memory_order_relaxed);
-    return n;
-}
-
-template <int PARTS, int CG>
-int launch_chain(const CUtensorMap& rows, const CUtensorMap& columns, const CUtensorMap& two, const Params& p, const AllFactors& f, cudaStream_t stream) {
-    auto kernel = k_muon_chain<PARTS, CG>;
+template <int KIND, int PARTS, int CG>
+int launch(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int sms, cudaStream_t stream) {
+    auto kernel = k_muon_tiles<KIND, PARTS, CG>;
     static std::atomic<uint64_t> allowed{0};
     FW_DO(allow_shared(kernel, kShared, allowed));
-    const int64_t tiles = (int64_t)p.steps * (2 * p.sym + p.apply), most = chain_grid<PARTS, CG>();
-    if (most < CG) return FRAMEWISE_B200_CUDA_ERROR;
-    cudaLaunchConfig_t c = {};
-    c.gridDim          = dim3((unsigned)std::min(most, std::max(p.sym, p.apply) * (int64_t)CG));
-    c.blockDim         = dim3(kThreads);
-    c.dynamicSmemBytes = kShared;
-    c.stream           = stream;
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeCooperative;
-    at[0].val.cooperative = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = CG, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
-    c.attrs    = at;
-    c.numAttrs = CG > 1 ? 2 : 1;
-    if (tiles >= INT32_MAX / 2) return FRAMEWISE_B200_BAD_ARGUMENT;
-    FW_TRY(cudaLaunchKernelEx(&c, kernel, rows, columns, two, p, f));
-    FW_LAUNCHED();
-    return FRAMEWISE_B200_OK;
+    return follow(kernel, std::min(p.tiles, sms / CG) * CG, kThreads, kShared, CG, stream, a, b, p);
 }
 
 template <typename X>
@@ -1073,36 +994,40 @@ int run_chain(Chain& c, const Rates& rates, const std::vector<Step>& steps, char
     constexpr int PARTS = sizeof(X) == 4 ? 2 : 1;
     const int sms = sm_count(), count = (int)c.entry.size();
     if (sms < 2) return FRAMEWISE_B200_CUDA_ERROR;
+    struct Shape {
+        int     pair, wide;
+        int64_t tiles;
+    };
     auto lay = [&](int pair, int wide, bool apply, bool write) {
         int64_t tiles = 0;
         const int rows = kRowsPerCta * pair;
         for (Entry& e : c.entry) {
-            const int64_t before = tiles;
+            if (write) (apply ? e.first_apply : e.first_sym) = (int)tiles;
             const int mt = e.mp / rows, nt = ((apply ? e.panels * 64 : e.mp) + wide - 1) / wide;
             if (apply) tiles += (int64_t)mt * nt;
             else for (int r = 0; r < mt; ++r) tiles += nt - r * rows / wide;
-            if (write) (apply ? e.first_apply : e.first_sym) = (int)before, (apply ? e.apply : e.sym) = (int)(tiles - before);
         }
         return tiles;
     };
     // The shape of the tiles whose time is the shortest by this count: clocks of a stage of 64 of K by what the products take or what
-    // a CTA can be fed (48 bytes a clock, measured), some thousand clocks a tile for what does not overlap, and whole rounds
-    // of the product with the fewest tiles.
-    int    pair = 1, wide = 64;
-    double least = 1e300, operations = 0;
-    int64_t depth = 0;
-    for (const Entry& e : c.entry) depth = std::max<int64_t>(depth, e.panels), operations += (double)e.mp * e.mp * (e.panels * 64.0 + e.mp) * 4;
-    for (int cg = 1; cg <= (c.pairs ? 2 : 1); ++cg)
-        for (int w = 64 * cg; w <= kMostWide; w *= 2) {
-            const double products = w * 2.0 * (PARTS == 2 ? 3 : 1), fed = PARTS * (kRowsPerCta + w / cg) * kDepth * 2 / 48.0, stage = std::max(products, fed);
-            const int64_t workers = sms / cg, sym = (lay(cg, w, false, false) + workers - 1) / workers, apply = (lay(cg, w, true, false) + workers - 1) / workers;
-            double inner = 0;
-            for (const Entry& e : c.entry) inner = std::max(inner, (e.m + 63) / 64.0);
-            const double time = sym * ((depth + inner) * stage + 6000) + apply * (inner * stage + 3000);
-            if (time < least) least = time, pair = cg, wide = w;
-        }
-    const int64_t sym = lay(pair, wide, false, true), apply = lay(pair, wide, true, true);
-    if (sym >= INT32_MAX / 4 || apply >= INT32_MAX / 4 || c.chunks >= INT32_MAX || c.blocks >= INT32_MAX || c.bytes / (kUnit * 2) >= INT32_MAX)
+    // a CTA can be fed (48 bytes a clock, measured), some thousand clocks a tile for what does not overlap, and whole rounds.
+    auto shape = [&](bool apply) {
+        Shape  best = {1, 64, 0};
+        double least = 1e300;
+        for (int pair = 1; pair <= (c.pairs ? 2 : 1); ++pair)
+            for (int wide = 64 * pair; wide <= kMostWide; wide *= 2) {
+                const double products = wide * 2.0 * (PARTS == 2 ? 3 : 1), fed = PARTS * (kRowsPerCta + wide / pair) * kDepth * 2 / 48.0;
+                const int64_t tiles = lay(pair, wide, apply, false), workers = sms / pair;
+                double stages = 0;
+                for (const Entry& e : c.entry) stages = std::max(stages, (double)(apply ? (e.m + 63) / 64 : e.panels));
+                const double time = (double)((tiles + workers - 1) / workers) * (stages * std::max(products, fed) + 3000);
+                if (time < least) least = time, best = {pair, wide, tiles};
+            }
+        lay(best.pair, best.wide, apply, true);
+        return best;
+    };
+    const Shape sym = shape(false), apply = shape(true);
+    if (sym.tiles >= INT32_MAX || apply.tiles >= INT32_MAX || c.chunks >= INT32_MAX || c.blocks >= INT32_MAX || c.bytes / (kUnit * 2) >= INT32_MAX)
         return FRAMEWISE_B200_BAD_ARGUMENT;
     FW_DO(bind_device());
     // 128 rows of a unit; 64 of them; 64 rows of two units
@@ -1111,16 +1036,10 @@ int run_chain(Chain& c, const Rates& rates, const std::vector<Step>& steps, char
     if (!map_of(&tall, work, false, 64, 128, units, 64, kUnit, 64, 128) || !map_of(&square, work, false, 64, 128, units, 64, kUnit, 64, 64) ||
         !map_of(&two, work, false, 64, 128, units, 64, kUnit, 64, 64, 2))
         return FRAMEWISE_B200_TENSOR_MAP;
-    FW_TRY(cudaMemsetAsync(c.failed, 0, (size_t)(64 + count) * 4, stream));
+    FW_TRY(cudaMemsetAsync(c.failed, 0, 4, stream));
     Steps abc;
-    AllFactors factors;
     abc.count = (int)steps.size();
-    for (size_t i = 0; i < steps.size(); ++i) {
-        const Step& s = steps[i];
-        abc.abc[3 * i] = s.a, abc.abc[3 * i + 1] = s.b, abc.abc[3 * i + 2] = s.c;
-        factors.step[i] = {std::ldexp(1.f, s.gram - 2 * s.x), std::ldexp(s.c, s.factor - 2 * s.gram), std::ldexp(s.b, s.factor - s.gram), std::ldexp(1.f, s.factor),
-                           std::ldexp(1.f, -s.factor - s.x), s.a, i + 1 < steps.size() ? std::ldexp(1.f, steps[i + 1].x) : 0.f};
-    }
+    for (size_t i = 0; i < steps.size(); ++i) abc.abc[3 * i] = steps[i].a, abc.abc[3 * i + 1] = steps[i].b, abc.abc[3 * i + 2] = steps[i].c;
     for (int i = 0; i < count; i += kSlots) {
         Slots s;
         s.count = std::min(kSlots, count - i), s.base = i, s.table = c.table;
@@ -1131,13 +1050,30 @@ int run_chain(Chain& c, const Rates& rates, const std::vector<Step>& steps, char
     }
     __half* const halves = reinterpret_cast<__half*>(work);
     FW_DO(follow(k_muon_begin<X, PARTS>, c.blocks, 256, 0, 1, stream, (const Entry*)c.table, count, rates, std::ldexp(1.f, steps[0].x), halves, abc));
+    auto go = [&](auto kind, const Shape& sh, Params& p) {
+        constexpr int KIND = decltype(kind)::value;
+        const int other = KIND == kLast ? kEpilogue * kTurn : 0;
+        p.tiles = (int)sh.tiles, p.wide = sh.wide;
+        p.stages = std::min(kMostStages, (kShared - 1024 - other) / ((kRowsPerCta + sh.wide / sh.pair) * kDepth * 2));
+        p.span = std::min(128, sh.wide / sh.pair);
+        const CUtensorMap& b = p.span == 64 ? square : KIND == kApply || KIND == kLast ? two : tall;
+        return sh.pair == 2 ? launch<KIND, PARTS, 2>(tall, b, p, sms, stream) : launch<KIND, PARTS, 1>(tall, b, p, sms, stream);
+    };
     Params p = {};
-    p.table = c.table, p.done = c.done, p.failed = c.failed, p.work = halves, p.count = count, p.steps = (int)steps.size(), p.wide = wide;
-    p.stages = std::min(kMostStages, (kShared - 1024 - kEpilogue * kTurn) / ((kRowsPerCta + wide / pair) * kDepth * 2));
-    p.span = std::min(128, wide / pair), p.sym = (int)sym, p.apply = (int)apply, p.rates = rates;
-    p.patience = (uint64_t)(4e9 + operations / 1e4);  // four seconds beside a step at 10 TFLOP/s
-    const CUtensorMap &columns = p.span == 64 ? square : tall, &both = p.span == 64 ? square : two;
-    return pair == 2 ? launch_chain<PARTS, 2>(tall, columns, both, p, factors, stream) : launch_chain<PARTS, 1>(tall, columns, both, p, factors, stream);
+    p.table = c.table, p.count = count, p.work = halves, p.failed = c.failed, p.rates = rates;
+    for (size_t i = 0; i < steps.size(); ++i) {
+        const Step& s = steps[i];
+        p.step = (int)i, p.from = (int)(i & 1);
+        p.product = std::ldexp(1.f, s.gram - 2 * s.x);
+        FW_DO(go(std::integral_constant<int, kGram>(), sym, p));
+        p.product = std::ldexp(s.c, s.factor - 2 * s.gram), p.old = std::ldexp(s.b, s.factor - s.gram), p.scale = std::ldexp(1.f, s.factor);
+        FW_DO(go(std::integral_constant<int, kSquare>(), sym, p));
+        const bool last = i + 1 == steps.size();
+        p.product = std::ldexp(1.f, -s.factor - s.x), p.old = s.a, p.scale = last ? 0.f : std::ldexp(1.f, steps[i + 1].x);
+        if (last) FW_DO(go(std::integral_constant<int, kLast>(), apply, p));
+        else FW_DO(go(std::integral_constant<int, kApply>(), apply, p));
+    }
+    return follow(k_muon_check<X>, sms, 256, 0, 1, stream, (const Entry*)c.table, count, (const int*)c.failed);
 }
 
 size_t bytes_for(const std::vector<Matrix>& list, int parts) {
