@@ -848,15 +848,220 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
     if (warp == 1) tmem_free<CG>(tmem, kColumns);
 }
 
+// ------------------------------------------------------------------------------------------ small matrices
+
+constexpr int kSmallM = 128, kSmallN = 256;  // a matrix that one CTA holds: X in registers, its operands, A and B in shared memory
+constexpr int kSmallThreads = 512;
+constexpr int kSmallPitch = kSmallN + 1;     // of the values on their way in and out
+__host__ __device__ constexpr int small_bytes(int parts) {
+    const int operands = parts * (kSmallN / 64 + 2) * kUnit * 2, values = kSmallM * kSmallPitch * 4;
+    return 1024 + (operands > values ? operands : values);
+}
+
+struct SmallSlot {  // `count` matrices of one shape, `stride` values apart
+    const void* grad;
+    float*      momentum;
+    void*       param;
+    float*      master;
+    int64_t     stride;
+    int         rows, cols, count;
+    float       rate;
+};
+struct SmallSlots {
+    int       count;
+    SmallSlot slot[kSlots];
+};
+
+// A step's factors, of what they are in Params.
+struct SmallStep {
+    float gram, square, of_gram, of_one, apply, a, operand, b, c;
+};
+struct SmallSteps {
+    int       count;
+    SmallStep step[kMostSteps];
+};
+
+// All steps of a matrix of at most 128 x 256 in one CTA, and its update: nothing but the gradient, the momentum and the parameter
+// crosses memory.  A row of X by four threads, 64 columns each (one unit's row), 32 columns of A and B.  What bounds it is latency:
+// three products a step, each behind a barrier, and what turns its sums into the next operands; SMALLUS.
+template <typename X>
+__global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_constant__ SmallSlots s, const Rates r, const __grid_constant__ SmallSteps steps) {
+    constexpr int PARTS = sizeof(X) == 4 ? 2 : 1;
+    extern __shared__ char shared_raw[];
+    __shared__ double   part[kSmallThreads / 32];
+    __shared__ uint64_t bar_at;
+    __shared__ uint32_t slot_at;
+    const uint32_t base = (smem_addr(shared_raw) + 1023u) & ~1023u, bar = smem_addr(&bar_at);
+    char* const    mem  = shared_raw + (base - smem_addr(shared_raw));
+    float* const   values = reinterpret_cast<float*>(mem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = warp % 4 * 32 + lane, group = warp / 4;
+    int at = 0, index = blockIdx.x;
+    while (index >= s.slot[at].count) index -= s.slot[at++].count;
+    const SmallSlot& m = s.slot[at];
+    const int  rows = m.rows, cols = m.cols, all = rows * cols;
+    const bool tall = rows > cols;
+    const int  small = min(rows, cols), wide = max(rows, cols), units = (wide + 63) / 64;
+    const X* const g = static_cast<const X*>(m.grad) + index * m.stride;
+    X* const       p = static_cast<X*>(m.param) + index * m.stride;
+    float* const   v = m.momentum ? m.momentum + index * m.stride : nullptr;
+    float* const   master = m.master ? m.master + index * m.stride : nullptr;
+
+    if (threadIdx.x == 0) {
+        bar_init(bar, 1);
+        bar_init_fence();
+    }
+    if (warp == 0) tmem_alloc<1>(smem_addr(&slot_at), kColumns);
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < all; i += kSmallThreads) {
+        float u = value(g[i]);
+        if (v) {
+            const float v0 = v[i], now = v0 + (u - v0) * r.keep;
+            v[i] = now;
+            u = direction(u, now, r);
+        }
+        const int line = i / cols, place = i - line * cols;
+        values[tall ? place * kSmallPitch + line : line * kSmallPitch + place] = u;
+        sum += (double)u * (double)u;
+    }
+#pragma unroll
+    for (int j = 16; j > 0; j >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, j);
+    if (lane == 0) part[warp] = sum;
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *const_cast<volatile uint32_t*>(&slot_at);
+    sum = 0.0;
+    for (int i = 0; i < kSmallThreads / 32; ++i) sum += part[i];
+    const double by = 1.0 / fmax(sqrt(sum), (double)r.eps);  // in 64 bits, as for larger matrices
+    const bool   far = !(by < 1e30);
+    const float  by32 = (float)by;
+    float x[64];
+    const bool mine = row < small;
+#pragma unroll
+    for (int j = 0; j < 64; ++j) {
+        const int col = group * 64 + j;
+        const float u = mine && col < wide ? values[row * kSmallPitch + col] : 0.f;
+        x[j] = far ? (float)(u * by) : u * by32;
+    }
+    __syncthreads();  // the operands take the values' place
+    float one = (float)(fmin(1.0, sqrt(sum) * by) * rsqrt((double)small));
+    const uint32_t x_at = base, s_at = base + PARTS * (kSmallN / 64) * (kUnit * 2);
+    constexpr int kXPart = kSmallN / 64 * kUnit * 2, kSPart = 2 * kUnit * 2;
+    // 8 values as an operand's 16 bytes: piece `piece` of this row in a unit
+    auto put8 = [&](uint32_t unit, int part_bytes, int piece, const float* v8, float scale) {
+        float2 two[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) two[j] = make_float2(v8[2 * j] * scale, v8[2 * j + 1] * scale);
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = part_of(two[j]);
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(unit + q * part_bytes + row * 128 + ((piece ^ (row & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                         : "memory");
+        }
+    };
+    auto put_x = [&](float scale) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) put8(x_at + group * kUnit * 2, kXPart, j, x + 8 * j, scale);
+    };
+    uint32_t phase = 0;
+    bool     ok = true;
+    // a product of the operands that all threads have written, by one of them; the others wait for it
+    auto multiply = [&](uint32_t d, uint32_t a, int a_part, uint32_t b, int b_part, uint32_t kind, int depth, bool b_mn) {
+        fence_before();
+        async_fence();
+        __syncthreads();
+        fence_after();
+        if (threadIdx.x == 0) {
+            bool add = false;
+#pragma unroll
+            for (int q = PARTS == 2 ? 0 : 2; q < 3; ++q)  // of two parts: the small products first
+                for (int k = 0; k < depth; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i, add = true)
+                        product<1>(tmem + d, operand(a + (q == 0 ? a_part : 0) + k * kUnit * 2 + i * 32, 8192),
+                                   operand(b + (q == 1 ? b_part : 0) + (b_mn ? (k * 4 + i) * 2048 : k * kUnit * 2 + i * 32), kUnit * 2), kind, add);
+            products_commit<1>(bar);
+        }
+        uint64_t since = 0;
+        for (int i = 1; ok; ++i) {
+            if (bar_try(bar, phase)) break;
+            if (i % 64) continue;
+            uint64_t now;
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+            if (since == 0) since = now;
+            if (now - since > 4000000000ull) ok = false;
+        }
+        phase ^= 1;
+        fence_after();
+    };
+    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
+    const int depth_x = units, depth_s = (small + 63) / 64;
+    put_x(steps.step[0].operand);
+    for (int i = 0; i < steps.count; ++i) {
+        const SmallStep& f = steps.step[i];
+        const float square = one * one, shift = square * (f.b + f.c * square);
+        one *= f.a + shift;
+        float2 pairs[16];
+        float* const sums = reinterpret_cast<float*>(pairs);
+        float a[32];
+        multiply(0, x_at, kXPart, x_at, kXPart, half_kind(128, 128, false), depth_x, false);  // A = X X^T
+        tmem_load32(tmem + lanes + group * 32, pairs);
+        tmem_loaded(pairs);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) a[j] = sums[j] * f.gram;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) put8(s_at + group / 2 * kUnit * 2, kSPart, group % 2 * 4 + j, a + 8 * j, 1.f);
+        multiply(128, s_at, kSPart, s_at, kSPart, half_kind(128, 128, false), depth_s, false);  // B = b A + c A A - t
+        tmem_load32(tmem + lanes + 128 + group * 32, pairs);
+        tmem_loaded(pairs);
+        const int hit = row - group * 32;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) a[j] = fmaf(f.of_gram, a[j], sums[j] * f.square) - (j == hit ? shift * f.of_one : 0.f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) put8(s_at + group / 2 * kUnit * 2, kSPart, group % 2 * 4 + j, a + 8 * j, 1.f);
+        multiply(256, s_at, kSPart, x_at, kXPart, half_kind(128, units * 64, true), depth_s, true);  // (a + t) X + B X
+        if (group < units) {
+#pragma unroll
+            for (int c = 0; c < 64; c += 32) {
+                tmem_load32(tmem + lanes + 256 + group * 64 + c, pairs);
+                tmem_loaded(pairs);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[c + j] = fmaf(f.a + shift, x[c + j], sums[j] * f.apply);
+            }
+        }
+        if (i + 1 < steps.count) put_x(steps.step[i + 1].operand);
+    }
+    ok = __syncthreads_and(ok);  // and all products have been read: the values take the operands' place again
+#pragma unroll
+    for (int j = 0; j < 64; ++j)
+        if (mine && group * 64 + j < wide) values[row * kSmallPitch + group * 64 + j] = ok ? x[j] : __uint_as_float(0x7fffffffu);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 0) tmem_free<1>(tmem, kColumns);
+    for (int i = threadIdx.x; i < all; i += kSmallThreads) {
+        const int line = i / cols, place = i - line * cols;
+        float o = values[tall ? place * kSmallPitch + line : line * kSmallPitch + place];
+        if (v) {
+            o = updated<X>(value(p[i]), master ? master[i] : 0.f, master != nullptr, o, r, m.rate);
+            if (master) master[i] = o;
+        }
+        put(p + i, o);
+    }
+}
+
 // ------------------------------------------------------------------------------------------ host side
 
-struct Matrix {
+struct Matrix {  // `count` of them, one after another
     void*       param;
     const void* grad;
     float*      momentum;
     float*      master;
     int64_t     rows, cols;
     double      rate;
+    bool        small() const { return std::min(rows, cols) <= kSmallM && std::max(rows, cols) <= kSmallN; }
 };
 
 // Powers of two that bring the operands of each step into the range of fp16, for singular values of at most one before.
@@ -1087,13 +1292,38 @@ size_t bytes_for(const std::vector<Matrix>& list, int parts) {
     return most;
 }
 
-int run(const std::vector<Matrix>& list, int dtype, const Rates& rates, const double* coefficients, int steps, void* work, size_t work_bytes,
-        cudaStream_t stream) {
-    if (list.empty()) return FRAMEWISE_B200_OK;
+template <typename X>
+int run_small(const std::vector<SmallSlot>& slots, const Rates& rates, const std::vector<Step>& steps, cudaStream_t stream) {
+    constexpr int PARTS = sizeof(X) == 4 ? 2 : 1;
+    static std::atomic<uint64_t> allowed{0};
+    FW_DO(allow_shared(k_muon_small<X>, small_bytes(PARTS), allowed));
+    SmallSteps f;
+    f.count = (int)steps.size();
+    for (size_t i = 0; i < steps.size(); ++i) {
+        const Step& t = steps[i];
+        f.step[i] = {std::ldexp(1.f, t.gram - 2 * t.x), std::ldexp(t.c, t.factor - 2 * t.gram), std::ldexp(t.b, t.factor - t.gram), std::ldexp(1.f, t.factor),
+                     std::ldexp(1.f, -t.factor - t.x), t.a, std::ldexp(1.f, t.x), t.b, t.c};
+    }
+    for (size_t i = 0; i < slots.size(); i += kSlots) {
+        SmallSlots s;
+        s.count = (int)std::min<size_t>(kSlots, slots.size() - i);
+        int64_t grid = 0;
+        for (int j = 0; j < s.count; ++j) s.slot[j] = slots[i + j], grid += s.slot[j].count;
+        k_muon_small<X><<<(unsigned)grid, kSmallThreads, small_bytes(PARTS), stream>>>(s, rates, f);
+        FW_LAUNCHED();
+    }
+    return FRAMEWISE_B200_OK;
+}
+
+// the matrices that a CTA holds, and the others
+int run(const std::vector<SmallSlot>& small, const std::vector<Matrix>& list, int dtype, const Rates& rates, const double* coefficients, int steps, void* work,
+        size_t work_bytes, cudaStream_t stream) {
+    if (list.empty() && small.empty()) return FRAMEWISE_B200_OK;
     const int parts = dtype == FRAMEWISE_B200_F32 ? 2 : 1;
     std::vector<Step> plan;
     if (!work || misaligned(work) || !coefficients || steps < 1 || steps > kMostSteps || !steps_of(coefficients, steps, &plan)) return FRAMEWISE_B200_BAD_ARGUMENT;
     if (work_bytes < bytes_for(list, parts)) return FRAMEWISE_B200_WORKSPACE;
+    FW_DO(dtype == FRAMEWISE_B200_F32 ? run_small<float>(small, rates, plan, stream) : run_small<__nv_bfloat16>(small, rates, plan, stream));
     for (size_t i = 0; i < list.size();) {
         const int64_t n = together(list.data() + i, (int64_t)(list.size() - i), parts);
         Chain c = chain_of(list.data() + i, n, parts, kMostSteps, work);
@@ -1107,24 +1337,34 @@ int run(const std::vector<Matrix>& list, int dtype, const Rates& rates, const do
 bool dtype_ok(int dtype) { return dtype == FRAMEWISE_B200_F32 || dtype == FRAMEWISE_B200_BF16; }
 
 // the matrices of a Muon step; those without values are passed over
-int muon_list(const framewise_b200_matrix* matrices, int64_t count, double lr, int adjust, std::vector<Matrix>* list) {
+int muon_list(const framewise_b200_matrix* matrices, int64_t count, double lr, int adjust, std::vector<SmallSlot>* small, std::vector<Matrix>* list) {
     if (count < 0 || (count > 0 && !matrices)) return FRAMEWISE_B200_BAD_ARGUMENT;
     for (int64_t i = 0; i < count; ++i) {
         const framewise_b200_matrix& m = matrices[i];
         if (m.rows < 0 || m.cols < 0) return FRAMEWISE_B200_BAD_ARGUMENT;
         if (m.rows == 0 || m.cols == 0) continue;
         const double by = adjust ? 0.2 * std::sqrt((double)std::max(m.rows, m.cols)) : std::sqrt(std::max(1.0, (double)m.rows / m.cols));
-        list->push_back({m.param, m.grad, m.momentum, m.master, m.rows, m.cols, lr * by});
+        const Matrix one = {m.param, m.grad, m.momentum, m.master, m.rows, m.cols, lr * by};
+        if (one.small()) small->push_back({m.grad, m.momentum, m.param, m.master, 0, (int)m.rows, (int)m.cols, 1, (float)one.rate});
+        else list->push_back(one);
     }
     return matrices_ok(list->data(), (int64_t)list->size()) ? FRAMEWISE_B200_OK : FRAMEWISE_B200_BAD_ARGUMENT;
 }
 
-std::vector<Matrix> batch_list(int64_t count, int64_t rows, int64_t cols, int dtype, const void* x, void* out) {
-    std::vector<Matrix> list;
-    const int64_t bytes = rows * cols * (dtype == FRAMEWISE_B200_F32 ? 4 : 2);
+// `count` matrices of one shape, one after another
+int batch_list(int64_t count, int64_t rows, int64_t cols, int dtype, const void* x, void* out, std::vector<SmallSlot>* small, std::vector<Matrix>* list) {
+    const int64_t values = rows * cols, bytes = values * (dtype == FRAMEWISE_B200_F32 ? 4 : 2);
+    const Matrix  one = {out, x, nullptr, nullptr, rows, cols, 0.0};
+    if (one.small()) {
+        for (int64_t i = 0; i < count; i += 1 << 30)
+            small->push_back({x ? static_cast<const char*>(x) + i * bytes : nullptr, nullptr, out ? static_cast<char*>(out) + i * bytes : nullptr, nullptr, values, (int)rows,
+                              (int)cols, (int)std::min<int64_t>(count - i, 1 << 30), 0.f});
+        return FRAMEWISE_B200_OK;
+    }
+    if (!matrices_ok(&one, 1)) return FRAMEWISE_B200_BAD_ARGUMENT;
     for (int64_t i = 0; i < count; ++i)
-        list.push_back({out ? static_cast<char*>(out) + i * bytes : nullptr, x ? static_cast<const char*>(x) + i * bytes : nullptr, nullptr, nullptr, rows, cols, 0.0});
-    return list;
+        list->push_back({out ? static_cast<char*>(out) + i * bytes : nullptr, x ? static_cast<const char*>(x) + i * bytes : nullptr, nullptr, nullptr, rows, cols, 0.0});
+    return FRAMEWISE_B200_OK;
 }
 
 }  // namespace
@@ -1132,28 +1372,33 @@ std::vector<Matrix> batch_list(int64_t count, int64_t rows, int64_t cols, int dt
 extern "C" {
 
 size_t framewise_b200_muon_bytes(const framewise_b200_matrix* matrices, int64_t count, int32_t dtype) {
-    std::vector<Matrix> list;
-    if (!dtype_ok(dtype) || muon_list(matrices, count, 0.0, 0, &list) != FRAMEWISE_B200_OK) return 0;
+    std::vector<SmallSlot> small;
+    std::vector<Matrix>    list;
+    if (!dtype_ok(dtype) || muon_list(matrices, count, 0.0, 0, &small, &list) != FRAMEWISE_B200_OK) return 0;
     return bytes_for(list, dtype == FRAMEWISE_B200_F32 ? 2 : 1);
 }
 
 int framewise_b200_muon(const framewise_b200_matrix* matrices, int64_t count, int32_t dtype, double lr, double beta, int32_t nesterov,
                         double weight_decay, int32_t match_rms, const double* coefficients, int32_t steps, double eps, int32_t follow,
                         void* work, size_t work_bytes, framewise_b200_stream_t stream) {
-    std::vector<Matrix> list;
+    std::vector<SmallSlot> small;
+    std::vector<Matrix>    list;
     if (!dtype_ok(dtype) || !(eps > 0)) return FRAMEWISE_B200_BAD_ARGUMENT;
-    FW_DO(muon_list(matrices, count, lr, match_rms, &list));
-    for (const Matrix& m : list)
-        if (!m.param || !m.grad || !m.momentum || (m.master && dtype == FRAMEWISE_B200_F32)) return FRAMEWISE_B200_BAD_ARGUMENT;
+    FW_DO(muon_list(matrices, count, lr, match_rms, &small, &list));
+    auto bad = [&](const auto& m) { return !m.param || !m.grad || !m.momentum || (m.master && dtype == FRAMEWISE_B200_F32); };
+    if (std::any_of(list.begin(), list.end(), bad) || std::any_of(small.begin(), small.end(), bad)) return FRAMEWISE_B200_BAD_ARGUMENT;
     const Rates rates = {(float)(1 - beta), (float)beta, nesterov ? 1.f : 0.f, (float)eps, (float)(1 - lr * weight_decay), follow};
-    return run(list, dtype, rates, coefficients, steps, work, work_bytes, stream);
+    return run(small, list, dtype, rates, coefficients, steps, work, work_bytes, stream);
 }
 
 size_t framewise_b200_orthogonalize_bytes(int64_t count, int64_t rows, int64_t cols, int32_t dtype) {
     if (!dtype_ok(dtype) || count < 0 || rows < 0 || cols < 0) return 0;
     if (count == 0 || rows == 0 || cols == 0) return 256;
-    const std::vector<Matrix> list = batch_list(std::min<int64_t>(count, kMostMatrices), rows, cols, dtype, nullptr, nullptr);
-    return matrices_ok(list.data(), (int64_t)list.size()) ? bytes_for(list, dtype == FRAMEWISE_B200_F32 ? 2 : 1) : 0;
+    std::vector<SmallSlot> small;
+    std::vector<Matrix>    list;
+    // more than a chain's go through the same scratch
+    if (batch_list(std::min<int64_t>(count, kMostMatrices), rows, cols, dtype, nullptr, nullptr, &small, &list) != FRAMEWISE_B200_OK) return 0;
+    return bytes_for(list, dtype == FRAMEWISE_B200_F32 ? 2 : 1);
 }
 
 int framewise_b200_orthogonalize(int64_t count, int64_t rows, int64_t cols, int32_t dtype, const void* x, void* out, const double* coefficients,
@@ -1161,10 +1406,11 @@ int framewise_b200_orthogonalize(int64_t count, int64_t rows, int64_t cols, int3
     if (!dtype_ok(dtype) || count < 0 || rows < 0 || cols < 0 || !(eps > 0)) return FRAMEWISE_B200_BAD_ARGUMENT;
     if (count == 0 || rows == 0 || cols == 0) return FRAMEWISE_B200_OK;
     if (!x || !out) return FRAMEWISE_B200_BAD_ARGUMENT;
-    const std::vector<Matrix> list = batch_list(count, rows, cols, dtype, x, out);
-    if (!matrices_ok(list.data(), (int64_t)list.size())) return FRAMEWISE_B200_BAD_ARGUMENT;
+    std::vector<SmallSlot> small;
+    std::vector<Matrix>    list;
+    FW_DO(batch_list(count, rows, cols, dtype, x, out, &small, &list));
     const Rates rates = {0.f, 0.f, 0.f, (float)eps, 1.f, 0};
-    return run(list, dtype, rates, coefficients, steps, work, work_bytes, stream);
+    return run(small, list, dtype, rates, coefficients, steps, work, work_bytes, stream);
 }
 
 }  // extern "C"
