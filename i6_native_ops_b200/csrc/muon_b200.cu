@@ -912,16 +912,41 @@ __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_co
     }
     if (warp == 0) tmem_alloc<1>(smem_addr(&slot_at), kColumns);
     double sum = 0.0;
-    for (int i = threadIdx.x; i < all; i += kSmallThreads) {
-        float u = value(g[i]);
-        if (v) {
-            const float v0 = v[i], now = v0 + (u - v0) * r.keep;
-            v[i] = now;
-            u = direction(u, now, r);
-        }
+    // four values at a time, of which a line's lie side by side
+    constexpr int kAhead = 4;
+    const bool wide4 = aligned4(g, v) && aligned4(p, master) && cols % 4 == 0;
+    auto place_of = [&](int i) {
         const int line = i / cols, place = i - line * cols;
-        values[tall ? place * kSmallPitch + line : line * kSmallPitch + place] = u;
-        sum += (double)u * (double)u;
+        return tall ? place * kSmallPitch + line : line * kSmallPitch + place;
+    };
+    const int hop = tall ? kSmallPitch : 1;
+    for (int i0 = threadIdx.x * 4; i0 < all; i0 += kSmallThreads * 4 * kAhead) {
+        float u[kAhead][4], old[kAhead][4];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int i = i0 + k * kSmallThreads * 4;
+            if (i >= all) continue;
+            load4(g + i, wide4, all - i, u[k]);
+            if (v) load4(v + i, wide4, all - i, old[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int i = i0 + k * kSmallThreads * 4;
+            if (i >= all) continue;
+            const int at = place_of(i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (!wide4 && i + j >= all) continue;
+                if (v) {
+                    old[k][j] += (u[k][j] - old[k][j]) * r.keep;
+                    if (!wide4) v[i + j] = old[k][j];
+                    u[k][j] = direction(u[k][j], old[k][j], r);
+                }
+                values[wide4 ? at + j * hop : place_of(i + j)] = u[k][j];
+                sum += (double)u[k][j] * (double)u[k][j];
+            }
+            if (v && wide4) *reinterpret_cast<float4*>(v + i) = make_float4(old[k][0], old[k][1], old[k][2], old[k][3]);
+        }
     }
 #pragma unroll
     for (int j = 16; j > 0; j >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, j);
@@ -1041,14 +1066,43 @@ __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_co
     __syncthreads();
     fence_after();
     if (warp == 0) tmem_free<1>(tmem, kColumns);
-    for (int i = threadIdx.x; i < all; i += kSmallThreads) {
-        const int line = i / cols, place = i - line * cols;
-        float o = values[tall ? place * kSmallPitch + line : line * kSmallPitch + place];
-        if (v) {
-            o = updated<X>(value(p[i]), master ? master[i] : 0.f, master != nullptr, o, r, m.rate);
-            if (master) master[i] = o;
+    for (int i0 = threadIdx.x * 4; i0 < all; i0 += kSmallThreads * 4 * kAhead) {
+        float was[kAhead][4], held[kAhead][4];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int i = i0 + k * kSmallThreads * 4;
+            if (i >= all || !v) continue;
+            load4(p + i, wide4, all - i, was[k]);
+            if (master) load4(master + i, wide4, all - i, held[k]);
         }
-        put(p + i, o);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int i = i0 + k * kSmallThreads * 4;
+            if (i >= all) continue;
+            const int at = place_of(i);
+            float o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (!wide4 && i + j >= all) continue;
+                o[j] = values[wide4 ? at + j * hop : place_of(i + j)];
+                if (v) o[j] = updated<X>(was[k][j], master ? held[k][j] : 0.f, master != nullptr, o[j], r, m.rate);
+                if (!wide4) {
+                    if (master) master[i + j] = o[j];
+                    put(p + i + j, o[j]);
+                }
+            }
+            if (wide4) {
+                if (master) *reinterpret_cast<float4*>(master + i) = make_float4(o[0], o[1], o[2], o[3]);
+                if constexpr (sizeof(X) == 4) {
+                    *reinterpret_cast<float4*>(p + i) = make_float4(o[0], o[1], o[2], o[3]);
+                } else {
+                    uint2 w;
+                    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w.x) : "f"(o[1]), "f"(o[0]));
+                    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w.y) : "f"(o[3]), "f"(o[2]));
+                    *reinterpret_cast<uint2*>(p + i) = w;
+                }
+            }
+        }
     }
 }
 
@@ -1076,15 +1130,21 @@ bool steps_of(const double* abc, int count, std::vector<Step>* steps) {
     for (int i = 0; i < count; ++i) {
         const double a = abc[3 * i], b = abc[3 * i + 1], c = abc[3 * i + 2];
         if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
-        double low = 0, high = 0, next = 0;  // of B, less any of its own values
-        for (int j = 0; j <= 4096; ++j) {
-            const double s = most * j / 4096, f = b * s * s + c * s * s * s * s;
-            low = std::min(low, f), high = std::max(high, f), next = std::max(next, std::fabs(s * (a + f)));
-        }
+        // B, less any of its own values, and the next singular values: largest at the range's end or where a derivative is zero
+        double low = 0, high = 0, next = 0;
+        auto meet = [&](double square) {
+            if (!(square >= 0)) return;
+            const double q = std::min(square, most * most), f = q * (b + c * q);
+            low = std::min(low, f), high = std::max(high, f), next = std::max(next, std::sqrt(q) * std::fabs(a + f));
+        };
+        meet(most * most);
+        meet(-b / (2 * c));
+        const double root = std::sqrt(9 * b * b - 20 * a * c);
+        meet((-3 * b + root) / (10 * c)), meet((-3 * b - root) / (10 * c));
+        if (c == 0) meet(-a / (3 * b));
         const double factor = 1.01 * (high - low);
         next *= 1.01;
-        Step s = {(float)a, (float)b, (float)c, exponent(most), exponent(most * most), exponent(factor)};
-        steps->push_back(s);
+        steps->push_back({(float)a, (float)b, (float)c, exponent(most), exponent(most * most), exponent(factor)});
         if (!(next < 1e6)) return false;
         most = std::max(next, 1e-6);
     }
