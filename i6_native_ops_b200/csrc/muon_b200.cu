@@ -42,10 +42,12 @@ constexpr int kMostWide     = 256;   // columns of a tile at most
 constexpr int kColumns      = 512;   // of tensor memory: a ring of accumulators
 constexpr int kMostAccs     = 8;
 constexpr int kDepth        = 64;    // K per stage: one part of both operands
-constexpr int kSegment      = 2;     // f32: steps of 64 of K after which an accumulator is added up in registers, for tensor cores cut
-                                     // off what they add, at 2^-24 of the sum a step, and never round it up.  A segment's small
-                                     // products come first, so that eight steps of it count: 6 x 500 x 2001 is off by SEGERR of
-                                     // its norm (plain 32 bits: 2.7e-6; segments of four stages, stage by stage: 5.1e-6)
+// f32: steps of 64 of K after which an accumulator is added up in registers, for tensor cores cut off what they add, at 2^-24 of the
+// sum a step, and never round it up.  What A A is off by shows most (b A and c A A undo each other where singular values are near
+// one), and it is the smallest product: there it is done after each step, and so in short sums, whose tiles wait for other things.
+// Off by, as a part of their norm (plain 32 bits): 500 x 2001 2.6e-6 (2.8e-6; four steps in A A as well 5.1e-6, two throughout
+// 3.4e-6, in 531 us for six instead of 480).
+__host__ __device__ constexpr int segment_of(bool square, int depth) { return square || depth <= 4 ? 1 : 4; }
 constexpr int kMostStages   = 12;
 constexpr int kEpilogue     = 8;     // warps that finish tiles
 constexpr int kThreads      = 64 + 32 * kEpilogue;
@@ -623,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
             const Entry m = p.table[t.e];
             const int limit = kApplies ? m.panels * 64 : m.mp;
             const uint32_t kind = half_kind(kTile, min(p.wide, limit - t.col), kBMn);
-            for (int k0 = 0; k0 < t.depth && ok; k0 += kSegments ? kSegment : t.depth) {
+            for (int k0 = 0; k0 < t.depth && ok; k0 += kSegments ? segment_of(KIND == kSquare, t.depth) : t.depth) {
                 ok = wait(freed + 8 * acc, acc_phase ^ 1);
                 if (!ok) break;
                 fence_after();
@@ -642,29 +644,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                     if (ok) fence_after();
                     return ok;
                 };
-                if constexpr (kSegments) {  // the small products of all steps, then the large ones
-                    int large[kSegment] = {};
-                    const int some = min(kSegment, t.depth - k0);
-#pragma unroll
-                    for (int k = 0; k < kSegment; ++k) {
-                        if (k >= some) continue;
+                if constexpr (kSegments) {  // the small products first
+                    const int k1 = min(t.depth, k0 + segment_of(KIND == kSquare, t.depth));
+                    for (int k = k0; k < k1; ++k) {
                         const int low = stage;
                         if (!arrived(stage, phase)) break;
                         next(stage, phase);
                         if (!arrived(stage, phase)) break;
-                        large[k] = stage;
-                        multiply(low, large[k], k > 0);
-                        multiply(large[k], low, true);
+                        multiply(low, stage, k > k0);
+                        multiply(stage, low, true);
                         products_commit<CG>(empty + 8 * low);
+                        multiply(stage, stage, true);
+                        products_commit<CG>(empty + 8 * stage);
                         next(stage, phase);
                     }
                     if (!ok) break;
-#pragma unroll
-                    for (int k = 0; k < kSegment; ++k) {
-                        if (k >= some) continue;
-                        multiply(large[k], large[k], true);
-                        products_commit<CG>(empty + 8 * large[k]);
-                    }
                 } else {
                     for (int k = 0; k < t.depth; ++k) {
                         if (!arrived(stage, phase)) break;
@@ -786,7 +780,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
 #pragma unroll
                 for (int j = 0; j < kMostWide / 2; ++j) total[j] = 0.f;
             }
-            for (int k0 = 0; k0 < t.depth; k0 += kSegments ? kSegment : t.depth) {
+            for (int k0 = 0; k0 < t.depth; k0 += kSegments ? segment_of(KIND == kSquare, t.depth) : t.depth) {
                 ok = __all_sync(0xffffffffu, wait(done + 8 * acc, acc_phase));
                 if (!ok) break;
                 fence_after();
@@ -854,7 +848,7 @@ constexpr int kSmallM = 128, kSmallN = 256;  // a matrix that one CTA holds: X i
 constexpr int kSmallThreads = 512;
 constexpr int kSmallPitch = kSmallN + 1;     // of the values on their way in and out
 __host__ __device__ constexpr int small_bytes(int parts) {
-    const int operands = parts * (kSmallN / 64 + 2) * kUnit * 2, values = kSmallM * kSmallPitch * 4;
+    const int operands = (parts * (kSmallN / 64) + 2 * 2) * kUnit * 2, values = kSmallM * kSmallPitch * 4;
     return 1024 + (operands > values ? operands : values);
 }
 
@@ -881,6 +875,8 @@ struct SmallSteps {
     SmallStep step[kMostSteps];
 };
 
+// A has two parts here for bf16 as well: with one, b A and c A A disagree about what A is, and results are off by up to 1.9 times their
+// own rounding (2 x 27; 1.24 times with two).
 // All steps of a matrix of at most 128 x 256 in one CTA, and its update: nothing but the gradient, the momentum and the parameter
 // crosses memory.  A row of X by four threads, 64 columns each (one unit's row), 32 columns of A and B.  What bounds it is latency:
 // three products a step, each behind a barrier, and what turns its sums into the next operands; SMALLUS.
@@ -973,40 +969,47 @@ __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_co
     const uint32_t x_at = base, s_at = base + PARTS * (kSmallN / 64) * (kUnit * 2);
     constexpr int kXPart = kSmallN / 64 * kUnit * 2, kSPart = 2 * kUnit * 2;
     // 8 values as an operand's 16 bytes: piece `piece` of this row in a unit
-    auto put8 = [&](uint32_t unit, int part_bytes, int piece, const float* v8, float scale) {
+    auto put8 = [&](auto parts, uint32_t unit, int part_bytes, int piece, float* v8, float scale, bool round = false) {
         float2 two[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) two[j] = make_float2(v8[2 * j] * scale, v8[2 * j + 1] * scale);
 #pragma unroll
-        for (int q = 0; q < PARTS; ++q) {
+        for (int q = 0; q < decltype(parts)::value; ++q) {
             uint32_t w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = part_of(two[j]);
             asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(unit + q * part_bytes + row * 128 + ((piece ^ (row & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
                          : "memory");
         }
+        if (round) {  // the values become what the parts hold
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v8[2 * j] -= two[j].x, v8[2 * j + 1] -= two[j].y;
+        }
     };
+    constexpr std::integral_constant<int, PARTS> of_type{};
+    constexpr std::integral_constant<int, 2>     both{};
     auto put_x = [&](float scale) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) put8(x_at + group * kUnit * 2, kXPart, j, x + 8 * j, scale);
+        for (int j = 0; j < 8; ++j) put8(of_type, x_at + group * kUnit * 2, kXPart, j, x + 8 * j, scale);
     };
     uint32_t phase = 0;
     bool     ok = true;
     // a product of the operands that all threads have written, by one of them; the others wait for it
-    auto multiply = [&](uint32_t d, uint32_t a, int a_part, uint32_t b, int b_part, uint32_t kind, int depth, bool b_mn) {
+    // each: accumulators for 64 of K, 128 columns apart (0: one for all)
+    auto multiply = [&](auto parts, int each, uint32_t d, uint32_t a, int a_part, uint32_t b, int b_part, uint32_t kind, int depth, bool b_mn) {
         fence_before();
         async_fence();
         __syncthreads();
         fence_after();
         if (threadIdx.x == 0) {
-            bool add = false;
+            for (int k = 0; k < depth; ++k)
 #pragma unroll
-            for (int q = PARTS == 2 ? 0 : 2; q < 3; ++q)  // of two parts: the small products first
-                for (int k = 0; k < depth; ++k)
+                for (int q = decltype(parts)::value == 2 ? 0 : 2; q < 3; ++q)  // of two parts: the small products first
 #pragma unroll
-                    for (int i = 0; i < 4; ++i, add = true)
-                        product<1>(tmem + d, operand(a + (q == 0 ? a_part : 0) + k * kUnit * 2 + i * 32, 8192),
-                                   operand(b + (q == 1 ? b_part : 0) + (b_mn ? (k * 4 + i) * 2048 : k * kUnit * 2 + i * 32), kUnit * 2), kind, add);
+                    for (int i = 0; i < 4; ++i)
+                        product<1>(tmem + d + (k * each + i * each / 4) * 128, operand(a + (q == 0 ? a_part : 0) + k * kUnit * 2 + i * 32, 8192),
+                                   operand(b + (q == 1 ? b_part : 0) + (b_mn ? (k * 4 + i) * 2048 : k * kUnit * 2 + i * 32), kUnit * 2), kind,
+                                   q > (decltype(parts)::value == 2 ? 0 : 2) || (each > 0 ? i * each % 4 != 0 : k > 0 || i > 0));
             products_commit<1>(bar);
         }
         uint64_t since = 0;
@@ -1022,7 +1025,9 @@ __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_co
         fence_after();
     };
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
-    const int depth_x = units, depth_s = (small + 63) / 64;
+    // f32: A A, whose errors show most (see segment_of), has as many accumulators as there is room for: 64 x 256 is off by 1.1e-6 of its norm, with
+    // one by 2.4e-6 (plain 32 bits: 1.4e-6)
+    const int depth_x = units, depth_s = (small + 63) / 64, each = PARTS == 2 ? 4 / depth_s : 0;
     put_x(steps.step[0].operand);
     for (int i = 0; i < steps.count; ++i) {
         const SmallStep& f = steps.step[i];
@@ -1031,27 +1036,35 @@ __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_co
         float2 pairs[16];
         float* const sums = reinterpret_cast<float*>(pairs);
         float a[32];
-        multiply(0, x_at, kXPart, x_at, kXPart, half_kind(128, 128, false), depth_x, false);  // A = X X^T
-        tmem_load32(tmem + lanes + group * 32, pairs);
-        tmem_loaded(pairs);
+        auto add_up = [&](int count, int col) {  // 32 columns
+            tmem_load32(tmem + lanes + col, pairs);
+            tmem_loaded(pairs);
+            for (int k = 1; k < count; ++k) {
+                float2 more[16];
+                tmem_load32(tmem + lanes + k * 128 + col, more);
+                tmem_loaded(more);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) pairs[j] = add2(pairs[j], more[j]);
+            }
+        };
+        multiply(of_type, 0, 0, x_at, kXPart, x_at, kXPart, half_kind(128, 128, false), depth_x, false);  // A = X X^T
+        add_up(1, group * 32);
 #pragma unroll
         for (int j = 0; j < 32; ++j) a[j] = sums[j] * f.gram;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) put8(s_at + group / 2 * kUnit * 2, kSPart, group % 2 * 4 + j, a + 8 * j, 1.f);
-        multiply(128, s_at, kSPart, s_at, kSPart, half_kind(128, 128, false), depth_s, false);  // B = b A + c A A - t
-        tmem_load32(tmem + lanes + 128 + group * 32, pairs);
-        tmem_loaded(pairs);
+        for (int j = 0; j < 4; ++j) put8(both, s_at + group / 2 * kUnit * 2, kSPart, group % 2 * 4 + j, a + 8 * j, 1.f, true);  // b A and c A A agree about A
+        multiply(both, each, 0, s_at, kSPart, s_at, kSPart, half_kind(128, 128, false), depth_s, false);  // B = b A + c A A - t
+        add_up(max(1, each * depth_s), group * 32);
         const int hit = row - group * 32;
 #pragma unroll
         for (int j = 0; j < 32; ++j) a[j] = fmaf(f.of_gram, a[j], sums[j] * f.square) - (j == hit ? shift * f.of_one : 0.f);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) put8(s_at + group / 2 * kUnit * 2, kSPart, group % 2 * 4 + j, a + 8 * j, 1.f);
-        multiply(256, s_at, kSPart, x_at, kXPart, half_kind(128, units * 64, true), depth_s, true);  // (a + t) X + B X
+        for (int j = 0; j < 4; ++j) put8(of_type, s_at + group / 2 * kUnit * 2, kSPart, group % 2 * 4 + j, a + 8 * j, 1.f);
+        multiply(of_type, 0, 256, s_at, kSPart, x_at, kXPart, half_kind(128, units * 64, true), depth_s, true);  // (a + t) X + B X
         if (group < units) {
 #pragma unroll
             for (int c = 0; c < 64; c += 32) {
-                tmem_load32(tmem + lanes + 256 + group * 64 + c, pairs);
-                tmem_loaded(pairs);
+                add_up(1, 256 + group * 64 + c);
 #pragma unroll
                 for (int j = 0; j < 32; ++j) x[c + j] = fmaf(f.a + shift, x[c + j], sums[j] * f.apply);
             }
