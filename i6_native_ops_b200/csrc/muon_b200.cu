@@ -13,8 +13,13 @@
 // finer, and all operands are bounded, so that powers of two (from the coefficients, for any matrix) keep them in its range.
 // Once singular values are near one, B is near (b + c) times the identity and undoes most of a X.  So a multiple t of the
 // identity is taken from B and added to a, where it costs no rounding: t = b s^2 + c s^4 for the singular value s that all
-// would have if they were equal (1 / sqrt(m) at first; a matrix below eps, which stays small, has small t).  Errors of bf16 results besides their own rounding: 64 x 256 0.93e-3 of the norm
-// (1.9e-3 without), 512 x 2048 0.6e-3 (1.3e-3); the rounding alone is 1.66e-3.
+// would have if they were equal (1 / sqrt(m) at first; a matrix below eps, which stays small, has small t).  Errors of bf16
+// results besides their own rounding, as a part of their norm: 64 x 256 0.93e-3 (1.9e-3 without t), 512 x 2048 0.6e-3
+// (1.3e-3); the rounding alone is 1.66e-3.
+//
+// Matrices of up to 128 x 256: k_muon_small, a CTA each, all in one launch.  Others go through a chain of launches together: two
+// passes over the gradients (k_muon_collect: momentum and norm; k_muon_begin: X), then a launch of k_muon_tiles for each product,
+// of which the last updates the parameters.
 #include "framewise_b200.h"
 #include "framewise_host.h"
 #include "tensor_core.h"
@@ -65,7 +70,7 @@ struct Entry {
     float*      master;     // or null
     double*     partial;    // sums of squares of the chunks
     float*      shift;      // per step: the multiple of the identity that B does without
-    float*      x[2];       // X, before and after a step
+    float*      x;          // X
     int         operand[2]; // its fp16 parts, as units of the workspace
     int         gram, factor; // A and B, likewise
     int         rows, cols; // of the parameter
@@ -283,7 +288,7 @@ __global__ void __launch_bounds__(256) k_muon_begin(const Entry* __restrict__ ta
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // a warp: 32 rows of four columns, 512 bytes of X
         const int row = (threadIdx.x / 32 & 1) * 32 + threadIdx.x % 32, col = (threadIdx.x / 64 + i * 4) * 4;
-        *reinterpret_cast<float4*>(m.x[0] + place(m.mp, row0 + row, panel * 64 + col)) = make_float4(x_of(row, col), x_of(row, col + 1), x_of(row, col + 2), x_of(row, col + 3));
+        *reinterpret_cast<float4*>(m.x + place(m.mp, row0 + row, panel * 64 + col)) = make_float4(x_of(row, col), x_of(row, col + 1), x_of(row, col + 2), x_of(row, col + 3));
     }
     __half* const op = work + (int64_t)m.operand[0] * kUnit + in_units(m.panels, row0, panel * 64);
     const int64_t plane = (int64_t)m.panels * m.mp * 64;
@@ -310,12 +315,12 @@ struct Params {
     const Entry* table;
     int     count, tiles, wide, stages;
     int     span;        // columns of the second operand that a copy brings
-    int     from, step;  // from: which X it starts from
+    int     from, step;  // from: which operands of X are read
     __half* work;
     int*    failed;      // a wait ran out
     float   product;     // factor of the finished sums
     float   old;         // kSquare: of A; kApply: a
-    float   scale;       // kSquare: of B; kApply: of the operands
+    float   scale;       // kSquare: of the identity; kApply: of the next operands
     Rates   rates;       // kLast
 };
 
@@ -484,9 +489,17 @@ __global__ void __launch_bounds__(256) k_muon_check(const Entry* __restrict__ ta
     }
 }
 
-// Tiles of 128 rows by up to 256 columns.  kGram: A = X X^T; kSquare: b A + c A A; of both the tiles on and above the diagonal,
-// what lies above it is written to both places.  kApply: a X + B X.  kLast: likewise, and the parameters' update.
-// CG: CTAs per tile (2: of 256 rows, each CTA with 128 of them and half of the second operand).
+// A product of all matrices of a chain, as tiles of 128 rows (CG 2: of 256, on a pair of CTAs, each with 128 of them and half of the
+// second operand) by up to 256 columns, dealt out in turn to CTAs that stay.
+//   kGram    A = X X^T       of both the tiles on and above the diagonal; what lies above it is written to both places
+//   kSquare  b A + c A A - t
+//   kApply   (a + t) X + B X; kLast: likewise, and the parameters' update
+// One warp asks for copies, one for products, eight finish tiles, a row a lane, while the next is multiplied.  What bounds it: products
+// and their feeding where m is 2048 (4 x 2048 x 8192 bf16, in us of which products at 1.69 PFLOP/s: A 124 of 85, B 43 of 21, X 232 of
+// 163; power lowers the clock in long runs), X in 32 bits and its latency where m is 512 (16 x 512 x 2048 bf16: A 25, B 17, X 44 of
+// 31 at the copy's rate).  Tried and not kept: all products in one cooperative launch in which a tile waits for its matrix's tiles
+// alone (3.9 us for a product of the smallest either way; 4 x 2048 x 8192 10 % slower: two stages of the ring went to the update),
+// X and results by the copy engine (its queue holds them up; the ring lost three stages: X 249), X brought to the second cache ahead.
 template <int KIND, int PARTS, int CG>
 __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
     constexpr bool kApplies = KIND == kApply || KIND == kLast;
@@ -690,8 +703,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
             const int64_t s_plane = (int64_t)m.mp * m.mp, x_plane = (int64_t)m.panels * m.mp * 64;
             const float shift = KIND == kGram ? 0.f : m.shift[p.step], old = kApplies ? p.old + shift : p.old;
             const int64_t at0 = kApplies ? place(m.mp, row, col0) : 0;
-            const float* const x_from = p.from ? m.x[1] : m.x[0];
-            float* const       x_to   = p.from ? m.x[0] : m.x[1];
             const int          target = KIND == kGram ? m.gram : KIND == kSquare ? m.factor : p.from ? m.operand[0] : m.operand[1];
             using X = std::conditional_t<PARTS == 2, float, __nv_bfloat16>;
             // (f32: the sums need the registers; half of the parameters at a time)
@@ -700,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
             const bool grains = KIND == kLast && by_grains<X>(m), early = grains && m.momentum && !kSegments;
             auto load_x = [&](int c, float4 (&x)[8]) {  // 32 columns of X
                 if (col0 + c >= limit) return;
-                const float4* const from = reinterpret_cast<const float4*>(x_from + at0 + (int64_t)(c / 32) * m.mp * 32);
+                const float4* const from = reinterpret_cast<const float4*>(m.x + at0 + (int64_t)(c / 32) * m.mp * 32);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = from[j * 32];
             };
@@ -720,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                     return;
                 }
                 if (KIND == kApply) {
-                    float4* const to = reinterpret_cast<float4*>(x_to + at0 + (int64_t)(c / 32) * m.mp * 32);
+                    float4* const to = reinterpret_cast<float4*>(m.x + at0 + (int64_t)(c / 32) * m.mp * 32);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) to[j * 32] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
                 } else if (row / 128 > col / 128) {
@@ -875,11 +886,11 @@ struct SmallSteps {
     SmallStep step[kMostSteps];
 };
 
-// A has two parts here for bf16 as well: with one, b A and c A A disagree about what A is, and results are off by up to 1.9 times their
-// own rounding (2 x 27; 1.24 times with two).
 // All steps of a matrix of at most 128 x 256 in one CTA, and its update: nothing but the gradient, the momentum and the parameter
 // crosses memory.  A row of X by four threads, 64 columns each (one unit's row), 32 columns of A and B.  What bounds it is latency:
-// three products a step, each behind a barrier, and what turns its sums into the next operands; SMALLUS.
+// three products a step, each behind a barrier, and what turns its sums into the next operands: 64 x 256 bf16 14 us and 5.6 a step, f32 14 and
+// 9.6 (a chain of launches: 80 and 136 for five steps, and 17 launches of the host's time).
+// A has two parts for bf16 as well: with one, results of few rows are off by up to 1.9 times their own rounding (2 x 27; 1.2 times with two).
 template <typename X>
 __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_constant__ SmallSlots s, const Rates r, const __grid_constant__ SmallSteps steps) {
     constexpr int PARTS = sizeof(X) == 4 ? 2 : 1;
@@ -1201,7 +1212,7 @@ Chain chain_of(const Matrix* matrices, int64_t count, int parts, int steps, void
         e.partial = w.take<double>(e.chunks);
         e.shift   = w.take<float>(steps);
         const int64_t values = (int64_t)e.panels * e.mp * 64;
-        for (int j = 0; j < 2; ++j) e.x[j] = w.take<float>(values);
+        e.x = w.take<float>(values);
         auto units = [&](int* at, int64_t halves) {
             w.used = (size_t)up((int64_t)w.used, kUnit * 2);
             *at = (int)(w.used / (kUnit * 2));
@@ -1214,14 +1225,14 @@ Chain chain_of(const Matrix* matrices, int64_t count, int parts, int steps, void
     return c;
 }
 
-// How many of the matrices, from the first on, go together: as many as some hundred megabytes hold.
-constexpr size_t kChainBytes = (size_t)1 << 30;
+// How many of the matrices, from the first on, go together: as many as two gigabytes hold.
+constexpr size_t kChainBytes = (size_t)2 << 30;
 int64_t together(const Matrix* matrices, int64_t count, int parts) {
     size_t bytes = 0;
     int64_t i = 0;
     for (; i < count && i < kMostMatrices; ++i) {
         const int64_t m = std::min(matrices[i].rows, matrices[i].cols), n = std::max(matrices[i].rows, matrices[i].cols);
-        const size_t more = (size_t)up(m, 256) * ((size_t)up(n, 128) * (8 + 4 * parts) + (size_t)up(m, 256) * 4 * parts);
+        const size_t more = (size_t)up(m, 256) * ((size_t)up(n, 128) * (4 + 4 * parts) + (size_t)up(m, 256) * 4 * parts);
         if (i > 0 && bytes + more > kChainBytes) break;
         bytes += more;
     }
@@ -1444,16 +1455,18 @@ int batch_list(int64_t count, int64_t rows, int64_t cols, int dtype, const void*
 
 extern "C" {
 
-size_t framewise_b200_muon_bytes(const framewise_b200_matrix* matrices, int64_t count, int32_t dtype) {
+size_t framewise_b200_muon_bytes(const framewise_b200_matrix* matrices, int64_t count, int32_t dtype) try {
     std::vector<SmallSlot> small;
     std::vector<Matrix>    list;
     if (!dtype_ok(dtype) || muon_list(matrices, count, 0.0, 0, &small, &list) != FRAMEWISE_B200_OK) return 0;
     return bytes_for(list, dtype == FRAMEWISE_B200_F32 ? 2 : 1);
+} catch (...) {  // no memory for the lists
+    return 0;
 }
 
 int framewise_b200_muon(const framewise_b200_matrix* matrices, int64_t count, int32_t dtype, double lr, double beta, int32_t nesterov,
                         double weight_decay, int32_t match_rms, const double* coefficients, int32_t steps, double eps, int32_t follow,
-                        void* work, size_t work_bytes, framewise_b200_stream_t stream) {
+                        void* work, size_t work_bytes, framewise_b200_stream_t stream) try {
     std::vector<SmallSlot> small;
     std::vector<Matrix>    list;
     if (!dtype_ok(dtype) || !(eps > 0)) return FRAMEWISE_B200_BAD_ARGUMENT;
@@ -1462,9 +1475,11 @@ int framewise_b200_muon(const framewise_b200_matrix* matrices, int64_t count, in
     if (std::any_of(list.begin(), list.end(), bad) || std::any_of(small.begin(), small.end(), bad)) return FRAMEWISE_B200_BAD_ARGUMENT;
     const Rates rates = {(float)(1 - beta), (float)beta, nesterov ? 1.f : 0.f, (float)eps, (float)(1 - lr * weight_decay), follow};
     return run(small, list, dtype, rates, coefficients, steps, work, work_bytes, stream);
+} catch (...) {
+    return FRAMEWISE_B200_BAD_ARGUMENT;
 }
 
-size_t framewise_b200_orthogonalize_bytes(int64_t count, int64_t rows, int64_t cols, int32_t dtype) {
+size_t framewise_b200_orthogonalize_bytes(int64_t count, int64_t rows, int64_t cols, int32_t dtype) try {
     if (!dtype_ok(dtype) || count < 0 || rows < 0 || cols < 0) return 0;
     if (count == 0 || rows == 0 || cols == 0) return 256;
     std::vector<SmallSlot> small;
@@ -1472,10 +1487,12 @@ size_t framewise_b200_orthogonalize_bytes(int64_t count, int64_t rows, int64_t c
     // more than a chain's go through the same scratch
     if (batch_list(std::min<int64_t>(count, kMostMatrices), rows, cols, dtype, nullptr, nullptr, &small, &list) != FRAMEWISE_B200_OK) return 0;
     return bytes_for(list, dtype == FRAMEWISE_B200_F32 ? 2 : 1);
+} catch (...) {
+    return 0;
 }
 
 int framewise_b200_orthogonalize(int64_t count, int64_t rows, int64_t cols, int32_t dtype, const void* x, void* out, const double* coefficients,
-                                 int32_t steps, double eps, void* work, size_t work_bytes, framewise_b200_stream_t stream) {
+                                 int32_t steps, double eps, void* work, size_t work_bytes, framewise_b200_stream_t stream) try {
     if (!dtype_ok(dtype) || count < 0 || rows < 0 || cols < 0 || !(eps > 0)) return FRAMEWISE_B200_BAD_ARGUMENT;
     if (count == 0 || rows == 0 || cols == 0) return FRAMEWISE_B200_OK;
     if (!x || !out) return FRAMEWISE_B200_BAD_ARGUMENT;
@@ -1484,6 +1501,8 @@ int framewise_b200_orthogonalize(int64_t count, int64_t rows, int64_t cols, int3
     FW_DO(batch_list(count, rows, cols, dtype, x, out, &small, &list));
     const Rates rates = {0.f, 0.f, 0.f, (float)eps, 1.f, 0};
     return run(small, list, dtype, rates, coefficients, steps, work, work_bytes, stream);
+} catch (...) {
+    return FRAMEWISE_B200_BAD_ARGUMENT;
 }
 
 }  // extern "C"

@@ -290,9 +290,13 @@ COEFFICIENTS: Triple = (3.4445, -4.7750, 2.0315)
 
 def _flat(coefficients: Union[Triple, Sequence[Triple]], steps: int) -> List[float]:
     """Three numbers per step, from those of one step or of all."""
-    rows = [tuple(c) for c in coefficients] if isinstance(coefficients[0], (tuple, list)) else [tuple(coefficients)] * int(steps)
+    try:
+        given = list(coefficients)
+        rows = [tuple(c) for c in given] if given and isinstance(given[0], (tuple, list)) else [tuple(float(c) for c in given)] * int(steps)
+    except TypeError:
+        rows = []
     if len(rows) != steps or any(len(r) != 3 for r in rows):
-        raise RuntimeError("coefficients must be three numbers, or three for each of the steps")
+        raise RuntimeError("steps must be in 1..100, and coefficients three numbers, or three for each of the steps")
     return [float(c) for r in rows for c in r]
 
 

@@ -168,10 +168,37 @@ def test_strides(fw, cuda):
     wide[..., 1:] = x
     assert torch.equal(fw.orthogonalize(wide[..., 1:]), want)
     check(fw.orthogonalize(x.mT), with_bound(x.mT))
-    for cut in (1, 2, 3):  # values that begin anywhere
-        flat = torch.zeros(x.numel() + cut, device=cuda)
-        flat[cut:] = x.reshape(-1)
-        assert torch.equal(fw.orthogonalize(flat[cut:].view(x.shape)), want)
+    for shape in ((3, 60, 80), (2, 140, 272), (2, 272, 140)):
+        for dtype in TYPES:
+            x = matrices(cuda, shape, dtype, seed=15)
+            want = fw.orthogonalize(x)
+            for cut in (1, 2, 3, 4):  # values that begin anywhere
+                flat = torch.zeros(x.numel() + cut, device=cuda, dtype=dtype)
+                flat[cut:] = x.reshape(-1)
+                assert torch.equal(fw.orthogonalize(flat[cut:].view(x.shape)), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(48, 96), (136, 264), (264, 136), (130, 257)])
+def test_parameters_that_begin_anywhere(fw, cuda, dtype, shape):
+    """Parameters, gradients, momentum and copies at any multiple of their type's size: the same bits."""
+    n = shape[0] * shape[1]
+
+    def cut(x, by):
+        flat = torch.empty(n + by, device=cuda, dtype=x.dtype)
+        flat[by:] = x.reshape(-1)
+        return flat[by:].view(shape)
+
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    p, g, v = torch.randn(shape, device=cuda, generator=gen).to(dtype), matrices(cuda, shape, dtype, seed=1), matrices(cuda, shape, seed=2)
+    m = None if dtype == torch.float32 else [p.float()]
+    first = [p.clone()], [v.clone()], None if m is None else [m[0].clone()]
+    fw.muon_step(first[0], [g], first[1], lr=0.1, master=first[2])
+    for by in ((1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (0, 0, 0, 1), (3, 2, 1, 5), (8, 4, 4, 4)):
+        again = [cut(p, by[0])], [cut(v, by[2])], None if m is None else [cut(m[0], by[3])]
+        fw.muon_step(again[0], [cut(g, by[1])], again[1], lr=0.1, master=again[2])
+        assert torch.equal(again[0][0], first[0][0]) and torch.equal(again[1][0], first[1][0])
+        assert m is None or torch.equal(again[2][0], first[2][0])
 
 
 def reference_step(p, g, v, lr, beta, nesterov, decay, match, dtype, steps=5):
@@ -188,13 +215,14 @@ def reference_step(p, g, v, lr, beta, nesterov, decay, match, dtype, steps=5):
     return (new, dv), (out, lr * s * 2 * (each + (want - exact).abs()) + 4 * U * (p.abs() + lr * s * exact.abs()))
 
 
-SHAPES = [(64, 64), (40, 200), (200, 40), (1, 9), (300, 129), (128, 256)]
+# up to 128 x 256 a CTA each, the others together; rows that begin at multiples of 16 bytes and elsewhere
+SHAPES = [(64, 64), (40, 200), (200, 41), (1, 9), (300, 129), (128, 256), (256, 520), (520, 136), (131, 262)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("nesterov,match", [(True, False), (False, True)])
 def test_step(fw, cuda, dtype, nesterov, match):
-    shapes = SHAPES * 5  # more than the arguments of a launch hold
+    shapes = SHAPES * 7  # more than the arguments of a launch hold, of either kind
     gen = torch.Generator(device="cuda").manual_seed(5)
     p = [torch.randn(s, device=cuda, generator=gen).to(dtype) for s in shapes]
     g = [matrices(cuda, s, dtype, seed=i) for i, s in enumerate(shapes)]
@@ -209,9 +237,9 @@ def test_step(fw, cuda, dtype, nesterov, match):
         close(p[i], (out, dout + r * out.abs()), f"parameter {i}")
 
 
-def test_copies(fw, cuda):
+@pytest.mark.parametrize("shapes", [SHAPES[:3], SHAPES[4:5], SHAPES[6:]])
+def test_copies(fw, cuda, shapes):
     """With a copy in 32 bits the parameter is its rounded value; with ``follow`` a change of the parameter is taken over."""
-    shapes = SHAPES[:3]
     gen = torch.Generator(device="cuda").manual_seed(5)
     master = [torch.randn(s, device=cuda, generator=gen) for s in shapes]
     p = [x.bfloat16() for x in master]
@@ -243,7 +271,7 @@ def test_a_zero_gradient_leaves_the_decay(fw, cuda):
 @pytest.mark.parametrize("dtype", TYPES)
 def test_optimizer(fw, cuda, dtype):
     gen = torch.Generator(device="cuda").manual_seed(0)
-    params = [torch.nn.Parameter(torch.randn(s, device=cuda, generator=gen).to(dtype)) for s in SHAPES[:4]]
+    params = [torch.nn.Parameter(torch.randn(s, device=cuda, generator=gen).to(dtype)) for s in SHAPES[2:7]]
     plain = [x.detach().clone() for x in params]
     momentum = [torch.zeros(x.shape, device=cuda) for x in plain]
     master = None if dtype == torch.float32 else [x.float() for x in plain]
@@ -340,6 +368,7 @@ def test_refusals(fw, cuda):
         (lambda: step([y], [g], [v], master=[v]), "no copies"),
         (lambda: step([y, y.bfloat16()], [g, g.bfloat16()], [v, v]), "share"),
         (lambda: step([y], [g.cpu()], [v]), "gradient"),
+        (lambda: step([y, y], [g, g], [v, v.clone()]), "twice"),
     ]
     for f, what in bad:
         with pytest.raises(RuntimeError, match=what):
