@@ -359,6 +359,8 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(X) == 4 && !TOP ? 4 : 3) k
         }
 #pragma unroll
         for (int j = 16; j > 0; j >>= 1) a = joined(a, {__shfl_xor_sync(0xffffffffu, a.m, j), __shfl_xor_sync(0xffffffffu, a.s, j), __shfl_xor_sync(0xffffffffu, a.t, j)});
+        // the lanes' sums may differ in their last bit: all go by the first's, so that equal logits have equal results
+        a = {__shfl_sync(0xffffffffu, a.m, 0), __shfl_sync(0xffffffffu, a.s, 0), __shfl_sync(0xffffffffu, a.t, 0)};
     }
     // the team's parts, pairs of warps at a time
     if (r.team > 1) {

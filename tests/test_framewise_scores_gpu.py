@@ -102,6 +102,11 @@ def check(fw, logits, labels, lens, top, grads=None):
     for name in ("log_probs", "entropy", "top_log_probs"):
         close(getattr(got, name).detach(), want[name], name)
     assert got.top_labels.dtype == labels.dtype and torch.equal(got.top_labels.long(), want["top_labels"])
+    # falling order to the last bit; equal logits have equal log probabilities, the label's among them
+    best = got.top_log_probs.detach()
+    assert bool((best[..., :-1] >= best[..., 1:]).all())
+    same = (want["top_labels"] == labels[..., None]) & kept(labels, lens, IGNORE)[..., None]
+    assert torch.equal(best[same], got.log_probs.detach()[..., None].expand_as(best)[same])
     close(z.grad, want["logits"], "logits")
     with torch.no_grad():
         again = fw.label_scores(logits, labels, top=top, seq_lens=lens, ignore_index=IGNORE)
@@ -352,3 +357,25 @@ def test_refusals(fw, cuda):
         dual = fa.make_dual(z.detach(), torch.ones_like(z))
         with pytest.raises(RuntimeError, match="forward-mode"):
             fw.label_scores(dual, t)
+
+
+def test_offsets_past_32_bits(fw, cuda):
+    """More than 2^31 logits, of which a few rows count: first and last ones."""
+    V, N = 12001, 180000
+    z = torch.zeros(1, N, V, device=cuda, dtype=torch.bfloat16)
+    t = torch.full((1, N), IGNORE, device=cuda, dtype=torch.int32)
+    at = torch.tensor([0, 1, N // 2, N - 2, N - 1], device=cuda)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    z[0, at] = (torch.randn(5, V, device=cuda, generator=gen) * 3).bfloat16()
+    t[0, at] = torch.randint(0, V, (5,), device=cuda, generator=gen, dtype=torch.int32)
+    zz = z.requires_grad_()
+    got = fw.label_scores(zz, t, top=3)
+    torch.autograd.backward([got.log_probs, got.entropy], [torch.ones(1, N, device=cuda), torch.ones(1, N, device=cuda)])
+    g = [torch.ones(1, 5, device=cuda), torch.ones(1, 5, device=cuda), None]
+    want = reference(z.detach()[:, at], t[:, at], None, 3, g)
+    for name in ("log_probs", "entropy", "top_log_probs"):
+        close(getattr(got, name).detach()[:, at], want[name], name)
+    assert torch.equal(got.top_labels[:, at].long(), want["top_labels"])
+    close(zz.grad[:, at], want["logits"], "logits")
+    zz.grad[:, at] = 0
+    assert float(zz.grad.abs().amax()) == 0.0
