@@ -227,45 +227,43 @@ __global__ void __launch_bounds__(256) k_muon_collect(const __grid_constant__ Sl
     }
 }
 
-// X = U / max(|U|, eps) in 32 bits and as operands: a CTA per 64 columns and rows, zeros where there are none.
+// X = U / max(|U|, eps) in 32 bits and as operands, zeros where there are none: a CTA takes kBlocks squares of 64 columns and rows, the
+// next of which is loaded while one is written.  (A square each: 204 us for 4 x 2048 x 8192 bf16, 184 with four;
+// its bytes at the copy's rate 123.)
+constexpr int kBlocks = 4;
 template <typename X, int PARTS>
-__global__ void __launch_bounds__(256) k_muon_begin(const Entry* __restrict__ table, int count, const Rates r, float scale, __half* work, const __grid_constant__ Steps steps) {
+__global__ void __launch_bounds__(256, 5) k_muon_begin(const Entry* __restrict__ table, int count, const Rates r, float scale, __half* work, const __grid_constant__ Steps steps) {
     __shared__ double part[8];
     __shared__ float  tile[64][65];
     next_may_start();
     former_is_done();
     const int   e = find(count, blockIdx.x, [&](int i) { return table[i].first_block; });
     const Entry& m = table[e];
-    const int block = blockIdx.x - m.first_block, panel = block / (m.mp / 64), row0 = block % (m.mp / 64) * 64;
+    const int first = (blockIdx.x - m.first_block) * kBlocks, high = m.mp / 64, blocks = min(kBlocks, m.panels * high - first);
     const X* const     g = static_cast<const X*>(m.grad);
     const float* const v = m.momentum;
-    const bool tall = m.rows > m.cols;
-    // neighbours in memory first: `line` of U as it lies, four values from `at` on
-    const int  lines = tall ? m.n : m.m, line0 = tall ? panel * 64 : row0, col0 = tall ? row0 : panel * 64;
-    const bool wide = aligned4(g, v) && m.cols % 4 == 0;
+    const bool tall = m.rows > m.cols, wide = aligned4(g, v) && m.cols % 4 == 0;
+    const int  lines = tall ? m.n : m.m, at = threadIdx.x % 16 * 4, l0 = threadIdx.x / 16;
+    // neighbours in memory first: lines of U as it lies, four values from `at` on
     float u[4][4], mom[4][4];
-    const int at = threadIdx.x % 16 * 4, l0 = threadIdx.x / 16, left = m.cols - col0 - at;
+    auto load = [&](int block) {
+        const int panel = block / high, row0 = block % high * 64;
+        const int line0 = tall ? panel * 64 : row0, col0 = tall ? row0 : panel * 64, left = m.cols - col0 - at;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int line = line0 + l0 + i * 16;
-        const bool some = line < lines && left > 0;
-        const int64_t from = some ? (int64_t)line * m.cols + col0 + at : 0;
-        load4(g + from, some && wide, some ? left : 0, u[i]);
-        if (v) load4(v + from, some && wide, some ? left : 0, mom[i]);
-    }
+        for (int i = 0; i < 4; ++i) {
+            const int line = line0 + l0 + i * 16;
+            const bool some = line < lines && left > 0;
+            const int64_t from = some ? (int64_t)line * m.cols + col0 + at : 0;
+            load4(g + from, some && wide, some ? left : 0, u[i]);
+            if (v) load4(v + from, some && wide, some ? left : 0, mom[i]);
+        }
+    };
+    load(first);
     double sum = 0.0;
     for (int i = threadIdx.x; i < m.chunks; i += 256) sum += m.partial[i];
 #pragma unroll
     for (int j = 16; j > 0; j >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, j);
     if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = sum;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float x = v ? direction(u[i][j], mom[i][j], r) : u[i][j];
-            if (tall) tile[at + j][l0 + i * 16] = x;
-            else tile[l0 + i * 16][at + j] = x;
-        }
     __syncthreads();
     sum = part[0];
     for (int i = 1; i < 8; ++i) sum += part[i];
@@ -273,7 +271,7 @@ __global__ void __launch_bounds__(256) k_muon_begin(const Entry* __restrict__ ta
     const double by = 1.0 / fmax(sqrt(sum), (double)r.eps);
     const bool   far = !(by < 1e30);
     const float  by32 = (float)by;
-    if (block == 0 && threadIdx.x == 0) {
+    if (first == 0 && threadIdx.x == 0) {
         float one = (float)(fmin(1.0, sqrt(sum) * by) * rsqrt((double)m.m));  // all singular values, if they are equal
         for (int i = 0; i < steps.count; ++i) {
             const float square = one * one, t = square * (steps.abc[3 * i + 1] + steps.abc[3 * i + 2] * square);
@@ -281,29 +279,39 @@ __global__ void __launch_bounds__(256) k_muon_begin(const Entry* __restrict__ ta
             one *= steps.abc[3 * i] + t;
         }
     }
-    auto x_of = [&](int row, int col) {
-        const float x = tile[row][col];
-        return far ? (float)(x * by) : x * by32;
-    };
+    for (int b = 0; b < blocks; ++b) {
+        if (b > 0) __syncthreads();  // the square before has been read
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {  // a warp: 32 rows of four columns, 512 bytes of X
-        const int row = (threadIdx.x / 32 & 1) * 32 + threadIdx.x % 32, col = (threadIdx.x / 64 + i * 4) * 4;
-        *reinterpret_cast<float4*>(m.x + place(m.mp, row0 + row, panel * 64 + col)) = make_float4(x_of(row, col), x_of(row, col + 1), x_of(row, col + 2), x_of(row, col + 3));
-    }
-    __half* const op = work + (int64_t)m.operand[0] * kUnit + in_units(m.panels, row0, panel * 64);
-    const int64_t plane = (int64_t)m.panels * m.mp * 64;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {  // a row's 128 bytes by eight lanes
-        const int row = threadIdx.x / 8 + i * 32, col = threadIdx.x % 8 * 8;
-        uint32_t w[PARTS][4];
+            for (int j = 0; j < 4; ++j) {
+                const float d = v ? direction(u[i][j], mom[i][j], r) : u[i][j], x = far ? (float)(d * by) : d * by32;
+                if (tall) tile[at + j][l0 + i * 16] = x;
+                else tile[l0 + i * 16][at + j] = x;
+            }
+        __syncthreads();
+        if (b + 1 < blocks) load(first + b + 1);
+        const int panel = (first + b) / high, row0 = (first + b) % high * 64;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float2 x = make_float2(x_of(row, col + 2 * j) * scale, x_of(row, col + 2 * j + 1) * scale);
-#pragma unroll
-            for (int q = 0; q < PARTS; ++q) w[q][j] = part_of(x);
+        for (int i = 0; i < 4; ++i) {  // a warp: 32 rows of four columns, 512 bytes of X
+            const int row = (threadIdx.x / 32 & 1) * 32 + threadIdx.x % 32, col = (threadIdx.x / 64 + i * 4) * 4;
+            *reinterpret_cast<float4*>(m.x + place(m.mp, row0 + row, panel * 64 + col)) = make_float4(tile[row][col], tile[row][col + 1], tile[row][col + 2], tile[row][col + 3]);
         }
+        __half* const op = work + (int64_t)m.operand[0] * kUnit + in_units(m.panels, row0, panel * 64);
+        const int64_t plane = (int64_t)m.panels * m.mp * 64;
 #pragma unroll
-        for (int q = 0; q < PARTS; ++q) *reinterpret_cast<uint4*>(op + q * plane + row * 64 + col) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
+        for (int i = 0; i < 2; ++i) {  // a row's 128 bytes by eight lanes
+            const int row = threadIdx.x / 8 + i * 32, col = threadIdx.x % 8 * 8;
+            uint32_t w[PARTS][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float2 x = make_float2(tile[row][col + 2 * j] * scale, tile[row][col + 2 * j + 1] * scale);
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q) w[q][j] = part_of(x);
+            }
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) *reinterpret_cast<uint4*>(op + q * plane + row * 64 + col) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
+        }
     }
 }
 
@@ -1036,8 +1044,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_co
         fence_after();
     };
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
-    // f32: A A, whose errors show most (see segment_of), has as many accumulators as there is room for: 64 x 256 is off by 1.1e-6 of its norm, with
-    // one by 2.4e-6 (plain 32 bits: 1.4e-6)
+    // f32: an accumulator for 64 of K, and for A A, whose errors show most (see segment_of), as many as there is room for: 64 x 256 is off
+    // by 1.1e-6 of its norm, with one accumulator each by 2.4e-6 (plain 32 bits: 1.4e-6)
     const int depth_x = units, depth_s = (small + 63) / 64, each = PARTS == 2 ? 4 / depth_s : 0;
     put_x(steps.step[0].operand);
     for (int i = 0; i < steps.count; ++i) {
@@ -1208,7 +1216,7 @@ Chain chain_of(const Matrix* matrices, int64_t count, int parts, int steps, void
         e.mp = (int)up(e.m, c.pairs ? 256 : 128), e.panels = (int)(up(e.n, c.pairs ? 128 : 64) / 64);
         e.chunks = (int)((m.rows * m.cols + kChunk - 1) / kChunk);
         e.first_chunk = (int)c.chunks, e.first_block = (int)c.blocks;
-        c.chunks += e.chunks, c.blocks += (int64_t)e.panels * (e.mp / 64);
+        c.chunks += e.chunks, c.blocks += ((int64_t)e.panels * (e.mp / 64) + kBlocks - 1) / kBlocks;
         e.partial = w.take<double>(e.chunks);
         e.shift   = w.take<float>(steps);
         const int64_t values = (int64_t)e.panels * e.mp * 64;
