@@ -1014,8 +1014,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_co
     uint32_t phase = 0;
     bool     ok = true;
     // a product of the operands that all threads have written, by one of them; the others wait for it
-    // each: accumulators for 64 of K, 128 columns apart (0: one for all)
-    auto multiply = [&](auto parts, int each, uint32_t d, uint32_t a, int a_part, uint32_t b, int b_part, uint32_t kind, int depth, bool b_mn) {
+    // each: accumulators for 64 of K, `apart` columns apart (0: one for all)
+    auto multiply = [&](auto parts, int each, int apart, uint32_t a, int a_part, uint32_t b, int b_part, uint32_t kind, int depth, bool b_mn) {
         fence_before();
         async_fence();
         __syncthreads();
@@ -1026,7 +1026,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_co
                 for (int q = decltype(parts)::value == 2 ? 0 : 2; q < 3; ++q)  // of two parts: the small products first
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        product<1>(tmem + d + (k * each + i * each / 4) * 128, operand(a + (q == 0 ? a_part : 0) + k * kUnit * 2 + i * 32, 8192),
+                        product<1>(tmem + (k * each + i * each / 4) * apart, operand(a + (q == 0 ? a_part : 0) + k * kUnit * 2 + i * 32, 8192),
                                    operand(b + (q == 1 ? b_part : 0) + (b_mn ? (k * 4 + i) * 2048 : k * kUnit * 2 + i * 32), kUnit * 2), kind,
                                    q > (decltype(parts)::value == 2 ? 0 : 2) || (each > 0 ? i * each % 4 != 0 : k > 0 || i > 0));
             products_commit<1>(bar);
@@ -1055,35 +1055,35 @@ __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_co
         float2 pairs[16];
         float* const sums = reinterpret_cast<float*>(pairs);
         float a[32];
-        auto add_up = [&](int count, int col) {  // 32 columns
+        auto add_up = [&](int count, int apart, int col) {  // 32 columns
             tmem_load32(tmem + lanes + col, pairs);
             tmem_loaded(pairs);
             for (int k = 1; k < count; ++k) {
                 float2 more[16];
-                tmem_load32(tmem + lanes + k * 128 + col, more);
+                tmem_load32(tmem + lanes + k * apart + col, more);
                 tmem_loaded(more);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) pairs[j] = add2(pairs[j], more[j]);
             }
         };
-        multiply(of_type, 0, 0, x_at, kXPart, x_at, kXPart, half_kind(128, 128, false), depth_x, false);  // A = X X^T
-        add_up(1, group * 32);
+        multiply(of_type, PARTS - 1, 128, x_at, kXPart, x_at, kXPart, half_kind(128, 128, false), depth_x, false);  // A = X X^T
+        add_up(PARTS == 2 ? depth_x : 1, 128, group * 32);
 #pragma unroll
         for (int j = 0; j < 32; ++j) a[j] = sums[j] * f.gram;
 #pragma unroll
         for (int j = 0; j < 4; ++j) put8(both, s_at + group / 2 * kUnit * 2, kSPart, group % 2 * 4 + j, a + 8 * j, 1.f, true);  // b A and c A A agree about A
-        multiply(both, each, 0, s_at, kSPart, s_at, kSPart, half_kind(128, 128, false), depth_s, false);  // B = b A + c A A - t
-        add_up(max(1, each * depth_s), group * 32);
+        multiply(both, each, 128, s_at, kSPart, s_at, kSPart, half_kind(128, 128, false), depth_s, false);  // B = b A + c A A - t
+        add_up(max(1, each * depth_s), 128, group * 32);
         const int hit = row - group * 32;
 #pragma unroll
         for (int j = 0; j < 32; ++j) a[j] = fmaf(f.of_gram, a[j], sums[j] * f.square) - (j == hit ? shift * f.of_one : 0.f);
 #pragma unroll
         for (int j = 0; j < 4; ++j) put8(of_type, s_at + group / 2 * kUnit * 2, kSPart, group % 2 * 4 + j, a + 8 * j, 1.f);
-        multiply(of_type, 0, 256, s_at, kSPart, x_at, kXPart, half_kind(128, units * 64, true), depth_s, true);  // (a + t) X + B X
+        multiply(of_type, PARTS - 1, 256, s_at, kSPart, x_at, kXPart, half_kind(128, units * 64, true), depth_s, true);  // (a + t) X + B X
         if (group < units) {
 #pragma unroll
             for (int c = 0; c < 64; c += 32) {
-                add_up(1, 256 + group * 64 + c);
+                add_up(PARTS == 2 ? depth_s : 1, 256, group * 64 + c);
 #pragma unroll
                 for (int j = 0; j < 32; ++j) x[c + j] = fmaf(f.a + shift, x[c + j], sums[j] * f.apply);
             }
