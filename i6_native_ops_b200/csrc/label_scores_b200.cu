@@ -25,8 +25,8 @@ using namespace tensor_core;
 constexpr int   kMostTop  = 32;      // alternatives: one per lane
 constexpr int   kWarps    = 8;       // per CTA
 constexpr int   kMostTeam = 64;      // warps that share a row: up to 8 CTAs
-constexpr int   kAhead    = 4;       // vectors of 8 logits that a lane has under way: a block
-constexpr int   kCells    = 16;      // blocks between looks for the best
+constexpr int   kCell     = 4;       // vectors of 8 logits that a lane has in a cell (see Best)
+constexpr int   kCells    = 16;      // cells of a lane between looks for the best
 constexpr int   kFew      = 8;       // alternatives that the lanes' largest cells alone single out well
 constexpr float kLog2e    = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNever    = -200.f;  // of an exponent of 2: zero in 32 bits
@@ -77,6 +77,10 @@ struct Raw<float> {
                      : "l"(x));
     }
     __device__ __forceinline__ void set(int i, const float* x) { w[i] = x ? *x : -INFINITY; }
+    __device__ __forceinline__ void none() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = -INFINITY;
+    }
     __device__ __forceinline__ float get(int i) const { return w[i]; }
 };
 template <>
@@ -89,41 +93,86 @@ struct Raw<__nv_bfloat16> {
         const uint32_t v = x ? *reinterpret_cast<const uint16_t*>(x) : 0xff80u;  // -inf
         w[i / 2] = i % 2 ? (w[i / 2] & 0xffffu) | v << 16 : v;
     }
+    __device__ __forceinline__ void none() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = 0xff80ff80u;
+    }
     __device__ __forceinline__ float get(int i) const { return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); }
 };
+// The largest of kCell vectors' values.
+__device__ __forceinline__ float largest(const Raw<float>* v) {
+    float a = max_nan(v[0].get(0), v[0].get(1), v[0].get(2)), b = max_nan(v[0].get(3), v[0].get(4), v[0].get(5));
+    a = max_nan(a, v[0].get(6), v[0].get(7));
+#pragma unroll
+    for (int i = 1; i < kCell; ++i) {
+        a = max_nan(max_nan(a, v[i].get(0), v[i].get(1)), v[i].get(2), v[i].get(3));
+        b = max_nan(max_nan(b, v[i].get(4), v[i].get(5)), v[i].get(6), v[i].get(7));
+    }
+    return max_nan(a, b);
+}
+// (Of the unpacked values the compiler would keep 64 until the sums are formed, some of them in local memory.)
+__device__ __forceinline__ float largest(const Raw<__nv_bfloat16>* v) {
+    uint32_t a = v[0].w[0];
+#pragma unroll
+    for (int i = 0; i < kCell; ++i)
+#pragma unroll
+        for (int j = i == 0 ? 1 : 0; j < 4; ++j) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(v[i].w[j]));
+    return max_nan(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u));
+}
 __device__ __forceinline__ float value(float x) { return x; }
 __device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162float(x); }
 
+// A lane has 128 bytes under way: a block of so many vectors.  (bf16, 20000 x 12001: half of them with the next half loaded before
+// they are worked on 111 us, and the gradient 184; this 107 and 170.)
+template <typename X>
+constexpr int kAhead = 128 / (8 * (int)sizeof(X));
+
 // A row in vectors of 8, 32 of them a step.  The vectors' addresses are aligned: the first begins `ahead` places before the row.
-// Places outside of the row are not read and hold -inf, which changes no sum.
+// Those from `low` to `high` are inside of it.
 template <typename X>
 struct Row {
     const X* x;
-    int      V, ahead, steps;
+    int      V, ahead, low, high;
     __device__ Row(const X* x, int V) : x(x), V(V) {
         ahead = (int)(reinterpret_cast<uintptr_t>(x) / sizeof(X) % 8);
-        steps = ((V + ahead + 7) / 8 + 31) / 32;
+        low = ahead > 0, high = (V + ahead) / 8;
     }
     __device__ __forceinline__ int first(int step, int lane) const { return (step * 32 + lane) * 8 - ahead; }
-    // A block: kAhead steps, `team` apart.
+    // A block: kAhead<X> steps, `team` apart.
     __device__ __forceinline__ bool inside(int step, int team) const {
-        return step * 256 >= ahead && (step + (kAhead - 1) * team + 1) * 256 - ahead <= V;
+        return step * 32 >= low && (step + (kAhead<X> - 1) * team + 1) * 32 <= high;
     }
-    __device__ __forceinline__ void load(int step, int team, int lane, Raw<X> (&v)[kAhead], bool aligned = true) const {
-        if (aligned && inside(step, team)) {
-            const X* const from = x + first(step, lane);
+    __device__ __forceinline__ void load_inside(int step, int team, int lane, Raw<X> (&v)[kAhead<X>]) const {
+        const X* const from = x + first(step, lane);
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) v[i].load(from + (int64_t)i * team * 256);
-        } else {
+        for (int i = 0; i < kAhead<X>; ++i) v[i].load(from + (int64_t)i * team * 256);
+    }
+    // The vectors inside of the row; -inf, which changes no sum, in place of others.
+    __device__ __forceinline__ void load_whole(int step, int team, int lane, Raw<X> (&v)[kAhead<X>]) const {
+        if (inside(step, team)) return load_inside(step, team, lane, v);
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const int at = first(step + i * team, lane);
-                if (aligned && at >= 0 && at + 8 <= V) {
-                    v[i].load(x + at);
-                } else {
+        for (int i = 0; i < kAhead<X>; ++i) {
+            const int q = (step + i * team) * 32 + lane;
+            if (q >= low && q < high) v[i].load(x + q * 8 - ahead);
+            else v[i].none();
+        }
+    }
+    // Where in the row the value is that a lane takes of the two vectors that lie partly outside; -1: none.
+    __device__ __forceinline__ int edge(int lane) const {
+        if (lane < 8) return low && lane >= ahead && lane - ahead < V ? lane - ahead : -1;
+        return lane < 16 && !(low && high == 0) && high * 8 - ahead + lane - 8 < V ? high * 8 - ahead + lane - 8 : -1;
+    }
+    // All values inside of the row, one by one where they are not `aligned` or a vector is not whole.
+    __device__ __forceinline__ void load(int step, int team, int lane, Raw<X> (&v)[kAhead<X>], bool aligned) const {
+        if (aligned && inside(step, team)) return load_inside(step, team, lane, v);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[i].set(j, at + j >= 0 && at + j < V ? x + at + j : nullptr);
-                }
+        for (int i = 0; i < kAhead<X>; ++i) {
+            const int at = first(step + i * team, lane);
+            if (aligned && at >= 0 && at + 8 <= V) {
+                v[i].load(x + at);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i].set(j, at + j >= 0 && at + j < V ? x + at + j : nullptr);
             }
         }
     }
@@ -159,6 +208,10 @@ __device__ __forceinline__ uint64_t joined(uint64_t list, uint64_t more, int lan
     return list;
 }
 
+// One copy of the networks, and six cells at a time in Best::look, so that the instructions stay in their cache (20000 x 12001 f32
+// with 8 alternatives: a dozen copies 225 us, one 213, six cells instead of a dozen 198).
+__device__ __noinline__ uint64_t merged(uint64_t list, uint64_t key, int lane) { return joined(list, sorted(key, lane), lane); }
+
 struct Sums {  // of a part of a row: maximum, sum of 2^d, sum of 2^d d
     float m, s, t;
 };
@@ -193,10 +246,10 @@ struct Room {
     uint64_t wait[64];
 };
 
-// The best that a warp has met.  While the sums are formed only the maximum of each cell, the 32 values that a lane has of a
-// block, is written down.  After kCells blocks, or at the row's end, those cells are read again whose maximum is no smaller
+// The best that a warp has met.  While the sums are formed only the maximum of each cell, 32 values of a lane in kCell steps
+// that the team takes in turn, is written down.  After kCells of them, or at the row's end, those cells are read again whose maximum is no smaller
 // than the `top`-th largest of the lanes' maxima: some more than `top` of them.  (Looking at each value while the sums are formed,
-// against the list so far: 26 instructions a value for the whole kernel, 20000 x 12001 f32 with 8 alternatives 664 us; 219 this way,
+// against the list so far: 26 instructions a value for the whole kernel, 20000 x 12001 f32 with 8 alternatives 664 us; 198 this way,
 // and 148 without alternatives.)
 struct Best {
     uint64_t list;    // the 32 largest so far, a lane each, in falling order
@@ -210,7 +263,7 @@ struct Best {
         __syncwarp();
         const uint64_t key = lane < min(count, 32) ? room.wait[lane] : 0, rest = lane + 32 < count ? room.wait[lane + 32] : 0;
         __syncwarp();
-        list  = joined(list, sorted(key, lane), lane);
+        list  = merged(list, key, lane);
         count = max(0, count - 32);
         if (lane < count) room.wait[lane] = rest;
         const uint64_t last = __shfl_sync(0xffffffffu, list, top - 1);
@@ -219,7 +272,7 @@ struct Best {
         __syncwarp();
     }
     template <typename X>
-    __device__ void look(const Row<X>& row, int step, int team, int blocks, int lane) {  // the first block's first step
+    __device__ void look(const Row<X>& row, int step, int team, int blocks, int lane) {  // blocks: of cells, from `step` on
         __syncwarp();
         float most = -INFINITY, second = -INFINITY;
         for (int b = 0; b < blocks; ++b) {
@@ -252,31 +305,40 @@ struct Best {
         int   block = -1;
         bool  before = false;
         float floor = -INFINITY;
-        constexpr int kLoads = 12;
+        const int begin = row.low * 8 - row.ahead;  // the vectors inside of the row
+        const uint32_t span = max(0, row.high - row.low) * 8;
+        constexpr int kLoads = 6;  // cells
         for (int i = 0; i < cells; i += kLoads) {
             float v[kLoads];
+            int   at[kLoads];
 #pragma unroll
             for (int q = 0; q < kLoads; ++q) {
-                v[q] = -INFINITY;
+                v[q] = -INFINITY, at[q] = begin - 1;
                 if (i + q >= cells) continue;
-                const int cell = room.near[i + q], at = row.first(step + (cell / 32 * kAhead + lane / 8) * team, cell % 32) + lane % 8;
+                const int cell = room.near[i + q];
                 const float c = room.cell[cell / 32][cell % 32];
                 if (cell / 32 != block && full && (c <= least || least != least)) continue;  // has been overtaken
-                if (at >= 0 && at < row.V) v[q] = value(row.x[at]);
+                at[q] = row.first(step + (cell / 32 * kCell + lane / 8) * team, cell % 32) + lane % 8;
+                if ((uint32_t)(at[q] - begin) < span) v[q] = value(row.x[at[q]]);
             }
 #pragma unroll
             for (int q = 0; q < kLoads; ++q) {
                 if (i + q >= cells) break;
-                const int cell = room.near[i + q], at = row.first(step + (cell / 32 * kAhead + lane / 8) * team, cell % 32) + lane % 8;
+                const int cell = room.near[i + q];
                 if (cell / 32 != block) block = cell / 32, before = full, floor = least;
-                const bool in = at >= 0 && at < row.V && !(v[q] < from) && !(before && (v[q] <= floor || floor != floor)) && !(v[q] < least);
+                const bool in = (uint32_t)(at[q] - begin) < span && !(v[q] < from) && !(before && (v[q] <= floor || floor != floor)) && !(v[q] < least);
                 const uint32_t lanes = __ballot_sync(0xffffffffu, in);
-                if (in) room.wait[count + __popc(lanes & ((1u << lane) - 1))] = key_of(v[q], at);
+                if (in) room.wait[count + __popc(lanes & ((1u << lane) - 1))] = key_of(v[q], at[q]);
                 count += __popc(lanes);
                 if (count >= 32) sort_in(lane);
             }
         }
         while (count > 0) sort_in(lane);
+    }
+    // one more value a lane; index < 0: none
+    __device__ __forceinline__ void take(float v, int index, int lane) {
+        const bool in = index >= 0 && !(v < least);
+        if (__any_sync(0xffffffffu, in)) list = merged(list, in ? key_of(v, index) : 0, lane);
     }
 };
 
@@ -310,30 +372,31 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(X) == 4 && !TOP ? 4 : 3) k
     Best b(room[TOP ? warp : 0], r.top);
     if (counts) {
         const Row<X> row(x, r.V);
-        constexpr bool kEarly = sizeof(X) == 2;  // the next block is loaded before this one is worked on
-        Raw<X> v[kAhead], next[kEarly ? kAhead : 1];
-        const int hop = r.team * kAhead;
-        int blocks = 0, looked = member;
-        if (member < row.steps) row.load(member, r.team, lane, v);
-        for (int step = member; step < row.steps; step += hop) {
-            const bool more = step + hop < row.steps;
-            if constexpr (kEarly)
-                if (more) row.load(step + hop, r.team, lane, next);
-            float all = max_nan(v[0].get(0), v[0].get(1), v[0].get(2)), other = max_nan(v[0].get(3), v[0].get(4), v[0].get(5));
-            all = max_nan(all, v[0].get(6), v[0].get(7));
+        constexpr int A = kAhead<X>;
+        Raw<X> v[A];
+        const int hop = r.team * A, steps = (row.high + 31) / 32, edge = member == 0 ? row.edge(lane) : -1;
+        int cells = 0, looked = member;
+        if (member < steps) row.load_whole(member, r.team, lane, v);
+        const float at_edge = edge >= 0 ? value(x[edge]) : 0.f;
+        if (edge >= 0) {
+            a.m = max_nan(a.m, at_edge);
+            a.s = exp2_approx(max_nan((at_edge - a.m) * kLog2e, kNever));
+        }
+        for (int step = member; step < steps; step += hop) {
+            const bool more = step + hop < steps;
+            float all = -FLT_MAX;
 #pragma unroll
-            for (int i = 1; i < kAhead; ++i) {
-                all   = max_nan(max_nan(all, v[i].get(0), v[i].get(1)), v[i].get(2), v[i].get(3));
-                other = max_nan(max_nan(other, v[i].get(4), v[i].get(5)), v[i].get(6), v[i].get(7));
+            for (int c = 0; c < A; c += kCell) {
+                const float of = largest(v + c);
+                all = max_nan(all, of);
+                if (TOP) room[warp].cell[cells++][lane] = of;
             }
-            all = max_nan(all, other);
-            if (TOP) room[warp].cell[blocks][lane] = all;
             const float m = max_nan(a.m, all);
             rescale(a, m);
             const float2 off = make_float2(-m, -m), scale = make_float2(kLog2e, kLog2e);
             float2 s = make_float2(0.f, 0.f), t = s;
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i)
+            for (int i = 0; i < A; ++i)
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                     float2 d = mul2(add2(make_float2(v[i].get(j), v[i].get(j + 1)), off), scale);
@@ -344,19 +407,13 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(X) == 4 && !TOP ? 4 : 3) k
                 }
             a.s += s.x + s.y;
             a.t += t.x + t.y;
-            if (TOP && (++blocks == kCells || !more)) {
-                b.look(row, looked, r.team, blocks, lane);
-                blocks = 0, looked = step + hop;
+            if (TOP && (cells == kCells || !more)) {
+                b.look(row, looked, r.team, cells, lane);
+                cells = 0, looked = step + hop;
             }
-            if (more) {
-                if constexpr (kEarly) {
-#pragma unroll
-                    for (int i = 0; i < kAhead; ++i) v[i] = next[i];
-                } else {
-                    row.load(step + hop, r.team, lane, v);
-                }
-            }
+            if (more) row.load_whole(step + hop, r.team, lane, v);
         }
+        if (TOP) b.take(at_edge, edge, lane);
 #pragma unroll
         for (int j = 16; j > 0; j >>= 1) a = joined(a, {__shfl_xor_sync(0xffffffffu, a.m, j), __shfl_xor_sync(0xffffffffu, a.s, j), __shfl_xor_sync(0xffffffffu, a.t, j)});
         // the lanes' sums may differ in their last bit: all go by the first's, so that equal logits have equal results
@@ -443,6 +500,7 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(X) == 4 ? 4 : 3) k_label_s
     const int64_t seq = (uint32_t)n / (uint32_t)r.T, at_t = (uint32_t)n % (uint32_t)r.T;
     X* const to = dz + n * r.V;
     const Row<X> row(to, r.V);
+    const int steps = (row.high + ((r.V + row.ahead) % 8 > 0) + 31) / 32;
     int64_t label = 0;
     const bool   counts = counted<L>(r, n, label);
     const float4 kept   = counts ? in.kept[n] : make_float4(0.f, -INFINITY, 0.f, 0.f);
@@ -465,7 +523,7 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(X) == 4 ? 4 : 3) k_label_s
     if (kept.y == -INFINITY) {  // does not count, or no class is possible
         const float none = c0 != c0 ? c0 : 0.f;
         const float v[8] = {none, none, none, none, none, none, none, none};
-        for (int step = member; step < row.steps; step += r.team) {
+        for (int step = member; step < steps; step += r.team) {
             const int at = row.first(step, lane);
             if (at >= 0 && at + 8 <= r.V) {
                 store8(to + at, v);
@@ -481,7 +539,7 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(X) == 4 ? 4 : 3) k_label_s
     // read by vectors where they are aligned in the logits as in the gradient
     const bool even = (reinterpret_cast<uintptr_t>(x) / sizeof(X)) % 8 == row.ahead;
     Row<X> from(x, r.V);
-    from.ahead = row.ahead, from.steps = row.steps;
+    from.ahead = row.ahead, from.low = row.low, from.high = row.high;
     const float2 off = make_float2(-kept.x, -kept.x), scale = make_float2(kLog2e, kLog2e), log2_s = make_float2(-kept.y, -kept.y);
     const float2 c0s = make_float2(c0, c0), c1s = make_float2(c1, c1);
     auto gradients = [&](float2 v) {
@@ -490,17 +548,14 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(X) == 4 ? 4 : 3) k_label_s
         return mul2(make_float2(exp2_approx(l.x), exp2_approx(l.y)), fma2(c1s, l, c0s));
     };
     auto gradient = [&](float v) { return gradients(make_float2(v, v)).x; };
-    constexpr bool kEarly = sizeof(X) == 2;
-    Raw<X> v[kAhead], next[kEarly ? kAhead : 1];
-    const int hop = r.team * kAhead;
-    if (member < row.steps) from.load(member, r.team, lane, v, even);
-    for (int step = member; step < row.steps; step += hop) {
-        const bool more = step + hop < row.steps;
-        if constexpr (kEarly)
-            if (more) from.load(step + hop, r.team, lane, next, even);
+    constexpr int A = kAhead<X>;
+    Raw<X> v[A];
+    const int hop = r.team * A;
+    if (member < steps) from.load(member, r.team, lane, v, even);
+    for (int step = member; step < steps; step += hop) {
         const bool inside = row.inside(step, r.team);
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
+        for (int i = 0; i < A; ++i) {
             float out[8];
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
@@ -516,14 +571,7 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(X) == 4 ? 4 : 3) k_label_s
                     if (at + j >= 0 && at + j < r.V) put(to + at + j, out[j]);
             }
         }
-        if (more) {
-            if constexpr (kEarly) {
-#pragma unroll
-                for (int i = 0; i < kAhead; ++i) v[i] = next[i];
-            } else {
-                from.load(step + hop, r.team, lane, v, even);
-            }
-        }
+        if (step + hop < steps) from.load(step + hop, r.team, lane, v, even);
     }
     // The label and the alternatives: by the warp that wrote their places.
     __syncwarp();

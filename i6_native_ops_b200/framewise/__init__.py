@@ -341,9 +341,9 @@ def muon_step(
     follow: bool = False,
 ) -> None:
     """One step of Muon over a list of matrices, in place: ``v += (1 - beta) (g - v)``, ``u = g + beta (v - g)`` (without
-    ``nesterov``: ``v``), ``p = p (1 - lr weight_decay) - lr s orthogonalize(u)``.  All matrices, of whatever shapes, go
-    through each product in one launch (256 of them, as far as a gigabyte of scratch holds them).  As after any operation in
-    place, graphs that saved a parameter before refuse their backward pass.
+    ``nesterov``: ``v``), ``p = p (1 - lr weight_decay) - lr s orthogonalize(u)``.  Matrices of up to 128 x 256 take one
+    launch, the others, of whatever shapes, go through each product in one launch (256 of them, as far as two gigabytes of
+    scratch hold them).  As after any operation in place, graphs that saved a parameter before refuse their backward pass.
 
     :param params: contiguous CUDA matrices, all float32 or all bfloat16
     :param momentum: per parameter a float32 tensor of its shape
