@@ -581,11 +581,14 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(X) == 4 ? 4 : 3) k_label_s
     if (lane == 0 && !listed && label >= 0 && label < r.V && mine((int)label)) put(to + label, gradient(value(x[label])) + g);
 }
 
-// Warps per row: enough to fill the SMs, a step each at least.  (See the launches' comment for what was measured.)
-int team_of(int64_t N, int64_t V, int most) {
-    const int64_t want = (int64_t)sm_count() * 16;
+// Warps per row: enough for `busy` on each SM, a step each at least.  Forward 8 of them, and more than a CTA's only where each has
+// 1024 logits: what is joined costs more than further warps bring.  (us without and with 8 alternatives, f32: 256 x 10025 5.0 and
+// 10.7, with 16 busy warps 6.2 and 18; 8 x 10025 3.8 and 8.5, with a team of 64 4.2 and 15; 16 x 100000 with a team of 8 11.4 and
+// 16.5, of 64 5.5 and 12.9.)  The gradient, where nothing is joined: 16.
+int team_of(int64_t N, int64_t V, int most, int busy) {
+    const int64_t want = (int64_t)sm_count() * busy;
     int team = 1;
-    while (team < most && N * team < want && team * 256 < V) team *= 2;
+    while (2 * team <= most && N * team < want && team * 256 < V) team *= 2;
     return team;
 }
 
@@ -595,9 +598,9 @@ bool sizes_ok(const framewise_b200_scores_shape* s) {
            s->top <= kMostTop && s->top <= s->V && (s->dtype == FRAMEWISE_B200_F32 || s->dtype == FRAMEWISE_B200_BF16);
 }
 
-Rows rows_of(const framewise_b200_scores_shape& s, const void* labels, const int32_t* lens, int most_team) {
+Rows rows_of(const framewise_b200_scores_shape& s, const void* labels, const int32_t* lens, int most_team, int busy) {
     Rows r = {};
-    r.N = s.B * s.T, r.T = (int)s.T, r.V = (int)s.V, r.top = s.top, r.team = team_of(r.N, s.V, most_team);
+    r.N = s.B * s.T, r.T = (int)s.T, r.V = (int)s.V, r.top = s.top, r.team = team_of(r.N, s.V, most_team, busy);
     r.stride_b = s.logits_stride_b, r.stride_t = s.logits_stride_t;
     r.labels = labels, r.lens = lens, r.ignore = s.ignore_index;
     return r;
@@ -632,7 +635,7 @@ int framewise_b200_scores_forward(const framewise_b200_scores_shape* shape, cons
     if (shape->B * shape->T == 0) return FRAMEWISE_B200_OK;
     if (!logits || !labels || !log_probs || !entropy || (shape->top > 0 && (!top_log_probs || !top_labels)) || reinterpret_cast<uintptr_t>(kept) % 16 != 0)
         return FRAMEWISE_B200_BAD_ARGUMENT;
-    const Rows   r   = rows_of(*shape, labels, seq_lens, kMostTeam);
+    const Rows   r   = rows_of(*shape, labels, seq_lens, (int)std::clamp<int64_t>(shape->V / 1024, kWarps, kMostTeam), 8);
     const Scored out = {log_probs, entropy, top_log_probs, top_labels, static_cast<float4*>(kept)};
     auto go = [&](auto x, auto l) {
         using X = decltype(x);
@@ -651,7 +654,7 @@ int framewise_b200_scores_backward(const framewise_b200_scores_shape* shape, con
     if (!logits || !labels || !kept || !grads || !grad_logits || reinterpret_cast<uintptr_t>(kept) % 16 != 0 ||
         (grads->top_log_probs && shape->top > 0 && !top_labels))
         return FRAMEWISE_B200_BAD_ARGUMENT;
-    const Rows r = rows_of(*shape, labels, seq_lens, 1 << 16);
+    const Rows r = rows_of(*shape, labels, seq_lens, 1 << 16, 16);
     Incoming   in = {};
     in.log_prob = grads->log_probs, in.log_prob_b = grads->log_probs_stride_b, in.log_prob_t = grads->log_probs_stride_t;
     in.entropy = grads->entropy, in.entropy_b = grads->entropy_stride_b, in.entropy_t = grads->entropy_stride_t;

@@ -132,6 +132,33 @@ def test_rows_shared_by_warps_and_ctas(fw, cuda, rows):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [1, 2, 6, 7, 8, 9, 15, 16, 17, 40])
+def test_rows_that_begin_anywhere(fw, cuda, dtype, V):
+    """Each row begins a value later than the one before, relative to the vectors that it is read in."""
+    wide = torch.randn(1, 17, 2 * V + 17, device=cuda, generator=torch.Generator(cuda).manual_seed(V)).to(dtype)
+    width = V + (V + 1) % 2  # odd, so that rows begin everywhere
+    z = wide.flatten()[: 17 * width].view(1, 17, width)[..., :V]
+    for first in range(3):
+        t = torch.arange(17, device=cuda).view(1, 17).to(torch.int32) % V
+        for top in sorted({0, 1, min(V, 5)}):
+            check(fw, wide.flatten()[first:][: 17 * width].view(1, 17, width)[..., :V] if first else z, t, None, top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [16383, 16385, 33001, 70001])
+def test_long_rows_by_several_ctas(fw, cuda, dtype, V):
+    for rows in (1, 5):
+        for top in (0, 9, 32):
+            check(fw, *inputs(cuda, dtype, 1, rows, V, seed=V + top, short=False), top)
+    z, t, _ = inputs(cuda, dtype, 1, 3, V, short=False, skip=0.0)
+    z[0, 0] = 0.5  # all equal: the first ones are the best
+    z[0, 1] = -INF
+    z[0, 1, V - 3 :] = 1.0
+    got, _ = check(fw, z, t, None, 4)
+    assert got.top_labels[0, 0].tolist() == [0, 1, 2, 3] and got.top_labels[0, 1].tolist() == [V - 3, V - 2, V - 1, 0]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,V", [(3, 5000), (5000, 700)])
 @pytest.mark.parametrize("order", ["equal", "few", "rising", "falling", "lowest", "zeros"])
 def test_equal_and_ordered_logits(fw, cuda, dtype, rows, V, order):
