@@ -1448,9 +1448,10 @@ int batch_list(int64_t count, int64_t rows, int64_t cols, int dtype, const void*
     const int64_t values = rows * cols, bytes = values * (dtype == FRAMEWISE_B200_F32 ? 4 : 2);
     const Matrix  one = {out, x, nullptr, nullptr, rows, cols, 0.0};
     if (one.small()) {
-        for (int64_t i = 0; i < count; i += 1 << 30)
+        constexpr int64_t kMost = 1 << 26;  // of a slot: the CTAs of a launch's slots stay below 2^31
+        for (int64_t i = 0; i < count; i += kMost)
             small->push_back({x ? static_cast<const char*>(x) + i * bytes : nullptr, nullptr, out ? static_cast<char*>(out) + i * bytes : nullptr, nullptr, values, (int)rows,
-                              (int)cols, (int)std::min<int64_t>(count - i, 1 << 30), 0.f});
+                              (int)cols, (int)std::min<int64_t>(count - i, kMost), 0.f});
         return FRAMEWISE_B200_OK;
     }
     if (!matrices_ok(&one, 1)) return FRAMEWISE_B200_BAD_ARGUMENT;

@@ -369,6 +369,8 @@ def test_refusals(fw, cuda):
         (lambda: step([y, y.bfloat16()], [g, g.bfloat16()], [v, v]), "share"),
         (lambda: step([y], [g.cpu()], [v]), "gradient"),
         (lambda: step([y, y], [g, g], [v, v.clone()]), "twice"),
+        (lambda: step([y, y.clone()], [g, g], [v, v]), "twice"),
+        (lambda: step([y.bfloat16()], [g.bfloat16()], [v], master=[v]), "twice"),
     ]
     for f, what in bad:
         with pytest.raises(RuntimeError, match=what):
