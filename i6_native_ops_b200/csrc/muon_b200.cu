@@ -1047,7 +1047,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_co
     // f32: an accumulator for 64 of K, and for A A, whose errors show most (see segment_of), as many as there is room for: 64 x 256 is off
     // by 1.1e-6 of its norm, with one accumulator each by 2.4e-6 (plain 32 bits: 1.4e-6)
     const int depth_x = units, depth_s = (small + 63) / 64, each = PARTS == 2 ? 4 / depth_s : 0;
-    put_x(steps.step[0].operand);
+    const bool square_too = group < 2 * depth_s;  // A and B have columns for this warp
+    if (group < units) put_x(steps.step[0].operand);
     for (int i = 0; i < steps.count; ++i) {
         const SmallStep& f = steps.step[i];
         const float square = one * one, shift = square * (f.b + f.c * square);
@@ -1066,19 +1067,23 @@ __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_co
                 for (int j = 0; j < 16; ++j) pairs[j] = add2(pairs[j], more[j]);
             }
         };
-        multiply(of_type, PARTS - 1, 128, x_at, kXPart, x_at, kXPart, half_kind(128, 128, false), depth_x, false);  // A = X X^T
-        add_up(PARTS == 2 ? depth_x : 1, 128, group * 32);
+        multiply(of_type, PARTS - 1, 128, x_at, kXPart, x_at, kXPart, half_kind(128, depth_s * 64, false), depth_x, false);  // A = X X^T
+        if (square_too) {
+            add_up(PARTS == 2 ? depth_x : 1, 128, group * 32);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) a[j] = sums[j] * f.gram;
+            for (int j = 0; j < 32; ++j) a[j] = sums[j] * f.gram;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) put8(both, s_at + group / 2 * kUnit * 2, kSPart, group % 2 * 4 + j, a + 8 * j, 1.f, true);  // b A and c A A agree about A
-        multiply(both, each, 128, s_at, kSPart, s_at, kSPart, half_kind(128, 128, false), depth_s, false);  // B = b A + c A A - t
-        add_up(max(1, each * depth_s), 128, group * 32);
-        const int hit = row - group * 32;
+            for (int j = 0; j < 4; ++j) put8(both, s_at + group / 2 * kUnit * 2, kSPart, group % 2 * 4 + j, a + 8 * j, 1.f, true);  // b A and c A A agree about A
+        }
+        multiply(both, each, 128, s_at, kSPart, s_at, kSPart, half_kind(128, depth_s * 64, false), depth_s, false);  // B = b A + c A A - t
+        if (square_too) {
+            add_up(max(1, each * depth_s), 128, group * 32);
+            const int hit = row - group * 32;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) a[j] = fmaf(f.of_gram, a[j], sums[j] * f.square) - (j == hit ? shift * f.of_one : 0.f);
+            for (int j = 0; j < 32; ++j) a[j] = fmaf(f.of_gram, a[j], sums[j] * f.square) - (j == hit ? shift * f.of_one : 0.f);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) put8(of_type, s_at + group / 2 * kUnit * 2, kSPart, group % 2 * 4 + j, a + 8 * j, 1.f);
+            for (int j = 0; j < 4; ++j) put8(of_type, s_at + group / 2 * kUnit * 2, kSPart, group % 2 * 4 + j, a + 8 * j, 1.f);
+        }
         multiply(of_type, PARTS - 1, 256, s_at, kSPart, x_at, kXPart, half_kind(128, units * 64, true), depth_s, true);  // (a + t) X + B X
         if (group < units) {
 #pragma unroll
@@ -1087,8 +1092,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_co
 #pragma unroll
                 for (int j = 0; j < 32; ++j) x[c + j] = fmaf(f.a + shift, x[c + j], sums[j] * f.apply);
             }
+            if (i + 1 < steps.count) put_x(steps.step[i + 1].operand);
         }
-        if (i + 1 < steps.count) put_x(steps.step[i + 1].operand);
     }
     ok = __syncthreads_and(ok);  // and all products have been read: the values take the operands' place again
 #pragma unroll
