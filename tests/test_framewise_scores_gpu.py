@@ -145,6 +145,27 @@ def test_rows_that_begin_anywhere(fw, cuda, dtype, V):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [3, 13, 300, 2051])
+def test_special_values_at_the_ends_of_rows(fw, cuda, dtype, V):
+    z, t, _ = inputs(cuda, dtype, 1, 40, V, seed=V, short=False, skip=0.0)
+    z[0, 0::5, 0] = -INF
+    z[0, 1::5, V - 1] = -INF
+    z[0, 2::5, 0] = torch.finfo(dtype).min
+    z[0, 3::5, V - 1] = 30.0
+    z[0, 4::5, : V - 1] = -INF
+    check(fw, z, t, None, 3)
+    for value in (float("nan"), INF):
+        for at in (0, V - 1):
+            bad = z.clone()
+            bad[0, 8:24, at] = value
+            got, fine = fw.label_scores(bad, t, top=3), fw.label_scores(z, t, top=3)
+            assert bool(got.log_probs[0, 8:24].isnan().all()) and bool(got.entropy[0, 8:24].isnan().all())
+            assert bool((got.top_labels[0, 8:24, 0] == at).all())
+            for a, b in zip(got, fine):
+                assert torch.equal(a[0, :8], b[0, :8]) and torch.equal(a[0, 24:], b[0, 24:])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("V", [16383, 16385, 33001, 70001])
 def test_long_rows_by_several_ctas(fw, cuda, dtype, V):
     for rows in (1, 5):
