@@ -896,8 +896,9 @@ struct SmallSteps {
 
 // All steps of a matrix of at most 128 x 256 in one CTA, and its update: nothing but the gradient, the momentum and the parameter
 // crosses memory.  A row of X by four threads, 64 columns each (one unit's row), 32 columns of A and B.  What bounds it is latency:
-// three products a step, each behind a barrier, and what turns its sums into the next operands: 64 x 256 bf16 14 us and 5.6 a step, f32 14 and
-// 9.6 (a chain of launches: 80 and 136 for five steps, and 17 launches of the host's time).
+// three products a step, each behind a barrier, and what turns its sums into the next operands: 64 x 256 bf16 14 us and 4.6 a step, f32 14 and
+// 9.2 (a chain of launches: 80 and 136 for five steps, and 17 launches of the host's time).  Descriptors counted up instead of formed for
+// each product, and waits that ask without a pause, changed nothing.
 // A has two parts for bf16 as well: with one, results of few rows are off by up to 1.9 times their own rounding (2 x 27; 1.2 times with two).
 template <typename X>
 __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_constant__ SmallSlots s, const Rates r, const __grid_constant__ SmallSteps steps) {
