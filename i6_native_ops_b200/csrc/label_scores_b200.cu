@@ -351,7 +351,8 @@ struct Scored {
 };
 
 // A row per team of r.team warps (1 to 8 of a CTA; 16 to 64: all of 2 to 8 CTAs of a cluster), which take its steps of 256
-// logits in turn.
+// logits in turn.  f32 without alternatives is bound by memory (20000 x 12001 6.5 TB/s), bf16 by exponentials and the instructions
+// around them (5.3 TB/s).  Three CTAs an SM where the registers of four do not do (f32 with 8 alternatives 221 us for 198).
 template <typename X, typename L, bool TOP>
 __global__ void __launch_bounds__(kWarps * 32, sizeof(X) == 4 && !TOP ? 4 : 3) k_label_scores(const X* __restrict__ z, const Rows r, const Scored out) {
     __shared__ Sums     part[kWarps];
