@@ -19,8 +19,8 @@ def fw():
     return m
 
 
-def reference(logits, labels, lens, top, grads):
-    """Results and gradient of positions in 64 bits, with a bound of each.
+def reference(logits, labels, lens, top, grads, best=None):
+    """Results and gradient of positions in 64 bits, with a bound of each; best: the order of the alternatives, by their logits without it.
 
     A difference to the maximum, ``spread``, is off by its rounding, that of its product with log2 e and of that constant (3U of
     itself), an exponential by 4 times 2^-22 of itself more than that; a lane adds V / 32 terms, two chains side by side, and
@@ -49,6 +49,8 @@ def reference(logits, labels, lens, top, grads):
     dlp = row + 6 * U * (torch.where(lp == -INF, 0.0, d.abs() + lp.abs()) + logs.abs())
     dH = row * (1 + M) + (p * spread * (de + 4 * U)).sum(1, keepdim=True) + (V / 16 + 128) * U * M + 8 * U * (logs.abs() + M)
     order = torch.sort(z, dim=1, descending=True, stable=True).indices[:, :top]
+    if best is not None and top:
+        order = best.reshape(-1, top)[ok].long()
     g, h, gt = (None if x is None else x.reshape(len(ok), -1)[ok].to(f64) for x in grads)
     zero = torch.zeros(len(t), 1, dtype=f64, device=z.device)
     g, h = zero if g is None else g, zero if h is None else h
@@ -92,20 +94,33 @@ def incoming(shape, top, seed=0, which=(True, True, True)):
     return [g if w else None for g, w in zip(full, which)]
 
 
+def check_order(z, best, log_probs):
+    """The largest logits (equal ones by their class), each once, in falling order of their log probabilities, equal ones by their class."""
+    assert bool((best.sort(1).values.diff(dim=1) > 0).all())
+    of, equal = z.gather(1, best), log_probs[:, :-1] == log_probs[:, 1:]
+    assert bool(torch.where(equal, best[:, :-1] < best[:, 1:], of[:, :-1] > of[:, 1:]).all())
+    if best.shape[1] < z.shape[1]:
+        rest, at = z.scatter(1, best, -INF).max(1)
+        last = of.amin(1)
+        assert bool(((rest < last) | ((rest == last) & ((at > best.where(of == last[:, None], -1).amax(1)) | (rest == -INF)))).all())
+
+
 def check(fw, logits, labels, lens, top, grads=None):
     grads = incoming(tuple(labels.shape), top) if grads is None else grads
-    want = reference(logits, labels, lens, top, grads)
     z = logits.detach().requires_grad_()
     got = fw.label_scores(z, labels, top=top, seq_lens=lens, ignore_index=IGNORE)
+    want = reference(logits, labels, lens, top, grads, got.top_labels)
     pairs = [(o, g) for o, g in zip(got, grads) if g is not None]
     torch.autograd.backward([o for o, _ in pairs], [g for _, g in pairs])
     for name in ("log_probs", "entropy", "top_log_probs"):
         close(getattr(got, name).detach(), want[name], name)
-    assert got.top_labels.dtype == labels.dtype and torch.equal(got.top_labels.long(), want["top_labels"])
+    best, ok = got.top_log_probs.detach(), kept(labels, lens, IGNORE)
+    assert got.top_labels.dtype == labels.dtype and bool((got.top_labels[~ok] == IGNORE).all())
+    if top:
+        check_order(logits.detach()[ok].float(), got.top_labels[ok].long(), best[ok])
     # falling order to the last bit; equal logits have equal log probabilities, the label's among them
-    best = got.top_log_probs.detach()
     assert bool((best[..., :-1] >= best[..., 1:]).all())
-    same = (want["top_labels"] == labels[..., None]) & kept(labels, lens, IGNORE)[..., None]
+    same = (got.top_labels.long() == labels[..., None]) & ok[..., None]
     assert torch.equal(best[same], got.log_probs.detach()[..., None].expand_as(best)[same])
     close(z.grad, want["logits"], "logits")
     with torch.no_grad():
@@ -236,6 +251,21 @@ def test_nan_and_infinity_stay_in_their_rows(fw, cuda, dtype):
     close(zz.grad[:, good], want["logits"])
     assert bool(zz.grad[:, ~good].isnan().all())
     assert got.top_labels[0, 3, 0] == 17 and got.top_labels[0, 4, 0] == 200 and got.top_labels[0, 5].tolist() == [0, 1, 2, 3]
+
+
+def test_equal_log_probabilities_go_by_class(fw, cuda):
+    """Logits a rounding apart, far below the row's largest: what is left of them after it is taken off is equal."""
+    z = torch.full((64, 500), -3.0, device=cuda)
+    z[:, 400] = 18.0
+    z[:, 7] = 5.0
+    z[:, 300] = torch.nextafter(torch.tensor(5.0), torch.tensor(6.0)).to(cuda)  # 5 - 18 and this - 18 round alike: ulps of 2^-21, 2^-20
+    z[:, 450] = 4.0
+    t = torch.zeros(64, dtype=torch.int64, device=cuda)
+    assert z[0, 7] != z[0, 300] and z[0, 7] - 18 == z[0, 300] - 18
+    for top, want in ((2, [400, 300]), (3, [400, 7, 300]), (4, [400, 7, 300, 450]), (32, [400, 7, 300, 450, 0, 1, 2, 3, 4, 5, 6] + list(range(8, 29)))):
+        got = fw.label_scores(z, t, top=top)
+        assert bool((got.top_labels == torch.tensor(want, device=cuda)).all())
+        assert bool((got.top_log_probs[:, 1] == got.top_log_probs[:, 2]).all()) if top > 2 else True
 
 
 def test_nothing_is_read_of_positions_that_do_not_count(fw, cuda):
