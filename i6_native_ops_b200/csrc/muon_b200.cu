@@ -41,7 +41,7 @@ using namespace tensor_core;
 
 constexpr int kMostMatrices = 256;   // of a chain of launches
 constexpr int kSlots        = 24;    // matrices in a launch's arguments
-constexpr int kChunk        = 16384; // values per CTA of the pass over gradients
+constexpr int kChunk        = 8192;  // values per CTA of the pass over gradients
 constexpr int kRowsPerCta   = 128;   // of a tile: the lanes of tensor memory
 constexpr int kMostWide     = 256;   // columns of a tile at most
 constexpr int kColumns      = 512;   // of tensor memory: a ring of accumulators
@@ -52,7 +52,8 @@ constexpr int kDepth        = 64;    // K per stage: one part of both operands
 // one), and it is the smallest product: there it is done after each step, and so in short sums, whose tiles wait for other things.
 // Off by, as a part of their norm (plain 32 bits): 500 x 2001 2.6e-6 (2.8e-6; four steps in A A as well 5.1e-6, two throughout
 // 3.4e-6, in 531 us for six instead of 480).
-__host__ __device__ constexpr int segment_of(bool square, int depth) { return square || depth <= 4 ? 1 : 4; }
+// Matrices of at most 128 rows, which fill a tile a step, have all their sums cut: 1 x 2869 was off by 1.3e-6 (plain 3.3e-7).
+__host__ __device__ constexpr int segment_of(bool always, int depth) { return always || depth <= 4 ? 1 : 4; }
 constexpr int kMostStages   = 12;
 constexpr int kEpilogue     = 8;     // warps that finish tiles
 constexpr int kThreads      = 64 + 32 * kEpilogue;
@@ -228,9 +229,10 @@ __global__ void __launch_bounds__(256) k_muon_collect(const __grid_constant__ Sl
 }
 
 // X = U / max(|U|, eps) in 32 bits and as operands, zeros where there are none: a CTA takes kBlocks squares of 64 columns and rows, the
-// next of which is loaded while one is written.  (A square each: 204 us for 4 x 2048 x 8192 bf16, 184 with four;
-// its bytes at the copy's rate 123.)
-constexpr int kBlocks = 4;
+// next of which is loaded while one is written.  (A square each: 204 us for 4 x 2048 x 8192 bf16, 184 with four, its bytes at the
+// copy's rate 123.  Smaller calls end sooner with more CTAs: all five steps of 6 x 500 x 2001 f32 487 us with four and chunks of 16384,
+// 472 with two and 8192; 16 x 512 x 2048 bf16 502 and 494; 8 x 2048 x 8192 bf16 5390 and 5430.)
+constexpr int kBlocks = 2;
 template <typename X, int PARTS>
 __global__ void __launch_bounds__(256, 5) k_muon_begin(const Entry* __restrict__ table, int count, const Rates r, float scale, __half* work, const __grid_constant__ Steps steps) {
     __shared__ double part[8];
@@ -566,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
 
     // Tile u: its matrix, and the first row and column.  Symmetric results: rows of tiles from the diagonal on.
     struct Tile {
-        int e, row, col, depth;
+        int e, row, col, depth, segment;
     };
     auto tile_at = [&](int u) -> Tile {
         Tile t;
@@ -591,6 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
             t.row = row * kTile;
         }
         t.depth = KIND == kGram ? m.panels : (m.m + 63) / 64;
+        t.segment = kSegments ? segment_of(KIND == kSquare || m.m <= 128, t.depth) : t.depth;
         return t;
     };
 
@@ -646,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
             const Entry m = p.table[t.e];
             const int limit = kApplies ? m.panels * 64 : m.mp;
             const uint32_t kind = half_kind(kTile, min(p.wide, limit - t.col), kBMn);
-            for (int k0 = 0; k0 < t.depth && ok; k0 += kSegments ? segment_of(KIND == kSquare, t.depth) : t.depth) {
+            for (int k0 = 0; k0 < t.depth && ok; k0 += t.segment) {
                 ok = wait(freed + 8 * acc, acc_phase ^ 1);
                 if (!ok) break;
                 fence_after();
@@ -666,7 +669,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                     return ok;
                 };
                 if constexpr (kSegments) {  // the small products first
-                    const int k1 = min(t.depth, k0 + segment_of(KIND == kSquare, t.depth));
+                    const int k1 = min(t.depth, k0 + t.segment);
                     for (int k = k0; k < k1; ++k) {
                         const int low = stage;
                         if (!arrived(stage, phase)) break;
@@ -799,7 +802,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
 #pragma unroll
                 for (int j = 0; j < kMostWide / 2; ++j) total[j] = 0.f;
             }
-            for (int k0 = 0; k0 < t.depth; k0 += kSegments ? segment_of(KIND == kSquare, t.depth) : t.depth) {
+            for (int k0 = 0; k0 < t.depth; k0 += t.segment) {
                 ok = __all_sync(0xffffffffu, wait(done + 8 * acc, acc_phase));
                 if (!ok) break;
                 fence_after();
