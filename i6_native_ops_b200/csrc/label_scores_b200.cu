@@ -249,7 +249,7 @@ struct Room {
 // The best that a warp has met.  While the sums are formed only the maximum of each cell, 32 values of a lane in kCell steps
 // that the team takes in turn, is written down.  After kCells of them, or at the row's end, those cells are read again whose maximum is no smaller
 // than the `top`-th largest of the lanes' maxima: some more than `top` of them.  (Looking at each value while the sums are formed,
-// against the list so far: 26 instructions a value for the whole kernel, 20000 x 12001 f32 with 8 alternatives 664 us; 198 this way,
+// against the list so far: 26 instructions a value for the whole kernel, 20000 x 12001 f32 with 8 alternatives 664 us; 202 this way,
 // and 148 without alternatives.)
 struct Best {
     uint64_t list;    // the 32 largest so far, a lane each, in falling order
