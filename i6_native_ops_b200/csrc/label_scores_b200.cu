@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(X) == 4 && !TOP ? 4 : 3) k
     if (member != 0 || !inside) return;
     // a row without a class that is possible has log probabilities of -inf and no entropy
     const float log2_s = log2f(a.s), entropy = a.s == 0.f ? 0.f : kLn2 * (log2_s - a.t / a.s);
-    // each operation rounded by itself: which logits have equal log probabilities does not hang on how they are compiled
+    // each operation rounded by itself, so that the label's and its alternative's are equal to the last bit
     const float log_s = logf(a.s);
     auto log_prob = [&](float v) { return a.s == 0.f ? -INFINITY : __fsub_rn(__fsub_rn(v, a.m), log_s); };
     if (lane == 0) {
@@ -467,18 +467,11 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(X) == 4 && !TOP ? 4 : 3) k
         if (out.kept) out.kept[n] = make_float4(a.m, log2_s, entropy, 0.f);
     }
     if constexpr (TOP) {
-        // Logits that differ may have equal log probabilities, those next to each other in the list: these too go by their class.
-        float      p = log_prob(value_of(b.list));
-        int        label_of = index_of(b.list);
-        const float former = __shfl_up_sync(0xffffffffu, p, 1);
-        const bool  in = lane < r.top;
-        if (counts && __any_sync(0xffffffffu, in && lane > 0 && p == former)) {
-            const uint64_t key = sorted(in ? key_of(p, label_of) : 0, lane);
-            p = value_of(key), label_of = index_of(key);
-        }
+        // In the order of the logits, which no rounding touches: what is left of two of them after the maximum and the logarithm are
+        // taken off may be equal, and the last bit of the sum, which hangs on how many warps share the row, then decided.
         if (lane < r.top) {
-            out.top_log_prob[n * r.top + lane] = counts ? p : 0.f;
-            static_cast<L*>(out.top_label)[n * r.top + lane] = counts ? (L)label_of : (L)r.ignore;
+            out.top_log_prob[n * r.top + lane] = counts ? log_prob(value_of(b.list)) : 0.f;
+            static_cast<L*>(out.top_label)[n * r.top + lane] = counts ? (L)index_of(b.list) : (L)r.ignore;
         }
     }
 }

@@ -135,8 +135,8 @@ def label_scores(
     :param seq_lens: (B,) int32 lengths, or a (T, B) index mask
     :param ignore_index: labels of positions that are left out
     :return: ``log_probs`` and ``entropy``, float32 in the shape of ``labels``; ``top_log_probs`` and ``top_labels``, (..., top):
-        the largest logits, in falling order of their log probabilities, equal ones by their class (NaN is the largest),
-        labels in the dtype of ``labels``.  Positions past their length or left out have 0 and the ignored label, and their logits are never read.
+        the largest logits in falling order, equal ones by their class (NaN is the largest), so that fewer are the first of
+        more; labels in the dtype of ``labels``.  Positions past their length or left out have 0 and the ignored label, and their logits are never read.
 
     A position whose logits are all -inf has log probabilities of -inf, entropy 0 and a gradient of 0; one with NaN or +inf
     has NaN.  A label outside 0..V-1 at a position that counts gives NaN, there and in that position's gradient.

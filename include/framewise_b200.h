@@ -148,8 +148,8 @@ typedef struct {
 
 /* For z = logits[b,t,:] and log p = z - log sum_v exp z[v]:
  *     log_probs[b,t] = log p[label];  entropy[b,t] = - sum_v p log p  (classes of z = -inf add nothing);
- *     top_labels[b,t,:], top_log_probs[b,t,:]: the `top` largest of z (equal ones by their index; NaN is the largest) and
- *     their log p, in falling order of it, equal ones by their index.
+ *     top_labels[b,t,:], top_log_probs[b,t,:]: the `top` largest of z in falling order (equal ones by their index; NaN is the
+ *     largest) and their log p.
  * Positions that do not count: 0, and `ignore_index` as labels.  A row of -inf alone: log probabilities -inf, entropy 0.
  * A row with NaN or +inf: NaN.  logits (B,T,V), labels (B,T) dense, outputs dense, f32.  `kept`: 16 B T bytes, 16-byte
  * aligned, for the backward pass, or NULL. */
