@@ -430,6 +430,7 @@ const char* framewise_b200_status_string(int status) {
         case FRAMEWISE_B200_WORKSPACE: return "buffer too small";
         case FRAMEWISE_B200_CUDA_ERROR: return "CUDA error";
         case FRAMEWISE_B200_TENSOR_MAP: return "a tensor map could not be made";
+        case FRAMEWISE_B200_OVERLAP: return "a tensor that is written is given twice, or overlaps another one or a gradient";
         default: return "unknown status";
     }
 }

@@ -542,15 +542,6 @@ void muon_step(const Tensors& params, const Tensors& grads, const Tensors& momen
         if (!master.empty()) check_state(master[i], p, torch::kFloat32, "master");
         list[i] = {p.data_ptr(), g.data_ptr(), momentum[i].data_ptr<float>(), master.empty() ? nullptr : master[i].data_ptr<float>(), p.size(0), p.size(1)};
     }
-    std::vector<const void*> seen;  // what is written
-    seen.reserve(3 * n);
-    for (const auto& m : list) {
-        if (m.rows * m.cols == 0) continue;
-        seen.push_back(m.param), seen.push_back(m.momentum);
-        if (m.master) seen.push_back(m.master);
-    }
-    std::sort(seen.begin(), seen.end());
-    TORCH_CHECK(std::adjacent_find(seen.begin(), seen.end()) == seen.end(), "Muon: a parameter or a state is given twice");
     const size_t need = framewise_b200_muon_bytes(list.data(), (int64_t)n, dtype);
     TORCH_CHECK(need > 0, "Muon: a parameter is too large");
     Tensor work = bytes(need, params[0]);

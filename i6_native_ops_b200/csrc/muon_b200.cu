@@ -1452,6 +1452,35 @@ int muon_list(const framewise_b200_matrix* matrices, int64_t count, double lr, i
     return matrices_ok(list->data(), (int64_t)list->size()) ? FRAMEWISE_B200_OK : FRAMEWISE_B200_BAD_ARGUMENT;
 }
 
+// Whether something that a step writes overlaps something else that it writes or reads.  (The momentum is written before the gradient
+// is read again, and matrices are not done in order.)
+bool overlaps(const framewise_b200_matrix* matrices, int64_t count, int64_t size) {
+    struct Range {
+        uintptr_t begin, end;
+        bool      written;
+    };
+    std::vector<Range> ranges;
+    ranges.reserve(4 * count);
+    for (int64_t i = 0; i < count; ++i) {
+        const framewise_b200_matrix& m = matrices[i];
+        if (m.rows == 0 || m.cols == 0) continue;
+        auto add = [&](const void* at, int64_t each, bool written) {
+            const uintptr_t begin = reinterpret_cast<uintptr_t>(at);
+            ranges.push_back({begin, begin + (uintptr_t)(m.rows * m.cols * each), written});
+        };
+        add(m.param, size, true), add(m.grad, size, false), add(m.momentum, 4, true);
+        if (m.master) add(m.master, 4, true);
+    }
+    std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+    uintptr_t written = 0, any = 0;  // where the ranges so far end
+    for (const Range& r : ranges) {
+        if (r.begin < (r.written ? any : written)) return true;
+        any = std::max(any, r.end);
+        if (r.written) written = std::max(written, r.end);
+    }
+    return false;
+}
+
 // `count` matrices of one shape, one after another
 int batch_list(int64_t count, int64_t rows, int64_t cols, int dtype, const void* x, void* out, std::vector<SmallSlot>* small, std::vector<Matrix>* list) {
     const int64_t values = rows * cols, bytes = values * (dtype == FRAMEWISE_B200_F32 ? 4 : 2);
@@ -1491,6 +1520,7 @@ int framewise_b200_muon(const framewise_b200_matrix* matrices, int64_t count, in
     FW_DO(muon_list(matrices, count, lr, match_rms, &small, &list));
     auto bad = [&](const auto& m) { return !m.param || !m.grad || !m.momentum || (m.master && dtype == FRAMEWISE_B200_F32); };
     if (std::any_of(list.begin(), list.end(), bad) || std::any_of(small.begin(), small.end(), bad)) return FRAMEWISE_B200_BAD_ARGUMENT;
+    if (overlaps(matrices, count, dtype == FRAMEWISE_B200_F32 ? 4 : 2)) return FRAMEWISE_B200_OVERLAP;
     const Rates rates = {(float)(1 - beta), (float)beta, nesterov ? 1.f : 0.f, (float)eps, (float)(1 - lr * weight_decay), follow};
     return run(small, list, dtype, rates, coefficients, steps, work, work_bytes, stream);
 } catch (...) {

@@ -345,7 +345,8 @@ def muon_step(
     launch, the others, of whatever shapes, go through each product in one launch (256 of them, as far as two gigabytes of
     scratch hold them).  As after any operation in place, graphs that saved a parameter before refuse their backward pass.
 
-    :param params: contiguous CUDA matrices, all float32 or all bfloat16
+    :param params: contiguous CUDA matrices, all float32 or all bfloat16.  Parameters, momentum and copies overlap neither each
+        other nor a gradient; gradients may be shared
     :param momentum: per parameter a float32 tensor of its shape
     :param adjust_lr: ``"original"`` (or None): ``s = sqrt(max(1, rows / cols))``; ``"match_rms_adamw"``: ``s = 0.2
         sqrt(max(rows, cols))``

@@ -32,7 +32,8 @@ enum {
     FRAMEWISE_B200_BAD_ARGUMENT = 1, /* null pointer, negative dimension, size past a limit, misaligned buffer */
     FRAMEWISE_B200_WORKSPACE    = 2, /* caller-provided buffer too small                                      */
     FRAMEWISE_B200_CUDA_ERROR   = 3, /* a CUDA call failed (see cudaGetLastError)                             */
-    FRAMEWISE_B200_TENSOR_MAP   = 4  /* the driver made no tensor map (or has no call for it)                 */
+    FRAMEWISE_B200_TENSOR_MAP   = 4, /* the driver made no tensor map (or has no call for it)                 */
+    FRAMEWISE_B200_OVERLAP      = 5  /* what is written is given twice, or overlaps something else of the call */
 };
 
 enum { FRAMEWISE_B200_F32 = 0, FRAMEWISE_B200_BF16 = 1 };
@@ -198,7 +199,8 @@ typedef struct {
  *     v = v + (g - v) (1 - beta);   u = nesterov ? g + (v - g) beta : v;   o = u orthogonalised as above
  *     x = x (1 - lr weight_decay) - lr s o,   s = sqrt(max(1, rows / cols)), or match_rms: 0.2 sqrt(max(rows, cols))
  * x being the master copy where there is one (the parameter is then x rounded once); follow: a copy of which its parameter
- * is not the rounded value starts from the parameter.  Matrices of up to 128 x 256 (either way round) take one launch, the
+ * is not the rounded value starts from the parameter.  What is written (params, momentum, masters) overlaps nothing else of the
+ * call; gradients may be shared.  Matrices of up to 128 x 256 (either way round) take one launch, the
  * others a chain of 3 steps + 3 launches together, 256 of them and two gigabytes of scratch at most at a time. */
 size_t framewise_b200_muon_bytes(const framewise_b200_matrix* matrices, int64_t count, int32_t dtype);
 int framewise_b200_muon(const framewise_b200_matrix* matrices, int64_t count, int32_t dtype, double lr, double beta,
