@@ -269,9 +269,9 @@ __global__ void __launch_bounds__(256, 5) k_muon_begin(const Entry* __restrict__
     __syncthreads();
     sum = part[0];
     for (int i = 1; i < 8; ++i) sum += part[i];
-    // |U| may be past the range of 32 bits (or below): 64 bits up to the quotient
+    // |U| may be past the range of 32 bits (or below), or its reciprocal where 32 bits hold few digits: 64 bits up to the quotient
     const double by = 1.0 / fmax(sqrt(sum), (double)r.eps);
-    const bool   far = !(by < 1e30);
+    const bool   far = !(by < 1e30 && by > 1e-30);
     const float  by32 = (float)by;
     if (first == 0 && threadIdx.x == 0) {
         float one = (float)(fmin(1.0, sqrt(sum) * by) * rsqrt((double)m.m));  // all singular values, if they are equal
@@ -977,7 +977,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_co
     sum = 0.0;
     for (int i = 0; i < kSmallThreads / 32; ++i) sum += part[i];
     const double by = 1.0 / fmax(sqrt(sum), (double)r.eps);  // in 64 bits, as for larger matrices
-    const bool   far = !(by < 1e30);
+    const bool   far = !(by < 1e30 && by > 1e-30);
     const float  by32 = (float)by;
     float x[64];
     const bool mine = row < small;
