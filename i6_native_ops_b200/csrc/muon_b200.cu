@@ -121,9 +121,10 @@ __device__ __forceinline__ int64_t in_units(int panels, int row, int col) {
 }
 
 struct Rates {
-    float keep, beta, nesterov;  // 1 - beta; nesterov: 0 or 1
-    float eps, decay;            // decay: 1 - lr weight_decay
-    int   follow;
+    double eps;
+    float  keep, beta, nesterov;  // 1 - beta; nesterov: 0 or 1
+    float  decay;                 // 1 - lr weight_decay
+    int    follow;
 };
 
 // The nearest fp16 numbers of two values, which keep what is left of them.
@@ -270,7 +271,7 @@ __global__ void __launch_bounds__(256, 5) k_muon_begin(const Entry* __restrict__
     sum = part[0];
     for (int i = 1; i < 8; ++i) sum += part[i];
     // |U| may be past the range of 32 bits (or below), or its reciprocal where 32 bits hold few digits: 64 bits up to the quotient
-    const double by = 1.0 / fmax(sqrt(sum), (double)r.eps);
+    const double by = sum == 0.0 ? 0.0 : 1.0 / fmax(sqrt(sum), r.eps);  // zeros stay zeros, however small eps is
     const bool   far = !(by < 1e30 && by > 1e-30);
     const float  by32 = (float)by;
     if (first == 0 && threadIdx.x == 0) {
@@ -976,7 +977,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_co
     const uint32_t tmem = *const_cast<volatile uint32_t*>(&slot_at);
     sum = 0.0;
     for (int i = 0; i < kSmallThreads / 32; ++i) sum += part[i];
-    const double by = 1.0 / fmax(sqrt(sum), (double)r.eps);  // in 64 bits, as for larger matrices
+    const double by = sum == 0.0 ? 0.0 : 1.0 / fmax(sqrt(sum), r.eps);  // in 64 bits, as for larger matrices
     const bool   far = !(by < 1e30 && by > 1e-30);
     const float  by32 = (float)by;
     float x[64];
@@ -1521,7 +1522,7 @@ int framewise_b200_muon(const framewise_b200_matrix* matrices, int64_t count, in
     auto bad = [&](const auto& m) { return !m.param || !m.grad || !m.momentum || (m.master && dtype == FRAMEWISE_B200_F32); };
     if (std::any_of(list.begin(), list.end(), bad) || std::any_of(small.begin(), small.end(), bad)) return FRAMEWISE_B200_BAD_ARGUMENT;
     if (overlaps(matrices, count, dtype == FRAMEWISE_B200_F32 ? 4 : 2)) return FRAMEWISE_B200_OVERLAP;
-    const Rates rates = {(float)(1 - beta), (float)beta, nesterov ? 1.f : 0.f, (float)eps, (float)(1 - lr * weight_decay), follow};
+    const Rates rates = {eps, (float)(1 - beta), (float)beta, nesterov ? 1.f : 0.f, (float)(1 - lr * weight_decay), follow};
     return run(small, list, dtype, rates, coefficients, steps, work, work_bytes, stream);
 } catch (...) {
     return FRAMEWISE_B200_BAD_ARGUMENT;
@@ -1547,7 +1548,7 @@ int framewise_b200_orthogonalize(int64_t count, int64_t rows, int64_t cols, int3
     std::vector<SmallSlot> small;
     std::vector<Matrix>    list;
     FW_DO(batch_list(count, rows, cols, dtype, x, out, &small, &list));
-    const Rates rates = {0.f, 0.f, 0.f, (float)eps, 1.f, 0};
+    const Rates rates = {eps, 0.f, 0.f, 0.f, 1.f, 0};
     return run(small, list, dtype, rates, coefficients, steps, work, work_bytes, stream);
 } catch (...) {
     return FRAMEWISE_B200_BAD_ARGUMENT;
