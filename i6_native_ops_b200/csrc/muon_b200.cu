@@ -143,6 +143,19 @@ __device__ __forceinline__ void former_is_done() { asm volatile("griddepcontrol.
 // what is made orthogonal, from the gradient and the new momentum
 __device__ __forceinline__ float direction(float g, float v, const Rates& r) { return r.nesterov != 0.f ? g + (v - g) * r.beta : v; }
 
+// 1 / max(|U|, eps), from the sum of squares.  |U| may be past the range of 32 bits, or below, and its reciprocal where 32 bits hold few
+// digits: two factors, of which the second is a power of two, and one but for those.
+struct Reciprocal {
+    float  first, second;
+    double both;
+    __device__ __forceinline__ Reciprocal(double sum, double eps) {
+        both = sum == 0.0 ? 0.0 : 1.0 / fmax(sqrt(sum), eps);  // zeros stay zeros, however small eps is
+        second = both > 1e30 ? 0x1p100f : both < 1e-30 ? 0x1p-100f : 1.f;
+        first  = (float)(both > 1e30 ? both * 0x1p-100 : both < 1e-30 ? both * 0x1p100 : both);
+    }
+    __device__ __forceinline__ float times(float u) const { return u * first * second; }
+};
+
 // four values in a row; `wide`: aligned for one access, else as many as there are (`left`)
 __device__ __forceinline__ void load4(const float* x, bool wide, int left, float (&v)[4]) {
     if (wide) {
@@ -270,12 +283,9 @@ __global__ void __launch_bounds__(256, 5) k_muon_begin(const Entry* __restrict__
     __syncthreads();
     sum = part[0];
     for (int i = 1; i < 8; ++i) sum += part[i];
-    // |U| may be past the range of 32 bits (or below), or its reciprocal where 32 bits hold few digits: 64 bits up to the quotient
-    const double by = sum == 0.0 ? 0.0 : 1.0 / fmax(sqrt(sum), r.eps);  // zeros stay zeros, however small eps is
-    const bool   far = !(by < 1e30 && by > 1e-30);
-    const float  by32 = (float)by;
+    const Reciprocal by(sum, r.eps);
     if (first == 0 && threadIdx.x == 0) {
-        float one = (float)(fmin(1.0, sqrt(sum) * by) * rsqrt((double)m.m));  // all singular values, if they are equal
+        float one = (float)(fmin(1.0, sqrt(sum) * by.both) * rsqrt((double)m.m));  // all singular values, if they are equal
         for (int i = 0; i < steps.count; ++i) {
             const float square = one * one, t = square * (steps.abc[3 * i + 1] + steps.abc[3 * i + 2] * square);
             m.shift[i] = t;
@@ -288,7 +298,7 @@ __global__ void __launch_bounds__(256, 5) k_muon_begin(const Entry* __restrict__
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float d = v ? direction(u[i][j], mom[i][j], r) : u[i][j], x = far ? (float)(d * by) : d * by32;
+                const float d = v ? direction(u[i][j], mom[i][j], r) : u[i][j], x = by.times(d);
                 if (tall) tile[at + j][l0 + i * 16] = x;
                 else tile[l0 + i * 16][at + j] = x;
             }
@@ -977,19 +987,17 @@ __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_co
     const uint32_t tmem = *const_cast<volatile uint32_t*>(&slot_at);
     sum = 0.0;
     for (int i = 0; i < kSmallThreads / 32; ++i) sum += part[i];
-    const double by = sum == 0.0 ? 0.0 : 1.0 / fmax(sqrt(sum), r.eps);  // in 64 bits, as for larger matrices
-    const bool   far = !(by < 1e30 && by > 1e-30);
-    const float  by32 = (float)by;
+    const Reciprocal by(sum, r.eps);
     float x[64];
     const bool mine = row < small;
 #pragma unroll
     for (int j = 0; j < 64; ++j) {
         const int col = group * 64 + j;
         const float u = mine && col < wide ? values[row * kSmallPitch + col] : 0.f;
-        x[j] = far ? (float)(u * by) : u * by32;
+        x[j] = by.times(u);
     }
     __syncthreads();  // the operands take the values' place
-    float one = (float)(fmin(1.0, sqrt(sum) * by) * rsqrt((double)small));
+    float one = (float)(fmin(1.0, sqrt(sum) * by.both) * rsqrt((double)small));
     const uint32_t x_at = base, s_at = base + PARTS * (kSmallN / 64) * (kUnit * 2);
     constexpr int kXPart = kSmallN / 64 * kUnit * 2, kSPart = 2 * kUnit * 2;
     // 8 values as an operand's 16 bytes: piece `piece` of this row in a unit
