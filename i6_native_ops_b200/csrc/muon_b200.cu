@@ -6,11 +6,12 @@
 // which makes of each singular value s the value s (a + b s^2 + c s^4): after some steps they are all near one.
 // Per step 2 m n m + 2 m m m + 2 m m n operations, of which half of the first two are not needed, for A and B are symmetric.
 //
-// X is held in 32 bits; the products' operands are rounded from it to fp16: one part (11 bits) for bf16 matrices, two parts
-// (22 bits, three products) for f32 ones.  a X is added in 32 bits, outside of the products: small singular values are those that
-// grow, by a factor of a step, and an error that a product made of X would grow with them.  What B's and A's roundings do is
-// a change of the factor B, small for small singular values, and does not grow.  fp16 rather than bf16: as fast, eight times
-// finer, and all operands are bounded, so that powers of two (from the coefficients, for any matrix) keep them in its range.
+// X is held in 32 bits; the products' operands are rounded from it to fp16: one part (11 bits) for bf16 matrices, but two of A
+// where it has up to 128 rows (see gram_parts), two parts (22 bits, three products) for f32 ones.  a X is added in 32 bits, outside of
+// the products: small singular values are those that grow, by a factor of a step, and an error that a product made of X would
+// grow with them.  What B's and A's roundings do is a change of the factor B, small for small singular values, and does not grow.  fp16
+// rather than bf16: as fast, eight times finer, and all operands are bounded, so that powers of two (from the coefficients, for any
+// matrix) keep them in its range.
 // Once singular values are near one, B is near (b + c) times the identity and undoes most of a X.  So a multiple t of the
 // identity is taken from B and added to a, where it costs no rounding: t = b s^2 + c s^4 for the singular value s that all
 // would have if they were equal (1 / sqrt(m) at first; a matrix below eps, which stays small, has small t).  Errors of bf16
@@ -54,6 +55,11 @@ constexpr int kDepth        = 64;    // K per stage: one part of both operands
 // 3.4e-6, in 531 us for six instead of 480).
 // Matrices of at most 128 rows, which fill a tile a step, have all their sums cut: 1 x 2869 was off by 1.3e-6 (plain 3.3e-7).
 __host__ __device__ constexpr int segment_of(bool always, int depth) { return always || depth <= 4 ? 1 : 4; }
+// Parts of A.  bf16 matrices of few rows have two of them: b A and c A A undo each other, and where B has few values their errors do not
+// average out (with one part, worst of 40 matrices, bf16 result: 2 x 257 off by 4.1e-3 of its norm, with two by 2.5e-3; 3 x 1024 3.3e-3 and
+// 2.2e-3; 128 x 300 1.86e-3 and 1.75e-3, of which the result's own rounding 1.67e-3; more rows gain as little and would pay three times
+// the product).
+__host__ __device__ constexpr int gram_parts(int parts, int m) { return m <= 128 ? 2 : parts; }
 constexpr int kMostStages   = 12;
 constexpr int kEpilogue     = 8;     // warps that finish tiles
 constexpr int kThreads      = 64 + 32 * kEpilogue;
@@ -622,9 +628,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
             const int a_first = a0 + (t.row / 128 + rank) * (KIND == kGram ? m.panels : s_row);
             // columns of the tile that there are and are this CTA's
             const int limit = kApplies ? m.panels * 64 : m.mp, have = min(p.wide, limit - t.col) / CG, from = t.col + rank * have;
-            const int copies = (have + p.span - 1) / p.span, span_bytes = p.span * kDepth * 2;
+            const int copies = (have + p.span - 1) / p.span, span_bytes = p.span * kDepth * 2, parts = KIND == kSquare ? gram_parts(PARTS, m.m) : PARTS;
             for (int k = 0; k < t.depth && ok; ++k) {
-                for (int q = PARTS - 1; q >= 0; --q) {  // the small part is met, and its stage free again, first
+                for (int q = parts - 1; q >= 0; --q) {  // the small part is met, and its stage free again, first
                     ok = wait(empty + 8 * stage, phase ^ 1);
                     if (!ok) break;
                     const uint32_t a = base + stage * stage_bytes, b = a + part_a, bar = CG == 2 ? in_cta(full + 8 * stage, 0) : full + 8 * stage;
@@ -679,29 +685,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                     if (ok) fence_after();
                     return ok;
                 };
-                if constexpr (kSegments) {  // the small products first
-                    const int k1 = min(t.depth, k0 + t.segment);
-                    for (int k = k0; k < k1; ++k) {
+                const int  k1 = kSegments ? min(t.depth, k0 + t.segment) : t.depth;
+                const bool two = kSegments || (KIND == kSquare && gram_parts(PARTS, m.m) == 2);
+                for (int k = k0; k < k1; ++k) {
+                    if (!arrived(stage, phase)) break;
+                    if (two) {  // the small products first
                         const int low = stage;
-                        if (!arrived(stage, phase)) break;
                         next(stage, phase);
                         if (!arrived(stage, phase)) break;
                         multiply(low, stage, k > k0);
                         multiply(stage, low, true);
                         products_commit<CG>(empty + 8 * low);
-                        multiply(stage, stage, true);
-                        products_commit<CG>(empty + 8 * stage);
-                        next(stage, phase);
                     }
-                    if (!ok) break;
-                } else {
-                    for (int k = 0; k < t.depth; ++k) {
-                        if (!arrived(stage, phase)) break;
-                        multiply(stage, stage, k > 0);
-                        products_commit<CG>(empty + 8 * stage);
-                        next(stage, phase);
-                    }
+                    multiply(stage, stage, two || k > k0);
+                    products_commit<CG>(empty + 8 * stage);
+                    next(stage, phase);
                 }
+                if (!ok) break;
                 products_commit<CG>(done + 8 * acc);
                 if (++acc == accs) acc = 0, acc_phase ^= 1;
             }
@@ -762,16 +762,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                 const int64_t at = in_units(kApplies ? m.panels : m.mp / 64, row, col);
                 __half* const to = p.work + (int64_t)target * kUnit;
                 const int64_t plane = KIND == kApply ? x_plane : s_plane;
+                const int of_gram = gram_parts(PARTS, m.m), parts = KIND == kGram ? of_gram : PARTS;
                 if (KIND == kSquare) {
 #pragma unroll
-                    for (int q = PARTS - 1; q >= 0; --q) {
+                    for (int q = 1; q >= 0; --q) {
+                        if (q >= of_gram) continue;
                         uint32_t w[16];
                         load_sector(p.work + (int64_t)m.gram * kUnit + q * plane + at, w), load_sector(p.work + (int64_t)m.gram * kUnit + q * plane + at + 16, w + 8);
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
                             const float2 a = __half22float2(reinterpret_cast<const __half2&>(w[j]));
-                            v[2 * j] = fmaf(old, a.x, q == PARTS - 1 ? v[2 * j] * p.product : v[2 * j]);
-                            v[2 * j + 1] = fmaf(old, a.y, q == PARTS - 1 ? v[2 * j + 1] * p.product : v[2 * j + 1]);
+                            v[2 * j] = fmaf(old, a.x, q == of_gram - 1 ? v[2 * j] * p.product : v[2 * j]);
+                            v[2 * j + 1] = fmaf(old, a.y, q == of_gram - 1 ? v[2 * j + 1] * p.product : v[2 * j + 1]);
                         }
                     }
                     const int hit = row - col;  // the diagonal's place among these columns
@@ -785,7 +787,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constan
                 }
                 const bool mirror = KIND != kApply && col / 128 > row / 128;
 #pragma unroll
-                for (int q = 0; q < PARTS; ++q) {
+                for (int q = 0; q < (KIND == kGram ? 2 : PARTS); ++q) {
+                    if (q >= parts) continue;
                     uint32_t w[16];
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
@@ -1245,7 +1248,7 @@ Chain chain_of(const Matrix* matrices, int64_t count, int parts, int steps, void
             w.take<__half>(halves);
         };
         for (int& at : e.operand) units(&at, parts * values);
-        units(&e.gram, (int64_t)parts * e.mp * e.mp), units(&e.factor, (int64_t)parts * e.mp * e.mp);
+        units(&e.gram, (int64_t)gram_parts(parts, e.m) * e.mp * e.mp), units(&e.factor, (int64_t)parts * e.mp * e.mp);
     }
     c.bytes = (size_t)up((int64_t)w.used, kUnit * 2);
     return c;
@@ -1258,7 +1261,7 @@ int64_t together(const Matrix* matrices, int64_t count, int parts) {
     int64_t i = 0;
     for (; i < count && i < kMostMatrices; ++i) {
         const int64_t m = std::min(matrices[i].rows, matrices[i].cols), n = std::max(matrices[i].rows, matrices[i].cols);
-        const size_t more = (size_t)up(m, 256) * ((size_t)up(n, 128) * (4 + 4 * parts) + (size_t)up(m, 256) * 4 * parts);
+        const size_t more = (size_t)up(m, 256) * ((size_t)up(n, 128) * (4 + 4 * parts) + (size_t)up(m, 256) * 2 * (parts + gram_parts(parts, (int)std::min<int64_t>(m, 256))));
         if (i > 0 && bytes + more > kChainBytes) break;
         bytes += more;
     }

@@ -320,8 +320,8 @@ def orthogonalize(
     :param coefficients: (a, b, c) of every step, or one such triple per step.  Those that let singular values grow past
         10^6 are refused
     :return: the same shape and dtype; there is no gradient.  X is held in 32 bits; the operands of the products have 11
-        bits for bfloat16 matrices and 22 for float32 ones, sums are formed in 32 bits in a fixed order.  A matrix with NaN or
-        an infinity becomes NaN, one of zeros stays as it is."""
+        bits for bfloat16 matrices (A 22 where the shorter side is at most 128) and 22 for float32 ones, sums are formed in
+        32 bits in a fixed order.  A matrix with NaN or an infinity becomes NaN, one of zeros stays as it is."""
     return core.orthogonalize(x, _flat(coefficients, steps), float(eps))
 
 

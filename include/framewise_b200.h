@@ -177,10 +177,11 @@ int framewise_b200_scores_backward(const framewise_b200_scores_shape* shape, con
 /* Orthogonalisation by Newton-Schulz products.  For X = x / max(|x|, eps) (Frobenius norm; matrices with more rows than
  * columns lie transposed) and each of `steps` triples (a, b, c) of `coefficients` (HOST array of 3 steps values):
  *     A = X X^T;  X = a X + (b A + c A A) X
- * X is held in 32 bits; the products' operands are rounded to 11 bits for bf16 matrices, 22 for f32 ones, the sums are
- * formed in 32 bits in a fixed order: equal calls give equal bits.  `count` dense matrices of rows x cols one after another,
- * out likewise (may be x).  eps: any positive number.  A matrix with NaN or an infinity becomes NaN; zeros stay zeros.  Coefficients that let a
- * singular value grow past 10^6 are refused.  The result of _bytes is 0 for sizes past the limits. */
+ * X is held in 32 bits; the products' operands are rounded to 11 bits for bf16 matrices (22 for A = X X^T where the shorter side is at most
+ * 128), to 22 for f32 ones, the sums are formed in 32 bits in a fixed order: equal calls give equal bits.  `count` dense matrices
+ * of rows x cols one after another, out likewise (may be x).  eps: any positive number.  A matrix with NaN or an infinity becomes
+ * NaN; zeros stay zeros.  Coefficients that let a singular value grow past 10^6 are refused.  The result of _bytes is 0 for sizes
+ * past the limits. */
 size_t framewise_b200_orthogonalize_bytes(int64_t count, int64_t rows, int64_t cols, int32_t dtype);
 int framewise_b200_orthogonalize(int64_t count, int64_t rows, int64_t cols, int32_t dtype, const void* x, void* out,
                                  const double* coefficients, int32_t steps, double eps, void* work, size_t work_bytes,
