@@ -122,8 +122,8 @@ __device__ __forceinline__ float largest(const Raw<__nv_bfloat16>* v) {
 __device__ __forceinline__ float value(float x) { return x; }
 __device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// A lane has 128 bytes under way: a block of so many vectors.  (bf16, 20000 x 12001: half of them with the next half loaded before
-// they are worked on 111 us, and the gradient 184; this 107 and 170.)
+// A lane has 128 bytes under way: a block of so many vectors.  (bf16, 20000 x 12001: 89 us, and the gradient 170; half of them with
+// the next half loaded before they are worked on took 4 and 14 us more.)
 template <typename X>
 constexpr int kAhead = 128 / (8 * (int)sizeof(X));
 
@@ -249,7 +249,7 @@ struct Room {
 // The best that a warp has met.  While the sums are formed only the maximum of each cell, 32 values of a lane in kCell steps
 // that the team takes in turn, is written down.  After kCells of them, or at the row's end, those cells are read again whose maximum is no smaller
 // than the `top`-th largest of the lanes' maxima: some more than `top` of them.  (Looking at each value while the sums are formed,
-// against the list so far: 26 instructions a value for the whole kernel, 20000 x 12001 f32 with 8 alternatives 664 us; 202 this way,
+// against the list so far: 26 instructions a value for the whole kernel, 20000 x 12001 f32 with 8 alternatives 664 us; 199 this way,
 // and 148 without alternatives.)
 struct Best {
     uint64_t list;    // the 32 largest so far, a lane each, in falling order
@@ -352,7 +352,7 @@ struct Scored {
 
 // A row per team of r.team warps (1 to 8 of a CTA; 16 to 64: all of 2 to 8 CTAs of a cluster), which take its steps of 256
 // logits in turn.  f32 without alternatives is bound by memory (20000 x 12001 6.5 TB/s), bf16 by exponentials and the instructions
-// around them (5.3 TB/s).  Three CTAs an SM where the registers of four do not do (f32 with 8 alternatives 221 us for 198).
+// around them (5.3 TB/s).  Three CTAs an SM where the registers of four do not do (f32 with 8 alternatives 221 us for 199).
 template <typename X, typename L, bool TOP>
 __global__ void __launch_bounds__(kWarps * 32, sizeof(X) == 4 && !TOP ? 4 : 3) k_label_scores(const X* __restrict__ z, const Rows r, const Scored out) {
     __shared__ Sums     part[kWarps];

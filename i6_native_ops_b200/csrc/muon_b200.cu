@@ -251,7 +251,8 @@ __global__ void __launch_bounds__(256) k_muon_collect(const __grid_constant__ Sl
 // X = U / max(|U|, eps) in 32 bits and as operands, zeros where there are none: a CTA takes kBlocks squares of 64 columns and rows, the
 // next of which is loaded while one is written.  (A square each: 204 us for 4 x 2048 x 8192 bf16, 184 with four, its bytes at the
 // copy's rate 123.  Smaller calls end sooner with more CTAs: all five steps of 6 x 500 x 2001 f32 487 us with four and chunks of 16384,
-// 472 with two and 8192; 16 x 512 x 2048 bf16 502 and 494; 8 x 2048 x 8192 bf16 5390 and 5430.)
+// 472 with two and 8192; 16 x 512 x 2048 bf16 502 and 494; 8 x 2048 x 8192 bf16 5390 and 5430.)  The loads ahead are kept across the
+// norm's division: 120 to 160 bytes a thread spill there, at five CTAs an SM.
 constexpr int kBlocks = 2;
 template <typename X, int PARTS>
 __global__ void __launch_bounds__(256, 5) k_muon_begin(const Entry* __restrict__ table, int count, const Rates r, float scale, __half* work, const __grid_constant__ Steps steps) {
@@ -527,6 +528,8 @@ __global__ void __launch_bounds__(256) k_muon_check(const Entry* __restrict__ ta
 // 31 at the copy's rate).  Tried and not kept: all products in one cooperative launch in which a tile waits for its matrix's tiles
 // alone (3.9 us for a product of the smallest either way; 4 x 2048 x 8192 10 % slower: two stages of the ring went to the update),
 // X and results by the copy engine (its queue holds them up; the ring lost three stages: X 249), X brought to the second cache ahead.
+// f32: the 128 sums a thread leave the last product no registers for parameters: it spills 336 to 344 bytes a thread and takes 91 us for
+// 12 x 500 x 2000, where a X + B X alone takes 54 (the other products spill 52 to 96; bf16 none).
 template <int KIND, int PARTS, int CG>
 __global__ void __launch_bounds__(kThreads, 1) k_muon_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
     constexpr bool kApplies = KIND == kApply || KIND == kLast;
@@ -916,6 +919,7 @@ struct SmallSteps {
 // three products a step, each behind a barrier, and what turns its sums into the next operands: 64 x 256 bf16 14 us and 4.6 a step, f32 14 and
 // 9.2 (a chain of launches: 80 and 136 for five steps, and 17 launches of the host's time).  Descriptors counted up instead of formed for
 // each product, and waits that ask without a pause, changed nothing.
+// (f32 spills 368 bytes a thread, bf16 108.)
 // A has two parts for bf16 as well: with one, results of few rows are off by up to 1.9 times their own rounding (2 x 27; 1.2 times with two).
 template <typename X>
 __global__ void __launch_bounds__(kSmallThreads, 1) k_muon_small(const __grid_constant__ SmallSlots s, const Rates r, const __grid_constant__ SmallSteps steps) {

@@ -341,9 +341,11 @@ def muon_step(
     follow: bool = False,
 ) -> None:
     """One step of Muon over a list of matrices, in place: ``v += (1 - beta) (g - v)``, ``u = g + beta (v - g)`` (without
-    ``nesterov``: ``v``), ``p = p (1 - lr weight_decay) - lr s orthogonalize(u)``.  Matrices of up to 128 x 256 take one
-    launch, the others, of whatever shapes, go through each product in one launch (256 of them, as far as two gigabytes of
-    scratch hold them).  As after any operation in place, graphs that saved a parameter before refuse their backward pass.
+    ``nesterov``: ``v``), ``p = p (1 - lr weight_decay) - lr s orthogonalize(u)``.  Matrices of up to 128 x 256 take a
+    launch for every 24 of them, the others, of whatever shapes, go through each product in one launch (256 of them, as far as
+    two gigabytes of scratch hold them).  Copies too get what :func:`orthogonalize` makes of the parameters' type: for
+    bfloat16 parameters the update is off by some 0.6e-3 to 1e-3 of its norm (up to 2e-3 where a matrix has a few rows), whether
+    or not there is a copy in 32 bits.  As after any operation in place, graphs that saved a parameter before refuse their backward pass.
 
     :param params: contiguous CUDA matrices, all float32 or all bfloat16.  Parameters, momentum and copies overlap neither each
         other nor a gradient; gradients may be shared

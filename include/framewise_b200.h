@@ -201,8 +201,9 @@ typedef struct {
  *     x = x (1 - lr weight_decay) - lr s o,   s = sqrt(max(1, rows / cols)), or match_rms: 0.2 sqrt(max(rows, cols))
  * x being the master copy where there is one (the parameter is then x rounded once); follow: a copy of which its parameter
  * is not the rounded value starts from the parameter.  What is written (params, momentum, masters) overlaps nothing else of the
- * call; gradients may be shared.  Matrices of up to 128 x 256 (either way round) take one launch, the
- * others a chain of 3 steps + 3 launches together, 256 of them and two gigabytes of scratch at most at a time. */
+ * call; gradients may be shared.  Matrices of up to 128 x 256 (either way round) take a launch for every 24 of them; the others go
+ * together, 256 of them and two gigabytes of scratch at most at a time, through a chain of 3 steps + 2 launches and one for every 24 of
+ * them. */
 size_t framewise_b200_muon_bytes(const framewise_b200_matrix* matrices, int64_t count, int32_t dtype);
 int framewise_b200_muon(const framewise_b200_matrix* matrices, int64_t count, int32_t dtype, double lr, double beta,
                         int32_t nesterov, double weight_decay, int32_t match_rms, const double* coefficients,
